@@ -107,6 +107,13 @@ enum {
      * limit (never expected: waits end when earlier tiles commit). Its query
      * window's output rows were written as NaN. */
     SPARDA_STATUS_PREFILL_WAIT_TIMEOUT = 1,
+    /* Offsets of packed sequences that fall or leave [0, N]. The rows of such
+     * a sequence were not written. */
+    SPARDA_STATUS_SEQUENCE_RANGE = 2,
+    /* A page index outside [0, n_pages), or a length or position outside the
+     * page table's row. The sequence's output rows were written as NaN
+     * (sparda_decode_paged); the new row was dropped (sparda_append_paged). */
+    SPARDA_STATUS_PAGE_RANGE = 4,
 };
 
 /*
@@ -836,6 +843,85 @@ SPARDA_API int sparda_offload_rebuild_sums(sparda_offload_t h, int64_t len, int6
 SPARDA_API int sparda_offload_fetch(sparda_offload_t h, const int32_t* sel, const int32_t* n_sel,
                                     int64_t sel_cap, int64_t block_size, int64_t len, int method,
                                     void* k_dst, void* v_dst, void* stream);
+
+/*
+ * ---- Batches of sequences of different lengths ----
+ * Three operators that need no padding: attention over packed prompts, the
+ * write of new keys and values into a cache of pages, and single-token
+ * attention over that cache. No counterpart in the reference, whose prefill
+ * and caches hold one length per batch (model/attention/base.py:11-32,
+ * model/attention/sparse.py:201-224). The offsets, lengths, positions and page
+ * tables are device arrays of int32 that the host does not read: the calls can
+ * be captured into a HIP graph and replayed as these change. Values out of
+ * range never lead to an access out of bounds; they raise a bit of the status
+ * word (sparda_status). The stream must belong to the current device.
+ *
+ * Packed sequences: sequence i is rows [cu_seqlens[i], cu_seqlens[i+1]) of N,
+ * 0 <= i < n_seqs; sequences may be empty. Rows before the first and behind the
+ * last sequence are neither read nor written.
+ *
+ * Pages: position p of sequence b is row p % page_size of page
+ * page_table[b * t_st + p / page_size], p < width * page_size. k_pages,
+ * v_pages: [n_pages, page_size, Hkv, D] of dtype, both with element strides
+ * (p_st, s_st, h_st, 1), rows 16-byte aligned; page_size a multiple of 16.
+ * Sequences may share pages. Entries of the table past a sequence's length are
+ * not read.
+ */
+
+/*
+ * Attention over packed prompts, grouped heads.
+ *   out[t,h*D+d] = sum_{s in A(t)} softmax_s(q[t,h].k[s,g] * scale) v[s,g,d],
+ *   g = h / (Hq/Hkv), A(t) = the rows of t's sequence, those up to t if causal.
+ * Sums and softmax statistics in fp32; for bf16 the weights are rounded to
+ * bf16 for the product with v.
+ *   q: [N,Hq,D] strides (q_st, q_sh, 1); k, v: [N,Hkv,D] strides (kv_st,
+ *   kv_sh, 1); out: [N,Hq*D] of dtype, stride out_st; D in {16, 32, 64, 128},
+ *   any Hq that Hkv divides. A row outside A(t) has no part in out[t], whatever
+ *   it holds. cu_seqlens: n_seqs + 1 offsets.
+ */
+SPARDA_API int sparda_prefill_packed(const void* q, int64_t q_st, int64_t q_sh,
+                                     const void* k, const void* v, int64_t kv_st, int64_t kv_sh,
+                                     int dtype, const int32_t* cu_seqlens, int64_t n_seqs, int64_t N,
+                                     int64_t Hq, int64_t Hkv, int64_t D, int causal, float scale,
+                                     void* out, int64_t out_st, void* stream);
+
+/*
+ * Writes new keys and values into the pages: row j of sequence i becomes
+ * position positions[i] + j.
+ *   k_new, v_new: [N,Hkv,D] of dtype, strides (new_st, new_sh, 1), rows 16-byte
+ *   aligned; cu_seqlens: the sequences' rows, or NULL: one row per sequence,
+ *   N = n_seqs. A sequence with a negative position takes no part. Two rows for
+ *   the same page row in one call leave either of them there.
+ */
+SPARDA_API int sparda_append_paged(void* k_pages, void* v_pages, int dtype, int64_t n_pages, int64_t page_size,
+                                   int64_t p_st, int64_t s_st, int64_t h_st, const int32_t* page_table,
+                                   int64_t t_st, int64_t width, const int32_t* positions,
+                                   const int32_t* cu_seqlens, int64_t n_seqs, const void* k_new,
+                                   const void* v_new, int64_t N, int64_t new_st, int64_t new_sh,
+                                   int64_t Hkv, int64_t D, void* stream);
+
+/* Workspace bytes sparda_decode_paged needs for these sizes (0: none). */
+SPARDA_API size_t sparda_decode_paged_workspace_bytes(int64_t B, int64_t width, int64_t page_size,
+                                                      int64_t Hq, int64_t Hkv, int64_t D, int dtype);
+
+/*
+ * Attention of one token per sequence over the paged cache:
+ *   out[b,h*D+d] = sum_{p < lengths[b]} softmax_p(q[b,h].k[p,g] * scale) v[p,g,d];
+ * zeros where lengths[b] is 0.
+ *   q: [B,Hq,D] of dtype, strides (q_sb, q_sh, 1), rows 16-byte aligned;
+ *   lengths: [B]; out: [B,Hq*D] of dtype, stride out_sb. The keys of the whole
+ *   batch are cut into equal shares over the workgroups; the shares of a
+ *   sequence are joined by a second launch through the workspace (written and
+ *   read within the call; calls that share one must be ordered on one stream).
+ *   The result depends on the batch's lengths through the order of summation.
+ */
+SPARDA_API int sparda_decode_paged(const void* q, int64_t q_sb, int64_t q_sh,
+                                   const void* k_pages, const void* v_pages, int dtype,
+                                   int64_t n_pages, int64_t page_size, int64_t p_st, int64_t s_st, int64_t h_st,
+                                   const int32_t* page_table, int64_t t_st, int64_t width,
+                                   const int32_t* lengths, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                   float scale, void* out, int64_t out_sb,
+                                   void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

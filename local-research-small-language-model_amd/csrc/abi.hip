@@ -921,4 +921,96 @@ SPARDA_API int sparda_offload_append_at_prefetch(sparda_offload_t h, const void*
                              static_cast<hipStream_t>(stream), &pf);
 }
 
+// ---- packed prompts and the paged cache ----
+
+SPARDA_API int sparda_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void* k, const void* v,
+                                     int64_t kv_st, int64_t kv_sh, int dtype, const int32_t* cu_seqlens,
+                                     int64_t n_seqs, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int causal,
+                                     float scale, void* out, int64_t out_st, void* stream) {
+    SPARDA_REQUIRE(q && k && v && cu_seqlens && out, SPARDA_ERR_NULL, "prefill_packed: null pointer");
+    SPARDA_REQUIRE(dtype_ok(dtype), SPARDA_ERR_DTYPE, "prefill_packed: dtype %d unsupported", dtype);
+    SPARDA_REQUIRE(n_seqs > 0 && N > 0 && Hq > 0 && Hkv > 0, SPARDA_ERR_SHAPE, "prefill_packed: sizes must be positive");
+    SPARDA_REQUIRE(head_dim_ok(D), SPARDA_ERR_SHAPE, "prefill_packed: head dim %lld not in {16,32,64,128}",
+                   (long long)D);
+    SPARDA_REQUIRE(Hq % Hkv == 0, SPARDA_ERR_SHAPE, "prefill_packed: Hq must be a multiple of Hkv");
+    SPARDA_REQUIRE(N < (1ll << 31) && n_seqs < (1ll << 31) && Hq <= 65535, SPARDA_ERR_SHAPE,
+                   "prefill_packed: too many rows, sequences or heads");
+    SPARDA_REQUIRE(N == 1 || out_st >= Hq * D, SPARDA_ERR_STRIDE, "prefill_packed: output rows overlap");
+    return launch_prefill_packed(q, q_st, q_sh, k, v, kv_st, kv_sh, dtype, cu_seqlens, n_seqs, N, Hq, Hkv, D,
+                                 causal != 0, scale, out, out_st, static_cast<hipStream_t>(stream));
+}
+
+// the pages' sizes and strides, common to both entries
+static int check_pages(const char* who, const void* k, const void* v, int dtype, int64_t n_pages, int64_t page_size,
+                       int64_t p_st, int64_t s_st, int64_t h_st, int64_t t_st, int64_t width, int64_t Hkv, int64_t D) {
+    SPARDA_REQUIRE(dtype_ok(dtype), SPARDA_ERR_DTYPE, "%s: dtype %d unsupported", who, dtype);
+    SPARDA_REQUIRE(n_pages > 0 && width > 0 && Hkv > 0, SPARDA_ERR_SHAPE, "%s: sizes must be positive", who);
+    SPARDA_REQUIRE(page_size >= 16 && page_size % 16 == 0, SPARDA_ERR_SHAPE,
+                   "%s: page size %lld is no positive multiple of 16", who, (long long)page_size);
+    SPARDA_REQUIRE(head_dim_ok(D), SPARDA_ERR_SHAPE, "%s: head dim %lld not in {16,32,64,128}", who, (long long)D);
+    SPARDA_REQUIRE(n_pages < (1ll << 31) && Hkv <= 65535 && page_size < (1ll << 31) && width <= 0x7fffffff / page_size,
+                   SPARDA_ERR_SHAPE, "%s: 2^31 pages, or 2^31 positions in a row of the table", who);
+    const int64_t ve = 16 / (dtype == SPARDA_F32 ? 4 : 2);
+    SPARDA_REQUIRE(p_st >= 0 && s_st >= 0 && h_st >= 0 && t_st >= 0, SPARDA_ERR_STRIDE, "%s: negative stride", who);
+    SPARDA_REQUIRE(aligned16(k) && aligned16(v) && p_st % ve == 0 && s_st % ve == 0 && h_st % ve == 0,
+                   SPARDA_ERR_STRIDE, "%s: the rows of the pages must be 16-byte aligned", who);
+    SPARDA_REQUIRE(s_st < (1ll << 26), SPARDA_ERR_STRIDE, "%s: 2^26 elements between rows of a page", who);
+    return 0;
+}
+
+SPARDA_API int sparda_append_paged(void* k_pages, void* v_pages, int dtype, int64_t n_pages, int64_t page_size,
+                                   int64_t p_st, int64_t s_st, int64_t h_st, const int32_t* page_table, int64_t t_st,
+                                   int64_t width, const int32_t* positions, const int32_t* cu_seqlens, int64_t n_seqs,
+                                   const void* k_new, const void* v_new, int64_t N, int64_t new_st, int64_t new_sh,
+                                   int64_t Hkv, int64_t D, void* stream) {
+    SPARDA_REQUIRE(k_pages && v_pages && page_table && positions && k_new && v_new, SPARDA_ERR_NULL,
+                   "append_paged: null pointer");
+    if (const int rc = check_pages("append_paged", k_pages, v_pages, dtype, n_pages, page_size, p_st, s_st, h_st, t_st,
+                                   width, Hkv, D))
+        return rc;
+    SPARDA_REQUIRE(n_seqs > 0 && N > 0 && n_seqs < (1ll << 31) && N < (1ll << 31), SPARDA_ERR_SHAPE,
+                   "append_paged: bad numbers of sequences or rows");
+    SPARDA_REQUIRE(cu_seqlens || N == n_seqs, SPARDA_ERR_SHAPE,
+                   "append_paged: without offsets every sequence takes one row (%lld rows, %lld sequences)",
+                   (long long)N, (long long)n_seqs);
+    const int64_t ve = 16 / (dtype == SPARDA_F32 ? 4 : 2);
+    SPARDA_REQUIRE(aligned16(k_new) && aligned16(v_new) && new_st % ve == 0 && new_sh % ve == 0, SPARDA_ERR_STRIDE,
+                   "append_paged: the new rows must be 16-byte aligned");
+    return launch_append_paged(k_pages, v_pages, n_pages, page_size, p_st, s_st, h_st, dtype, page_table, t_st, width,
+                               positions, cu_seqlens, n_seqs, k_new, v_new, N, new_st, new_sh, Hkv, D,
+                               static_cast<hipStream_t>(stream));
+}
+
+SPARDA_API size_t sparda_decode_paged_workspace_bytes(int64_t B, int64_t width, int64_t page_size, int64_t Hq,
+                                                      int64_t Hkv, int64_t D, int dtype) {
+    if (B <= 0 || width <= 0 || page_size <= 0 || Hkv <= 0 || Hq < Hkv || D <= 0) return 0;
+    return decode_paged_workspace_bytes(B, width * page_size, Hq, Hkv, D, dtype);
+}
+
+SPARDA_API int sparda_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k_pages, const void* v_pages,
+                                   int dtype, int64_t n_pages, int64_t page_size, int64_t p_st, int64_t s_st,
+                                   int64_t h_st, const int32_t* page_table, int64_t t_st, int64_t width,
+                                   const int32_t* lengths, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, float scale,
+                                   void* out, int64_t out_sb, void* workspace, size_t workspace_bytes, void* stream) {
+    SPARDA_REQUIRE(q && k_pages && v_pages && page_table && lengths && out, SPARDA_ERR_NULL,
+                   "decode_paged: null pointer");
+    if (const int rc = check_pages("decode_paged", k_pages, v_pages, dtype, n_pages, page_size, p_st, s_st, h_st, t_st,
+                                   width, Hkv, D))
+        return rc;
+    SPARDA_REQUIRE(B > 0 && B <= 65535 && Hq > 0 && Hq <= 65535, SPARDA_ERR_SHAPE,
+                   "decode_paged: sequences and query heads must be in [1, 65535]");
+    SPARDA_REQUIRE(Hq % Hkv == 0, SPARDA_ERR_SHAPE, "decode_paged: Hq must be a multiple of Hkv");
+    SPARDA_REQUIRE(B * cdiv(width * page_size, 16) < (1ll << 31), SPARDA_ERR_SHAPE, "decode_paged: too many positions");
+    const int64_t ve = 16 / (dtype == SPARDA_F32 ? 4 : 2);
+    SPARDA_REQUIRE(aligned16(q) && q_sb % ve == 0 && q_sh % ve == 0, SPARDA_ERR_STRIDE,
+                   "decode_paged: the rows of q must be 16-byte aligned");
+    SPARDA_REQUIRE(B == 1 || out_sb >= Hq * D, SPARDA_ERR_STRIDE, "decode_paged: output rows overlap");
+    const size_t need = decode_paged_workspace_bytes(B, width * page_size, Hq, Hkv, D, dtype);
+    SPARDA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)), SPARDA_ERR_WORKSPACE,
+                   "decode_paged: workspace of %zu bytes needed, 16-byte aligned", need);
+    return launch_decode_paged(q, q_sb, q_sh, k_pages, v_pages, n_pages, page_size, p_st, s_st, h_st, dtype,
+                               page_table, t_st, width, lengths, B, Hq, Hkv, D, scale, out, out_sb,
+                               need ? workspace : nullptr, static_cast<hipStream_t>(stream));
+}
+
 }  // extern "C"

@@ -38,6 +38,24 @@ int launch_prefill_routed(const void* q, int64_t q_sb, int64_t q_st, int64_t q_s
 
 // copy the device's status word (SPARDA_STATUS_* bits) to out, clearing it when asked
 int launch_read_status(uint32_t* out, int clear, hipStream_t stream);
+// the current device's status word, for kernels of other sources
+int status_word(uint32_t** word);
+
+// packed prompts (prefill_packed.hip)
+int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void* k, const void* v, int64_t kv_st,
+                          int64_t kv_sh, int dtype, const int32_t* cu, int64_t n, int64_t N, int64_t Hq, int64_t Hkv,
+                          int64_t D, int causal, float scale, void* out, int64_t out_st, hipStream_t stream);
+
+// the paged cache (paged.hip); cap = table entries x page size
+int launch_append_paged(void* k, void* v, int64_t n_pages, int64_t ps, int64_t p_st, int64_t s_st, int64_t h_st,
+                        int dtype, const int32_t* table, int64_t t_st, int64_t width, const int32_t* positions,
+                        const int32_t* cu, int64_t n, const void* k_new, const void* v_new, int64_t N, int64_t new_st,
+                        int64_t new_sh, int64_t Hkv, int64_t D, hipStream_t stream);
+size_t decode_paged_workspace_bytes(int64_t B, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D, int dtype);
+int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k, const void* v, int64_t n_pages,
+                        int64_t ps, int64_t p_st, int64_t s_st, int64_t h_st, int dtype, const int32_t* table,
+                        int64_t t_st, int64_t width, const int32_t* len, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                        float scale, void* out, int64_t out_sb, void* workspace, hipStream_t stream);
 
 // dense (no selection lists) bf16 prefill, D = 64 (prefill_dense.hip)
 bool prefill_dense_supported(int dtype, int64_t Hq, int64_t Hkv, int64_t D, int64_t q_sb, int64_t q_st,

@@ -1,0 +1,555 @@
+// A key-value cache in pages (sparda_append_paged, sparda_decode_paged): pages
+// of ps rows [ps, Hkv, D], position p of sequence b in row p % ps of page
+// table[b, p / ps].
+#include "common.h"
+#include "kernels.h"
+#include "mfma.h"
+
+namespace sparda {
+
+namespace {
+
+constexpr float kPgLog2e = 1.4426950408889634f;
+
+// the pages and the table, as both kernels read them (strides in elements)
+struct Pages {
+    int64_t p_st, s_st, h_st;      // page, row, head
+    const int32_t* table;
+    int64_t t_st;                  // between the sequences' rows of the table
+    int width;                     // entries of a row
+    int n_pages;
+};
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+
+// One wavefront per new row: its sequence (64 offsets at a time), its page, then
+// the row's heads in 16-byte pieces.
+__global__ void __launch_bounds__(256)
+append_paged_kernel(char* __restrict__ k, char* __restrict__ v, Pages pg, int ps, const int32_t* __restrict__ positions,
+                    const int32_t* __restrict__ cu, int n, const char* __restrict__ k_new,
+                    const char* __restrict__ v_new, int64_t N, int64_t new_st, int64_t new_sh, int Hkv, int row_bytes,
+                    int es, uint32_t* __restrict__ status) {
+    const int lane = threadIdx.x % kWave;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if (t >= N) return;
+    int seq = -1;
+    int64_t at = 0;                               // the row's place among its sequence's new rows
+    if (cu == nullptr) {
+        seq = static_cast<int>(t);
+    } else {
+        // the last sequence that starts at or before t, when t is one of its rows
+        for (int i0 = 0; i0 < n; i0 += kWave) {
+            const int i = i0 + lane;
+            const uint64_t m = __ballot(i < n && cu[i < n ? i : n] <= t);
+            if (m == 0) break;
+            seq = i0 + 63 - __builtin_clzll(m);
+            if (m != ~0ull) break;
+        }
+        seq = __builtin_amdgcn_readfirstlane(seq);
+        if (seq < 0) return;
+        const int c0 = __builtin_amdgcn_readfirstlane(cu[seq]), c1 = __builtin_amdgcn_readfirstlane(cu[seq + 1]);
+        if (t >= c1) return;                      // behind the last sequence
+        at = t - c0;
+    }
+    const int p0 = __builtin_amdgcn_readfirstlane(positions[seq]);
+    if (p0 < 0) return;                           // a sequence that takes no part
+    const int64_t pos = p0 + at;
+    const int64_t slot = pos / ps;
+    int page = -1;
+    if (slot < pg.width) page = __builtin_amdgcn_readfirstlane(pg.table[seq * pg.t_st + slot]);
+    if (page < 0 || page >= pg.n_pages) {         // the row is dropped
+        if (lane == 0) atomicOr(status, static_cast<uint32_t>(SPARDA_STATUS_PAGE_RANGE));
+        return;
+    }
+    const int64_t to = (page * pg.p_st + (pos - slot * ps) * pg.s_st) * es;
+    const int64_t from = t * new_st * es;
+    const int per = row_bytes / 16;               // pieces of a head's row
+    for (int c = lane; c < Hkv * per; c += kWave) {
+        const int h = c / per, o = (c - h * per) * 16;
+        const int64_t src = from + h * new_sh * es + o, dst = to + h * pg.h_st * es + o;
+        *reinterpret_cast<uint4*>(k + dst) = *reinterpret_cast<const uint4*>(k_new + src);
+        *reinterpret_cast<uint4*>(v + dst) = *reinterpret_cast<const uint4*>(v_new + src);
+    }
+}
+
+int launch_append_paged(void* k, void* v, int64_t n_pages, int64_t ps, int64_t p_st, int64_t s_st, int64_t h_st,
+                        int dtype, const int32_t* table, int64_t t_st, int64_t width, const int32_t* positions,
+                        const int32_t* cu, int64_t n, const void* k_new, const void* v_new, int64_t N, int64_t new_st,
+                        int64_t new_sh, int64_t Hkv, int64_t D, hipStream_t stream) {
+    uint32_t* status;
+    if (const int rc = status_word(&status)) return rc;
+    const Pages pg{p_st, s_st, h_st, table, t_st, static_cast<int>(width), static_cast<int>(n_pages)};
+    const int es = dtype == SPARDA_F32 ? 4 : 2;
+    hipLaunchKernelGGL(append_paged_kernel, dim3(static_cast<unsigned>(cdiv(N, 4))), dim3(256), 0, stream,
+                       static_cast<char*>(k), static_cast<char*>(v), pg, static_cast<int>(ps), positions, cu,
+                       static_cast<int>(n), static_cast<const char*>(k_new), static_cast<const char*>(v_new), N, new_st,
+                       new_sh, static_cast<int>(Hkv), static_cast<int>(D * es), es, status);
+    return check_hip(hipGetLastError(), "append_paged_kernel");
+}
+
+// ---------------------------------------------------------------------------
+// decode
+// ---------------------------------------------------------------------------
+
+namespace {
+
+// Shares of a launch. A sequence's keys are walked in steps of 16 kTiles keys.
+// All steps of the batch are cut into shares of the same number of steps, so
+// that long and short sequences load the workgroups alike: the share length is
+// the total over `target`, at least `least`, and sequence b takes
+// n_b = max(1, ceil(steps_b / share)) consecutive items, at most target + B of
+// them in all. Every workgroup derives this from the lengths for itself.
+struct Share {
+    int seq;         // -1: no sequence has this item
+    int part, parts; // the item's place among its sequence's
+    int first;       // the sequence's first item
+    int share;       // steps of an item
+    int len;         // the sequence's length, cut to the table's capacity
+    bool bad;        // the length is out of range
+};
+
+__device__ __forceinline__ int paged_steps(int len, int cap, int step) {
+    const int c = len < 0 ? 0 : len > cap ? cap : len;
+    return static_cast<int>((static_cast<int64_t>(c) + step - 1) / step);
+}
+
+__device__ __forceinline__ int wave_sum_i32(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+    return v;
+}
+__device__ __forceinline__ int wave_scan_i32(int v) {  // inclusive
+    const int lane = threadIdx.x % kWave;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const int w = __shfl_up(v, o, kWave);
+        if (lane >= o) v += w;
+    }
+    return v;
+}
+
+// Steps of an item. The total stays below 2^31 (checked by the host against the capacity).
+__device__ __forceinline__ int paged_share(const int32_t* __restrict__ len, int B, int cap, int step, int target,
+                                           int least) {
+    const int lane = threadIdx.x % kWave;
+    int total = 0;
+    for (int b0 = 0; b0 < B; b0 += kWave) total += b0 + lane < B ? paged_steps(len[b0 + lane], cap, step) : 0;
+    total = __builtin_amdgcn_readfirstlane(wave_sum_i32(total));
+    const int share = (total + target - 1) / target;
+    return share > least ? share : least;
+}
+
+// The item's sequence (by_item), or sequence `want`'s items. Wave-uniform.
+__device__ __forceinline__ Share paged_item(const int32_t* __restrict__ len, int B, int cap, int step, int target,
+                                            int least, bool by_item, int want) {
+    const int lane = threadIdx.x % kWave;
+    Share r{-1, 0, 0, 0, paged_share(len, B, cap, step, target, least), 0, false};
+    int before = 0;
+    for (int b0 = 0; b0 < B; b0 += kWave) {
+        const int b = b0 + lane;
+        const int n = b < B ? max(1, (paged_steps(len[b], cap, step) + r.share - 1) / r.share) : 0;
+        const int end = before + wave_scan_i32(n);      // items of sequences 0 .. b
+        const uint64_t m = __ballot(b < B && (by_item ? end > want : b == want));
+        if (m != 0) {
+            const int at = __builtin_ctzll(m);
+            r.seq = b0 + at;
+            r.parts = __builtin_amdgcn_readfirstlane(__shfl(n, at, kWave));
+            r.first = __builtin_amdgcn_readfirstlane(__shfl(end, at, kWave)) - r.parts;
+            r.part = by_item ? want - r.first : 0;
+            const int l = __builtin_amdgcn_readfirstlane(len[r.seq]);
+            r.bad = l < 0 || l > cap;
+            r.len = l < 0 ? 0 : l > cap ? cap : l;
+            return r;
+        }
+        before = __builtin_amdgcn_readfirstlane(__shfl(end, kWave - 1, kWave));
+    }
+    return r;
+}
+
+template <int DT>
+struct PagedType;
+template <>
+struct PagedType<SPARDA_BF16> {
+    static constexpr int kTiles = 2;   // 16-key tiles of a step
+    typedef short E;
+};
+template <>
+struct PagedType<SPARDA_F32> {
+    static constexpr int kTiles = 1;
+    typedef float E;
+};
+
+// The operands of one step, as loaded
+template <int DT, int D>
+struct PagedStep {
+    static constexpr int kTiles = PagedType<DT>::kTiles;
+    static constexpr int kQ = DT == SPARDA_F32 ? D / 16 : (D + 31) / 32;   // 16-byte pieces of K a lane holds per tile
+    static constexpr int kV = D / 16;                                       // elements of V per key a lane holds
+    typedef typename PagedType<DT>::E VRow __attribute__((ext_vector_type(kV)));
+    uint4 k[kTiles][kQ];
+    VRow v[kTiles][4];
+};
+
+struct PagedDecode {
+    const void* q;
+    int64_t q_sb, q_sh;
+    const void *k, *v;
+    Pages pg;
+    int ps16;                     // 16-key tiles of a page
+    const int32_t* len;
+    int B, cap;
+    int Hq, Hkv, R, head_tiles;   // head tiles of 16 query heads per KV head
+    int target, least;
+    float scale_log2;
+    void* out;
+    int64_t out_sb;
+    float *part_o, *part_ml;      // [items, Hq, D], [items, Hq, 2]
+    uint32_t* status;
+};
+
+}  // namespace
+
+// One workgroup of W wavefronts per (KV head, tile of up to 16 of its query
+// heads, item). The heads are the 16 columns of the matrix products:
+//     S^T[key, head] = K[key, :] . Q[head, :]
+//     P = exp2(S scale log2 e - m[head])
+//     O^T[d, head] += V^T[d, key] . P^T[key, head]
+// Wavefront w walks the steps w, w + W, ... of the share with its own (m, l, O);
+// K and V go straight from the pages to the operand registers, the next step's
+// under the present one's arithmetic, and S^T's layout is already that of the
+// P operand, so nothing passes through LDS before the wavefronts are joined. A
+// tile's 16 keys lie in one page (pages hold a multiple of 16 rows), so that its
+// base address is a scalar.
+template <int DT, int D, int W>
+__global__ void __launch_bounds__(W* kWave) decode_paged_kernel(PagedDecode a) {
+    typedef PagedStep<DT, D> Step;
+    constexpr int kTiles = Step::kTiles, kV = Step::kV, kQ = Step::kQ, kStep = 16 * kTiles;
+    extern __shared__ float lds[];
+    const int lane = threadIdx.x % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int c16 = lane % 16, grp = lane / 16;
+    const int heads = a.Hkv * a.head_tiles;
+    const int item = blockIdx.x / heads, gt = blockIdx.x % heads;
+    const int g = gt / a.head_tiles, h0 = gt % a.head_tiles * 16;
+    const int nh = a.R - h0 < 16 ? a.R - h0 : 16;           // query heads of the tile
+    const Share sh = paged_item(a.len, a.B, a.cap, kStep, a.target, a.least, true, item);
+    if (sh.seq < 0) return;                                 // workgroup-uniform
+    const int b = sh.seq, len = sh.len;
+    const int steps = paged_steps(len, a.cap, kStep);
+    const int s_end = min(steps, (sh.part + 1) * sh.share);
+    bool bad = sh.bad;
+
+    // this lane's column of Q
+    uint4 qr[kQ];
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) qr[i] = uint4{0, 0, 0, 0};
+    {
+        const int64_t qo = b * a.q_sb + static_cast<int64_t>(g * a.R + h0 + c16) * a.q_sh;
+#pragma unroll
+        for (int i = 0; i < kQ; ++i) {
+            const int d = DT == SPARDA_F32 ? 16 * i + 4 * grp : 32 * i + 8 * grp;
+            if (c16 < nh && d < D)
+                qr[i] = *reinterpret_cast<const uint4*>(static_cast<const char*>(a.q) + (qo + d) * (DT == SPARDA_F32 ? 4 : 2));
+        }
+    }
+
+    // the walk over the table: tile 2 u (or u) of step u in page `page`, `rem` tiles into it
+    const int32_t* row = a.pg.table + b * a.pg.t_st;
+    const int tile0 = (sh.part * sh.share + wave) * kTiles;
+    int page = tile0 / a.ps16, rem = tile0 % a.ps16;
+    const int adv_p = W * kTiles / a.ps16, adv_r = W * kTiles % a.ps16;
+    const int last_tile = (len - 1) / 16;
+    typedef typename PagedType<DT>::E E;
+    const E* kg = static_cast<const E*>(a.k) + g * a.pg.h_st;
+    const E* vg = static_cast<const E*>(a.v) + g * a.pg.h_st;
+    const int s_st = static_cast<int>(a.pg.s_st);
+    auto load = [&](int u, Step& x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            int tile = u * kTiles + t, p = page, r = rem;
+            if (t == 1) {
+                if (tile > last_tile) --tile;                // past the end: the step's first tile again, masked
+                else if (++r == a.ps16) r = 0, ++p;
+            }
+            int id = row[p];
+            if (id < 0 || id >= a.pg.n_pages) bad = true, id = 0;
+            const int last = len - 1 - 16 * tile;            // rows past the end read the last one
+            const int64_t base = id * a.pg.p_st + static_cast<int64_t>(16 * r) * a.pg.s_st;
+            const E* kb = kg + base;
+            const E* vb = vg + base;
+            const int kr = c16 < last ? c16 : last;
+#pragma unroll
+            for (int i = 0; i < kQ; ++i) {
+                const int d = DT == SPARDA_F32 ? 16 * i + 4 * grp : 32 * i + 8 * grp;
+                x.k[t][i] = uint4{0, 0, 0, 0};
+                if (D >= 32 || DT == SPARDA_F32 || d < D)
+                    x.k[t][i] = *reinterpret_cast<const uint4*>(kb + (kr * s_st + d));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int vr = 4 * grp + i < last ? 4 * grp + i : last;
+                x.v[t][i] = *reinterpret_cast<const typename Step::VRow*>(vb + (vr * s_st + kV * c16));
+            }
+        }
+        rem += adv_r;
+        page += adv_p;
+        if (rem >= a.ps16) rem -= a.ps16, ++page;
+    };
+
+    float m = -__builtin_inff(), l = 0.0f;                   // the column's maximum (log2 units), this lane's part of its sum
+    f32x4 o[kV];
+#pragma unroll
+    for (int j = 0; j < kV; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto compute = [&](int u, Step& x) __attribute__((always_inline)) {
+        f32x4 s[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < kQ; ++i) {
+                if constexpr (DT == SPARDA_F32) {
+                    const f32x4 ka = __builtin_bit_cast(f32x4, x.k[t][i]), qb = __builtin_bit_cast(f32x4, qr[i]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(ka[e], qb[e], s[t], 0, 0, 0);
+                } else {
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.k[t][i]),
+                                                                   __builtin_bit_cast(bf16x8, qr[i]), s[t], 0, 0, 0);
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) s[t] *= a.scale_log2;
+        const int key0 = u * kStep;
+        if (key0 + kStep > len) {                            // the last step: its keys past the end weigh nothing
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (key0 + 16 * t + 4 * grp + i >= len) {
+                        s[t][i] = -__builtin_inff();
+#pragma unroll
+                        for (int j = 0; j < kV; ++j) x.v[t][i][j] = 0;
+                    }
+        }
+        float mx = m;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][i]);
+        // (builtin swaps: both lanes of a pair see the same two values)
+        float2 r2 = rows16_swap(mx);
+        mx = fmaxf(r2.x, r2.y);
+        r2 = rows32_swap(mx);
+        mx = fmaxf(r2.x, r2.y);
+        const float ref = mx == -__builtin_inff() ? 0.0f : mx;
+        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+        m = mx;
+        l *= alpha;
+        float p[kTiles][4];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[t][i] = __builtin_amdgcn_exp2f(s[t][i] - ref);
+                l += p[t][i];
+            }
+#pragma unroll
+        for (int j = 0; j < kV; ++j) o[j] *= alpha;
+        if constexpr (DT == SPARDA_F32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < kV; ++j)
+                    o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[0][i][j], p[0][i], o[j], 0, 0, 0);
+        } else {
+            // P is rounded to bf16 for the product (the sum l keeps it in fp32)
+            bf16x8 pb;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pb[e] = static_cast<__bf16>(p[e / 4][e % 4]);
+#pragma unroll
+            for (int j = 0; j < kV; ++j) {
+                typedef short s16x8 __attribute__((ext_vector_type(8)));
+                s16x8 va;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) va[e] = x.v[e / 4][e % 4][j];
+                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), pb, o[j], 0, 0, 0);
+            }
+        }
+    };
+
+    int u = sh.part * sh.share + wave;
+    if (u < s_end) {
+        Step x, y;
+        load(u, x);
+        while (true) {                                       // wave-uniform
+            if (u + W < s_end) load(u + W, y);
+            compute(u, x);
+            u += W;
+            if (u >= s_end) break;
+            if (u + W < s_end) load(u + W, x);
+            compute(u, y);
+            u += W;
+            if (u >= s_end) break;
+        }
+    }
+    l = pair32_sum(pair16_sum(l));
+
+    // ---- the wavefronts' partials, joined in order ----
+    float* lo = lds;                                          // [W][nh][D]
+    float* lm = lds + W * nh * D;                             // [W][16][2]
+    int* lbad = reinterpret_cast<int*>(lm + W * 32);          // [W]
+    if (c16 < nh) {
+        // O^T tile j, row 4 grp + i: dim kV (4 grp + i) + j
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < kV; ++j) lo[(wave * nh + c16) * D + kV * (4 * grp + i) + j] = o[j][i];
+        if (grp == 0) {
+            lm[(wave * 16 + c16) * 2] = m;
+            lm[(wave * 16 + c16) * 2 + 1] = l;
+        }
+    }
+    const bool any_bad = __ballot(bad) != 0;
+    if (lane == 0) lbad[wave] = any_bad ? 1 : 0;
+    __syncthreads();
+    int bads = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) bads |= lbad[w];
+    if (bads != 0 && threadIdx.x == 0) atomicOr(a.status, static_cast<uint32_t>(SPARDA_STATUS_PAGE_RANGE));
+    for (int e = threadIdx.x; e < nh * D; e += W * kWave) {
+        const int c = e / D, d = e % D;
+        float M = lm[c * 2];
+#pragma unroll
+        for (int w = 1; w < W; ++w) M = fmaxf(M, lm[(w * 16 + c) * 2]);
+        const float ref = M == -__builtin_inff() ? 0.0f : M;
+        float L = 0.0f, O = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float wt = __builtin_amdgcn_exp2f(lm[(w * 16 + c) * 2] - ref);
+            L = __builtin_fmaf(wt, lm[(w * 16 + c) * 2 + 1], L);
+            O = __builtin_fmaf(wt, lo[(w * nh + c) * D + d], O);
+        }
+        if (bads != 0) O = L = __builtin_nanf("");
+        const int h = g * a.R + h0 + c;
+        if (sh.parts == 1) {
+            store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d, len == 0 && bads == 0 ? 0.0f : O / L);
+        } else {
+            const int64_t at = static_cast<int64_t>(item) * a.Hq + h;
+            a.part_o[at * D + d] = O;
+            if (d == 0) {
+                a.part_ml[at * 2] = M;
+                a.part_ml[at * 2 + 1] = L;
+            }
+        }
+    }
+}
+
+// Joins the items of a sequence, one workgroup per (query head, sequence): the
+// items' weights once in LDS, then dims over the lanes and the items over
+// 256 / D thread groups, added in group order.
+template <int DT, int D>
+__global__ void __launch_bounds__(256) decode_paged_join_kernel(PagedDecode a) {
+    constexpr int kStep = 16 * PagedType<DT>::kTiles, kG = 256 / D;
+    __shared__ float red[256], lsum[kG];
+    const int b = blockIdx.y, h = blockIdx.x;
+    const Share sh = paged_item(a.len, a.B, a.cap, kStep, a.target, a.least, false, b);
+    if (sh.parts <= 1) return;                                // written by its one item
+    const int d = threadIdx.x % D, gr = threadIdx.x / D;
+    const int64_t at0 = static_cast<int64_t>(sh.first) * a.Hq + h;
+    float M = -__builtin_inff();
+    for (int i = threadIdx.x % kWave; i < sh.parts; i += kWave) M = fmaxf(M, a.part_ml[(at0 + static_cast<int64_t>(i) * a.Hq) * 2]);
+    M = wave_max(M);
+    const float ref = M == -__builtin_inff() ? 0.0f : M;
+    float L = 0.0f, O = 0.0f;
+    for (int i = gr; i < sh.parts; i += kG) {
+        const int64_t at = at0 + static_cast<int64_t>(i) * a.Hq;
+        const float wt = __builtin_amdgcn_exp2f(a.part_ml[at * 2] - ref);
+        L = __builtin_fmaf(wt, a.part_ml[at * 2 + 1], L);
+        O = __builtin_fmaf(wt, a.part_o[at * D + d], O);
+    }
+    red[threadIdx.x] = O;
+    if (d == 0) lsum[gr] = L;
+    __syncthreads();
+    if (gr != 0) return;
+    float sum = 0.0f, den = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kG; ++i) {
+        sum += red[i * D + d];
+        den += lsum[i];
+    }
+    store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d, sum / den);
+}
+
+namespace {
+
+constexpr int kPgWaves = 4;
+constexpr int kPgLeast = 2 * kPgWaves;   // steps of the smallest share
+constexpr int64_t kPgGroups = 1024;      // workgroups aimed at
+
+struct PagedPlan {
+    int64_t heads, target, items;
+};
+PagedPlan paged_plan(int64_t B, int64_t cap, int64_t Hq, int64_t Hkv, int dtype) {
+    const int64_t heads = Hkv * cdiv(Hq / Hkv, 16), step = dtype == SPARDA_F32 ? 16 : 32;
+    int64_t target = cdiv(kPgGroups, heads);
+    int64_t items = target + B;
+    const int64_t most = B * cdiv(cdiv(cap, step), kPgLeast);  // every share the smallest
+    if (items > most) items = most;
+    return {heads, target, items};
+}
+
+}  // namespace
+
+size_t decode_paged_workspace_bytes(int64_t B, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D, int dtype) {
+    const PagedPlan p = paged_plan(B, cap, Hq, Hkv, dtype);
+    // one item a sequence: written by the item itself
+    return p.items <= B ? 0 : static_cast<size_t>(p.items * Hq * (D + 2)) * sizeof(float);
+}
+
+int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k, const void* v, int64_t n_pages,
+                        int64_t ps, int64_t p_st, int64_t s_st, int64_t h_st, int dtype, const int32_t* table,
+                        int64_t t_st, int64_t width, const int32_t* len, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                        float scale, void* out, int64_t out_sb, void* workspace, hipStream_t stream) {
+    PagedDecode a{};
+    if (const int rc = status_word(&a.status)) return rc;
+    const int64_t cap = width * ps, R = Hq / Hkv;
+    const PagedPlan p = paged_plan(B, cap, Hq, Hkv, dtype);
+    a.q = q, a.q_sb = q_sb, a.q_sh = q_sh, a.k = k, a.v = v;
+    a.pg = Pages{p_st, s_st, h_st, table, t_st, static_cast<int>(width), static_cast<int>(n_pages)};
+    a.ps16 = static_cast<int>(ps / 16), a.len = len, a.B = static_cast<int>(B), a.cap = static_cast<int>(cap);
+    a.Hq = static_cast<int>(Hq), a.Hkv = static_cast<int>(Hkv), a.R = static_cast<int>(R);
+    a.head_tiles = static_cast<int>(cdiv(R, 16));
+    a.target = static_cast<int>(p.target), a.least = kPgLeast;
+    a.scale_log2 = scale * kPgLog2e, a.out = out, a.out_sb = out_sb;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = workspace ? a.part_o + p.items * Hq * D : nullptr;
+    if (p.items * p.heads >= (int64_t(1) << 31)) return set_error(SPARDA_ERR_SHAPE, "decode_paged: grid too large");
+    const dim3 grid(static_cast<unsigned>(p.items * p.heads));
+    const int nh = static_cast<int>(R < 16 ? R : 16);
+    const size_t lds = (static_cast<size_t>(kPgWaves) * nh * D + kPgWaves * 33) * sizeof(float);
+#define SPARDA_PGD(DT_, D_)                                                                                       \
+    do {                                                                                                          \
+        hipLaunchKernelGGL((decode_paged_kernel<DT_, D_, kPgWaves>), grid, dim3(kPgWaves * kWave), lds, stream, a); \
+        if (p.items > B)                                                                                          \
+            hipLaunchKernelGGL((decode_paged_join_kernel<DT_, D_>), dim3(static_cast<unsigned>(Hq), static_cast<unsigned>(B)), \
+                               dim3(256), 0, stream, a);                                                          \
+    } while (0)
+#define SPARDA_PGD_D(DT_)                     \
+    switch (D) {                              \
+        case 16: SPARDA_PGD(DT_, 16); break;  \
+        case 32: SPARDA_PGD(DT_, 32); break;  \
+        case 64: SPARDA_PGD(DT_, 64); break;  \
+        default: SPARDA_PGD(DT_, 128); break; \
+    }
+    if (dtype == SPARDA_F32) SPARDA_PGD_D(SPARDA_F32)
+    else SPARDA_PGD_D(SPARDA_BF16)
+#undef SPARDA_PGD_D
+#undef SPARDA_PGD
+    return check_hip(hipGetLastError(), "decode_paged_kernel");
+}
+
+}  // namespace sparda

@@ -32,6 +32,8 @@
 // K A operands are read straight from memory; V is staged per wavefront in
 // LDS, half a block at a time (XOR-swizzled 16-byte chunks), and read
 // transposed with ds_read_b64_tr_b16.
+#include <atomic>
+
 #include "common.h"
 #include "kernels.h"
 #include "mfma.h"
@@ -884,6 +886,20 @@ __global__ void read_status_kernel(uint32_t* __restrict__ out, int clear) {
     if (threadIdx.x == 0) {
         *out = clear ? atomicExch(&g_sparda_status, 0u) : atomicOr(&g_sparda_status, 0u);
     }
+}
+
+int status_word(uint32_t** word) {
+    // the address per device, asked for once
+    constexpr int kDevices = 64;
+    static std::atomic<uint32_t*> known[kDevices];
+    int dev = 0;
+    SPARDA_HIP(hipGetDevice(&dev));
+    if (dev >= 0 && dev < kDevices && (*word = known[dev].load(std::memory_order_relaxed)) != nullptr) return 0;
+    void* p = nullptr;
+    SPARDA_HIP(hipGetSymbolAddress(&p, HIP_SYMBOL(g_sparda_status)));
+    *word = static_cast<uint32_t*>(p);
+    if (dev >= 0 && dev < kDevices) known[dev].store(*word, std::memory_order_relaxed);
+    return 0;
 }
 
 int launch_read_status(uint32_t* out, int clear, hipStream_t stream) {

@@ -127,6 +127,13 @@ SIGNATURES = {
     "sparda_offload_append": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p]),
     "sparda_offload_rebuild_sums": (_int, [_p, _i64, _i64, _p, _p]),
     "sparda_offload_fetch": (_int, [_p, _p, _p, _i64, _i64, _i64, _int, _p, _p, _p]),
+    "sparda_prefill_packed": (_int, [_p, _i64, _i64, _p, _p, _i64, _i64, _int, _p, _i64, _i64, _i64, _i64, _i64, _int,
+                                     _f32, _p, _i64, _p]),
+    "sparda_append_paged": (_int, [_p, _p, _int, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _p,
+                                   _i64, _i64, _i64, _i64, _i64, _p]),
+    "sparda_decode_paged_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _int]),
+    "sparda_decode_paged": (_int, [_p, _i64, _i64, _p, _p, _int, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p,
+                                   _i64, _i64, _i64, _i64, _f32, _p, _i64, _p, _size, _p]),
 }
 
 _lock = threading.Lock()

@@ -479,6 +479,8 @@ class DecodeWorkspace:
 
 
 STATUS_PREFILL_WAIT_TIMEOUT = 1
+STATUS_SEQUENCE_RANGE = 2
+STATUS_PAGE_RANGE = 4
 
 
 def status(device=None, clear: bool = True) -> int:
@@ -1134,6 +1136,171 @@ def _prefetch_args(spec: dict, B: int, Hkv: int, D: int, block_size: int, dev):
                            float(scale), sel.data_ptr(), n_sel.data_ptr(), cap, k_dst.data_ptr(), v_dst.data_ptr(),
                            stage, parts, part)
     return pf, (f, sums, sel, n_sel, k_dst, v_dst)
+
+
+# ---------------------------------------------------------------------------
+# batches of sequences of different lengths: packed prompts, a cache in pages
+# ---------------------------------------------------------------------------
+
+def _int32_array(t: torch.Tensor, dim: int, what: str) -> torch.Tensor:
+    if t.dtype != torch.int32:
+        raise TypeError(f"sparda: {what} must be an int32 tensor, got {t.dtype}")
+    if t.dim() != dim or (t.numel() > 0 and t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"sparda: {what} must have {dim} dimension(s), the last one contiguous")
+    return t
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """Rows of 16-byte pieces: innermost stride 1, the others and the address multiples of 16 bytes."""
+    n = 16 // t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % n == 0 for s in t.stride()[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _check_out(out: torch.Tensor, shape, dtype) -> torch.Tensor:
+    if out.dtype != dtype or tuple(out.shape) != tuple(shape) or out.stride(-1) != 1:
+        raise ValueError(f"sparda: out must be {dtype} of shape {tuple(shape)} with contiguous rows")
+    return out
+
+
+def prefill_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                   causal: bool = True, scale: Optional[float] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention over packed prompts of different lengths.
+
+    q [N,Hq,D], k/v [N,Hkv,D] (same dtype): sequence i is the rows
+    [cu_seqlens[i], cu_seqlens[i+1]) (int32 on the device, read when the kernel
+    runs) and attends to itself alone, causally unless causal=False; query head
+    h reads KV head h // (Hq // Hkv). Sequences may be empty; rows of `out`
+    outside every sequence keep what they hold (with out=None: anything).
+    Returns out [N,Hq*D]. Offsets that fall or leave [0, N]: that sequence's
+    rows are not written and status() has STATUS_SEQUENCE_RANGE.
+    """
+    dev = require_device(q, k, v, cu_seqlens, out)
+    _inference_only(q, k, v)
+    if not (q.dtype == k.dtype == v.dtype):
+        raise TypeError("sparda: q, k, v must share a dtype")
+    code = _dtype_code(q)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError(f"sparda: prefill_packed takes q [N,Hq,D] and k, v [N,Hkv,D], got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    cu = _int32_array(cu_seqlens, 1, "cu_seqlens")
+    if cu.numel() < 1:
+        raise ValueError("sparda: cu_seqlens holds one offset more than there are sequences")
+    q, k, v = _rowmajor(q), _rowmajor(k), _rowmajor(v)
+    if k.stride() != v.stride():
+        k, v = k.contiguous(), v.contiguous()
+    N, Hq, D = q.shape
+    if scale is None:
+        scale = default_scale(D)
+    if out is None:
+        out = torch.empty((N, Hq * D), dtype=q.dtype, device=dev)
+    else:
+        _check_out(out, (N, Hq * D), q.dtype)
+    if N == 0 or cu.numel() == 1:
+        return out
+    with torch.cuda.device(dev):
+        call("sparda_prefill_packed", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(), k.stride(0),
+             k.stride(1), code, cu.data_ptr(), cu.numel() - 1, N, Hq, k.shape[1], D, int(causal), float(scale),
+             out.data_ptr(), out.stride(0), _stream(dev))
+    return out
+
+
+def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor) -> None:
+    if k_pages.dtype != v_pages.dtype:
+        raise TypeError("sparda: k_pages and v_pages must share a dtype")
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+        raise ValueError("sparda: k_pages and v_pages must be [pages,page_size,Hkv,D] with the same strides")
+    if k_pages.stride(-1) != 1:
+        raise ValueError("sparda: the last dimension of the pages must be contiguous")
+    _int32_array(page_table, 2, "page_table")
+
+
+def append_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, positions: torch.Tensor,
+                 k_new: torch.Tensor, v_new: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None) -> None:
+    """Writes new keys and values into the pages of a cache, in place.
+
+    k_pages/v_pages [pages,page_size,Hkv,D], page_table int32 [B,width]:
+    position p of sequence b is row p % page_size of page page_table[b, p //
+    page_size]. k_new/v_new [B,Hkv,D]: one row per sequence, written at
+    positions[b] (int32 [B] on the device); with cu_seqlens (int32 [B+1])
+    k_new/v_new [N,Hkv,D] are packed, and row j of sequence b goes to
+    positions[b] + j. A sequence with a negative position takes no part; a row
+    whose page is missing or outside the cache is dropped and status() has
+    STATUS_PAGE_RANGE.
+    """
+    dev = require_device(k_pages, v_pages, page_table, positions, k_new, v_new, cu_seqlens)
+    _inference_only(k_pages, v_pages, k_new, v_new)
+    _check_pages(k_pages, v_pages, page_table)
+    code = _dtype_code(k_pages)
+    if k_new.dtype != k_pages.dtype or v_new.dtype != k_pages.dtype:
+        raise TypeError("sparda: the new rows and the pages must share a dtype")
+    P, ps, Hkv, D = k_pages.shape
+    B, width = page_table.shape
+    if k_new.dim() != 3 or k_new.shape != v_new.shape or tuple(k_new.shape[1:]) != (Hkv, D):
+        raise ValueError(f"sparda: the new rows must be [N,{Hkv},{D}], got {tuple(k_new.shape)}, {tuple(v_new.shape)}")
+    if _int32_array(positions, 1, "positions").numel() != B:
+        raise ValueError(f"sparda: {positions.numel()} positions for {B} sequences")
+    N = k_new.shape[0]
+    if cu_seqlens is None:
+        if N != B:
+            raise ValueError(f"sparda: {N} new rows for {B} sequences: give cu_seqlens, or one row for each")
+    elif _int32_array(cu_seqlens, 1, "cu_seqlens").numel() != B + 1:
+        raise ValueError(f"sparda: cu_seqlens must hold {B + 1} offsets")
+    if N == 0 or B == 0:
+        return
+    k_new, v_new = _rows16(k_new), _rows16(v_new)
+    if k_new.stride() != v_new.stride():
+        k_new, v_new = k_new.contiguous(), v_new.contiguous()
+    with torch.cuda.device(dev):
+        call("sparda_append_paged", k_pages.data_ptr(), v_pages.data_ptr(), code, P, ps, *k_pages.stride()[:3],
+             page_table.data_ptr(), page_table.stride(0), width, positions.data_ptr(),
+             cu_seqlens.data_ptr() if cu_seqlens is not None else None, B, k_new.data_ptr(), v_new.data_ptr(), N,
+             k_new.stride(0), k_new.stride(1), Hkv, D, _stream(dev))
+
+
+def decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                 lengths: torch.Tensor, scale: Optional[float] = None,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one token per sequence over a cache in pages.
+
+    q [B,Hq,D]; k_pages/v_pages [pages,page_size,Hkv,D] and page_table int32
+    [B,width] as in ``append_paged``; lengths int32 [B] on the device: sequence
+    b attends to its positions [0, lengths[b]). Returns out [B,Hq*D]: zeros for
+    a length of 0, NaN (and STATUS_PAGE_RANGE in status()) where a page index or
+    the length is out of range.
+    """
+    dev = require_device(q, k_pages, v_pages, page_table, lengths, out)
+    _inference_only(q, k_pages, v_pages)
+    _check_pages(k_pages, v_pages, page_table)
+    code = _dtype_code(q)
+    if q.dtype != k_pages.dtype:
+        raise TypeError("sparda: q and the pages must share a dtype")
+    P, ps, Hkv, D = k_pages.shape
+    B, width = page_table.shape
+    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != D:
+        raise ValueError(f"sparda: decode_paged takes q [{B},Hq,{D}] for this cache, got {tuple(q.shape)}")
+    if _int32_array(lengths, 1, "lengths").numel() != B:
+        raise ValueError(f"sparda: {lengths.numel()} lengths for {B} sequences")
+    Hq = q.shape[1]
+    q = _rows16(q)
+    if scale is None:
+        scale = default_scale(D)
+    if out is None:
+        out = torch.empty((B, Hq * D), dtype=q.dtype, device=dev)
+    else:
+        _check_out(out, (B, Hq * D), q.dtype)
+    if B == 0:
+        return out
+    nbytes = _lib.load().sparda_decode_paged_workspace_bytes(B, width, ps, Hq, Hkv, D, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with torch.cuda.device(dev):
+        call("sparda_decode_paged", q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(),
+             code, P, ps, *k_pages.stride()[:3], page_table.data_ptr(), page_table.stride(0), width,
+             lengths.data_ptr(), B, Hq, Hkv, D, float(scale), out.data_ptr(), out.stride(0),
+             ws.data_ptr() if ws is not None else None, nbytes, _stream(dev))
+    return out
 
 
 def block_sums(k: torch.Tensor, pos: int, n: int, block_size: int, sums: torch.Tensor) -> torch.Tensor:
