@@ -135,19 +135,18 @@ struct PackedPrefill {
 // against them.
 template <int D, int NT, int CW, int KG, int KB>
 __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(PackedPrefill a) {
-    constexpr int kCols = 32 * NT, kBM = CW * kCols, kThreads = CW * kWave;
-    constexpr int kPieces = D / 8, kSR = KB * kPieces / kThreads, kRowStep = kThreads / kPieces;
+    constexpr int kCols = 32 * NT, kBM = CW * kCols;
+    constexpr int kPieces = D / 8, kRun = kWave / kPieces, kRuns = KB / (CW * kRun);
+    static_assert(kRuns * CW * kRun == KB, "whole runs");
     constexpr int kKS = D / 16, kDT = D / 32, kHalves = KB / 32;
     __shared__ union {
         PackedStage<D, KB, KG> st;
         PackedMerge<NT * kDT * 16, CW, NT, KG> mg;
-        float ref[KG][CW][NT][32];
     } sm;
     __shared__ int flag;
     const int lane = threadIdx.x % kWave;
     const int wv = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int wave = wv % CW, kg = wv / CW;
-    const int tid = wave * kWave + lane;
     const int col = lane % 32, hf = lane / 32;
     const int g = blockIdx.x % a.Hkv;
     const int64_t slot = a.slots - 1 - blockIdx.x / a.Hkv;    // a sequence's last windows, the longest walks, first
@@ -181,56 +180,54 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
         for (int kk = 0; kk < kKS; ++kk) qreg[tt][kk] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(qp + 16 * kk));
     }
 
-    const int srow = tid / kPieces, spiece = tid % kPieces, kv_st = static_cast<int>(a.kv_st);
-    typedef unsigned int StageV __attribute__((ext_vector_type(4 * kSR)));
-    auto fetch = [&](int j, StageV& nk, StageV& nv) __attribute__((always_inline)) {
+    // Staging goes from memory to LDS without registers, 16 bytes a lane, lanes in
+    // LDS order: lane i of a load holds place i % kPieces of row i / kPieces, and
+    // fetches the piece that belongs there. A wavefront loads every CW-th run of
+    // kRun rows. Rows behind the sequence repeat its last one.
+    const int srow = wave * kRun + lane / kPieces, kv_st = static_cast<int>(a.kv_st);
+    auto stage = [&](int j, int buf) __attribute__((always_inline)) {
+        typedef const __attribute__((address_space(1))) void* G;
+        typedef __attribute__((address_space(3))) void* L;
         const int row0 = j * KB, last = len - 1 - row0;
-        const uint16_t* kr = kb + static_cast<int64_t>(row0) * a.kv_st;
-        const uint16_t* vr = vb + static_cast<int64_t>(row0) * a.kv_st;
+        const char* kr = reinterpret_cast<const char*>(kb + static_cast<int64_t>(row0) * a.kv_st);
+        const char* vr = reinterpret_cast<const char*>(vb + static_cast<int64_t>(row0) * a.kv_st);
 #pragma unroll
-        for (int i = 0; i < kSR; ++i) {
-            int r = srow + i * kRowStep;
-            r = r < last ? r : last;
-            const uint32_t at = static_cast<uint32_t>(r * kv_st + 8 * spiece);
-            const uint4 x = *reinterpret_cast<const uint4*>(kr + at);
-            const uint4 y = *reinterpret_cast<const uint4*>(vr + at);
-            nk[4 * i] = x.x; nk[4 * i + 1] = x.y; nk[4 * i + 2] = x.z; nk[4 * i + 3] = x.w;
-            nv[4 * i] = y.x; nv[4 * i + 1] = y.y; nv[4 * i + 2] = y.z; nv[4 * i + 3] = y.w;
-        }
-    };
-    auto stash = [&](int j, int buf, StageV& nk, StageV& nv) __attribute__((always_inline)) {
-        const int rows = len - j * KB;
-#pragma unroll
-        for (int i = 0; i < kSR; ++i) {
-            const int r = srow + i * kRowStep, at = r * D + 8 * pk_piece<D>(r, spiece);
-            uint4 x{nk[4 * i], nk[4 * i + 1], nk[4 * i + 2], nk[4 * i + 3]};
-            uint4 y{nv[4 * i], nv[4 * i + 1], nv[4 * i + 2], nv[4 * i + 3]};
-            if (r >= rows) x = y = uint4{0, 0, 0, 0};         // behind the sequence: weightless, and finite
-            *reinterpret_cast<uint4*>(&sm.st.k[buf][kg][at]) = x;
-            *reinterpret_cast<uint4*>(&sm.st.v[buf][kg][at]) = y;
+        for (int i = 0; i < kRuns; ++i) {
+            const int r = i * CW * kRun, row = srow + r < last ? srow + r : last;
+            // (rows a multiple of 16 apart place their pieces alike)
+            const uint32_t at = 2 * static_cast<uint32_t>(row * kv_st + 8 * pk_piece<D>(srow + r, lane % kPieces));
+            __builtin_amdgcn_global_load_lds((G)(kr + at), (L)&sm.st.k[buf][kg][(r + wave * kRun) * D], 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((G)(vr + at), (L)&sm.st.v[buf][kg][(r + wave * kRun) * D], 16, 0, 0);
         }
     };
 
-    // the references: the first 32 keys straight from memory
+    // the columns' maxima over the keys [0, upto), straight from memory
     float ref[NT], l[NT];
-    {
-        bf16x8 ka[kKS];
-        const uint16_t* kr = kb + static_cast<int64_t>(col < len ? col : len - 1) * a.kv_st + 8 * hf;
+    auto take_refs = [&](int upto) __attribute__((always_inline)) {
 #pragma unroll
-        for (int kk = 0; kk < kKS; ++kk) ka[kk] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(kr + 16 * kk));
+        for (int tt = 0; tt < NT; ++tt) ref[tt] = -__builtin_inff();
+        for (int key0 = 0; key0 < upto; key0 += 32) {
+            bf16x8 ka[kKS];
+            const uint16_t* kr = kb + static_cast<int64_t>(key0 + col < len ? key0 + col : len - 1) * a.kv_st + 8 * hf;
+#pragma unroll
+            for (int kk = 0; kk < kKS; ++kk) ka[kk] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(kr + 16 * kk));
+#pragma unroll
+            for (int tt = 0; tt < NT; ++tt) {
+                f32x16 s{};
+#pragma unroll
+                for (int kk = 0; kk < kKS; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[kk], qreg[tt][kk], s, 0, 0, 0);
+                const int mine = lim[tt] - key0 - 4 * hf;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    ref[tt] = fmaxf(ref[tt], 8 * (i / 4) + i % 4 <= mine ? s[i] * a.scale_log2 : -__builtin_inff());
+            }
+        }
 #pragma unroll
         for (int tt = 0; tt < NT; ++tt) {
-            f32x16 s{};
-#pragma unroll
-            for (int kk = 0; kk < kKS; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[kk], qreg[tt][kk], s, 0, 0, 0);
-            float m = -__builtin_inff();
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (8 * (i / 4) + 4 * hf + i % 4 <= lim[tt]) m = fmaxf(m, s[i] * a.scale_log2);
-            const float2 r2 = rows32_swap(m);
+            const float2 r2 = rows32_swap(ref[tt]);
             ref[tt] = fmaxf(r2.x, r2.y);
         }
-    }
+    };
 
     f32x16 o[NT][kDT];
     auto clear = [&]() __attribute__((always_inline)) {
@@ -241,7 +238,6 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
             for (int dt = 0; dt < kDT; ++dt) o[tt][dt] = f32x16{};
         }
     };
-    clear();
 
     // operand reads of 32 keys: K rows at this lane's key, V transposed (a 16-lane
     // group reads 4 rows x 16 dims, lane j of it row j / 4, dims 4 (j % 4) .. +3);
@@ -258,12 +254,21 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
     bool odd = false;  // infinities or NaN in V at a place that some column may not attend
 
     // 32 keys from key0 on, staged at row 32 half of the buffer
-    auto compute = [&](int buf, int half, int key0, bool maxima) __attribute__((always_inline)) {
+    auto compute = [&](int buf, int half, int key0) __attribute__((always_inline)) {
         bf16x8 ka[kKS], va[kDT][2];
         const uint16_t* ks = &sm.st.k[buf][kg][32 * half * D];
         const uint16_t* vs = &sm.st.v[buf][kg][32 * half * D];
 #pragma unroll
         for (int kk = 0; kk < kKS; ++kk) ka[kk] = lds_read8(ks + k_at[kk]);
+        f32x16 s[NT];
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt) {
+            s[tt] = f32x16{};
+#pragma unroll
+            for (int kk = 0; kk < kKS; ++kk)
+                s[tt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[kk], qreg[tt][kk], s[tt], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // V's operands take K's registers
         // V^T operand: dim 32 dt + col, keys 16 c + 4 hf .. +3 and 8 further
 #pragma unroll
         for (int dt = 0; dt < kDT; ++dt)
@@ -274,19 +279,21 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
                 va[dt][c] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
             }
         const bool edge = a.causal ? key0 + 31 > w_first : key0 + 32 > len;
-        if (edge && a.causal) {
+        if (edge) {
             // a weight of 0 times inf is NaN: such values are cleared here, and added
             // after the walk to the columns that do attend them
-            auto bad2 = [](uint32_t x) { return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u; };
-            bool any = false;
+            // (an exponent of all ones carries into the sign's place)
+            uint32_t any = 0;
 #pragma unroll
             for (int dt = 0; dt < kDT; ++dt)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const uint4 x = __builtin_bit_cast(uint4, va[dt][c]);
-                    any = any || bad2(x.x) || bad2(x.y) || bad2(x.z) || bad2(x.w);
+                    any |= ((x.x & 0x7f807f80u) + 0x00800080u) | ((x.y & 0x7f807f80u) + 0x00800080u) |
+                           ((x.z & 0x7f807f80u) + 0x00800080u) | ((x.w & 0x7f807f80u) + 0x00800080u);
                 }
-            if (__ballot(any) != 0) {
+            any &= 0x80008000u;
+            if (__ballot(any != 0) != 0) {
                 odd = true;
                 typedef short s16x8 __attribute__((ext_vector_type(8)));
 #pragma unroll
@@ -302,17 +309,6 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
         }
 #pragma unroll
         for (int tt = 0; tt < NT; ++tt) {
-            f32x16 s{};
-#pragma unroll
-            for (int kk = 0; kk < kKS; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[kk], qreg[tt][kk], s, 0, 0, 0);
-            if (maxima) {
-                float m = ref[tt];
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (key0 + 8 * (i / 4) + 4 * hf + i % 4 <= lim[tt]) m = fmaxf(m, s[i] * a.scale_log2);
-                ref[tt] = m;
-                continue;
-            }
             const float neg = ref[tt] == -__builtin_inff() ? 0.0f : -ref[tt];
             bf16x8 pb[2];
             float sum = 0.0f;
@@ -320,7 +316,7 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
                 const int mine = lim[tt] - key0 - 4 * hf;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale_log2, neg));
+                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, neg));
                     p = 8 * (i / 4) + i % 4 <= mine ? p : 0.0f;
                     sum += p;
                     pb[i / 8][i % 8] = static_cast<__bf16>(p);
@@ -328,7 +324,7 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
             } else {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale_log2, neg));
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, neg));
                     sum += p;
                     pb[i / 8][i % 8] = static_cast<__bf16>(p);
                 }
@@ -342,59 +338,129 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
         }
     };
 
-    // step i: group kg computes block i KG + kg from buffer i & 1 while its next is loaded
-    const int steps = (nblk + KG - 1) / KG;
-    for (int mode = 0;; ++mode) {                             // 0: against ref; 1: the exact maxima; 2: against those
-        if (threadIdx.x == 0) flag = 0;
-        StageV nk{}, nv{};
-        if (kg < nblk) {
-            fetch(kg, nk, nv);
-            stash(kg, 0, nk, nv);
+    // A block all of whose keys every column attends, in units of 32 keys x 32
+    // columns: while a unit's exponentials are taken, the next one's scores and the
+    // last one's output products are on the matrix cores (sched_group_barrier lays
+    // the products between the vector instructions).
+    auto compute_block = [&](int buf, int next) __attribute__((always_inline)) {
+        constexpr int kU = kHalves * NT;
+        static_assert(kHalves <= 2, "");
+        constexpr int kMfma = kKS + 2 * kDT;                  // products of a unit
+        const uint16_t* ks = &sm.st.k[buf][kg][0];
+        const uint16_t* vs = &sm.st.v[buf][kg][0];
+        bf16x8 ka[kKS], va[2][kDT][2], pb[2][2];                // (two sets of V: NT = 1)
+        f32x16 s[2];
+        float neg[NT];
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt) neg[tt] = ref[tt] == -__builtin_inff() ? 0.0f : -ref[tt];
+        auto read_k = [&](int half) __attribute__((always_inline)) {
+#pragma unroll
+            for (int kk = 0; kk < kKS; ++kk) ka[kk] = lds_read8(ks + k_at[kk] + 32 * half * D);
+        };
+        auto read_v = [&](int half, bf16x8 (&x)[kDT][2]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int dt = 0; dt < kDT; ++dt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const i16x4 lo = lds_read_tr(vs + v_at[dt][0] + (32 * half + 16 * c) * D);
+                    const i16x4 hi = lds_read_tr(vs + v_at[dt][1] + (32 * half + 16 * c) * D);
+                    x[dt][c] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+        };
+        auto qk = [&](int u) __attribute__((always_inline)) {
+            f32x16 x{};
+#pragma unroll
+            for (int kk = 0; kk < kKS; ++kk) x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[kk], qreg[u % NT][kk], x, 0, 0, 0);
+            s[u & 1] = x;
+        };
+        auto pv = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int dt = 0; dt < kDT; ++dt)
+                    o[u % NT][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[NT == 1 ? u & 1 : 0][dt][c], pb[u & 1][c], o[u % NT][dt], 0, 0, 0);
+        };
+        read_k(0);
+        qk(0);
+        read_v(0, va[0]);
+        if (NT == 1 && kU > 1) read_k(1);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (u == kU - 1) {
+                // the last reads of LDS, then the next block's loads: a read behind them would wait for them
+                if (NT == 1 && kU > 1) {
+                    read_v(u, va[1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                stage(next, buf ^ 1);
+            }
+            if (u + 1 < kU) qk(u + 1);
+            if (u + 2 < kU && (u + 2) % NT == 0) read_k((u + 2) / NT);  // (its last unit's scores are under way)
+            if (u > 0) {
+                pv(u - 1);
+                if (NT > 1 && u % NT == 0) read_v(u / NT, va[0]);
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u & 1][i], a.scale_log2, neg[u % NT]));
+                pb[u & 1][i / 8][i % 8] = static_cast<__bf16>(p);
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+                const bf16x2 one{static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
+#pragma unroll
+                for (int e = 0; e < 8; e += 2)
+                    sum = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{pb[u & 1][c][e], pb[u & 1][c][e + 1]}, one, sum, false);
+            }
+            l[u % NT] += sum;
+#pragma unroll
+            for (int i = 0; i < kMfma; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 48 / kMfma, 0);
+            }
         }
-        if (kg + KG < nblk) fetch(kg + KG, nk, nv);
+        __builtin_amdgcn_sched_barrier(0);
+        pv(kU - 1);
+    };
+
+    // step i: group kg computes block i KG + kg from buffer i & 1 while its next is loaded
+    // (first the steps whose blocks every column of the workgroup attends)
+    const int steps = (nblk + KG - 1) / KG, whole = (a.causal ? col0 / a.R + 1 : len) / KB / KG;
+    for (int pass = 0;; ++pass) {
+        if (threadIdx.x == 0) flag = 0;
+        if (kg < nblk) stage(kg, 0);
+        take_refs(pass == 0 && w_end > 32 ? 32 : w_end);
+        clear();
         __syncthreads();
-        for (int i = 0; i < steps; ++i) {
-            const int buf = i & 1, j = i * KG + kg;
+        int i = 0;
+        for (; i < whole; ++i) {
+            const int j = i * KG + kg;
+            compute_block(i & 1, j + KG < nblk ? j + KG : j);  // (no next one: a block that nobody reads)
+            __syncthreads();
+        }
+        for (; i < steps; ++i) {
+            const int buf = i & 1, j = i * KG + kg, key0 = j * KB;
+            if (j + KG < nblk) stage(j + KG, buf ^ 1);
 #pragma unroll 1
             for (int hh = 0; hh < kHalves; ++hh)
-                if (j < nblk && j * KB + 32 * hh < w_end) compute(buf, hh, j * KB + 32 * hh, mode == 1);
-            if (j + KG < nblk) {
-                stash(j + KG, buf ^ 1, nk, nv);
-                if (j + 2 * KG < nblk) fetch(j + 2 * KG, nk, nv);
-            }
+                if (key0 + 32 * hh < w_end) compute(buf, hh, key0 + 32 * hh);
             __syncthreads();
         }
-        if (mode == 2) break;
-        if (mode == 0) {
-            bool over = false;
+        if (pass == 1) break;
+        bool over = false;
 #pragma unroll
-            for (int tt = 0; tt < NT; ++tt) over = over || (live && (!(l[tt] <= kPkGuard) || ref[tt] == -__builtin_inff()));
-            if (__ballot(over) != 0 && lane == 0) atomicOr(&flag, 1);
-            __syncthreads();
-            if (flag == 0) break;                             // workgroup-uniform
-            __syncthreads();                                  // (read by all before it is cleared)
-#pragma unroll
-            for (int tt = 0; tt < NT; ++tt) ref[tt] = -__builtin_inff();
-        } else {
-#pragma unroll
-            for (int tt = 0; tt < NT; ++tt) {
-                const float2 r2 = rows32_swap(ref[tt]);
-                ref[tt] = fmaxf(r2.x, r2.y);
-                if (KG > 1 && hf == 0) sm.ref[kg][wave][tt][col] = ref[tt];
-            }
-            if constexpr (KG > 1) {
-                __syncthreads();
-#pragma unroll
-                for (int tt = 0; tt < NT; ++tt)
-                    for (int x = 0; x < KG; ++x) ref[tt] = fmaxf(ref[tt], sm.ref[x][wave][tt][col]);
-                __syncthreads();
-            }
-            clear();
-        }
+        for (int tt = 0; tt < NT; ++tt) over = over || (live && (!(l[tt] <= kPkGuard) || ref[tt] == -__builtin_inff()));
+        if (__ballot(over) != 0 && lane == 0) atomicOr(&flag, 1);
+        __syncthreads();
+        if (flag == 0) break;                                 // workgroup-uniform
+        __syncthreads();                                      // (read by all before it is cleared)
     }
     if (__ballot(odd) != 0) {                                 // wave-uniform
         // the values cleared above: a positive weight times inf or NaN is that value
-        for (int key = w_first / 32 * 32; key < w_end; ++key) {
+        for (int key = (a.causal ? w_first : len) / 32 * 32; key < w_end; ++key) {
             if (key / KB % KG != kg) continue;
             const uint16_t* vr = vb + static_cast<int64_t>(key) * a.kv_st + 4 * hf;
 #pragma unroll
@@ -492,11 +558,15 @@ int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void*
             if (force == 1) SPARDA_PKM(64, 2, 1, 4, 32);
             else if (force == 2) SPARDA_PKM(64, 1, 1, 4, 32);
             else if (force == 3) SPARDA_PKM(64, 1, 4, 1, 64);
-            else if (force == 4) SPARDA_PKM(64, 2, 2, 2, 64);
+            else if (force == 4) SPARDA_PKM(64, 2, 4, 2, 64);
+            else if (force == 5) SPARDA_PKM(64, 1, 4, 2, 64);
+            else if (force == 6) SPARDA_PKM(64, 2, 4, 1, 32);
             else SPARDA_PKM(64, 2, 4, 1, 64);
         } else {
             if (force == 1 || force == 2) SPARDA_PKM(128, 1, 1, 4, 32);
-            else if (force == 4) SPARDA_PKM(128, 1, 2, 2, 32);
+            else if (force == 4) SPARDA_PKM(128, 1, 4, 2, 64);
+            else if (force == 5) SPARDA_PKM(128, 1, 4, 2, 32);
+            else if (force == 6) SPARDA_PKM(128, 1, 4, 1, 32);
             else SPARDA_PKM(128, 1, 4, 1, 64);
         }
 #undef SPARDA_PKM
