@@ -15,6 +15,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -43,6 +44,10 @@ struct Entries {
     decltype(&sparda_rows_residual) rows_residual;
     decltype(&sparda_norm_gemv) norm_gemv;
     decltype(&sparda_teacher_mass) teacher_mass;
+    decltype(&sparda_prefill_packed) prefill_packed;
+    decltype(&sparda_append_paged) append_paged;
+    decltype(&sparda_decode_paged) decode_paged;
+    decltype(&sparda_decode_paged_workspace_bytes) decode_paged_workspace_bytes;
 } g;
 
 // the call is not of the common form: the Python operator takes it
@@ -116,6 +121,13 @@ struct Args {
         need(t.scalar_type() == at::kLong && t.numel() == 1);
         return static_cast<const int64_t*>(t.data_ptr());
     }
+    const int32_t* ints(PyObject* o, int64_t n) {
+        const at::Tensor& t = tensor(o, 1);
+        need(t.scalar_type() == at::kInt && t.numel() == n && (n == 1 || t.stride(0) == 1));
+        return static_cast<const int32_t*>(t.data_ptr());
+    }
+    // the launch goes to the current device
+    void on_current() const { need(c10::impl::VirtualGuardImpl(at::kCUDA).getDevice().index() == device); }
     at::Tensor empty(at::IntArrayRef sizes, at::ScalarType dt) const {
         return at::empty(sizes, at::TensorOptions().dtype(dt).device(at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device))));
     }
@@ -482,6 +494,81 @@ PyObject* teacher_mass(PyObject* const* a) {
                   out);
 }
 
+// prefill_packed(q, k, v, cu_seqlens, causal, scale)
+PyObject* prefill_packed(PyObject* const* a) {
+    Args x;
+    const at::Tensor& q = x.operand(a[0], 3);
+    const at::Tensor& k = x.operand(a[1], 3);
+    const at::Tensor& v = x.operand(a[2], 3);
+    const at::Tensor& cu = x.tensor(a[3], 1);
+    const int causal = as_bool(a[4]);
+    const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2);
+    need(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type() && same_strides(k, v));
+    need(k.sizes() == v.sizes() && k.size(0) == N && k.size(2) == D && N > 0);
+    need(cu.scalar_type() == at::kInt && cu.numel() > 1 && cu.stride(0) == 1);
+    const float scale = scale_or(a[5], D);
+    x.on_current();
+    const at::Tensor out = x.empty({N, Hq * D}, q.scalar_type());
+    return result(run(g.prefill_packed, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(), k.stride(0),
+                      k.stride(1), code(q), static_cast<const int32_t*>(cu.data_ptr()), cu.numel() - 1, N, Hq, k.size(1),
+                      D, causal, scale, out.data_ptr(), out.stride(0), x.stream()),
+                  out);
+}
+
+struct PagesArg {
+    const at::Tensor &k, &v, &table;
+    int64_t P, ps, Hkv, D, B, width;
+    PagesArg(Args& x, PyObject* const* a)
+        : k(x.operand(a[0], 4)), v(x.operand(a[1], 4)), table(x.tensor(a[2], 2)), P(k.size(0)), ps(k.size(1)),
+          Hkv(k.size(2)), D(k.size(3)), B(table.size(0)), width(table.size(1)) {
+        need(k.scalar_type() == v.scalar_type() && k.sizes() == v.sizes() && same_strides(k, v));
+        need(table.scalar_type() == at::kInt && B > 0 && (width == 1 || table.stride(1) == 1));
+    }
+};
+// rows of 16-byte pieces
+inline bool rows16(const at::Tensor& t) { return aligned(t, 16) && strides_of(t, 16 / t.element_size()); }
+
+// append_paged(k_pages, v_pages, page_table, positions, k_new, v_new, cu_seqlens): an int (its status), or None
+PyObject* append_paged(PyObject* const* a) {
+    Args x;
+    const PagesArg p(x, a);
+    const int32_t* pos = x.ints(a[3], p.B);
+    const at::Tensor& kn = x.operand(a[4], 3);
+    const at::Tensor& vn = x.operand(a[5], 3);
+    need(kn.scalar_type() == p.k.scalar_type() && vn.scalar_type() == p.k.scalar_type() && kn.sizes() == vn.sizes());
+    const int64_t N = kn.size(0);
+    need(N > 0 && kn.size(1) == p.Hkv && kn.size(2) == p.D && same_strides(kn, vn) && rows16(kn) && rows16(vn));
+    const int32_t* cu = a[6] != Py_None ? x.ints(a[6], p.B + 1) : nullptr;
+    need(cu != nullptr || N == p.B);
+    x.on_current();
+    return PyLong_FromLong(run(g.append_paged, p.k.data_ptr(), p.v.data_ptr(), code(p.k), p.P, p.ps, p.k.stride(0),
+                               p.k.stride(1), p.k.stride(2), static_cast<const int32_t*>(p.table.data_ptr()),
+                               p.table.stride(0), p.width, pos, cu, p.B, kn.data_ptr(), vn.data_ptr(), N, kn.stride(0),
+                               kn.stride(1), p.Hkv, p.D, x.stream()));
+}
+
+// decode_paged(q, k_pages, v_pages, page_table, lengths, scale)
+PyObject* decode_paged(PyObject* const* a) {
+    Args x;
+    const at::Tensor& q = x.operand(a[0], 3);
+    const PagesArg p(x, a + 1);
+    const int32_t* len = x.ints(a[4], p.B);
+    const int64_t Hq = q.size(1);
+    need(q.scalar_type() == p.k.scalar_type() && q.size(0) == p.B && q.size(2) == p.D && rows16(q));
+    const float scale = scale_or(a[5], p.D);
+    x.on_current();
+    const size_t bytes = g.decode_paged_workspace_bytes(p.B, p.width, p.ps, Hq, p.Hkv, p.D, code(q));
+    at::Tensor part;  // the shares' partials, held until the launch is enqueued
+    if (bytes > 0) part = x.empty({static_cast<int64_t>(bytes)}, at::kByte);
+    const at::Tensor out = x.empty({p.B, Hq * p.D}, q.scalar_type());
+    return result(run(g.decode_paged, q.data_ptr(), q.stride(0), q.stride(1), p.k.data_ptr(), p.v.data_ptr(), code(q),
+                      p.P, p.ps, p.k.stride(0), p.k.stride(1), p.k.stride(2),
+                      static_cast<const int32_t*>(p.table.data_ptr()), p.table.stride(0), p.width, len, p.B, Hq, p.Hkv,
+                      p.D, scale, out.data_ptr(), out.stride(0), bytes > 0 ? part.data_ptr() : nullptr, bytes,
+                      x.stream()),
+                  out);
+}
+
 // bind(raw_stream, addresses): the current-stream query and the entry points' addresses, in Entries' order
 PyObject* bind(PyObject*, PyObject* args) {
     PyObject *raw, *list;
@@ -521,6 +608,9 @@ PyMethodDef kMethods[] = {
     SPARDA_FAST(rows_residual, 3),
     SPARDA_FAST(norm_gemv, 3),
     SPARDA_FAST(teacher_mass, 5),
+    SPARDA_FAST(prefill_packed, 6),
+    SPARDA_FAST(append_paged, 7),
+    SPARDA_FAST(decode_paged, 6),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

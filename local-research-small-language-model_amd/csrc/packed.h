@@ -36,17 +36,18 @@ __device__ __forceinline__ int64_t packed_first(int c, int i, int64_t N, int R, 
 __device__ __forceinline__ PackedWindow packed_window(const int32_t* __restrict__ cu, int n, int64_t N, int R, int BM,
                                                       int64_t slot, bool& bad) {
     const int lane = threadIdx.x % kWave;
-    int seq = 0;
+    int seq = 0, c0 = 0, c1 = 0;
     for (int i0 = 0; i0 < n; i0 += kWave) {
-        const int i = i0 + lane;
-        const bool before = i < n && packed_first(cu[i < n ? i : n - 1], i, N, R, BM) <= slot;
-        const uint64_t m = __ballot(before);
-        if (m == 0) break;                      // (offsets that rise: no later sequence either)
-        seq = i0 + 63 - __builtin_clzll(m);
+        const int i = i0 + lane < n ? i0 + lane : n - 1;
+        const int a0 = cu[i], a1 = cu[i + 1];   // (both at once: no second load behind the search)
+        const uint64_t m = __ballot(i0 + lane < n && packed_first(a0, i, N, R, BM) <= slot);
+        if (m == 0 && i0 > 0) break;            // (offsets that rise: no later sequence either)
+        const int at = m == 0 ? 0 : 63 - __builtin_clzll(m);
+        seq = i0 + at;
+        c0 = __builtin_amdgcn_readlane(a0, at);
+        c1 = __builtin_amdgcn_readlane(a1, at);
         if (m != ~0ull) break;
     }
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    const int c0 = __builtin_amdgcn_readfirstlane(cu[seq]), c1 = __builtin_amdgcn_readfirstlane(cu[seq + 1]);
     bad = c0 < 0 || c1 < c0 || c1 > N;
     PackedWindow w{-1, 0, 0, 0};
     const bool own = bad;

@@ -527,12 +527,265 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
     }
 }
 
+// ---------------------------------------------------------------------------
+// fp32, D = 64 and 128, on the matrix cores
+// ---------------------------------------------------------------------------
+
+namespace {
+
+constexpr int kPfWaves = 4;
+
+struct PackedPrefillF32 {
+    const float* q;
+    int64_t q_st, q_sh;
+    const float *k, *v;
+    int64_t kv_st, kv_sh;
+    const int32_t* cu;
+    int n;
+    int64_t N;
+    int Hkv, R, causal;
+    int64_t slots;
+    float scale_log2;
+    float* out;
+    int64_t out_st;
+    uint32_t* status;
+};
+
+template <int D>
+struct PackedStepF32 {
+    f32x4 k[D / 16];                 // key c16, dims 16 c + 4 grp .. +3
+    float v[4][D / 16];              // key 4 grp + i, dims D / 16 c16 ..
+};
+
+}  // namespace
+
+// One workgroup of 4 wavefronts per (KV head, window of 16 NT columns of one
+// sequence; columns as in the bf16 kernel). The wavefronts take the steps of 16 keys
+// in turn, each with its own running (m, l, O) of every column, and are joined in
+// order at the end. K and V go straight from memory to the operand registers, the
+// next step's under the present one's products, and the score layout is already
+// that of the P operand (v_mfma_f32_16x16x4_f32: 16 keys x 16 columns take D
+// products, 32 cycles each: the fp32 matrix rate bounds it).
+template <int D, int NT>
+__global__ void __launch_bounds__(kPfWaves* kWave, 2) prefill_packed_f32_kernel(PackedPrefillF32 a) {
+    constexpr int kV = D / 16, kBM = 16 * NT;
+    typedef PackedStepF32<D> Step;
+    __shared__ struct {
+        f32x4 o[kPfWaves - 1][NT][kV][kWave];
+        float m[kPfWaves - 1][NT][kWave], l[kPfWaves - 1][NT][kWave];
+        int odd[kPfWaves];
+    } sm;
+    const int lane = threadIdx.x % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int c16 = lane % 16, grp = lane / 16;
+    const int g = blockIdx.x % a.Hkv;
+    const int64_t slot = a.slots - 1 - blockIdx.x / a.Hkv;
+    bool bad;
+    const PackedWindow w = packed_window(a.cu, a.n, a.N, a.R, kBM, slot, bad);
+    if (bad && threadIdx.x == 0) atomicOr(a.status, static_cast<uint32_t>(SPARDA_STATUS_SEQUENCE_RANGE));
+    if (w.seq < 0) return;                                    // workgroup-uniform
+    const int len = w.len, ncol = len * a.R, col0 = static_cast<int>(w.win) * kBM;
+    const int w_first = col0 / a.R, w_last = (col0 + kBM <= ncol ? col0 + kBM - 1 : ncol - 1) / a.R;
+    const int w_end = a.causal ? w_last + 1 : len;            // keys of the window
+    const float* kb = a.k + static_cast<int64_t>(w.row0) * a.kv_st + static_cast<int64_t>(g) * a.kv_sh;
+    const float* vb = a.v + static_cast<int64_t>(w.row0) * a.kv_st + static_cast<int64_t>(g) * a.kv_sh;
+
+    int tok[NT], lim[NT];
+    f32x4 qr[NT][kV];
+#pragma unroll
+    for (int tt = 0; tt < NT; ++tt) {
+        const int c = col0 + 16 * tt + c16 < ncol ? col0 + 16 * tt + c16 : ncol - 1;
+        tok[tt] = c / a.R;
+        lim[tt] = a.causal ? tok[tt] : len - 1;
+        const float* qp = a.q + (w.row0 + static_cast<int64_t>(tok[tt])) * a.q_st +
+                          static_cast<int64_t>(g * a.R + c % a.R) * a.q_sh + 4 * grp;
+#pragma unroll
+        for (int x = 0; x < kV; ++x) qr[tt][x] = *reinterpret_cast<const f32x4*>(qp + 16 * x);
+    }
+    const int kv_st = static_cast<int>(a.kv_st);
+    auto load = [&](int u, Step& x) __attribute__((always_inline)) {
+        const int last = len - 1 - 16 * u;                    // rows past the end read the last one
+        const float* kr = kb + static_cast<int64_t>(16 * u) * a.kv_st;
+        const float* vr = vb + static_cast<int64_t>(16 * u) * a.kv_st;
+        const uint32_t ka = static_cast<uint32_t>((c16 < last ? c16 : last) * kv_st + 4 * grp);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) x.k[e] = *reinterpret_cast<const f32x4*>(kr + ka + 16 * e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t va = static_cast<uint32_t>((4 * grp + i < last ? 4 * grp + i : last) * kv_st + kV * c16);
+#pragma unroll
+            for (int j = 0; j < kV; j += 4) {
+                const f32x4 y = *reinterpret_cast<const f32x4*>(vr + va + j);
+                x.v[i][j] = y[0]; x.v[i][j + 1] = y[1]; x.v[i][j + 2] = y[2]; x.v[i][j + 3] = y[3];
+            }
+        }
+    };
+
+    float m[NT], l[NT];                                       // log2 units; this lane's part of the sum
+    f32x4 o[NT][kV];
+#pragma unroll
+    for (int tt = 0; tt < NT; ++tt) {
+        m[tt] = -__builtin_inff();
+        l[tt] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kV; ++j) o[tt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    bool odd = false;                                         // V not finite at a place that some column may not attend
+    auto compute = [&](int u, Step& x) __attribute__((always_inline)) {
+        const int key0 = 16 * u;
+        const bool edge = a.causal ? key0 + 15 > w_first : key0 + 16 > len;
+        f32x4 s[NT];
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt) s[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < kV; ++e)
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+                for (int tt = 0; tt < NT; ++tt)
+                    s[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[e][y], qr[tt][e][y], s[tt], 0, 0, 0);
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt) s[tt] *= a.scale_log2;
+        if (edge) {
+            // (a weight of 0 times inf is NaN: such values are cleared here, and added at the end to the columns
+            // that do attend them)
+            float vm = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < kV; ++j) vm = __builtin_elementwise_maximum(vm, __builtin_fabsf(x.v[i][j]));
+            if (__ballot(!(vm < __builtin_inff())) != 0) {
+                odd = true;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < kV; ++j) x.v[i][j] = __builtin_fabsf(x.v[i][j]) < __builtin_inff() ? x.v[i][j] : 0.0f;
+            }
+#pragma unroll
+            for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (key0 + 4 * grp + i > lim[tt]) s[tt][i] = -__builtin_inff();
+        }
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt) {
+            float mx = fmaxf(fmaxf(s[tt][0], s[tt][1]), fmaxf(s[tt][2], s[tt][3]));
+            float2 r2 = rows16_swap(mx);
+            mx = fmaxf(r2.x, r2.y);
+            r2 = rows32_swap(mx);
+            mx = fmaxf(m[tt], fmaxf(r2.x, r2.y));
+            const float ref = mx == -__builtin_inff() ? 0.0f : mx;
+            const float alpha = __builtin_amdgcn_exp2f(m[tt] - ref);
+            m[tt] = mx;
+            l[tt] *= alpha;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[tt][i] = __builtin_amdgcn_exp2f(s[tt][i] - ref);
+                l[tt] += s[tt][i];
+            }
+#pragma unroll
+            for (int j = 0; j < kV; ++j) o[tt][j] *= alpha;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < kV; ++j)
+#pragma unroll
+                for (int tt = 0; tt < NT; ++tt)
+                    o[tt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[i][j], s[tt][i], o[tt][j], 0, 0, 0);
+    };
+
+    const int steps = (w_end + 15) / 16;
+    int u = wave;
+    if (u < steps) {
+        Step x, y;
+        load(u, x);
+        while (true) {                                        // wave-uniform
+            if (u + kPfWaves < steps) load(u + kPfWaves, y);
+            compute(u, x);
+            u += kPfWaves;
+            if (u >= steps) break;
+            if (u + kPfWaves < steps) load(u + kPfWaves, x);
+            compute(u, y);
+            u += kPfWaves;
+            if (u >= steps) break;
+        }
+    }
+#pragma unroll
+    for (int tt = 0; tt < NT; ++tt) l[tt] = pair32_sum(pair16_sum(l[tt]));
+
+    // ---- join the wavefronts, in order ----
+    if (lane == 0) sm.odd[wave] = odd ? 1 : 0;
+    if (wave > 0) {
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt) {
+#pragma unroll
+            for (int j = 0; j < kV; ++j) sm.o[wave - 1][tt][j][lane] = o[tt][j];
+            sm.m[wave - 1][tt][lane] = m[tt];
+            sm.l[wave - 1][tt][lane] = l[tt];
+        }
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int tt = 0; tt < NT; ++tt) {
+        float M = m[tt];
+#pragma unroll
+        for (int x = 0; x < kPfWaves - 1; ++x) M = fmaxf(M, sm.m[x][tt][lane]);
+        const float ref = M == -__builtin_inff() ? 0.0f : M;
+        float wt = __builtin_amdgcn_exp2f(m[tt] - ref);
+        l[tt] *= wt;
+#pragma unroll
+        for (int j = 0; j < kV; ++j) o[tt][j] *= wt;
+#pragma unroll
+        for (int x = 0; x < kPfWaves - 1; ++x) {
+            wt = __builtin_amdgcn_exp2f(sm.m[x][tt][lane] - ref);
+            l[tt] = __builtin_fmaf(wt, sm.l[x][tt][lane], l[tt]);
+#pragma unroll
+            for (int j = 0; j < kV; ++j) o[tt][j] += sm.o[x][tt][j][lane] * wt;
+        }
+    }
+    if ((sm.odd[0] | sm.odd[1] | sm.odd[2] | sm.odd[3]) != 0) {
+        // the values cleared above: a positive weight times inf or NaN is that value
+        for (int key = (a.causal ? w_first : len) / 16 * 16; key < w_end; ++key) {
+            const float* vr = vb + static_cast<int64_t>(key) * a.kv_st + 4 * kV * grp;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < kV; ++j) {
+                    const float f = vr[kV * i + j];
+#pragma unroll
+                    for (int tt = 0; tt < NT; ++tt)
+                        if (!(__builtin_fabsf(f) < __builtin_inff()) && key <= lim[tt]) o[tt][j][i] += f;
+                }
+        }
+    }
+    // O^T tile j, row 4 grp + i: dim kV (4 grp + i) + j
+#pragma unroll
+    for (int tt = 0; tt < NT; ++tt) {
+        const int c = col0 + 16 * tt + c16;
+        if (c >= ncol) continue;
+        const float inv = 1.0f / l[tt];
+        float* op = a.out + (w.row0 + static_cast<int64_t>(tok[tt])) * a.out_st +
+                    static_cast<int64_t>(g * a.R + c % a.R) * D + 4 * kV * grp;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < kV; j += 4)
+                *reinterpret_cast<f32x4*>(op + kV * i + j) =
+                    f32x4{o[tt][j][i] * inv, o[tt][j + 1][i] * inv, o[tt][j + 2][i] * inv, o[tt][j + 3][i] * inv};
+    }
+}
+
+// 16-byte rows and 32-bit offsets within a block of keys
 static bool packed_matrix_cores(const void* q, int64_t q_st, int64_t q_sh, const void* k, const void* v, int64_t kv_st,
                                 int64_t kv_sh, int dtype, int64_t N, int64_t R, int64_t D, const void* out,
                                 int64_t out_st) {
-    auto al = [](const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
-    return dtype == SPARDA_BF16 && (D == 64 || D == 128) && N * R < (int64_t(1) << 31) - 256 && al(q, 16) && al(k, 16) && al(v, 16) &&
-           al(out, 8) && q_st % 8 == 0 && q_sh % 8 == 0 && kv_st >= 0 && kv_st < (1 << 24) && kv_st % 8 == 0 && kv_sh % 8 == 0 && out_st % 4 == 0;
+    const int64_t ve = dtype == SPARDA_F32 ? 4 : 8;
+    auto al16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    return (D == 64 || D == 128) && N * R < (int64_t(1) << 31) - 256 && al16(q) && al16(k) && al16(v) && al16(out) &&
+           q_st % ve == 0 && q_sh % ve == 0 && kv_st >= 0 && kv_st < (1 << 24) && kv_st % ve == 0 && kv_sh % ve == 0 &&
+           out_st % ve == 0;
 }
 
 int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void* k, const void* v, int64_t kv_st,
@@ -542,11 +795,31 @@ int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void*
     if (const int rc = status_word(&status)) return rc;
     const int64_t R = Hq / Hkv;
     const float sl = scale * kPkLog2e;
-    if (packed_matrix_cores(q, q_st, q_sh, k, v, kv_st, kv_sh, dtype, N, R, D, out, out_st)) {
+    const bool cores = packed_matrix_cores(q, q_st, q_sh, k, v, kv_st, kv_sh, dtype, N, R, D, out, out_st);
+    if (cores && dtype == SPARDA_F32) {
+        PackedPrefillF32 a{static_cast<const float*>(q), q_st, q_sh, static_cast<const float*>(k),
+                           static_cast<const float*>(v), kv_st, kv_sh, cu, static_cast<int>(n), N, static_cast<int>(Hkv),
+                           static_cast<int>(R), causal, 0, sl, static_cast<float*>(out), out_st, status};
+#define SPARDA_PKF(D_, NT_)                                                                                       \
+    do {                                                                                                          \
+        a.slots = packed_slots(N, n, R, 16 * NT_);                                                                \
+        if (a.slots * Hkv >= (int64_t(1) << 31)) return set_error(SPARDA_ERR_SHAPE, "prefill_packed: grid too large"); \
+        hipLaunchKernelGGL((prefill_packed_f32_kernel<D_, NT_>), dim3(static_cast<unsigned>(a.slots * Hkv)),      \
+                           dim3(kPfWaves * kWave), 0, stream, a);                                                 \
+    } while (0)
+        // wider windows read K and V for more columns, narrow ones are more workgroups:
+        // us of 16 / 48 columns, 12/4 heads of 64: N=512 12.9 / 21.2, 3 x 500 24.8 / 36.5,
+        // N=1501 54.9 / 62.8, N=4000 294 / 238
+        if (D == 128) SPARDA_PKF(128, 1);
+        else if (N * Hq <= 2048 * 16) SPARDA_PKF(64, 1);
+        else SPARDA_PKF(64, 3);
+#undef SPARDA_PKF
+        return check_hip(hipGetLastError(), "prefill_packed_f32_kernel");
+    }
+    if (cores) {
         PackedPrefill a{static_cast<const uint16_t*>(q), q_st, q_sh, static_cast<const uint16_t*>(k),
                         static_cast<const uint16_t*>(v), kv_st, kv_sh, cu, static_cast<int>(n), N, static_cast<int>(Hkv),
                         static_cast<int>(R), causal, 0, sl, static_cast<uint16_t*>(out), out_st, status};
-        static const int force = getenv("PKV") ? atoi(getenv("PKV")) : 0;
 #define SPARDA_PKM(D_, NT_, CW_, KG_, KB_)                                                                        \
     do {                                                                                                          \
         a.slots = packed_slots(N, n, R, 32 * NT_ * CW_);                                                          \
@@ -554,19 +827,29 @@ int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void*
         hipLaunchKernelGGL((prefill_packed_kernel<D_, NT_, CW_, KG_, KB_>), dim3(static_cast<unsigned>(a.slots * Hkv)), \
                            dim3(CW_ * KG_ * kWave), 0, stream, a);                                                \
     } while (0)
+        // W: windows of 128 columns, NB: 64-key blocks of a mean sequence. Wide windows
+        // stage a block for the most columns; key groups and small windows cut a
+        // window's serial walk where windows are few against the 256 CUs (a group's sums
+        // cost a merge, so that short walks are not cut). us of (tiles a wavefront, wavefronts,
+        // key groups) = (2,4,1) / (1,4,1) / (1,4,2) / (1,2,2) / (1,1,4), 12/4 heads of 64, causal:
+        //   N=64 7.8 / 6.0 / 7.4 / 5.8 / 5.8   N=1000 22.8 / 15.2 / 14.3 / 11.1 / 10.8
+        //   N=2048 38.8 / 25.0 / 23.1 / 19.4 / 21.1   N=4096 70.2 / 49.0 / 42.8 / 44.7 / 56.1
+        //   4 x 1024 38.1 / 25.8 / 22.8 / 23.0 / 30.1   16 x 256 15.6 / 13.3 / 16.3 / 16.2 / 21.8
+        //   N=8192 152 / 129 / 136 / 138 / 173   16 x 1024 67.2 / 59.5 / 72.8 / 72.9 / 105
+        //   N=16384 433 / 433 / 479 / 507 / 622   N=32768 1550 / 1627   8 x 8192 847 / 879
+        // and of (1,4,1) / (1,4,2) / (1,2,2 of 32 keys), heads of 128:
+        //   32/8: N=512 14.7 / 15.9 / 12.4   N=1000 23.2 / 22.9 / 22.2   N=2048 50.5 / 51.3 / 56.2
+        //   8 x 250 21.7 / 31.9 / 25.9   8 x 2000 385 / 459 / 507   8/1: N=8192 169 / 149 / 164
+        const int64_t W = cdiv(N * Hq, 128), NB = cdiv(cdiv(N, n), 64), cus = 256;
         if (D == 64) {
-            if (force == 1) SPARDA_PKM(64, 2, 1, 4, 32);
-            else if (force == 2) SPARDA_PKM(64, 1, 1, 4, 32);
-            else if (force == 3) SPARDA_PKM(64, 1, 4, 1, 64);
-            else if (force == 4) SPARDA_PKM(64, 2, 4, 2, 64);
-            else if (force == 5) SPARDA_PKM(64, 1, 4, 2, 64);
-            else if (force == 6) SPARDA_PKM(64, 2, 4, 1, 32);
+            if (2 * W <= cus) SPARDA_PKM(64, 1, 1, 4, 32);
+            else if (W <= cus && NB >= 8) SPARDA_PKM(64, 1, 2, 2, 64);
+            else if (W <= 2 * cus && NB >= 16) SPARDA_PKM(64, 1, 4, 2, 64);
+            else if (W <= 8 * cus || NB < 32) SPARDA_PKM(64, 1, 4, 1, 64);
             else SPARDA_PKM(64, 2, 4, 1, 64);
         } else {
-            if (force == 1 || force == 2) SPARDA_PKM(128, 1, 1, 4, 32);
-            else if (force == 4) SPARDA_PKM(128, 1, 4, 2, 64);
-            else if (force == 5) SPARDA_PKM(128, 1, 4, 2, 32);
-            else if (force == 6) SPARDA_PKM(128, 1, 4, 1, 32);
+            if (2 * W <= cus || (W <= cus && NB >= 8)) SPARDA_PKM(128, 1, 2, 2, 32);
+            else if (W <= 2 * cus && NB >= 64) SPARDA_PKM(128, 1, 4, 2, 64);
             else SPARDA_PKM(128, 1, 4, 1, 64);
         }
 #undef SPARDA_PKM

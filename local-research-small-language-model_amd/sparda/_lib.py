@@ -188,7 +188,8 @@ def fail(name: str, rc: int) -> None:
 # entry points the native host path calls, in the order of its table
 _HOST_ENTRIES = ("compress", "route", "prefill", "prefill_routed", "prefill_chunked", "decode",
                  "decode_workspace_bytes", "decode_selected", "decode_dense_workspace_bytes", "decode_sums", "produce",
-                 "produce_at", "produce_cache_at", "ffn_decode", "rows_residual", "norm_gemv", "teacher_mass")
+                 "produce_at", "produce_cache_at", "ffn_decode", "rows_residual", "norm_gemv", "teacher_mass",
+                 "prefill_packed", "append_paged", "decode_paged", "decode_paged_workspace_bytes")
 
 
 class _NoHost:

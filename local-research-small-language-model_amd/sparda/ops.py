@@ -1177,6 +1177,10 @@ def prefill_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
     Returns out [N,Hq*D]. Offsets that fall or leave [0, N]: that sequence's
     rows are not written and status() has STATUS_SEQUENCE_RANGE.
     """
+    if out is None:
+        r = _host.prefill_packed(q, k, v, cu_seqlens, causal, scale)
+        if r is not None:
+            return r if type(r) is not int else _lib.fail("sparda_prefill_packed", r)
     dev = require_device(q, k, v, cu_seqlens, out)
     _inference_only(q, k, v)
     if not (q.dtype == k.dtype == v.dtype):
@@ -1230,6 +1234,9 @@ def append_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch
     whose page is missing or outside the cache is dropped and status() has
     STATUS_PAGE_RANGE.
     """
+    r = _host.append_paged(k_pages, v_pages, page_table, positions, k_new, v_new, cu_seqlens)
+    if r is not None:
+        return None if r == 0 else _lib.fail("sparda_append_paged", r)
     dev = require_device(k_pages, v_pages, page_table, positions, k_new, v_new, cu_seqlens)
     _inference_only(k_pages, v_pages, k_new, v_new)
     _check_pages(k_pages, v_pages, page_table)
@@ -1271,6 +1278,10 @@ def decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     a length of 0, NaN (and STATUS_PAGE_RANGE in status()) where a page index or
     the length is out of range.
     """
+    if out is None:
+        r = _host.decode_paged(q, k_pages, v_pages, page_table, lengths, scale)
+        if r is not None:
+            return r if type(r) is not int else _lib.fail("sparda_decode_paged", r)
     dev = require_device(q, k_pages, v_pages, page_table, lengths, out)
     _inference_only(q, k_pages, v_pages)
     _check_pages(k_pages, v_pages, page_table)
