@@ -101,13 +101,14 @@ namespace {
 // All steps of the batch are cut into shares of the same number of steps, so
 // that long and short sequences load the workgroups alike: the share length is
 // the total over `target`, at least `least`, and sequence b takes
-// n_b = max(1, ceil(steps_b / share)) consecutive items, at most target + B of
-// them in all. Every workgroup derives this from the lengths for itself.
+// n_b = max(1, ceil(steps_b / share)) consecutive items of about equal length, at
+// most target + B of them in all. Every workgroup derives this from the lengths
+// for itself.
 struct Share {
     int seq;         // -1: no sequence has this item
     int part, parts; // the item's place among its sequence's
     int first;       // the sequence's first item
-    int share;       // steps of an item
+    int share;       // steps of each of them
     int len;         // the sequence's length, cut to the table's capacity
     bool bad;        // the length is out of range
 };
@@ -161,6 +162,7 @@ __device__ __forceinline__ Share paged_item(const int32_t* __restrict__ len, int
             r.first = __builtin_amdgcn_readfirstlane(__shfl(end, at, kWave)) - r.parts;
             r.part = by_item ? want - r.first : 0;
             const int l = __builtin_amdgcn_readfirstlane(len[r.seq]);
+            r.share = (paged_steps(l, cap, step) + r.parts - 1) / r.parts;
             r.bad = l < 0 || l > cap;
             r.len = l < 0 ? 0 : l > cap ? cap : l;
             return r;
@@ -194,6 +196,8 @@ struct PagedStep {
     VRow v[kTiles][4];
 };
 
+constexpr int kPgJoin = 512;        // threads of a join
+
 struct PagedDecode {
     const void* q;
     int64_t q_sb, q_sh;
@@ -204,6 +208,7 @@ struct PagedDecode {
     int B, cap;
     int Hq, Hkv, R, head_tiles;   // head tiles of 16 query heads per KV head
     int target, least;
+    int lds_heads;                // heads of the largest tile
     float scale_log2;
     void* out;
     int64_t out_sb;
@@ -213,27 +218,45 @@ struct PagedDecode {
 
 }  // namespace
 
-// One workgroup of W wavefronts per (KV head, tile of up to 16 of its query
-// heads, item). The heads are the 16 columns of the matrix products:
+// One output of an item: the sequence's, or the item's partial.
+template <int DT, int D>
+__device__ __forceinline__ void paged_store(const PagedDecode& a, const Share& sh, int item, int h, int d, float O, float M,
+                                            float L, bool bad) {
+    if (sh.parts == 1) {
+        // (an empty sequence: zeros)
+        store_elem<DT>(a.out, sh.seq * a.out_sb + static_cast<int64_t>(h) * D + d, sh.len == 0 && !bad ? 0.0f : O / L);
+    } else {
+        const int64_t at = static_cast<int64_t>(item) * a.Hq + h;
+        a.part_o[at * D + d] = O;
+        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(M, L);
+    }
+}
+
+// One workgroup of W = HG KW wavefronts per (HG head tiles, item): a head tile is
+// up to 16 query heads of one KV head, and the HG tiles' wavefronts read the same
+// positions at the same time, so that neighbouring heads' rows, which lie side by
+// side in a page, are fetched together. The heads of a tile are the 16 columns of
+// the matrix products:
 //     S^T[key, head] = K[key, :] . Q[head, :]
 //     P = exp2(S scale log2 e - m[head])
 //     O^T[d, head] += V^T[d, key] . P^T[key, head]
-// Wavefront w walks the steps w, w + W, ... of the share with its own (m, l, O);
-// K and V go straight from the pages to the operand registers, the next step's
-// under the present one's arithmetic, and S^T's layout is already that of the
+// The KW wavefronts of a tile take the steps of the share in turn, each with its own
+// (m, l, O); K and V go straight from the pages to the operand registers, the next
+// step's under the present one's arithmetic, and S^T's layout is already that of the
 // P operand, so nothing passes through LDS before the wavefronts are joined. A
 // tile's 16 keys lie in one page (pages hold a multiple of 16 rows), so that its
 // base address is a scalar.
-template <int DT, int D, int W>
-__global__ void __launch_bounds__(W* kWave) decode_paged_kernel(PagedDecode a) {
+template <int DT, int D, int HG, int KW>
+__global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : 4) decode_paged_kernel(PagedDecode a) {
     typedef PagedStep<DT, D> Step;
-    constexpr int kTiles = Step::kTiles, kV = Step::kV, kQ = Step::kQ, kStep = 16 * kTiles;
+    constexpr int kTiles = Step::kTiles, kV = Step::kV, kQ = Step::kQ, kStep = 16 * kTiles, W = KW;
     extern __shared__ float lds[];
     const int lane = threadIdx.x % kWave;
-    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int wv = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int wave = wv / HG;                               // among the wavefronts of a head tile
     const int c16 = lane % 16, grp = lane / 16;
-    const int heads = a.Hkv * a.head_tiles;
-    const int item = blockIdx.x / heads, gt = blockIdx.x % heads;
+    const int groups = a.Hkv * a.head_tiles / HG;
+    const int item = blockIdx.x / groups, gt = blockIdx.x % groups * HG + wv % HG;
     const int g = gt / a.head_tiles, h0 = gt % a.head_tiles * 16;
     const int nh = a.R - h0 < 16 ? a.R - h0 : 16;           // query heads of the tile
     const Share sh = paged_item(a.len, a.B, a.cap, kStep, a.target, a.least, true, item);
@@ -398,114 +421,212 @@ __global__ void __launch_bounds__(W* kWave) decode_paged_kernel(PagedDecode a) {
     }
     l = pair32_sum(pair16_sum(l));
 
-    // ---- the wavefronts' partials, joined in order ----
-    float* lo = lds;                                          // [W][nh][D]
-    float* lm = lds + W * nh * D;                             // [W][16][2]
-    int* lbad = reinterpret_cast<int*>(lm + W * 32);          // [W]
-    if (c16 < nh) {
+    const bool any_bad = __ballot(bad) != 0;                  // wave-uniform
+    if constexpr (KW == 1) {
+        if (any_bad && lane == 0) atomicOr(a.status, static_cast<uint32_t>(SPARDA_STATUS_PAGE_RANGE));
+        if (c16 >= nh) return;
+        const int h = g * a.R + h0 + c16;
         // O^T tile j, row 4 grp + i: dim kV (4 grp + i) + j
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < kV; ++j) lo[(wave * nh + c16) * D + kV * (4 * grp + i) + j] = o[j][i];
-        if (grp == 0) {
-            lm[(wave * 16 + c16) * 2] = m;
-            lm[(wave * 16 + c16) * 2 + 1] = l;
-        }
-    }
-    const bool any_bad = __ballot(bad) != 0;
-    if (lane == 0) lbad[wave] = any_bad ? 1 : 0;
-    __syncthreads();
-    int bads = 0;
+            for (int j = 0; j < kV; ++j)
+                paged_store<DT, D>(a, sh, item, h, kV * (4 * grp + i) + j, any_bad ? __builtin_nanf("") : o[j][i], m, l, any_bad);
+    } else {
+        // ---- the wavefronts' partials, joined in order: thread -> (head, dim) ----
+        const int hg = wv % HG;
+        float* lo = lds + hg * KW * (a.lds_heads * (D + 4) + 33);     // [KW][lds_heads][D + 4]
+        float* lm = lo + KW * a.lds_heads * (D + 4);                  // [KW][16][2]
+        int* lbad = reinterpret_cast<int*>(lm + KW * 32);             // [KW]
+        if (c16 < nh) {
 #pragma unroll
-    for (int w = 0; w < W; ++w) bads |= lbad[w];
-    if (bads != 0 && threadIdx.x == 0) atomicOr(a.status, static_cast<uint32_t>(SPARDA_STATUS_PAGE_RANGE));
-    for (int e = threadIdx.x; e < nh * D; e += W * kWave) {
-        const int c = e / D, d = e % D;
-        float M = lm[c * 2];
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int w = 1; w < W; ++w) M = fmaxf(M, lm[(w * 16 + c) * 2]);
-        const float ref = M == -__builtin_inff() ? 0.0f : M;
-        float L = 0.0f, O = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float wt = __builtin_amdgcn_exp2f(lm[(w * 16 + c) * 2] - ref);
-            L = __builtin_fmaf(wt, lm[(w * 16 + c) * 2 + 1], L);
-            O = __builtin_fmaf(wt, lo[(w * nh + c) * D + d], O);
-        }
-        if (bads != 0) O = L = __builtin_nanf("");
-        const int h = g * a.R + h0 + c;
-        if (sh.parts == 1) {
-            store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d, len == 0 && bads == 0 ? 0.0f : O / L);
-        } else {
-            const int64_t at = static_cast<int64_t>(item) * a.Hq + h;
-            a.part_o[at * D + d] = O;
-            if (d == 0) {
-                a.part_ml[at * 2] = M;
-                a.part_ml[at * 2 + 1] = L;
+                for (int j = 0; j < kV; ++j) lo[(wave * a.lds_heads + c16) * (D + 4) + kV * (4 * grp + i) + j] = o[j][i];
+            if (grp == 0) {
+                lm[(wave * 16 + c16) * 2] = m;
+                lm[(wave * 16 + c16) * 2 + 1] = l;
             }
+        }
+        if (lane == 0) lbad[wave] = any_bad ? 1 : 0;
+        __syncthreads();
+        int bads = 0;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) bads |= lbad[w];
+        if (bads != 0 && wave == 0 && lane == 0) atomicOr(a.status, static_cast<uint32_t>(SPARDA_STATUS_PAGE_RANGE));
+        for (int e = wave * kWave + lane; e < nh * D; e += KW * kWave) {
+            const int c = e / D, d = e % D;
+            float mw[KW], M = -__builtin_inff();
+#pragma unroll
+            for (int w = 0; w < KW; ++w) {
+                mw[w] = lm[(w * 16 + c) * 2];
+                M = fmaxf(M, mw[w]);
+            }
+            const float ref = M == -__builtin_inff() ? 0.0f : M;
+            float L = 0.0f, O = 0.0f;
+#pragma unroll
+            for (int w = 0; w < KW; ++w) {
+                const float wt = __builtin_amdgcn_exp2f(mw[w] - ref);
+                L = __builtin_fmaf(wt, lm[(w * 16 + c) * 2 + 1], L);
+                O = __builtin_fmaf(wt, lo[(w * a.lds_heads + c) * (D + 4) + d], O);
+            }
+            paged_store<DT, D>(a, sh, item, g * a.R + h0 + c, d, bads ? __builtin_nanf("") : O, M, L, bads != 0);
         }
     }
 }
 
 // Joins the items of a sequence, one workgroup per (query head, sequence): the
-// items' weights once in LDS, then dims over the lanes and the items over
-// 256 / D thread groups, added in group order.
+// items' weights once into LDS, then dims over the lanes and the items over the
+// thread groups (8 loads in flight each), added in group order.
 template <int DT, int D>
-__global__ void __launch_bounds__(256) decode_paged_join_kernel(PagedDecode a) {
-    constexpr int kStep = 16 * PagedType<DT>::kTiles, kG = 256 / D;
-    __shared__ float red[256], lsum[kG];
-    const int b = blockIdx.y, h = blockIdx.x;
+__global__ void __launch_bounds__(kPgJoin) decode_paged_join_kernel(PagedDecode a) {
+    constexpr int kStep = 16 * PagedType<DT>::kTiles, kG = kPgJoin / D, kChunk = 1024, kJW = kPgJoin / kWave;
+    __shared__ float red[kPgJoin], wts[kChunk], rm[kJW], rl[kJW];
+    const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, wave = tid / kWave;
     const Share sh = paged_item(a.len, a.B, a.cap, kStep, a.target, a.least, false, b);
     if (sh.parts <= 1) return;                                // written by its one item
-    const int d = threadIdx.x % D, gr = threadIdx.x / D;
-    const int64_t at0 = static_cast<int64_t>(sh.first) * a.Hq + h;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + static_cast<int64_t>(sh.first) * a.Hq + h;
+    const float* po = a.part_o + (static_cast<int64_t>(sh.first) * a.Hq + h) * D + tid % D;
+    const int64_t st = static_cast<int64_t>(a.Hq) * D;
+    float first[8];                                           // the thread's first items, under the weights' latency
+#pragma unroll
+    for (int e = 0; e < 8; ++e) first[e] = tid / D + e * kG < sh.parts ? po[(tid / D + e * kG) * st] : 0.0f;
     float M = -__builtin_inff();
-    for (int i = threadIdx.x % kWave; i < sh.parts; i += kWave) M = fmaxf(M, a.part_ml[(at0 + static_cast<int64_t>(i) * a.Hq) * 2]);
+    for (int i = tid; i < sh.parts; i += kPgJoin) M = fmaxf(M, ml[static_cast<int64_t>(i) * a.Hq].x);
     M = wave_max(M);
+    if (tid % kWave == 0) rm[wave] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJW; ++w) M = fmaxf(M, rm[w]);
     const float ref = M == -__builtin_inff() ? 0.0f : M;
     float L = 0.0f, O = 0.0f;
-    for (int i = gr; i < sh.parts; i += kG) {
-        const int64_t at = at0 + static_cast<int64_t>(i) * a.Hq;
-        const float wt = __builtin_amdgcn_exp2f(a.part_ml[at * 2] - ref);
-        L = __builtin_fmaf(wt, a.part_ml[at * 2 + 1], L);
-        O = __builtin_fmaf(wt, a.part_o[at * D + d], O);
-    }
-    red[threadIdx.x] = O;
-    if (d == 0) lsum[gr] = L;
-    __syncthreads();
-    if (gr != 0) return;
-    float sum = 0.0f, den = 0.0f;
+    for (int c0 = 0; c0 < sh.parts; c0 += kChunk) {
+        const int n = sh.parts - c0 < kChunk ? sh.parts - c0 : kChunk;
+        if (c0 > 0) __syncthreads();                          // the last chunk's weights have been read
+        for (int i = tid; i < n; i += kPgJoin) {
+            const float2 x = ml[static_cast<int64_t>(c0 + i) * a.Hq];
+            const float wt = __builtin_amdgcn_exp2f(x.x - ref);
+            wts[i] = wt;
+            L = __builtin_fmaf(wt, x.y, L);
+        }
+        __syncthreads();
+        int i = tid / D;
+        if (c0 == 0) {
 #pragma unroll
-    for (int i = 0; i < kG; ++i) {
-        sum += red[i * D + d];
-        den += lsum[i];
+            for (int e = 0; e < 8; ++e) O = i + e * kG < n ? __builtin_fmaf(wts[i + e * kG], first[e], O) : O;
+            i += 8 * kG;
+        }
+        for (; i + 7 * kG < n; i += 8 * kG) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = po[(c0 + i + e * kG) * st];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) O = __builtin_fmaf(wts[i + e * kG], x[e], O);
+        }
+        for (; i < n; i += kG) O = __builtin_fmaf(wts[i], po[(c0 + i) * st], O);
     }
-    store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d, sum / den);
+    L = wave_sum(L);
+    if (tid % kWave == 0) rl[wave] = L;
+    red[tid] = O;
+    __syncthreads();
+    if (tid >= D) return;
+    float den = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kJW; ++w) den += rl[w];
+#pragma unroll
+    for (int i = 1; i < kG; ++i) O += red[i * D + tid];
+    store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + tid, O / den);
+}
+
+// The same for few items a sequence: one thread per (query head, dim), items in order.
+template <int DT, int D>
+__global__ void __launch_bounds__(256) decode_paged_join_few_kernel(PagedDecode a) {
+    constexpr int kStep = 16 * PagedType<DT>::kTiles;
+    const int b = blockIdx.y, h = blockIdx.x * (256 / D) + threadIdx.x / D, d = threadIdx.x % D;
+    const Share sh = paged_item(a.len, a.B, a.cap, kStep, a.target, a.least, false, b);
+    if (sh.parts <= 1 || h >= a.Hq) return;                   // written by its one item
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + static_cast<int64_t>(sh.first) * a.Hq + h;
+    const float* po = a.part_o + (static_cast<int64_t>(sh.first) * a.Hq + h) * D + d;
+    const int64_t st = static_cast<int64_t>(a.Hq) * D;
+    float m = -__builtin_inff(), L = 0.0f, O = 0.0f;
+    for (int i0 = 0; i0 < sh.parts; i0 += 8) {
+        float2 x[8];
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int i = i0 + e < sh.parts ? i0 + e : sh.parts - 1;
+            x[e] = ml[static_cast<int64_t>(i) * a.Hq];
+            y[e] = po[i * st];
+        }
+        float M = m;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) M = fmaxf(M, x[e].x);
+        const float ref = M == -__builtin_inff() ? 0.0f : M, alpha = __builtin_amdgcn_exp2f(m - ref);
+        L *= alpha;
+        O *= alpha;
+        m = M;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (i0 + e < sh.parts) {
+                const float wt = __builtin_amdgcn_exp2f(x[e].x - ref);
+                L = __builtin_fmaf(wt, x[e].y, L);
+                O = __builtin_fmaf(wt, y[e], O);
+            }
+    }
+    store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d, O / L);
 }
 
 namespace {
 
-constexpr int kPgWaves = 4;
-constexpr int kPgLeast = 2 * kPgWaves;   // steps of the smallest share
-constexpr int64_t kPgGroups = 1024;      // workgroups aimed at
-
+// How a launch is cut. us, 12/4 heads of 64 and 32/8 of 128 where named:
+//  - A table whose sequences are short, or a batch that gives every CU a workgroup:
+//    one item a sequence, written straight to the output, no second launch
+//    (B=1, 300 positions 6.3 against 8.2 in shares; B=64, 1000: 12.5 / 15.3; B=128,
+//    300: 8.7 / 12.6). Fewer and longer sequences are faster in shares (B=1, 1000:
+//    10.3 / 8.3).
+//  - Many (sequence, head) pairs: workgroups of 2 or 4 neighbouring heads, which
+//    fetch whole rows of a page at a time (B=32, 16384, 32/8 heads of 128: 257
+//    against 290 with one head a workgroup; 8/8 heads of 64: 137 / 180).
+//  - Otherwise one head a workgroup: four wavefronts on its keys make four times
+//    fewer partials for the join (B=1, 131000: 31.4 / 35). About as many
+//    workgroups as the chip holds: shares of half the length cost a longer join
+//    (B=1, 131000: 34), twice the length a longer walk (B=8, 16384: 26.2 / 25.4).
 struct PagedPlan {
-    int64_t heads, target, items;
+    int hg, kw;              // head tiles, and wavefronts for each, of a workgroup
+    int64_t target, least;   // items aimed at, steps of the smallest item
+    int64_t items, groups;   // items at most, workgroups an item
+    bool few;                // a sequence has few items
 };
-PagedPlan paged_plan(int64_t B, int64_t cap, int64_t Hq, int64_t Hkv, int dtype) {
-    const int64_t heads = Hkv * cdiv(Hq / Hkv, 16), step = dtype == SPARDA_F32 ? 16 : 32;
-    int64_t target = cdiv(kPgGroups, heads);
-    int64_t items = target + B;
-    const int64_t most = B * cdiv(cdiv(cap, step), kPgLeast);  // every share the smallest
-    if (items > most) items = most;
-    return {heads, target, items};
+PagedPlan paged_plan(int64_t B, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D, int dtype) {
+    const int64_t R = Hq / Hkv, heads = Hkv * cdiv(R, 16), steps = cdiv(cap, dtype == SPARDA_F32 ? 16 : 32);
+    const int even = heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
+    const bool eight = (R < 16 ? R : 16) * (D + 4) + 33 <= 2048;  // eight wavefronts' partials fit 64 KB of LDS
+    PagedPlan p{1, 4, 1, 4, 0, 0, false};
+    if (steps <= 16 || (steps <= 64 && B * heads >= 128)) {
+        p.least = steps;
+        if (eight && steps > 8 && B * heads < 512) p.kw = 8;
+    } else if (eight && B * heads >= 128 && even > 1) {
+        p.hg = even;
+        p.kw = 8 / even;
+        // (items are target + B at most: whole rounds of 512 workgroups, half of one at least beside the B)
+        const int64_t round = cdiv(512, heads / even);
+        p.target = cdiv(B + round / 2, round) * round - B;
+    } else {
+        p.target = (D == 128 ? 512 : 1024) / heads - B / 2;
+    }
+    if (p.target < 1) p.target = 1;
+    p.groups = heads / p.hg;
+    p.items = p.target + B;
+    const int64_t most = B * cdiv(steps, p.least);   // every share the smallest
+    if (p.items > most) p.items = most;
+    p.few = p.items <= 16 * B;
+    return p;
 }
 
 }  // namespace
 
 size_t decode_paged_workspace_bytes(int64_t B, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D, int dtype) {
-    const PagedPlan p = paged_plan(B, cap, Hq, Hkv, dtype);
+    const PagedPlan p = paged_plan(B, cap, Hq, Hkv, D, dtype);
     // one item a sequence: written by the item itself
     return p.items <= B ? 0 : static_cast<size_t>(p.items * Hq * (D + 2)) * sizeof(float);
 }
@@ -517,26 +638,34 @@ int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k
     PagedDecode a{};
     if (const int rc = status_word(&a.status)) return rc;
     const int64_t cap = width * ps, R = Hq / Hkv;
-    const PagedPlan p = paged_plan(B, cap, Hq, Hkv, dtype);
+    const PagedPlan p = paged_plan(B, cap, Hq, Hkv, D, dtype);
     a.q = q, a.q_sb = q_sb, a.q_sh = q_sh, a.k = k, a.v = v;
     a.pg = Pages{p_st, s_st, h_st, table, t_st, static_cast<int>(width), static_cast<int>(n_pages)};
     a.ps16 = static_cast<int>(ps / 16), a.len = len, a.B = static_cast<int>(B), a.cap = static_cast<int>(cap);
     a.Hq = static_cast<int>(Hq), a.Hkv = static_cast<int>(Hkv), a.R = static_cast<int>(R);
     a.head_tiles = static_cast<int>(cdiv(R, 16));
-    a.target = static_cast<int>(p.target), a.least = kPgLeast;
+    a.target = static_cast<int>(p.target), a.least = static_cast<int>(p.least);
+    a.lds_heads = static_cast<int>(R < 16 ? R : 16);
     a.scale_log2 = scale * kPgLog2e, a.out = out, a.out_sb = out_sb;
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = workspace ? a.part_o + p.items * Hq * D : nullptr;
-    if (p.items * p.heads >= (int64_t(1) << 31)) return set_error(SPARDA_ERR_SHAPE, "decode_paged: grid too large");
-    const dim3 grid(static_cast<unsigned>(p.items * p.heads));
-    const int nh = static_cast<int>(R < 16 ? R : 16);
-    const size_t lds = (static_cast<size_t>(kPgWaves) * nh * D + kPgWaves * 33) * sizeof(float);
+    if (p.items * p.groups >= (int64_t(1) << 31)) return set_error(SPARDA_ERR_SHAPE, "decode_paged: grid too large");
+    const dim3 grid(static_cast<unsigned>(p.items * p.groups));
+#define SPARDA_PGD_W(DT_, D_, HG_, KW_)                                                                           \
+    hipLaunchKernelGGL((decode_paged_kernel<DT_, D_, HG_, KW_>), grid, dim3(HG_ * KW_ * kWave),                   \
+                       KW_ > 1 ? HG_ * KW_ * (a.lds_heads * ((D_) + 4) + 33) * sizeof(float) : 0, stream, a)
 #define SPARDA_PGD(DT_, D_)                                                                                       \
     do {                                                                                                          \
-        hipLaunchKernelGGL((decode_paged_kernel<DT_, D_, kPgWaves>), grid, dim3(kPgWaves * kWave), lds, stream, a); \
-        if (p.items > B)                                                                                          \
+        if (p.hg == 4) SPARDA_PGD_W(DT_, D_, 4, 2);                                                               \
+        else if (p.hg == 2) SPARDA_PGD_W(DT_, D_, 2, 4);                                                          \
+        else if (p.kw == 4) SPARDA_PGD_W(DT_, D_, 1, 4);                                                          \
+        else SPARDA_PGD_W(DT_, D_, 1, 8);                                                                         \
+        if (p.items > B && p.few)                                                                                 \
+            hipLaunchKernelGGL((decode_paged_join_few_kernel<DT_, D_>),                                           \
+                               dim3(static_cast<unsigned>(cdiv(Hq, 256 / D_)), static_cast<unsigned>(B)), dim3(256), 0, stream, a); \
+        else if (p.items > B)                                                                                     \
             hipLaunchKernelGGL((decode_paged_join_kernel<DT_, D_>), dim3(static_cast<unsigned>(Hq), static_cast<unsigned>(B)), \
-                               dim3(256), 0, stream, a);                                                          \
+                               dim3(kPgJoin), 0, stream, a);                                                      \
     } while (0)
 #define SPARDA_PGD_D(DT_)                     \
     switch (D) {                              \
@@ -548,6 +677,7 @@ int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k
     if (dtype == SPARDA_F32) SPARDA_PGD_D(SPARDA_F32)
     else SPARDA_PGD_D(SPARDA_BF16)
 #undef SPARDA_PGD_D
+#undef SPARDA_PGD_W
 #undef SPARDA_PGD
     return check_hip(hipGetLastError(), "decode_paged_kernel");
 }
