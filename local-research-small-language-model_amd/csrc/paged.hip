@@ -247,7 +247,7 @@ __device__ __forceinline__ void paged_store(const PagedDecode& a, const Share& s
 // tile's 16 keys lie in one page (pages hold a multiple of 16 rows), so that its
 // base address is a scalar.
 template <int DT, int D, int HG, int KW>
-__global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : 4) decode_paged_kernel(PagedDecode a) {
+__global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : DT == SPARDA_F32 ? 3 : 4) decode_paged_kernel(PagedDecode a) {
     typedef PagedStep<DT, D> Step;
     constexpr int kTiles = Step::kTiles, kV = Step::kV, kQ = Step::kQ, kStep = 16 * kTiles, W = KW;
     extern __shared__ float lds[];
@@ -332,28 +332,27 @@ __global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : 4) decode_paged_
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
             s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            f32x4 s4[4] = {s[t], s[t], s[t], s[t]};          // (fp32: four short sums, whose roundings are smaller)
 #pragma unroll
             for (int i = 0; i < kQ; ++i) {
                 if constexpr (DT == SPARDA_F32) {
                     const f32x4 ka = __builtin_bit_cast(f32x4, x.k[t][i]), qb = __builtin_bit_cast(f32x4, qr[i]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(ka[e], qb[e], s[t], 0, 0, 0);
+                    for (int e = 0; e < 4; ++e) s4[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(ka[e], qb[e], s4[e], 0, 0, 0);
                 } else {
                     s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.k[t][i]),
                                                                    __builtin_bit_cast(bf16x8, qr[i]), s[t], 0, 0, 0);
                 }
             }
+            if constexpr (DT == SPARDA_F32) s[t] = (s4[0] + s4[1]) + (s4[2] + s4[3]);
         }
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) s[t] *= a.scale_log2;
-        const int key0 = u * kStep;
-        if (key0 + kStep > len) {                            // the last step: its keys past the end weigh nothing
+        const int left = len - u * kStep - 4 * grp;          // this lane's keys 16 t + i below it are the sequence's
+        if (u * kStep + kStep > len) {                       // the last step: the others weigh nothing
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (key0 + 16 * t + 4 * grp + i >= len) {
-                        s[t][i] = -__builtin_inff();
+                    if (16 * t + i >= left) {
 #pragma unroll
                         for (int j = 0; j < kV; ++j) x.v[t][i][j] = 0;
                     }
@@ -362,7 +361,7 @@ __global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : 4) decode_paged_
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][i]);
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, 16 * t + i < left ? s[t][i] * a.scale_log2 : -__builtin_inff());
         // (builtin swaps: both lanes of a pair see the same two values)
         float2 r2 = rows16_swap(mx);
         mx = fmaxf(r2.x, r2.y);
@@ -372,12 +371,14 @@ __global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : 4) decode_paged_
         const float alpha = __builtin_amdgcn_exp2f(m - ref);
         m = mx;
         l *= alpha;
+        // one rounding between a score and its distance from the reference, which
+        // is small where the weight is not
         float p[kTiles][4];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                p[t][i] = __builtin_amdgcn_exp2f(s[t][i] - ref);
+                p[t][i] = 16 * t + i < left ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.scale_log2, -ref)) : 0.0f;
                 l += p[t][i];
             }
 #pragma unroll

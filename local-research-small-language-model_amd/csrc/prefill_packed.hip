@@ -39,9 +39,8 @@ prefill_packed_general_kernel(const void* __restrict__ q, int64_t q_st, int64_t 
     float m = -__builtin_inff(), l = 0.0f, o0 = 0.0f, o1 = 0.0f;
     for (int s0 = 0; s0 < keys; s0 += kWave) {
         const int s = s0 + lane;
-        float x = -__builtin_inff();
+        float x = -__builtin_inff(), acc = 0.0f;
         if (s < keys) {
-            float acc = 0.0f;
             const int64_t ko = kvo + s * kv_st;
             for (int d = 0; d < D; ++d) acc = __builtin_fmaf(load_elem<DT>(q, qo + d), load_elem<DT>(k, ko + d), acc);
             x = acc * scale_log2;
@@ -49,7 +48,7 @@ prefill_packed_general_kernel(const void* __restrict__ q, int64_t q_st, int64_t 
         const float mx = fmaxf(m, wave_max(x));
         const float ref = mx == -__builtin_inff() ? 0.0f : mx;
         const float alpha = __builtin_amdgcn_exp2f(m - ref);
-        float p = __builtin_amdgcn_exp2f(x - ref);
+        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc, scale_log2, -ref));
         if (s >= keys) p = 0.0f;
         l = l * alpha + wave_sum(p);
         o0 *= alpha;
@@ -634,18 +633,25 @@ __global__ void __launch_bounds__(kPfWaves* kWave, 2) prefill_packed_f32_kernel(
     auto compute = [&](int u, Step& x) __attribute__((always_inline)) {
         const int key0 = 16 * u;
         const bool edge = a.causal ? key0 + 15 > w_first : key0 + 16 > len;
-        f32x4 s[NT];
+        // kC short sums a score: no product waits for the one before, and the roundings are smaller
+        constexpr int kC = NT == 1 ? 4 : 2;
+        f32x4 s[NT], sc[NT][kC];
 #pragma unroll
-        for (int tt = 0; tt < NT; ++tt) s[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+            for (int c = 0; c < kC; ++c) sc[tt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < kV; ++e)
 #pragma unroll
             for (int y = 0; y < 4; ++y)
 #pragma unroll
                 for (int tt = 0; tt < NT; ++tt)
-                    s[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[e][y], qr[tt][e][y], s[tt], 0, 0, 0);
+                    sc[tt][y % kC] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[e][y], qr[tt][e][y], sc[tt][y % kC], 0, 0, 0);
 #pragma unroll
-        for (int tt = 0; tt < NT; ++tt) s[tt] *= a.scale_log2;
+        for (int tt = 0; tt < NT; ++tt) {
+            s[tt] = sc[tt][0] + sc[tt][1];
+            if constexpr (kC == 4) s[tt] += sc[tt][2] + sc[tt][3];
+        }
         if (edge) {
             // (a weight of 0 times inf is NaN: such values are cleared here, and added at the end to the columns
             // that do attend them)
@@ -661,26 +667,28 @@ __global__ void __launch_bounds__(kPfWaves* kWave, 2) prefill_packed_f32_kernel(
 #pragma unroll
                     for (int j = 0; j < kV; ++j) x.v[i][j] = __builtin_fabsf(x.v[i][j]) < __builtin_inff() ? x.v[i][j] : 0.0f;
             }
-#pragma unroll
-            for (int tt = 0; tt < NT; ++tt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (key0 + 4 * grp + i > lim[tt]) s[tt][i] = -__builtin_inff();
         }
 #pragma unroll
         for (int tt = 0; tt < NT; ++tt) {
-            float mx = fmaxf(fmaxf(s[tt][0], s[tt][1]), fmaxf(s[tt][2], s[tt][3]));
+            float mx = m[tt];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float y = s[tt][i] * a.scale_log2;
+                mx = fmaxf(mx, edge && key0 + 4 * grp + i > lim[tt] ? -__builtin_inff() : y);
+            }
             float2 r2 = rows16_swap(mx);
             mx = fmaxf(r2.x, r2.y);
             r2 = rows32_swap(mx);
-            mx = fmaxf(m[tt], fmaxf(r2.x, r2.y));
+            mx = fmaxf(r2.x, r2.y);
             const float ref = mx == -__builtin_inff() ? 0.0f : mx;
             const float alpha = __builtin_amdgcn_exp2f(m[tt] - ref);
             m[tt] = mx;
             l[tt] *= alpha;
+            // one rounding between a score and its distance from the reference, which is small where the weight is not
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                s[tt][i] = __builtin_amdgcn_exp2f(s[tt][i] - ref);
+                s[tt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, -ref));
+                if (edge && key0 + 4 * grp + i > lim[tt]) s[tt][i] = 0.0f;
                 l[tt] += s[tt][i];
             }
 #pragma unroll
