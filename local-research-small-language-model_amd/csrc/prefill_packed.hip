@@ -550,25 +550,19 @@ struct PackedPrefillF32 {
     uint32_t* status;
 };
 
-template <int D>
-struct PackedStepF32 {
-    f32x4 k[D / 16];                 // key c16, dims 16 c + 4 grp .. +3
-    float v[4][D / 16];              // key 4 grp + i, dims D / 16 c16 ..
-};
-
 }  // namespace
 
 // One workgroup of 4 wavefronts per (KV head, window of 16 NT columns of one
-// sequence; columns as in the bf16 kernel). The wavefronts take the steps of 16 keys
-// in turn, each with its own running (m, l, O) of every column, and are joined in
-// order at the end. K and V go straight from memory to the operand registers, the
-// next step's under the present one's products, and the score layout is already
+// sequence; columns as in the bf16 kernel). The wavefronts take the steps of 16
+// keys in turn, each with its own running (m, l, O) of every column, and are joined
+// in order at the end. K and V go straight from memory to the operand registers: the
+// next step's K once the scores are taken, its V once the output products are, each
+// under the other's products. The score layout is already
 // that of the P operand (v_mfma_f32_16x16x4_f32: 16 keys x 16 columns take D
 // products, 32 cycles each: the fp32 matrix rate bounds it).
 template <int D, int NT>
-__global__ void __launch_bounds__(kPfWaves* kWave, 2) prefill_packed_f32_kernel(PackedPrefillF32 a) {
-    constexpr int kV = D / 16, kBM = 16 * NT;
-    typedef PackedStepF32<D> Step;
+__global__ void __launch_bounds__(kPfWaves* kWave, D == 64 && NT == 1 ? 3 : 2) prefill_packed_f32_kernel(PackedPrefillF32 a) {
+    constexpr int kV = D / 16, kBM = 16 * NT, kStep = 16;
     __shared__ struct {
         f32x4 o[kPfWaves - 1][NT][kV][kWave];
         float m[kPfWaves - 1][NT][kWave], l[kPfWaves - 1][NT][kWave];
@@ -602,20 +596,26 @@ __global__ void __launch_bounds__(kPfWaves* kWave, 2) prefill_packed_f32_kernel(
         for (int x = 0; x < kV; ++x) qr[tt][x] = *reinterpret_cast<const f32x4*>(qp + 16 * x);
     }
     const int kv_st = static_cast<int>(a.kv_st);
-    auto load = [&](int u, Step& x) __attribute__((always_inline)) {
-        const int last = len - 1 - 16 * u;                    // rows past the end read the last one
-        const float* kr = kb + static_cast<int64_t>(16 * u) * a.kv_st;
-        const float* vr = vb + static_cast<int64_t>(16 * u) * a.kv_st;
-        const uint32_t ka = static_cast<uint32_t>((c16 < last ? c16 : last) * kv_st + 4 * grp);
+    f32x4 kr[kV];                    // key c16, dims 16 c + 4 grp .. +3
+    float vr[4][kV];                 // key 4 grp + i, dims kV c16 ..
+    auto load_k = [&](int u) __attribute__((always_inline)) {
+        const int last = len - 1 - kStep * u;                 // rows past the end read the last one
+        const float* p = kb + static_cast<int64_t>(kStep * u) * a.kv_st;
+        const uint32_t at = static_cast<uint32_t>((c16 < last ? c16 : last) * kv_st + 4 * grp);
 #pragma unroll
-        for (int e = 0; e < kV; ++e) x.k[e] = *reinterpret_cast<const f32x4*>(kr + ka + 16 * e);
+        for (int e = 0; e < kV; ++e) kr[e] = *reinterpret_cast<const f32x4*>(p + at + 16 * e);
+    };
+    auto load_v = [&](int u) __attribute__((always_inline)) {
+        const int last = len - 1 - kStep * u;
+        const float* p = vb + static_cast<int64_t>(kStep * u) * a.kv_st;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t va = static_cast<uint32_t>((4 * grp + i < last ? 4 * grp + i : last) * kv_st + kV * c16);
+            const int key = 4 * grp + i;
+            const uint32_t at = static_cast<uint32_t>((key < last ? key : last) * kv_st + kV * c16);
 #pragma unroll
             for (int j = 0; j < kV; j += 4) {
-                const f32x4 y = *reinterpret_cast<const f32x4*>(vr + va + j);
-                x.v[i][j] = y[0]; x.v[i][j + 1] = y[1]; x.v[i][j + 2] = y[2]; x.v[i][j + 3] = y[3];
+                const f32x4 y = *reinterpret_cast<const f32x4*>(p + at + j);
+                vr[i][j] = y[0]; vr[i][j + 1] = y[1]; vr[i][j + 2] = y[2]; vr[i][j + 3] = y[3];
             }
         }
     };
@@ -630,28 +630,28 @@ __global__ void __launch_bounds__(kPfWaves* kWave, 2) prefill_packed_f32_kernel(
         for (int j = 0; j < kV; ++j) o[tt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     bool odd = false;                                         // V not finite at a place that some column may not attend
-    auto compute = [&](int u, Step& x) __attribute__((always_inline)) {
-        const int key0 = 16 * u;
-        const bool edge = a.causal ? key0 + 15 > w_first : key0 + 16 > len;
-        // kC short sums a score: no product waits for the one before, and the roundings are smaller
-        constexpr int kC = NT == 1 ? 4 : 2;
-        f32x4 s[NT], sc[NT][kC];
+    const int steps = (w_end + kStep - 1) / kStep;
+    if (wave < steps) {
+        load_k(wave);
+        load_v(wave);
+    }
+    for (int u = wave; u < steps; u += kPfWaves) {            // wave-uniform
+        const int key0 = kStep * u, next = u + kPfWaves < steps ? u + kPfWaves : u;
+        const bool edge = a.causal ? key0 + kStep - 1 > w_first : key0 + kStep > len;
+        // two short sums a score: fewer products that wait for the one before, and smaller roundings
+        f32x4 s[NT], s2[NT];
 #pragma unroll
-        for (int tt = 0; tt < NT; ++tt)
-#pragma unroll
-            for (int c = 0; c < kC; ++c) sc[tt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int tt = 0; tt < NT; ++tt) s[tt] = s2[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < kV; ++e)
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
+            for (int y = 0; y < 4; y += 2)
 #pragma unroll
-                for (int tt = 0; tt < NT; ++tt)
-                    sc[tt][y % kC] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[e][y], qr[tt][e][y], sc[tt][y % kC], 0, 0, 0);
-#pragma unroll
-        for (int tt = 0; tt < NT; ++tt) {
-            s[tt] = sc[tt][0] + sc[tt][1];
-            if constexpr (kC == 4) s[tt] += sc[tt][2] + sc[tt][3];
-        }
+                for (int tt = 0; tt < NT; ++tt) {
+                    s[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[e][y], qr[tt][e][y], s[tt], 0, 0, 0);
+                    s2[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[e][y + 1], qr[tt][e][y + 1], s2[tt], 0, 0, 0);
+                }
+        load_k(next);                                         // (the last step: its own again)
         if (edge) {
             // (a weight of 0 times inf is NaN: such values are cleared here, and added at the end to the columns
             // that do attend them)
@@ -659,40 +659,41 @@ __global__ void __launch_bounds__(kPfWaves* kWave, 2) prefill_packed_f32_kernel(
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < kV; ++j) vm = __builtin_elementwise_maximum(vm, __builtin_fabsf(x.v[i][j]));
+                for (int j = 0; j < kV; ++j) vm = __builtin_elementwise_maximum(vm, __builtin_fabsf(vr[i][j]));
             if (__ballot(!(vm < __builtin_inff())) != 0) {
                 odd = true;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < kV; ++j) x.v[i][j] = __builtin_fabsf(x.v[i][j]) < __builtin_inff() ? x.v[i][j] : 0.0f;
+                    for (int j = 0; j < kV; ++j)
+                        vr[i][j] = __builtin_fabsf(vr[i][j]) < __builtin_inff() ? vr[i][j] : 0.0f;
             }
         }
 #pragma unroll
         for (int tt = 0; tt < NT; ++tt) {
+            const int left = lim[tt] - key0 - 4 * grp;        // this lane's keys up to it are allowed
             float mx = m[tt];
+            s[tt] += s2[tt];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float y = s[tt][i] * a.scale_log2;
-                mx = fmaxf(mx, edge && key0 + 4 * grp + i > lim[tt] ? -__builtin_inff() : y);
-            }
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, i <= left ? s[tt][i] * a.scale_log2 : -__builtin_inff());
             float2 r2 = rows16_swap(mx);
             mx = fmaxf(r2.x, r2.y);
             r2 = rows32_swap(mx);
             mx = fmaxf(r2.x, r2.y);
             const float ref = mx == -__builtin_inff() ? 0.0f : mx;
             const float alpha = __builtin_amdgcn_exp2f(m[tt] - ref);
+            if (__ballot(mx != m[tt]) != 0) {                 // wave-uniform: some column's maximum rose
+#pragma unroll
+                for (int j = 0; j < kV; ++j) o[tt][j] *= alpha;
+                l[tt] *= alpha;
+            }
             m[tt] = mx;
-            l[tt] *= alpha;
             // one rounding between a score and its distance from the reference, which is small where the weight is not
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                s[tt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, -ref));
-                if (edge && key0 + 4 * grp + i > lim[tt]) s[tt][i] = 0.0f;
+                s[tt][i] = i <= left ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, -ref)) : 0.0f;
                 l[tt] += s[tt][i];
             }
-#pragma unroll
-            for (int j = 0; j < kV; ++j) o[tt][j] *= alpha;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -700,24 +701,8 @@ __global__ void __launch_bounds__(kPfWaves* kWave, 2) prefill_packed_f32_kernel(
             for (int j = 0; j < kV; ++j)
 #pragma unroll
                 for (int tt = 0; tt < NT; ++tt)
-                    o[tt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[i][j], s[tt][i], o[tt][j], 0, 0, 0);
-    };
-
-    const int steps = (w_end + 15) / 16;
-    int u = wave;
-    if (u < steps) {
-        Step x, y;
-        load(u, x);
-        while (true) {                                        // wave-uniform
-            if (u + kPfWaves < steps) load(u + kPfWaves, y);
-            compute(u, x);
-            u += kPfWaves;
-            if (u >= steps) break;
-            if (u + kPfWaves < steps) load(u + kPfWaves, x);
-            compute(u, y);
-            u += kPfWaves;
-            if (u >= steps) break;
-        }
+                    o[tt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[i][j], s[tt][i], o[tt][j], 0, 0, 0);
+        load_v(next);
     }
 #pragma unroll
     for (int tt = 0; tt < NT; ++tt) l[tt] = pair32_sum(pair16_sum(l[tt]));
@@ -755,13 +740,13 @@ __global__ void __launch_bounds__(kPfWaves* kWave, 2) prefill_packed_f32_kernel(
     }
     if ((sm.odd[0] | sm.odd[1] | sm.odd[2] | sm.odd[3]) != 0) {
         // the values cleared above: a positive weight times inf or NaN is that value
-        for (int key = (a.causal ? w_first : len) / 16 * 16; key < w_end; ++key) {
-            const float* vr = vb + static_cast<int64_t>(key) * a.kv_st + 4 * kV * grp;
+        for (int key = (a.causal ? w_first : len) / kStep * kStep; key < w_end; ++key) {
+            const float* vp = vb + static_cast<int64_t>(key) * a.kv_st + 4 * kV * grp;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < kV; ++j) {
-                    const float f = vr[kV * i + j];
+                    const float f = vp[kV * i + j];
 #pragma unroll
                     for (int tt = 0; tt < NT; ++tt)
                         if (!(__builtin_fabsf(f) < __builtin_inff()) && key <= lim[tt]) o[tt][j][i] += f;
@@ -815,12 +800,11 @@ int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void*
         hipLaunchKernelGGL((prefill_packed_f32_kernel<D_, NT_>), dim3(static_cast<unsigned>(a.slots * Hkv)),      \
                            dim3(kPfWaves * kWave), 0, stream, a);                                                 \
     } while (0)
-        // wider windows read K and V for more columns, narrow ones are more workgroups:
-        // us of 16 / 48 columns, 12/4 heads of 64: N=512 12.9 / 21.2, 3 x 500 24.8 / 36.5,
-        // N=1501 54.9 / 62.8, N=4000 294 / 238
+        // wider windows read K and V for more columns, narrow ones are more workgroups: us of 16 / 32
+        // columns, 12/4 heads of 64: N=512 12.7 / 16.2, 3 x 500 25.4 / 26.7, N=1501 47.6 / 52.8, N=4000 232 / 225
         if (D == 128) SPARDA_PKF(128, 1);
         else if (N * Hq <= 2048 * 16) SPARDA_PKF(64, 1);
-        else SPARDA_PKF(64, 3);
+        else SPARDA_PKF(64, 2);
 #undef SPARDA_PKF
         return check_hip(hipGetLastError(), "prefill_packed_f32_kernel");
     }
