@@ -252,3 +252,50 @@ def test_packed_captured_and_replayed_with_other_offsets(dtype):
         eager = sparda.prefill_packed(qd, kd, vd, cud)
         assert torch.equal(out, eager)
         check(out, q, k, v, np.array(cu), rows=range(0, N, 23))
+
+
+# sizes on either side of the limits at which the work is cut differently
+CUTS = [(BF, 12, 4, 64, [500]), (BF, 12, 4, 64, [2000]), (BF, 12, 4, 64, [4200]), (BF, 12, 4, 64, [700] * 8),
+        (BF, 12, 4, 64, [9000, 13001]), (BF, 16, 16, 64, [1500, 600]), (BF, 32, 8, 128, [400]), (BF, 8, 2, 128, [4300]),
+        (BF, 32, 8, 128, [150] * 10), (BF, 32, 8, 128, [3000, 2000]), (F32, 12, 4, 64, [3000]), (F32, 8, 1, 128, [1000, 700])]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,Hq,Hkv,D,lengths", CUTS, ids=str)
+def test_packed_prompts_at_every_cut_of_the_work(dtype, Hq, Hkv, D, lengths, causal):
+    """Ordinary values; keys that rise far above the first ones; one value that is
+    not finite: sampled rows against float64, and every row for where it shows."""
+    print(f"[case] packed cut {dtype} {Hq}/{Hkv}x{D} {lengths} causal={causal}", flush=True)
+    cu = offsets(lengths)
+    N = int(cu[-1])
+    cud = torch.from_numpy(cu).to(DEV)
+    q, k, v = inputs(N, Hq, Hkv, D, dtype, seed=N, std=2.0)
+    rows = sorted({int(c) + d for c in cu for d in (-2, -1, 0, 1, 31, 32, 63, 64) if 0 <= c + d < N}
+                  | {int(x) for x in np.random.default_rng(N).integers(0, N, 12)})
+    qd, vd = q.to(DEV), v.to(DEV)
+    clean = sparda.prefill_packed(qd, k.to(DEV), vd, cud, causal=causal)
+    check(clean, q, k, v, cu, causal, rows=rows)
+    high = k.clone()
+    high[N // 3::5] *= 15
+    check(sparda.prefill_packed(qd, high.to(DEV), vd, cud, causal=causal), q, high, v, cu, causal, rows=rows)
+    last = len(lengths) - 1
+    a, b = int(cu[last]), int(cu[last + 1])
+    for at in (a, a + (b - a) // 2 + 1, b - 1):
+        v2 = v.clone()
+        v2[at, Hkv - 1, 5] = float("inf")
+        got = sparda.prefill_packed(qd, k.to(DEV), v2.to(DEV), cud, causal=causal).view(N, Hq, D)
+        hit = torch.zeros(N, Hq, D, dtype=torch.bool)
+        hit[(at if causal else a):b, Hq - Hq // Hkv:, 5] = True
+        assert torch.equal(~torch.isfinite(got).cpu(), hit)
+        torch.testing.assert_close(got.cpu()[~hit].float(), clean.cpu().view(N, Hq, D)[~hit].float(), rtol=0, atol=0)
+
+
+def test_packed_more_sequences_than_lanes_and_long_ones():
+    print("[case] packed 130 sequences of up to 700", flush=True)
+    r = np.random.default_rng(7)
+    lengths = np.where(r.random(130) < 0.1, r.integers(300, 700, 130), r.integers(0, 40, 130))
+    cu = offsets(lengths)
+    N = int(cu[-1])
+    q, k, v = inputs(N, 12, 4, 64, BF, seed=3)
+    got = sparda.prefill_packed(q.to(DEV), k.to(DEV), v.to(DEV), torch.from_numpy(cu).to(DEV))
+    check(got, q, k, v, cu, rows=range(0, N, 17))
