@@ -362,11 +362,7 @@ __global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : DT == SPARDA_F32
         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) mx = fmaxf(mx, 16 * t + i < left ? s[t][i] * a.scale_log2 : -__builtin_inff());
-        // (builtin swaps: both lanes of a pair see the same two values)
-        float2 r2 = rows16_swap(mx);
-        mx = fmaxf(r2.x, r2.y);
-        r2 = rows32_swap(mx);
-        mx = fmaxf(r2.x, r2.y);
+        mx = pair32_max(pair16_max(mx));
         const float ref = mx == -__builtin_inff() ? 0.0f : mx;
         const float alpha = __builtin_amdgcn_exp2f(m - ref);
         m = mx;
@@ -526,6 +522,7 @@ __global__ void __launch_bounds__(kPgJoin) decode_paged_join_kernel(PagedDecode 
         }
         for (; i < n; i += kG) O = __builtin_fmaf(wts[i], po[(c0 + i) * st], O);
     }
+    asm volatile("s_nop 1" : "+v"(L));  // the wait states of the reduction's first DPP, on every way out of the loop
     L = wave_sum(L);
     if (tid % kWave == 0) rl[wave] = L;
     red[tid] = O;

@@ -100,6 +100,13 @@ struct PackedMerge {
 template <int N, int CW, int NT>
 struct PackedMerge<N, CW, NT, 1> {};
 
+// A barrier behind loads to LDS: they are counted by vmcnt, and the barrier itself
+// does not wait for a wavefront's own.
+__device__ __forceinline__ void staged_barrier() {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), the other counters at their maximum
+    __syncthreads();
+}
+
 struct PackedPrefill {
     const uint16_t* q;
     int64_t q_st, q_sh;
@@ -222,10 +229,7 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
             }
         }
 #pragma unroll
-        for (int tt = 0; tt < NT; ++tt) {
-            const float2 r2 = rows32_swap(ref[tt]);
-            ref[tt] = fmaxf(r2.x, r2.y);
-        }
+        for (int tt = 0; tt < NT; ++tt) ref[tt] = pair32_max(ref[tt]);
     };
 
     f32x16 o[NT][kDT];
@@ -433,12 +437,12 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
         if (kg < nblk) stage(kg, 0);
         take_refs(pass == 0 && w_end > 32 ? 32 : w_end);
         clear();
-        __syncthreads();
+        staged_barrier();
         int i = 0;
         for (; i < whole; ++i) {
             const int j = i * KG + kg;
             compute_block(i & 1, j + KG < nblk ? j + KG : j);  // (no next one: a block that nobody reads)
-            __syncthreads();
+            staged_barrier();
         }
         for (; i < steps; ++i) {
             const int buf = i & 1, j = i * KG + kg, key0 = j * KB;
@@ -446,7 +450,7 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
 #pragma unroll 1
             for (int hh = 0; hh < kHalves; ++hh)
                 if (key0 + 32 * hh < w_end) compute(buf, hh, key0 + 32 * hh);
-            __syncthreads();
+            staged_barrier();
         }
         if (pass == 1) break;
         bool over = false;
@@ -676,10 +680,7 @@ __global__ void __launch_bounds__(kPfWaves* kWave, D == 64 && NT == 1 ? 3 : 2) p
             s[tt] += s2[tt];
 #pragma unroll
             for (int i = 0; i < 4; ++i) mx = fmaxf(mx, i <= left ? s[tt][i] * a.scale_log2 : -__builtin_inff());
-            float2 r2 = rows16_swap(mx);
-            mx = fmaxf(r2.x, r2.y);
-            r2 = rows32_swap(mx);
-            mx = fmaxf(r2.x, r2.y);
+            mx = pair32_max(pair16_max(mx));
             const float ref = mx == -__builtin_inff() ? 0.0f : mx;
             const float alpha = __builtin_amdgcn_exp2f(m[tt] - ref);
             if (__ballot(mx != m[tt]) != 0) {                 // wave-uniform: some column's maximum rose
