@@ -41,6 +41,11 @@ append_paged_kernel(char* __restrict__ k, char* __restrict__ v, Pages pg, int ps
     if (cu == nullptr) {
         seq = static_cast<int>(t);
     } else {
+        if (t == 0) {                             // the first row's wavefront looks at every pair of offsets
+            bool wrong = false;
+            for (int i = lane; i < n; i += kWave) wrong = wrong || cu[i] < 0 || cu[i + 1] < cu[i] || cu[i + 1] > N;
+            if (__ballot(wrong) != 0 && lane == 0) atomicOr(status, static_cast<uint32_t>(SPARDA_STATUS_SEQUENCE_RANGE));
+        }
         // the last sequence that starts at or before t, when t is one of its rows
         for (int i0 = 0; i0 < n; i0 += kWave) {
             const int i = i0 + lane;

@@ -1232,7 +1232,7 @@ def append_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch
     k_new/v_new [N,Hkv,D] are packed, and row j of sequence b goes to
     positions[b] + j. A sequence with a negative position takes no part; a row
     whose page is missing or outside the cache is dropped and status() has
-    STATUS_PAGE_RANGE.
+    STATUS_PAGE_RANGE (STATUS_SEQUENCE_RANGE for offsets that fall or leave [0, N]).
     """
     r = _host.append_paged(k_pages, v_pages, page_table, positions, k_new, v_new, cu_seqlens)
     if r is not None:

@@ -235,6 +235,18 @@ def test_append_rows_without_a_page_are_dropped():
         assert torch.equal(kp[:, :, 0, 0].float().cpu(), want) and torch.equal(vp[:, :, 0, 0].float().cpu(), want)
 
 
+@pytest.mark.parametrize("cu", [[0, 3, 9], [0, 5, 2], [-1, 2, 4]], ids=str)
+def test_append_offsets_out_of_range_raise_the_status(cu):
+    print(f"[case] append offsets {cu}", flush=True)
+    kp, vp = torch.zeros(4, 16, 1, 64, dtype=BF, device=DEV), torch.zeros(4, 16, 1, 64, dtype=BF, device=DEV)
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=DEV)
+    kn = torch.ones(6, 1, 64, dtype=BF, device=DEV)
+    sparda.status()
+    sparda.append_paged(kp, vp, table, torch.zeros(2, dtype=torch.int32, device=DEV), kn, kn,
+                        cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=DEV))
+    assert sparda.status() & sparda.STATUS_SEQUENCE_RANGE
+
+
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
 def test_paged_decode_captured_and_replayed(dtype):
     # two graphs, each with its own workspace, replayed in turn as lengths and tables change
@@ -339,3 +351,113 @@ def test_a_server_prefills_and_decodes(dtype, Hq, Hkv, D):
     for _ in range(3):
         step([0, 2, 3])
     assert sparda.status() == 0
+
+
+_FIRST_CALLS_CAPTURED = r"""
+import sys
+sys.path[:0] = sys.argv[1:3]
+import torch
+import sparda
+t = lambda *s: torch.randn(*s, device="cuda").to(torch.bfloat16)
+i = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+q, k, v, cu = t(40, 6, 64), t(40, 2, 64), t(40, 2, 64), i(0, 25, 40)
+kp, vp, table, zero, n = t(8, 16, 2, 64), t(8, 16, 2, 64), i(3, 1, 5, 2).view(2, 2), i(0, 0), i(25, 15)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    a = sparda.prefill_packed(q, k, v, cu)
+    sparda.append_paged(kp, vp, table, zero, k, v, cu_seqlens=cu)
+    b = sparda.decode_paged(q[:2], kp, vp, table, n)
+for _ in range(3):
+    a.zero_(), b.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(a, sparda.prefill_packed(q, k, v, cu))
+    assert torch.equal(b, sparda.decode_paged(q[:2], kp, vp, table, n))
+assert sparda.status() == 0
+print("CAPTURED", flush=True)
+"""
+
+
+def test_first_calls_of_a_process_can_be_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    pkg = os.path.join(root, "local-research-small-language-model_amd")
+    print("[case] first calls in a capture, fresh process", flush=True)
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALLS_CAPTURED, root, pkg], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "CAPTURED" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
+
+
+def test_operators_on_a_side_stream_and_without_the_native_host_path():
+    print("[case] paged and packed on a side stream, through Python", flush=True)
+    from sparda import ops
+    g = torch.Generator().manual_seed(5)
+    q, k, v = (torch.randn(90, h, 64, generator=g).to(BF).to(DEV) for h in (6, 2, 2))
+    cu = torch.tensor([0, 33, 90], dtype=torch.int32, device=DEV)
+    table = torch.tensor([[1, 7, 3, -1], [0, 2, 4, 6]], dtype=torch.int32, device=DEV)
+    zero, n = torch.zeros(2, dtype=torch.int32, device=DEV), torch.tensor([33, 57], dtype=torch.int32, device=DEV)
+
+    def all_three():
+        kp, vp = torch.zeros(8, 16, 2, 64, dtype=BF, device=DEV), torch.zeros(8, 16, 2, 64, dtype=BF, device=DEV)
+        a = sparda.prefill_packed(q, k, v, cu)
+        sparda.append_paged(kp, vp, table, zero, k, v, cu_seqlens=cu)
+        return a, kp, vp, sparda.decode_paged(q[:2], kp, vp, table, n)
+
+    want = all_three()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = all_three()
+    side.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+    class Off:
+        def __getattr__(self, name):
+            return lambda *args: None
+
+    host, ops._host = ops._host, Off()
+    try:
+        got = all_three()
+    finally:
+        ops._host = host
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_refusals_of_tensors_that_do_not_fit():
+    q, kv = torch.zeros(4, 2, 64, dtype=BF, device=DEV), torch.zeros(4, 1, 64, dtype=BF, device=DEV)
+    pages, table = torch.zeros(3, 16, 1, 64, dtype=BF, device=DEV), torch.zeros(4, 1, dtype=torch.int32, device=DEV)
+    n = torch.zeros(4, dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 4], dtype=torch.int32, device=DEV)
+    for exc, call in [
+            (TypeError, lambda: sparda.prefill_packed(q, kv.float(), kv, cu)),
+            (TypeError, lambda: sparda.prefill_packed(q, kv, kv, cu.long())),
+            (TypeError, lambda: sparda.prefill_packed(q.half(), kv.half(), kv.half(), cu)),
+            (ValueError, lambda: sparda.prefill_packed(q, kv[:3], kv[:3], cu)),
+            (ValueError, lambda: sparda.prefill_packed(q, kv, kv, cu.view(1, 2))),
+            (ValueError, lambda: sparda.prefill_packed(q, kv, kv, cu, out=torch.zeros(4, 64, dtype=BF, device=DEV))),
+            (ValueError, lambda: sparda.prefill_packed(torch.zeros(4, 3, 64, dtype=BF, device=DEV),
+                                                       torch.zeros(4, 2, 64, dtype=BF, device=DEV),
+                                                       torch.zeros(4, 2, 64, dtype=BF, device=DEV), cu)),
+            (TypeError, lambda: sparda.append_paged(pages, pages, table, n, kv.float(), kv.float())),
+            (TypeError, lambda: sparda.append_paged(pages, pages, table.long(), n, kv, kv)),
+            (ValueError, lambda: sparda.append_paged(pages, pages, table, n[:3], kv, kv)),
+            (ValueError, lambda: sparda.append_paged(pages, pages, table, n, kv[:3], kv[:3])),
+            (ValueError, lambda: sparda.append_paged(pages, pages, table, n, kv, kv, cu_seqlens=cu)),
+            (ValueError, lambda: sparda.append_paged(pages, pages.transpose(1, 2), table, n, kv, kv)),
+            (ValueError, lambda: sparda.append_paged(pages[:, :8], pages[:, :8], table, n, kv, kv)),
+            (TypeError, lambda: sparda.decode_paged(q.float(), pages, pages, table, n)),
+            (TypeError, lambda: sparda.decode_paged(q, pages, pages, table, n.long())),
+            (ValueError, lambda: sparda.decode_paged(q[:3], pages, pages, table, n)),
+            (ValueError, lambda: sparda.decode_paged(q, pages, pages, table[:, :0], n)),
+            (ValueError, lambda: sparda.decode_paged(q, pages, pages, table, n[:2]))]:
+        with pytest.raises(exc):
+            call()
+    grad = q.clone().requires_grad_(True)
+    for call in (lambda: sparda.prefill_packed(grad, kv, kv, cu), lambda: sparda.decode_paged(grad, pages, pages, table, n)):
+        with pytest.raises(RuntimeError, match="inference-only"):
+            call()
+    with torch.no_grad():
+        assert sparda.decode_paged(grad, pages, pages, table, n).shape == (4, 128)
