@@ -494,6 +494,9 @@ PyObject* teacher_mass(PyObject* const* a) {
                   out);
 }
 
+// rows of 16-byte pieces
+inline bool rows16(const at::Tensor& t) { return aligned(t, 16) && strides_of(t, 16 / t.element_size()); }
+
 // prefill_packed(q, k, v, cu_seqlens, causal, scale)
 PyObject* prefill_packed(PyObject* const* a) {
     Args x;
@@ -504,7 +507,7 @@ PyObject* prefill_packed(PyObject* const* a) {
     const int causal = as_bool(a[4]);
     const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2);
     need(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type() && same_strides(k, v));
-    need(k.sizes() == v.sizes() && k.size(0) == N && k.size(2) == D && N > 0);
+    need(k.sizes() == v.sizes() && k.size(0) == N && k.size(2) == D && N > 0 && rows16(q) && rows16(k) && rows16(v));
     need(cu.scalar_type() == at::kInt && cu.numel() > 1 && cu.stride(0) == 1);
     const float scale = scale_or(a[5], D);
     x.on_current();
@@ -525,9 +528,6 @@ struct PagesArg {
         need(table.scalar_type() == at::kInt && B > 0 && (width == 1 || table.stride(1) == 1));
     }
 };
-// rows of 16-byte pieces
-inline bool rows16(const at::Tensor& t) { return aligned(t, 16) && strides_of(t, 16 / t.element_size()); }
-
 // append_paged(k_pages, v_pages, page_table, positions, k_new, v_new, cu_seqlens): an int (its status), or None
 PyObject* append_paged(PyObject* const* a) {
     Args x;

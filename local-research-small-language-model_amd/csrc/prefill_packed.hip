@@ -69,7 +69,7 @@ prefill_packed_general_kernel(const void* __restrict__ q, int64_t q_st, int64_t 
 }
 
 // ---------------------------------------------------------------------------
-// bf16, D = 64 and 128, on the matrix cores
+// bf16, D = 32, 64 and 128, on the matrix cores
 // ---------------------------------------------------------------------------
 
 namespace {
@@ -83,7 +83,8 @@ constexpr float kPkGuard = 18446744073709551616.0f;  // 2^64
 // 4 consecutive rows at 4 consecutive pieces (V, transposed) do too.
 template <int D>
 __device__ __forceinline__ int pk_piece(int r, int c) {
-    if constexpr (D == 64) return c ^ ((r >> 1 & 1) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1));
+    if constexpr (D == 32) return c ^ (r >> 2 & 3);
+    else if constexpr (D == 64) return c ^ ((r >> 1 & 1) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1));
     else return c ^ ((r & 3) << 2 | (r >> 2 & 3));
 }
 
@@ -777,7 +778,7 @@ static bool packed_matrix_cores(const void* q, int64_t q_st, int64_t q_sh, const
                                 int64_t out_st) {
     const int64_t ve = dtype == SPARDA_F32 ? 4 : 8;
     auto al16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    return (D == 64 || D == 128) && N * R < (int64_t(1) << 31) - 256 && al16(q) && al16(k) && al16(v) && al16(out) &&
+    return (D == 64 || D == 128 || (D == 32 && dtype == SPARDA_BF16)) && N * R < (int64_t(1) << 31) - 256 && al16(q) && al16(k) && al16(v) && al16(out) &&
            q_st % ve == 0 && q_sh % ve == 0 && kv_st >= 0 && kv_st < (1 << 24) && kv_st % ve == 0 && kv_sh % ve == 0 &&
            out_st % ve == 0;
 }
@@ -834,7 +835,9 @@ int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void*
         //   32/8: N=512 14.7 / 15.9 / 12.4   N=1000 23.2 / 22.9 / 22.2   N=2048 50.5 / 51.3 / 56.2
         //   8 x 250 21.7 / 31.9 / 25.9   8 x 2000 385 / 459 / 507   8/1: N=8192 169 / 149 / 164
         const int64_t W = cdiv(N * Hq, 128), NB = cdiv(cdiv(N, n), 64), cus = 256;
-        if (D == 64) {
+        if (D == 32) {
+            SPARDA_PKM(32, 1, 4, 1, 64);
+        } else if (D == 64) {
             if (2 * W <= cus) SPARDA_PKM(64, 1, 1, 4, 32);
             else if (W <= cus && NB >= 8) SPARDA_PKM(64, 1, 2, 2, 64);
             else if (W <= 2 * cus && NB >= 16) SPARDA_PKM(64, 1, 4, 2, 64);

@@ -1192,7 +1192,7 @@ def prefill_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
     cu = _int32_array(cu_seqlens, 1, "cu_seqlens")
     if cu.numel() < 1:
         raise ValueError("sparda: cu_seqlens holds one offset more than there are sequences")
-    q, k, v = _rowmajor(q), _rowmajor(k), _rowmajor(v)
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
     if k.stride() != v.stride():
         k, v = k.contiguous(), v.contiguous()
     N, Hq, D = q.shape

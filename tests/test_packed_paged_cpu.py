@@ -60,7 +60,8 @@ def decode(q=P, q_sb=768, q_sh=64, k=P, v=P, dtype=1, pages=10, ps=64, p_st=1638
     (-1, dict(q=None)), (-1, dict(k=None)), (-1, dict(v=None)), (-1, dict(table=None)), (-1, dict(lens=None)),
     (-1, dict(out=None)), (-2, dict(B=0)), (-2, dict(B=1 << 17)), (-2, dict(Hq=14)), (-2, dict(Hq=0)),
     (-2, dict(B=65535, width=1 << 24)), (-5, dict(q=P + 4)), (-5, dict(q_sb=764)), (-5, dict(q_sh=60)),
-    (-5, dict(out_sb=700)), (-4, dict(ws=None)), (-4, dict(nbytes=16)), (-4, dict(ws=P + 8))], ids=str)
+    (-5, dict(out_sb=700)), (-4, dict(ws=None, width=64)), (-4, dict(nbytes=16, width=64)),
+    (-4, dict(ws=P + 8, width=64))], ids=str)
 def test_decode_paged_argument_errors(code, bad):
     _expect(code, "sparda_decode_paged", *decode(**bad))
 
