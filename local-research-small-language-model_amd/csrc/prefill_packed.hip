@@ -16,7 +16,9 @@ constexpr float kPkLog2e = 1.4426950408889634f;
 
 // One wavefront per (row, query head): lane j takes key j of 64 at a time, the
 // running maximum and sum are the wave's, and each lane then holds dims lane and
-// lane + 64 of the output. Any head dim up to 128, any strides.
+// lane + 64 of the output. Any head dim up to 128, any strides: heads of 16, and
+// rows that no 16-byte load can reach. Bound by its own loads, a lane reading a K row
+// of its own.
 template <int DT>
 __global__ void __launch_bounds__(256)
 prefill_packed_general_kernel(const void* __restrict__ q, int64_t q_st, int64_t q_sh, const void* __restrict__ k,
@@ -532,17 +534,17 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
 }
 
 // ---------------------------------------------------------------------------
-// fp32, D = 64 and 128, on the matrix cores
+// keys straight from memory: fp32, and bf16 where sequences are short
 // ---------------------------------------------------------------------------
 
 namespace {
 
-constexpr int kPfWaves = 4;
+constexpr int kPdWaves = 4;
 
-struct PackedPrefillF32 {
-    const float* q;
+struct PackedDirect {
+    const void* q;
     int64_t q_st, q_sh;
-    const float *k, *v;
+    const void *k, *v;
     int64_t kv_st, kv_sh;
     const int32_t* cu;
     int n;
@@ -550,28 +552,52 @@ struct PackedPrefillF32 {
     int Hkv, R, causal;
     int64_t slots;
     float scale_log2;
-    float* out;
+    void* out;
     int64_t out_st;
     uint32_t* status;
 };
 
+template <int DT>
+struct PackedElem {
+    typedef float E;
+    static constexpr int kTiles = 1;   // 16-key tiles of a step
+};
+template <>
+struct PackedElem<SPARDA_BF16> {
+    typedef short E;
+    static constexpr int kTiles = 2;
+};
+
+__device__ __forceinline__ bool packed_odd(float x) { return !(__builtin_fabsf(x) < __builtin_inff()); }
+__device__ __forceinline__ bool packed_odd(short x) { return (x & 0x7f80) == 0x7f80; }
+__device__ __forceinline__ float packed_f32(float x) { return x; }
+__device__ __forceinline__ float packed_f32(short x) { return bf16_to_f32(static_cast<uint16_t>(x)); }
+__device__ __forceinline__ void packed_put(float& o, float x) { o = x; }
+__device__ __forceinline__ void packed_put(short& o, float x) { o = __builtin_bit_cast(short, static_cast<__bf16>(x)); }
+
 }  // namespace
 
 // One workgroup of 4 wavefronts per (KV head, window of 16 NT columns of one
-// sequence; columns as in the bf16 kernel). The wavefronts take the steps of 16
-// keys in turn, each with its own running (m, l, O) of every column, and are joined
-// in order at the end. K and V go straight from memory to the operand registers: the
-// next step's K once the scores are taken, its V once the output products are, each
-// under the other's products. The score layout is already
-// that of the P operand (v_mfma_f32_16x16x4_f32: 16 keys x 16 columns take D
-// products, 32 cycles each: the fp32 matrix rate bounds it).
-template <int D, int NT>
-__global__ void __launch_bounds__(kPfWaves* kWave, D == 64 && NT == 1 ? 3 : 2) prefill_packed_f32_kernel(PackedPrefillF32 a) {
-    constexpr int kV = D / 16, kBM = 16 * NT, kStep = 16;
+// sequence; columns as in the staged kernel). The wavefronts take the steps of 16 keys
+// (bf16: 32) in turn, each with its own running (m, l, O) of every column, and are
+// joined in order at the end: a walk is four times shorter and knows no barrier. K
+// and V go straight from memory to the operand registers: the next step's K once
+// the scores are taken, its V once the output products are, each under the other's
+// products. The score layout of v_mfma_f32_16x16x4_f32 / 16x16x32_bf16 is already that
+// of the P operand. Bound in fp32 by the matrix rate (16 keys x 16 columns take D / 2
+// products of 32 cycles), in bf16 by the loads, K and V being read once for every
+// 16 NT columns: hence for short sequences alone.
+template <int DT, int D, int NT>
+__global__ void __launch_bounds__(kPdWaves* kWave, 2) prefill_packed_direct_kernel(PackedDirect a) {
+    typedef typename PackedElem<DT>::E E;
+    constexpr bool kF32 = DT == SPARDA_F32;
+    constexpr int kTiles = PackedElem<DT>::kTiles, kStep = 16 * kTiles, kBM = 16 * NT;
+    constexpr int kV = D / 16, kQ = kF32 ? D / 16 : D / 32, kPiece = kF32 ? 4 : 8;  // elements of V a lane holds per key, pieces of K, their elements
+    typedef E Row __attribute__((ext_vector_type(kV)));
     __shared__ struct {
-        f32x4 o[kPfWaves - 1][NT][kV][kWave];
-        float m[kPfWaves - 1][NT][kWave], l[kPfWaves - 1][NT][kWave];
-        int odd[kPfWaves];
+        f32x4 o[kPdWaves - 1][NT][kV][kWave];
+        float m[kPdWaves - 1][NT][kWave], l[kPdWaves - 1][NT][kWave];
+        int odd[kPdWaves];
     } sm;
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
@@ -585,44 +611,45 @@ __global__ void __launch_bounds__(kPfWaves* kWave, D == 64 && NT == 1 ? 3 : 2) p
     const int len = w.len, ncol = len * a.R, col0 = static_cast<int>(w.win) * kBM;
     const int w_first = col0 / a.R, w_last = (col0 + kBM <= ncol ? col0 + kBM - 1 : ncol - 1) / a.R;
     const int w_end = a.causal ? w_last + 1 : len;            // keys of the window
-    const float* kb = a.k + static_cast<int64_t>(w.row0) * a.kv_st + static_cast<int64_t>(g) * a.kv_sh;
-    const float* vb = a.v + static_cast<int64_t>(w.row0) * a.kv_st + static_cast<int64_t>(g) * a.kv_sh;
+    const E* kb = static_cast<const E*>(a.k) + static_cast<int64_t>(w.row0) * a.kv_st + static_cast<int64_t>(g) * a.kv_sh;
+    const E* vb = static_cast<const E*>(a.v) + static_cast<int64_t>(w.row0) * a.kv_st + static_cast<int64_t>(g) * a.kv_sh;
 
     int tok[NT], lim[NT];
-    f32x4 qr[NT][kV];
+    uint4 qr[NT][kQ];                // dims 4 kPiece x + kPiece grp ..
 #pragma unroll
     for (int tt = 0; tt < NT; ++tt) {
         const int c = col0 + 16 * tt + c16 < ncol ? col0 + 16 * tt + c16 : ncol - 1;
         tok[tt] = c / a.R;
         lim[tt] = a.causal ? tok[tt] : len - 1;
-        const float* qp = a.q + (w.row0 + static_cast<int64_t>(tok[tt])) * a.q_st +
-                          static_cast<int64_t>(g * a.R + c % a.R) * a.q_sh + 4 * grp;
+        const E* qp = static_cast<const E*>(a.q) + (w.row0 + static_cast<int64_t>(tok[tt])) * a.q_st +
+                      static_cast<int64_t>(g * a.R + c % a.R) * a.q_sh + kPiece * grp;
 #pragma unroll
-        for (int x = 0; x < kV; ++x) qr[tt][x] = *reinterpret_cast<const f32x4*>(qp + 16 * x);
+        for (int x = 0; x < kQ; ++x) qr[tt][x] = *reinterpret_cast<const uint4*>(qp + 4 * kPiece * x);
     }
     const int kv_st = static_cast<int>(a.kv_st);
-    f32x4 kr[kV];                    // key c16, dims 16 c + 4 grp .. +3
-    float vr[4][kV];                 // key 4 grp + i, dims kV c16 ..
+    uint4 kr[kTiles][kQ];            // key 16 t + c16, dims as q
+    Row vr[kTiles][4];               // key 16 t + 4 grp + i, dims kV c16 ..
     auto load_k = [&](int u) __attribute__((always_inline)) {
         const int last = len - 1 - kStep * u;                 // rows past the end read the last one
-        const float* p = kb + static_cast<int64_t>(kStep * u) * a.kv_st;
-        const uint32_t at = static_cast<uint32_t>((c16 < last ? c16 : last) * kv_st + 4 * grp);
+        const E* p = kb + static_cast<int64_t>(kStep * u) * a.kv_st;
 #pragma unroll
-        for (int e = 0; e < kV; ++e) kr[e] = *reinterpret_cast<const f32x4*>(p + at + 16 * e);
+        for (int t = 0; t < kTiles; ++t) {
+            const int key = 16 * t + c16;
+            const uint32_t at = static_cast<uint32_t>((key < last ? key : last) * kv_st + kPiece * grp);
+#pragma unroll
+            for (int x = 0; x < kQ; ++x) kr[t][x] = *reinterpret_cast<const uint4*>(p + at + 4 * kPiece * x);
+        }
     };
     auto load_v = [&](int u) __attribute__((always_inline)) {
         const int last = len - 1 - kStep * u;
-        const float* p = vb + static_cast<int64_t>(kStep * u) * a.kv_st;
+        const E* p = vb + static_cast<int64_t>(kStep * u) * a.kv_st;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int key = 4 * grp + i;
-            const uint32_t at = static_cast<uint32_t>((key < last ? key : last) * kv_st + kV * c16);
+        for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-            for (int j = 0; j < kV; j += 4) {
-                const f32x4 y = *reinterpret_cast<const f32x4*>(p + at + j);
-                vr[i][j] = y[0]; vr[i][j + 1] = y[1]; vr[i][j + 2] = y[2]; vr[i][j + 3] = y[3];
+            for (int i = 0; i < 4; ++i) {
+                const int key = 16 * t + 4 * grp + i;
+                vr[t][i] = *reinterpret_cast<const Row*>(p + static_cast<uint32_t>((key < last ? key : last) * kv_st + kV * c16));
             }
-        }
     };
 
     float m[NT], l[NT];                                       // log2 units; this lane's part of the sum
@@ -640,47 +667,70 @@ __global__ void __launch_bounds__(kPfWaves* kWave, D == 64 && NT == 1 ? 3 : 2) p
         load_k(wave);
         load_v(wave);
     }
-    for (int u = wave; u < steps; u += kPfWaves) {            // wave-uniform
-        const int key0 = kStep * u, next = u + kPfWaves < steps ? u + kPfWaves : u;
+    for (int u = wave; u < steps; u += kPdWaves) {            // wave-uniform
+        const int key0 = kStep * u, next = u + kPdWaves < steps ? u + kPdWaves : u;
         const bool edge = a.causal ? key0 + kStep - 1 > w_first : key0 + kStep > len;
-        // two short sums a score: fewer products that wait for the one before, and smaller roundings
-        f32x4 s[NT], s2[NT];
+        f32x4 s[NT][kTiles];
 #pragma unroll
-        for (int tt = 0; tt < NT; ++tt) s[tt] = s2[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < kTiles; ++t) {
+            // (fp32: two short sums a score, fewer products that wait for the one before and smaller roundings)
+            f32x4 s2[NT];
 #pragma unroll
-        for (int e = 0; e < kV; ++e)
+            for (int tt = 0; tt < NT; ++tt) s[tt][t] = s2[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int y = 0; y < 4; y += 2)
+            for (int x = 0; x < kQ; ++x) {
+                if constexpr (kF32) {
+                    const f32x4 ka = __builtin_bit_cast(f32x4, kr[t][x]);
 #pragma unroll
-                for (int tt = 0; tt < NT; ++tt) {
-                    s[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[e][y], qr[tt][e][y], s[tt], 0, 0, 0);
-                    s2[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[e][y + 1], qr[tt][e][y + 1], s2[tt], 0, 0, 0);
+                    for (int y = 0; y < 4; y += 2)
+#pragma unroll
+                        for (int tt = 0; tt < NT; ++tt) {
+                            const f32x4 qb = __builtin_bit_cast(f32x4, qr[tt][x]);
+                            s[tt][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(ka[y], qb[y], s[tt][t], 0, 0, 0);
+                            s2[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(ka[y + 1], qb[y + 1], s2[tt], 0, 0, 0);
+                        }
+                } else {
+#pragma unroll
+                    for (int tt = 0; tt < NT; ++tt)
+                        s[tt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[t][x]),
+                                                                           __builtin_bit_cast(bf16x8, qr[tt][x]), s[tt][t], 0, 0, 0);
                 }
+            }
+            if constexpr (kF32) {
+#pragma unroll
+                for (int tt = 0; tt < NT; ++tt) s[tt][t] += s2[tt];
+            }
+        }
         load_k(next);                                         // (the last step: its own again)
         if (edge) {
             // (a weight of 0 times inf is NaN: such values are cleared here, and added at the end to the columns
             // that do attend them)
-            float vm = 0.0f;
+            bool any = false;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < kV; ++j) vm = __builtin_elementwise_maximum(vm, __builtin_fabsf(vr[i][j]));
-            if (__ballot(!(vm < __builtin_inff())) != 0) {
-                odd = true;
+            for (int t = 0; t < kTiles; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < kV; ++j)
-                        vr[i][j] = __builtin_fabsf(vr[i][j]) < __builtin_inff() ? vr[i][j] : 0.0f;
+                    for (int j = 0; j < kV; ++j) any |= packed_odd(vr[t][i][j]);
+            if (__ballot(any) != 0) {
+                odd = true;
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < kV; ++j) vr[t][i][j] = packed_odd(vr[t][i][j]) ? 0 : vr[t][i][j];
             }
         }
 #pragma unroll
         for (int tt = 0; tt < NT; ++tt) {
-            const int left = lim[tt] - key0 - 4 * grp;        // this lane's keys up to it are allowed
+            const int left = lim[tt] - key0 - 4 * grp;        // this lane's keys 16 t + i up to it are allowed
             float mx = m[tt];
-            s[tt] += s2[tt];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, i <= left ? s[tt][i] * a.scale_log2 : -__builtin_inff());
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    mx = fmaxf(mx, 16 * t + i <= left ? s[tt][t][i] * a.scale_log2 : -__builtin_inff());
             mx = pair32_max(pair16_max(mx));
             const float ref = mx == -__builtin_inff() ? 0.0f : mx;
             const float alpha = __builtin_amdgcn_exp2f(m[tt] - ref);
@@ -692,18 +742,39 @@ __global__ void __launch_bounds__(kPfWaves* kWave, D == 64 && NT == 1 ? 3 : 2) p
             m[tt] = mx;
             // one rounding between a score and its distance from the reference, which is small where the weight is not
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[tt][i] = i <= left ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, -ref)) : 0.0f;
-                l[tt] += s[tt][i];
-            }
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[tt][t][i] = 16 * t + i <= left ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][t][i], a.scale_log2, -ref)) : 0.0f;
+                    l[tt] += s[tt][t][i];
+                }
         }
+        if constexpr (kF32) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < kV; ++j)
+                for (int j = 0; j < kV; ++j)
+#pragma unroll
+                    for (int tt = 0; tt < NT; ++tt)
+                        o[tt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[0][i][j], s[tt][0][i], o[tt][j], 0, 0, 0);
+        } else {
+            // P is rounded to bf16 for the product (the sum l keeps it in fp32)
+            bf16x8 pb[NT];
+#pragma unroll
+            for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) pb[tt][e] = static_cast<__bf16>(s[tt][e / 4][e % 4]);
+#pragma unroll
+            for (int j = 0; j < kV; ++j) {
+                typedef short s16x8 __attribute__((ext_vector_type(8)));
+                s16x8 va;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) va[e] = vr[e / 4][e % 4][j];
 #pragma unroll
                 for (int tt = 0; tt < NT; ++tt)
-                    o[tt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[i][j], s[tt][i], o[tt][j], 0, 0, 0);
+                    o[tt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), pb[tt], o[tt][j], 0, 0, 0);
+            }
+        }
         load_v(next);
     }
 #pragma unroll
@@ -726,14 +797,14 @@ __global__ void __launch_bounds__(kPfWaves* kWave, D == 64 && NT == 1 ? 3 : 2) p
     for (int tt = 0; tt < NT; ++tt) {
         float M = m[tt];
 #pragma unroll
-        for (int x = 0; x < kPfWaves - 1; ++x) M = fmaxf(M, sm.m[x][tt][lane]);
+        for (int x = 0; x < kPdWaves - 1; ++x) M = fmaxf(M, sm.m[x][tt][lane]);
         const float ref = M == -__builtin_inff() ? 0.0f : M;
         float wt = __builtin_amdgcn_exp2f(m[tt] - ref);
         l[tt] *= wt;
 #pragma unroll
         for (int j = 0; j < kV; ++j) o[tt][j] *= wt;
 #pragma unroll
-        for (int x = 0; x < kPfWaves - 1; ++x) {
+        for (int x = 0; x < kPdWaves - 1; ++x) {
             wt = __builtin_amdgcn_exp2f(sm.m[x][tt][lane] - ref);
             l[tt] = __builtin_fmaf(wt, sm.l[x][tt][lane], l[tt]);
 #pragma unroll
@@ -743,15 +814,15 @@ __global__ void __launch_bounds__(kPfWaves* kWave, D == 64 && NT == 1 ? 3 : 2) p
     if ((sm.odd[0] | sm.odd[1] | sm.odd[2] | sm.odd[3]) != 0) {
         // the values cleared above: a positive weight times inf or NaN is that value
         for (int key = (a.causal ? w_first : len) / kStep * kStep; key < w_end; ++key) {
-            const float* vp = vb + static_cast<int64_t>(key) * a.kv_st + 4 * kV * grp;
+            const E* vp = vb + static_cast<int64_t>(key) * a.kv_st + 4 * kV * grp;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < kV; ++j) {
-                    const float f = vp[kV * i + j];
+                    const E f = vp[kV * i + j];
 #pragma unroll
                     for (int tt = 0; tt < NT; ++tt)
-                        if (!(__builtin_fabsf(f) < __builtin_inff()) && key <= lim[tt]) o[tt][j][i] += f;
+                        if (packed_odd(f) && key <= lim[tt]) o[tt][j][i] += packed_f32(f);
                 }
         }
     }
@@ -761,14 +832,19 @@ __global__ void __launch_bounds__(kPfWaves* kWave, D == 64 && NT == 1 ? 3 : 2) p
         const int c = col0 + 16 * tt + c16;
         if (c >= ncol) continue;
         const float inv = 1.0f / l[tt];
-        float* op = a.out + (w.row0 + static_cast<int64_t>(tok[tt])) * a.out_st +
-                    static_cast<int64_t>(g * a.R + c % a.R) * D + 4 * kV * grp;
+        E* op = static_cast<E*>(a.out) + (w.row0 + static_cast<int64_t>(tok[tt])) * a.out_st +
+                static_cast<int64_t>(g * a.R + c % a.R) * D + 4 * kV * grp;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+            Row y;
 #pragma unroll
-            for (int j = 0; j < kV; j += 4)
-                *reinterpret_cast<f32x4*>(op + kV * i + j) =
-                    f32x4{o[tt][j][i] * inv, o[tt][j + 1][i] * inv, o[tt][j + 2][i] * inv, o[tt][j + 3][i] * inv};
+            for (int j = 0; j < kV; ++j) {
+                E e;
+                packed_put(e, o[tt][j][i] * inv);
+                y[j] = e;
+            }
+            *reinterpret_cast<Row*>(op + kV * i) = y;
+        }
     }
 }
 
@@ -778,7 +854,7 @@ static bool packed_matrix_cores(const void* q, int64_t q_st, int64_t q_sh, const
                                 int64_t out_st) {
     const int64_t ve = dtype == SPARDA_F32 ? 4 : 8;
     auto al16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    return (D == 64 || D == 128 || (D == 32 && dtype == SPARDA_BF16)) && N * R < (int64_t(1) << 31) - 256 && al16(q) && al16(k) && al16(v) && al16(out) &&
+    return (D == 32 || D == 64 || D == 128) && N * R < (int64_t(1) << 31) - 256 && al16(q) && al16(k) && al16(v) && al16(out) &&
            q_st % ve == 0 && q_sh % ve == 0 && kv_st >= 0 && kv_st < (1 << 24) && kv_st % ve == 0 && kv_sh % ve == 0 &&
            out_st % ve == 0;
 }
@@ -791,24 +867,33 @@ int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void*
     const int64_t R = Hq / Hkv;
     const float sl = scale * kPkLog2e;
     const bool cores = packed_matrix_cores(q, q_st, q_sh, k, v, kv_st, kv_sh, dtype, N, R, D, out, out_st);
-    if (cores && dtype == SPARDA_F32) {
-        PackedPrefillF32 a{static_cast<const float*>(q), q_st, q_sh, static_cast<const float*>(k),
-                           static_cast<const float*>(v), kv_st, kv_sh, cu, static_cast<int>(n), N, static_cast<int>(Hkv),
-                           static_cast<int>(R), causal, 0, sl, static_cast<float*>(out), out_st, status};
-#define SPARDA_PKF(D_, NT_)                                                                                       \
+    const bool f32 = dtype == SPARDA_F32;
+    // bf16 without staging: where 16-column windows leave every CU at most one workgroup and sequences are short, the
+    // walk's latency is all there is. us of this form / the staged ones below, causal: 12/4 heads of 64: N=1
+    // 4.0 / 5.1, 37 4.2 / 5.6, 256 5.7 / 6.2, 350 6.5 / 6.7, 512 8.8 / 7.3, 4 x 128 6.7 / 6.3, 16 x 32 4.8 / 5.6;
+    // 4/4 heads: N=384 6.3 / 6.6, 512 7.0 / 7.1; 8/1 heads of 128: N=400 9.2 / 10.9, 4 x 200 11.2 / 9.4; 32/8: N=128
+    // 6.8 / 8.0, 256 10.3 / 9.4
+    if (cores && (f32 || (N * Hq <= 16 * 256 && N <= 384 * n))) {
+        PackedDirect a{q, q_st, q_sh, k, v, kv_st, kv_sh, cu, static_cast<int>(n), N, static_cast<int>(Hkv),
+                       static_cast<int>(R), causal, 0, sl, out, out_st, status};
+#define SPARDA_PKD(DT_, D_, NT_)                                                                                  \
     do {                                                                                                          \
         a.slots = packed_slots(N, n, R, 16 * NT_);                                                                \
         if (a.slots * Hkv >= (int64_t(1) << 31)) return set_error(SPARDA_ERR_SHAPE, "prefill_packed: grid too large"); \
-        hipLaunchKernelGGL((prefill_packed_f32_kernel<D_, NT_>), dim3(static_cast<unsigned>(a.slots * Hkv)),      \
-                           dim3(kPfWaves * kWave), 0, stream, a);                                                 \
+        hipLaunchKernelGGL((prefill_packed_direct_kernel<DT_, D_, NT_>), dim3(static_cast<unsigned>(a.slots * Hkv)), \
+                           dim3(kPdWaves * kWave), 0, stream, a);                                                 \
     } while (0)
-        // wider windows read K and V for more columns, narrow ones are more workgroups: us of 16 / 32
+        // fp32: wider windows read K and V for more columns, narrow ones are more workgroups: us of 16 / 32
         // columns, 12/4 heads of 64: N=512 12.7 / 16.2, 3 x 500 25.4 / 26.7, N=1501 47.6 / 52.8, N=4000 232 / 225
-        if (D == 128) SPARDA_PKF(128, 1);
-        else if (N * Hq <= 2048 * 16) SPARDA_PKF(64, 1);
-        else SPARDA_PKF(64, 2);
-#undef SPARDA_PKF
-        return check_hip(hipGetLastError(), "prefill_packed_f32_kernel");
+        if (!f32 && D == 32) SPARDA_PKD(SPARDA_BF16, 32, 1);
+        else if (!f32 && D == 64) SPARDA_PKD(SPARDA_BF16, 64, 1);
+        else if (!f32) SPARDA_PKD(SPARDA_BF16, 128, 1);
+        else if (D == 32) SPARDA_PKD(SPARDA_F32, 32, 1);
+        else if (D == 128) SPARDA_PKD(SPARDA_F32, 128, 1);
+        else if (N * Hq <= 2048 * 16) SPARDA_PKD(SPARDA_F32, 64, 1);
+        else SPARDA_PKD(SPARDA_F32, 64, 2);
+#undef SPARDA_PKD
+        return check_hip(hipGetLastError(), "prefill_packed_direct_kernel");
     }
     if (cores) {
         PackedPrefill a{static_cast<const uint16_t*>(q), q_st, q_sh, static_cast<const uint16_t*>(k),

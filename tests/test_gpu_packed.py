@@ -257,7 +257,8 @@ def test_packed_captured_and_replayed_with_other_offsets(dtype):
 # sizes on either side of the limits at which the work is cut differently
 CUTS = [(BF, 12, 4, 64, [500]), (BF, 12, 4, 64, [2000]), (BF, 12, 4, 64, [4200]), (BF, 12, 4, 64, [700] * 8),
         (BF, 12, 4, 64, [9000, 13001]), (BF, 16, 16, 64, [1500, 600]), (BF, 32, 8, 128, [400]), (BF, 12, 4, 32, [900, 77]), (BF, 6, 2, 16, [300, 40]), (F32, 6, 2, 32, [300, 40]), (BF, 8, 2, 128, [4300]),
-        (BF, 32, 8, 128, [150] * 10), (BF, 32, 8, 128, [3000, 2000]), (F32, 12, 4, 64, [3000]), (F32, 8, 1, 128, [1000, 700])]
+        (BF, 32, 8, 128, [150] * 10), (BF, 32, 8, 128, [3000, 2000]), (F32, 12, 4, 64, [3000]), (F32, 8, 1, 128, [1000, 700]),
+        (BF, 12, 4, 64, [300, 41]), (BF, 8, 2, 128, [260, 33]), (BF, 8, 4, 32, [380, 100]), (F32, 6, 2, 32, [2000])]
 
 
 @pytest.mark.parametrize("causal", [True, False])
@@ -299,3 +300,45 @@ def test_packed_more_sequences_than_lanes_and_long_ones():
     q, k, v = inputs(N, 12, 4, 64, BF, seed=3)
     got = sparda.prefill_packed(q.to(DEV), k.to(DEV), v.to(DEV), torch.from_numpy(cu).to(DEV))
     check(got, q, k, v, cu, rows=range(0, N, 17))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("Hq,Hkv,D", [(12, 4, 64), (8, 1, 128), (6, 2, 32)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_short_sequences_in_a_large_batch(dtype, Hq, Hkv, D, causal):
+    """Many short sequences of odd lengths between rows of no sequence that hold
+    NaN, and, in one of them, a value that is not finite and keys whose scores are -inf."""
+    print(f"[case] packed large batch {dtype} {Hq}/{Hkv}x{D} causal={causal}", flush=True)
+    cu = offsets([5, 0, 64, 1, 130, 33, 120, 31] * 6, start=3)
+    N = int(cu[-1]) + 9
+    q, k, v = inputs(N, Hq, Hkv, D, dtype, seed=D)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    for x in (q, k, v):
+        x[:3] = float("nan")
+        x[N - 9:] = float("nan")
+    cud = torch.from_numpy(cu).to(DEV)
+    out = torch.full((N, Hq * D), 7.0, dtype=dtype, device=DEV)
+    sparda.prefill_packed(q.to(DEV), k.to(DEV), v.to(DEV), cud, causal=causal, out=out)
+    assert (out[:3] == 7).all() and (out[N - 9:] == 7).all()
+    rows = sorted({int(c) + d for c in cu for d in (-2, -1, 0, 1, 15, 16, 31, 32) if 3 <= c + d < N - 9})
+    check(out, q, k, v, cu, causal, rows=rows)
+    a, b = int(cu[20]), int(cu[21])                  # a sequence of 130
+    k2, v2 = k.clone(), v.clone()
+    k2[a:a + 40, 0, 0] = -float("inf")               # of the first KV head
+    v2[a + 77, Hkv - 1, 5] = float("nan")
+    R, got = Hq // Hkv, sparda.prefill_packed(q.to(DEV), k2.to(DEV), v2.to(DEV), cud, causal=causal).view(N, Hq, D).cpu().float()
+    nan = torch.zeros(N, Hq, D, dtype=torch.bool)
+    nan[(a + 77 if causal else a):b, Hq - R:, 5] = True
+    if causal:
+        nan[a:a + 40, :R] = True                     # every key weighs nothing: 0 / 0
+    inside = slice(3, N - 9)
+    assert torch.equal(torch.isnan(got)[inside], nan[inside])
+    same = torch.ones(N, Hq, D, dtype=torch.bool)
+    same[a:b] = False
+    torch.testing.assert_close(got[inside][same[inside]], out.view(N, Hq, D).cpu().float()[inside][same[inside]], rtol=0, atol=0)
+    qn, kn, vn = (np32(x).astype(np.float64) for x in (q, k, v))
+    for t in range(a + 41, b, 7):
+        e = t + 1 if causal else b
+        want, bf, f32 = attend(qn[t, :R], kn[a + 40:e, 0], vn[a + 40:e, 0], D ** -0.5)
+        ok = ~nan[t, :R].numpy()
+        assert (np.abs(got[t, :R].numpy() - want)[ok] <= (bf if dtype == BF else f32)[ok]).all()
