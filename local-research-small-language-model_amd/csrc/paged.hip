@@ -424,75 +424,68 @@ __global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : DT == SPARDA_F32
     l = pair32_sum(pair16_sum(l));
 
     const bool any_bad = __ballot(bad) != 0;                  // wave-uniform
-    if constexpr (KW == 1) {
-        if (any_bad && lane == 0) atomicOr(a.status, static_cast<uint32_t>(SPARDA_STATUS_PAGE_RANGE));
-        if (c16 >= nh) return;
-        const int h = g * a.R + h0 + c16;
-        // O^T tile j, row 4 grp + i: dim kV (4 grp + i) + j
+    // ---- the wavefronts' partials, joined in order: thread -> (head, dim) ----
+    const int hg = wv % HG;
+    float* lo = lds + hg * KW * (a.lds_heads * (D + 4) + 33);     // [KW][lds_heads][D + 4]
+    float* lm = lo + KW * a.lds_heads * (D + 4);                  // [KW][16][2]
+    int* lbad = reinterpret_cast<int*>(lm + KW * 32);             // [KW]
+    if (c16 < nh) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < kV; ++j)
-                paged_store<DT, D>(a, sh, item, h, kV * (4 * grp + i) + j, any_bad ? __builtin_nanf("") : o[j][i], m, l, any_bad);
-    } else {
-        // ---- the wavefronts' partials, joined in order: thread -> (head, dim) ----
-        const int hg = wv % HG;
-        float* lo = lds + hg * KW * (a.lds_heads * (D + 4) + 33);     // [KW][lds_heads][D + 4]
-        float* lm = lo + KW * a.lds_heads * (D + 4);                  // [KW][16][2]
-        int* lbad = reinterpret_cast<int*>(lm + KW * 32);             // [KW]
-        if (c16 < nh) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < kV; ++j) lo[(wave * a.lds_heads + c16) * (D + 4) + kV * (4 * grp + i) + j] = o[j][i];
-            if (grp == 0) {
-                lm[(wave * 16 + c16) * 2] = m;
-                lm[(wave * 16 + c16) * 2 + 1] = l;
-            }
+            for (int j = 0; j < kV; ++j) lo[(wave * a.lds_heads + c16) * (D + 4) + kV * (4 * grp + i) + j] = o[j][i];
+        if (grp == 0) {
+            lm[(wave * 16 + c16) * 2] = m;
+            lm[(wave * 16 + c16) * 2 + 1] = l;
         }
-        if (lane == 0) lbad[wave] = any_bad ? 1 : 0;
-        __syncthreads();
-        int bads = 0;
+    }
+    if (lane == 0) lbad[wave] = any_bad ? 1 : 0;
+    __syncthreads();
+    int bads = 0;
 #pragma unroll
-        for (int w = 0; w < KW; ++w) bads |= lbad[w];
-        if (bads != 0 && wave == 0 && lane == 0) atomicOr(a.status, static_cast<uint32_t>(SPARDA_STATUS_PAGE_RANGE));
-        for (int e = wave * kWave + lane; e < nh * D; e += KW * kWave) {
-            const int c = e / D, d = e % D;
-            float mw[KW], M = -__builtin_inff();
+    for (int w = 0; w < KW; ++w) bads |= lbad[w];
+    if (bads != 0 && wave == 0 && lane == 0) atomicOr(a.status, static_cast<uint32_t>(SPARDA_STATUS_PAGE_RANGE));
+    for (int e = wave * kWave + lane; e < nh * D; e += KW * kWave) {
+        const int c = e / D, d = e % D;
+        float mw[KW], M = -__builtin_inff();
 #pragma unroll
-            for (int w = 0; w < KW; ++w) {
-                mw[w] = lm[(w * 16 + c) * 2];
-                M = fmaxf(M, mw[w]);
-            }
-            const float ref = M == -__builtin_inff() ? 0.0f : M;
-            float L = 0.0f, O = 0.0f;
-#pragma unroll
-            for (int w = 0; w < KW; ++w) {
-                const float wt = __builtin_amdgcn_exp2f(mw[w] - ref);
-                L = __builtin_fmaf(wt, lm[(w * 16 + c) * 2 + 1], L);
-                O = __builtin_fmaf(wt, lo[(w * a.lds_heads + c) * (D + 4) + d], O);
-            }
-            paged_store<DT, D>(a, sh, item, g * a.R + h0 + c, d, bads ? __builtin_nanf("") : O, M, L, bads != 0);
+        for (int w = 0; w < KW; ++w) {
+            mw[w] = lm[(w * 16 + c) * 2];
+            M = fmaxf(M, mw[w]);
         }
+        const float ref = M == -__builtin_inff() ? 0.0f : M;
+        float L = 0.0f, O = 0.0f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+            const float wt = __builtin_amdgcn_exp2f(mw[w] - ref);
+            L = __builtin_fmaf(wt, lm[(w * 16 + c) * 2 + 1], L);
+            O = __builtin_fmaf(wt, lo[(w * a.lds_heads + c) * (D + 4) + d], O);
+        }
+        paged_store<DT, D>(a, sh, item, g * a.R + h0 + c, d, bads ? __builtin_nanf("") : O, M, L, bads != 0);
     }
 }
 
-// Joins the items of a sequence, one workgroup per (query head, sequence): the
-// items' weights once into LDS, then dims over the lanes and the items over the
-// thread groups (8 loads in flight each), added in group order.
+// Joins the items of a sequence, one workgroup per (32 dims of a query head, sequence):
+//     M = max m_i, out = sum exp2(m_i - M) O_i / sum exp2(m_i - M) l_i.
+// The items' weights once into LDS, then dims over the lanes and the items over the
+// thread groups (8 loads in flight each), added in group order. Bound by two
+// latencies, the weights' and the partials' (3.7 to 5.4 us): with a whole head a
+// workgroup 1 x 20000 positions take 12.8 against 11.7 us, 1 x 131000 31.6 / 30.8,
+// with 16 dims 8 x 16384 26.1 / 25.5.
 template <int DT, int D>
 __global__ void __launch_bounds__(kPgJoin) decode_paged_join_kernel(PagedDecode a) {
-    constexpr int kStep = 16 * PagedType<DT>::kTiles, kG = kPgJoin / D, kChunk = 1024, kJW = kPgJoin / kWave;
+    constexpr int JD = D < 32 ? D : 32;                       // dims of a workgroup
+    constexpr int kStep = 16 * PagedType<DT>::kTiles, kG = kPgJoin / JD, kChunk = 1024, kJW = kPgJoin / kWave;
     __shared__ float red[kPgJoin], wts[kChunk], rm[kJW], rl[kJW];
-    const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, wave = tid / kWave;
+    const int b = blockIdx.y, h = blockIdx.x / (D / JD), d0 = blockIdx.x % (D / JD) * JD, tid = threadIdx.x, wave = tid / kWave;
     const Share sh = paged_item(a.len, a.B, a.cap, kStep, a.target, a.least, false, b);
     if (sh.parts <= 1) return;                                // written by its one item
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + static_cast<int64_t>(sh.first) * a.Hq + h;
-    const float* po = a.part_o + (static_cast<int64_t>(sh.first) * a.Hq + h) * D + tid % D;
+    const float* po = a.part_o + (static_cast<int64_t>(sh.first) * a.Hq + h) * D + d0 + tid % JD;
     const int64_t st = static_cast<int64_t>(a.Hq) * D;
     float first[8];                                           // the thread's first items, under the weights' latency
 #pragma unroll
-    for (int e = 0; e < 8; ++e) first[e] = tid / D + e * kG < sh.parts ? po[(tid / D + e * kG) * st] : 0.0f;
+    for (int e = 0; e < 8; ++e) first[e] = tid / JD + e * kG < sh.parts ? po[(tid / JD + e * kG) * st] : 0.0f;
     float M = -__builtin_inff();
     for (int i = tid; i < sh.parts; i += kPgJoin) M = fmaxf(M, ml[static_cast<int64_t>(i) * a.Hq].x);
     M = wave_max(M);
@@ -512,7 +505,7 @@ __global__ void __launch_bounds__(kPgJoin) decode_paged_join_kernel(PagedDecode 
             L = __builtin_fmaf(wt, x.y, L);
         }
         __syncthreads();
-        int i = tid / D;
+        int i = tid / JD;
         if (c0 == 0) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) O = i + e * kG < n ? __builtin_fmaf(wts[i + e * kG], first[e], O) : O;
@@ -532,13 +525,13 @@ __global__ void __launch_bounds__(kPgJoin) decode_paged_join_kernel(PagedDecode 
     if (tid % kWave == 0) rl[wave] = L;
     red[tid] = O;
     __syncthreads();
-    if (tid >= D) return;
+    if (tid >= JD) return;
     float den = 0.0f;
 #pragma unroll
     for (int w = 0; w < kJW; ++w) den += rl[w];
 #pragma unroll
-    for (int i = 1; i < kG; ++i) O += red[i * D + tid];
-    store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + tid, O / den);
+    for (int i = 1; i < kG; ++i) O += red[i * JD + tid];
+    store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d0 + tid, O / den);
 }
 
 // The same for few items a sequence: one thread per (query head, dim), items in order.
@@ -656,7 +649,7 @@ int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k
     const dim3 grid(static_cast<unsigned>(p.items * p.groups));
 #define SPARDA_PGD_W(DT_, D_, HG_, KW_)                                                                           \
     hipLaunchKernelGGL((decode_paged_kernel<DT_, D_, HG_, KW_>), grid, dim3(HG_ * KW_ * kWave),                   \
-                       KW_ > 1 ? HG_ * KW_ * (a.lds_heads * ((D_) + 4) + 33) * sizeof(float) : 0, stream, a)
+                       HG_ * KW_ * (a.lds_heads * ((D_) + 4) + 33) * sizeof(float), stream, a)
 #define SPARDA_PGD(DT_, D_)                                                                                       \
     do {                                                                                                          \
         if (p.hg == 4) SPARDA_PGD_W(DT_, D_, 4, 2);                                                               \
@@ -667,8 +660,8 @@ int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k
             hipLaunchKernelGGL((decode_paged_join_few_kernel<DT_, D_>),                                           \
                                dim3(static_cast<unsigned>(cdiv(Hq, 256 / D_)), static_cast<unsigned>(B)), dim3(256), 0, stream, a); \
         else if (p.items > B)                                                                                     \
-            hipLaunchKernelGGL((decode_paged_join_kernel<DT_, D_>), dim3(static_cast<unsigned>(Hq), static_cast<unsigned>(B)), \
-                               dim3(kPgJoin), 0, stream, a);                                                      \
+            hipLaunchKernelGGL((decode_paged_join_kernel<DT_, D_>),                                               \
+                               dim3(static_cast<unsigned>(Hq * (D_ < 32 ? 1 : D_ / 32)), static_cast<unsigned>(B)), dim3(kPgJoin), 0, stream, a); \
     } while (0)
 #define SPARDA_PGD_D(DT_)                     \
     switch (D) {                              \
