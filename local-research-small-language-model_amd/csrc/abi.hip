@@ -933,7 +933,7 @@ SPARDA_API int sparda_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, 
     SPARDA_REQUIRE(head_dim_ok(D), SPARDA_ERR_SHAPE, "prefill_packed: head dim %lld not in {16,32,64,128}",
                    (long long)D);
     SPARDA_REQUIRE(Hq % Hkv == 0, SPARDA_ERR_SHAPE, "prefill_packed: Hq must be a multiple of Hkv");
-    SPARDA_REQUIRE(N < (1ll << 31) && n_seqs < (1ll << 31) && Hq <= 65535, SPARDA_ERR_SHAPE,
+    SPARDA_REQUIRE(N < (1ll << 31) && n_seqs <= (1ll << 30) && Hq <= 65535, SPARDA_ERR_SHAPE,
                    "prefill_packed: too many rows, sequences or heads");
     SPARDA_REQUIRE(N == 1 || out_st >= Hq * D, SPARDA_ERR_STRIDE, "prefill_packed: output rows overlap");
     return launch_prefill_packed(q, q_st, q_sh, k, v, kv_st, kv_sh, dtype, cu_seqlens, n_seqs, N, Hq, Hkv, D,
@@ -968,7 +968,7 @@ SPARDA_API int sparda_append_paged(void* k_pages, void* v_pages, int dtype, int6
     if (const int rc = check_pages("append_paged", k_pages, v_pages, dtype, n_pages, page_size, p_st, s_st, h_st, t_st,
                                    width, Hkv, D))
         return rc;
-    SPARDA_REQUIRE(n_seqs > 0 && N > 0 && n_seqs < (1ll << 31) && N < (1ll << 31), SPARDA_ERR_SHAPE,
+    SPARDA_REQUIRE(n_seqs > 0 && N > 0 && N < (1ll << 31) && (n_seqs <= (1ll << 30) || !cu_seqlens), SPARDA_ERR_SHAPE,
                    "append_paged: bad numbers of sequences or rows");
     SPARDA_REQUIRE(cu_seqlens || N == n_seqs, SPARDA_ERR_SHAPE,
                    "append_paged: without offsets every sequence takes one row (%lld rows, %lld sequences)",
