@@ -602,8 +602,14 @@ __global__ void __launch_bounds__(kPdWaves* kWave, 2) prefill_packed_direct_kern
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int c16 = lane % 16, grp = lane / 16;
-    const int g = blockIdx.x % a.Hkv;
-    const int64_t slot = a.slots - 1 - blockIdx.x / a.Hkv;
+    // A sequence's windows grow with their index. Where the chip holds all workgroups at
+    // once, no later one evens out the CUs' loads: every other round of 256 runs
+    // backwards. us against the plain order, fp32, 12/4 heads of 64: N=1000 25.1 / 27.0, N=1501 42.8 /
+    // 47.3, 3 x 500 22.0 / 23.9, 20 x 75 11.5 / 10.8; with more workgroups, N=4000 234 / 229.
+    uint32_t at = blockIdx.x;
+    if (gridDim.x <= 5 * 256 && at / 256 % 2 == 1 && (at / 256 + 1) * 256 <= gridDim.x) at = at / 256 * 256 + 255 - at % 256;
+    const int g = at % a.Hkv;
+    const int64_t slot = a.slots - 1 - at / a.Hkv;
     bool bad;
     const PackedWindow w = packed_window(a.cu, a.n, a.N, a.R, kBM, slot, bad);
     if (bad && threadIdx.x == 0) atomicOr(a.status, static_cast<uint32_t>(SPARDA_STATUS_SEQUENCE_RANGE));
@@ -884,7 +890,7 @@ int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void*
                            dim3(kPdWaves * kWave), 0, stream, a);                                                 \
     } while (0)
         // fp32: wider windows read K and V for more columns, narrow ones are more workgroups: us of 16 / 32
-        // columns, 12/4 heads of 64: N=512 12.7 / 16.2, 3 x 500 25.4 / 26.7, N=1501 47.6 / 52.8, N=4000 232 / 225
+        // columns, 12/4 heads of 64: N=512 12.7 / 16.2, 3 x 500 22.0 / 26.7, N=1501 42.8 / 52.8, N=4000 232 / 225
         if (!f32 && D == 32) SPARDA_PKD(SPARDA_BF16, 32, 1);
         else if (!f32 && D == 64) SPARDA_PKD(SPARDA_BF16, 64, 1);
         else if (!f32) SPARDA_PKD(SPARDA_BF16, 128, 1);
