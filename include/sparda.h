@@ -875,8 +875,9 @@ SPARDA_API int sparda_offload_fetch(sparda_offload_t h, const int32_t* sel, cons
  * Sums and softmax statistics in fp32; for bf16 the weights are rounded to
  * bf16 for the product with v.
  *   q: [N,Hq,D] strides (q_st, q_sh, 1); k, v: [N,Hkv,D] strides (kv_st,
- *   kv_sh, 1); out: [N,Hq*D] of dtype, stride out_st; D in {16, 32, 64, 128},
- *   any Hq that Hkv divides. A row outside A(t) has no part in out[t], whatever
+ *   kv_sh, 1); out: [N,Hq*D] of dtype, stride out_st; all rows 16-byte aligned,
+ *   0 <= kv_st < 2^24; D in {16, 32, 64, 128}, any Hq that Hkv divides,
+ *   N * Hq / Hkv < 2^31 - 256, n_seqs <= 2^30. A row outside A(t) has no part in out[t], whatever
  *   it holds. cu_seqlens: n_seqs + 1 offsets.
  */
 SPARDA_API int sparda_prefill_packed(const void* q, int64_t q_st, int64_t q_sh,

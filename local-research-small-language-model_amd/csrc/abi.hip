@@ -935,6 +935,14 @@ SPARDA_API int sparda_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, 
     SPARDA_REQUIRE(Hq % Hkv == 0, SPARDA_ERR_SHAPE, "prefill_packed: Hq must be a multiple of Hkv");
     SPARDA_REQUIRE(N < (1ll << 31) && n_seqs <= (1ll << 30) && Hq <= 65535, SPARDA_ERR_SHAPE,
                    "prefill_packed: too many rows, sequences or heads");
+    // (columns are counted in 32 bits, and so are the elements of a block of 64 keys)
+    SPARDA_REQUIRE(N * (Hq / Hkv) < (1ll << 31) - 256, SPARDA_ERR_SHAPE, "prefill_packed: too many rows and heads");
+    const int64_t ve = 16 / (dtype == SPARDA_F32 ? 4 : 2);
+    SPARDA_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && q_st % ve == 0 && q_sh % ve == 0 &&
+                       kv_st % ve == 0 && kv_sh % ve == 0 && out_st % ve == 0,
+                   SPARDA_ERR_STRIDE, "prefill_packed: the rows must be 16-byte aligned");
+    SPARDA_REQUIRE(kv_st >= 0 && kv_st < (1ll << 24), SPARDA_ERR_STRIDE,
+                   "prefill_packed: rows of k and v must lie less than 2^24 elements apart");
     SPARDA_REQUIRE(N == 1 || out_st >= Hq * D, SPARDA_ERR_STRIDE, "prefill_packed: output rows overlap");
     return launch_prefill_packed(q, q_st, q_sh, k, v, kv_st, kv_sh, dtype, cu_seqlens, n_seqs, N, Hq, Hkv, D,
                                  causal != 0, scale, out, out_st, static_cast<hipStream_t>(stream));

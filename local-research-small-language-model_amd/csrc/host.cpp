@@ -508,7 +508,7 @@ PyObject* prefill_packed(PyObject* const* a) {
     const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2);
     need(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type() && same_strides(k, v));
     need(k.sizes() == v.sizes() && k.size(0) == N && k.size(2) == D && N > 0 && rows16(q) && rows16(k) && rows16(v));
-    need(cu.scalar_type() == at::kInt && cu.numel() > 1 && cu.stride(0) == 1);
+    need(k.stride(0) < (int64_t(1) << 24) && cu.scalar_type() == at::kInt && cu.numel() > 1 && cu.stride(0) == 1);
     const float scale = scale_or(a[5], D);
     x.on_current();
     const at::Tensor out = x.empty({N, Hq * D}, q.scalar_type());

@@ -14,62 +14,6 @@ constexpr float kPkLog2e = 1.4426950408889634f;
 
 }  // namespace
 
-// One wavefront per (row, query head): lane j takes key j of 64 at a time, the
-// running maximum and sum are the wave's, and each lane then holds dims lane and
-// lane + 64 of the output. Any head dim up to 128, any strides: heads of 16, and
-// rows that no 16-byte load can reach. Bound by its own loads, a lane reading a K row
-// of its own.
-template <int DT>
-__global__ void __launch_bounds__(256)
-prefill_packed_general_kernel(const void* __restrict__ q, int64_t q_st, int64_t q_sh, const void* __restrict__ k,
-                              const void* __restrict__ v, int64_t kv_st, int64_t kv_sh,
-                              const int32_t* __restrict__ cu, int n, int64_t N, int Hq, int R, int D, int causal,
-                              float scale_log2, void* __restrict__ out, int64_t out_st, uint32_t* __restrict__ status) {
-    const int lane = threadIdx.x % kWave;
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int64_t slot = item / Hq;
-    const int h = static_cast<int>(item % Hq);
-    if (slot >= packed_slots(N, n, 1, 1)) return;
-    bool bad;
-    const PackedWindow w = packed_window(cu, n, N, 1, 1, slot, bad);
-    if (bad && lane == 0) atomicOr(status, static_cast<uint32_t>(SPARDA_STATUS_SEQUENCE_RANGE));
-    if (w.seq < 0) return;
-    const int64_t t = w.row0 + w.win;
-    const int keys = causal ? static_cast<int>(w.win) + 1 : w.len;
-    const int64_t qo = t * q_st + static_cast<int64_t>(h) * q_sh;
-    const int64_t kvo = static_cast<int64_t>(w.row0) * kv_st + static_cast<int64_t>(h / R) * kv_sh;
-    float m = -__builtin_inff(), l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int s0 = 0; s0 < keys; s0 += kWave) {
-        const int s = s0 + lane;
-        float x = -__builtin_inff(), acc = 0.0f;
-        if (s < keys) {
-            const int64_t ko = kvo + s * kv_st;
-            for (int d = 0; d < D; ++d) acc = __builtin_fmaf(load_elem<DT>(q, qo + d), load_elem<DT>(k, ko + d), acc);
-            x = acc * scale_log2;
-        }
-        const float mx = fmaxf(m, wave_max(x));
-        const float ref = mx == -__builtin_inff() ? 0.0f : mx;
-        const float alpha = __builtin_amdgcn_exp2f(m - ref);
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc, scale_log2, -ref));
-        if (s >= keys) p = 0.0f;
-        l = l * alpha + wave_sum(p);
-        o0 *= alpha;
-        o1 *= alpha;
-        m = mx;
-        const int cnt = keys - s0 < kWave ? keys - s0 : kWave;
-        for (int j = 0; j < cnt; ++j) {
-            const float pj = __shfl(p, j, kWave);
-            const int64_t vo = kvo + static_cast<int64_t>(s0 + j) * kv_st;
-            if (lane < D) o0 = __builtin_fmaf(pj, load_elem<DT>(v, vo + lane), o0);
-            if (lane + kWave < D) o1 = __builtin_fmaf(pj, load_elem<DT>(v, vo + lane + kWave), o1);
-        }
-    }
-    const float inv = 1.0f / l;
-    const int64_t oo = t * out_st + static_cast<int64_t>(h) * D;
-    if (lane < D) store_elem<DT>(out, oo + lane, o0 * inv);
-    if (lane + kWave < D) store_elem<DT>(out, oo + lane + kWave, o1 * inv);
-}
-
 // ---------------------------------------------------------------------------
 // bf16, D = 32, 64 and 128, on the matrix cores
 // ---------------------------------------------------------------------------
@@ -141,7 +85,10 @@ struct PackedPrefill {
 // allowed to every column), taken before the walk from memory, so that every key
 // group has it and nothing is rescaled. A sum past 2^64, or a first tile of -inf
 // alone, sends the workgroup over its keys twice more: for the exact maxima, then
-// against them.
+// against them. Bound by the matrix cores and the exponentials, which share the
+// issue slots: 16384 tokens of 12/4 heads of 64 take 407-430 us = 960-1010 TFLOP/s of
+// the 1210 that a large library product reaches (matrix cores busy 50% of the time by the
+// counters), 8 sequences of 16000 in all, 32/8 heads of 128, 376 us = 900 TFLOP/s.
 template <int D, int NT, int CW, int KG, int KB>
 __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(PackedPrefill a) {
     constexpr int kCols = 32 * NT, kBM = CW * kCols;
@@ -534,7 +481,7 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
 }
 
 // ---------------------------------------------------------------------------
-// keys straight from memory: fp32, and bf16 where sequences are short
+// keys straight from memory: fp32, heads of 16, and bf16 where sequences are short
 // ---------------------------------------------------------------------------
 
 namespace {
@@ -578,21 +525,26 @@ __device__ __forceinline__ void packed_put(short& o, float x) { o = __builtin_bi
 }  // namespace
 
 // One workgroup of 4 wavefronts per (KV head, window of 16 NT columns of one
-// sequence; columns as in the staged kernel). The wavefronts take the steps of 16 keys
-// (bf16: 32) in turn, each with its own running (m, l, O) of every column, and are
-// joined in order at the end: a walk is four times shorter and knows no barrier. K
-// and V go straight from memory to the operand registers: the next step's K once
-// the scores are taken, its V once the output products are, each under the other's
+// sequence; columns as in the staged kernel). The wavefronts take the steps of 16
+// keys (bf16: 32) in turn, each with its own running (m, l, O) of every column, and
+// are joined in order at the end: a walk is four times shorter and knows no barrier. K
+// and V go straight from memory to the operand registers: the next step's K once the
+// scores are taken, its V once the output products are, each under the other's
 // products. The score layout of v_mfma_f32_16x16x4_f32 / 16x16x32_bf16 is already that
 // of the P operand. Bound in fp32 by the matrix rate (16 keys x 16 columns take D / 2
-// products of 32 cycles), in bf16 by the loads, K and V being read once for every
-// 16 NT columns: hence for short sequences alone.
+// products of 32 cycles) and by how evenly the windows fall on the CUs, in bf16 by
+// the loads, K and V being read once for every 16 NT columns: hence for short
+// sequences, and for heads of 16, which fill no 32-row product. Measured: 37 tokens
+// of 12/4 heads of 64 in bf16 4.2 us, three sequences of 1501 tokens in all in fp32 22-24
+// us (48-52 TFLOP/s; the matrix cores are busy a third of it), 8000 tokens of 8/2 heads of
+// 128 in fp32 1081 us (121 TFLOP/s of the 154 that a large library product reaches).
 template <int DT, int D, int NT>
 __global__ void __launch_bounds__(kPdWaves* kWave, 2) prefill_packed_direct_kernel(PackedDirect a) {
     typedef typename PackedElem<DT>::E E;
     constexpr bool kF32 = DT == SPARDA_F32;
     constexpr int kTiles = PackedElem<DT>::kTiles, kStep = 16 * kTiles, kBM = 16 * NT;
-    constexpr int kV = D / 16, kQ = kF32 ? D / 16 : D / 32, kPiece = kF32 ? 4 : 8;  // elements of V a lane holds per key, pieces of K, their elements
+    constexpr int kV = D / 16, kQ = kF32 ? D / 16 : (D + 31) / 32, kPiece = kF32 ? 4 : 8;  // elements of V a lane holds per key, pieces of K, their elements
+    constexpr bool kHalf = !kF32 && D == 16;                  // half of the lanes hold 16 dims (the others' are zero)
     typedef E Row __attribute__((ext_vector_type(kV)));
     __shared__ struct {
         f32x4 o[kPdWaves - 1][NT][kV][kWave];
@@ -630,7 +582,10 @@ __global__ void __launch_bounds__(kPdWaves* kWave, 2) prefill_packed_direct_kern
         const E* qp = static_cast<const E*>(a.q) + (w.row0 + static_cast<int64_t>(tok[tt])) * a.q_st +
                       static_cast<int64_t>(g * a.R + c % a.R) * a.q_sh + kPiece * grp;
 #pragma unroll
-        for (int x = 0; x < kQ; ++x) qr[tt][x] = *reinterpret_cast<const uint4*>(qp + 4 * kPiece * x);
+        for (int x = 0; x < kQ; ++x) {
+            qr[tt][x] = uint4{0, 0, 0, 0};
+            if (!kHalf || grp < 2) qr[tt][x] = *reinterpret_cast<const uint4*>(qp + 4 * kPiece * x);
+        }
     }
     const int kv_st = static_cast<int>(a.kv_st);
     uint4 kr[kTiles][kQ];            // key 16 t + c16, dims as q
@@ -643,7 +598,10 @@ __global__ void __launch_bounds__(kPdWaves* kWave, 2) prefill_packed_direct_kern
             const int key = 16 * t + c16;
             const uint32_t at = static_cast<uint32_t>((key < last ? key : last) * kv_st + kPiece * grp);
 #pragma unroll
-            for (int x = 0; x < kQ; ++x) kr[t][x] = *reinterpret_cast<const uint4*>(p + at + 4 * kPiece * x);
+            for (int x = 0; x < kQ; ++x) {
+                kr[t][x] = uint4{0, 0, 0, 0};
+                if (!kHalf || grp < 2) kr[t][x] = *reinterpret_cast<const uint4*>(p + at + 4 * kPiece * x);
+            }
         }
     };
     auto load_v = [&](int u) __attribute__((always_inline)) {
@@ -854,17 +812,6 @@ __global__ void __launch_bounds__(kPdWaves* kWave, 2) prefill_packed_direct_kern
     }
 }
 
-// 16-byte rows and 32-bit offsets within a block of keys
-static bool packed_matrix_cores(const void* q, int64_t q_st, int64_t q_sh, const void* k, const void* v, int64_t kv_st,
-                                int64_t kv_sh, int dtype, int64_t N, int64_t R, int64_t D, const void* out,
-                                int64_t out_st) {
-    const int64_t ve = dtype == SPARDA_F32 ? 4 : 8;
-    auto al16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    return (D == 32 || D == 64 || D == 128) && N * R < (int64_t(1) << 31) - 256 && al16(q) && al16(k) && al16(v) && al16(out) &&
-           q_st % ve == 0 && q_sh % ve == 0 && kv_st >= 0 && kv_st < (1 << 24) && kv_st % ve == 0 && kv_sh % ve == 0 &&
-           out_st % ve == 0;
-}
-
 int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void* k, const void* v, int64_t kv_st,
                           int64_t kv_sh, int dtype, const int32_t* cu, int64_t n, int64_t N, int64_t Hq, int64_t Hkv,
                           int64_t D, int causal, float scale, void* out, int64_t out_st, hipStream_t stream) {
@@ -872,39 +819,50 @@ int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void*
     if (const int rc = status_word(&status)) return rc;
     const int64_t R = Hq / Hkv;
     const float sl = scale * kPkLog2e;
-    const bool cores = packed_matrix_cores(q, q_st, q_sh, k, v, kv_st, kv_sh, dtype, N, R, D, out, out_st);
     const bool f32 = dtype == SPARDA_F32;
     // bf16 without staging: where 16-column windows leave every CU at most one workgroup and sequences are short, the
     // walk's latency is all there is. us of this form / the staged ones below, causal: 12/4 heads of 64: N=1
     // 4.0 / 5.1, 37 4.2 / 5.6, 256 5.7 / 6.2, 350 6.5 / 6.7, 512 8.8 / 7.3, 4 x 128 6.7 / 6.3, 16 x 32 4.8 / 5.6;
     // 4/4 heads: N=384 6.3 / 6.6, 512 7.0 / 7.1; 8/1 heads of 128: N=400 9.2 / 10.9, 4 x 200 11.2 / 9.4; 32/8: N=128
     // 6.8 / 8.0, 256 10.3 / 9.4
-    if (cores && (f32 || (N * Hq <= 16 * 256 && N <= 384 * n))) {
+    if (f32 || D == 16 || (N * Hq <= 16 * 256 && N <= 384 * n)) {
         PackedDirect a{q, q_st, q_sh, k, v, kv_st, kv_sh, cu, static_cast<int>(n), N, static_cast<int>(Hkv),
                        static_cast<int>(R), causal, 0, sl, out, out_st, status};
-#define SPARDA_PKD(DT_, D_, NT_)                                                                                  \
+#define SPARDA_PKD_N(DT_, D_, NT_)                                                                                \
     do {                                                                                                          \
         a.slots = packed_slots(N, n, R, 16 * NT_);                                                                \
         if (a.slots * Hkv >= (int64_t(1) << 31)) return set_error(SPARDA_ERR_SHAPE, "prefill_packed: grid too large"); \
         hipLaunchKernelGGL((prefill_packed_direct_kernel<DT_, D_, NT_>), dim3(static_cast<unsigned>(a.slots * Hkv)), \
                            dim3(kPdWaves * kWave), 0, stream, a);                                                 \
     } while (0)
-        // fp32: wider windows read K and V for more columns, narrow ones are more workgroups: us of 16 / 32
-        // columns, 12/4 heads of 64: N=512 12.7 / 16.2, 3 x 500 22.0 / 26.7, N=1501 42.8 / 52.8, N=4000 232 / 225
-        if (!f32 && D == 32) SPARDA_PKD(SPARDA_BF16, 32, 1);
-        else if (!f32 && D == 64) SPARDA_PKD(SPARDA_BF16, 64, 1);
-        else if (!f32) SPARDA_PKD(SPARDA_BF16, 128, 1);
-        else if (D == 32) SPARDA_PKD(SPARDA_F32, 32, 1);
-        else if (D == 128) SPARDA_PKD(SPARDA_F32, 128, 1);
-        else if (N * Hq <= 2048 * 16) SPARDA_PKD(SPARDA_F32, 64, 1);
-        else SPARDA_PKD(SPARDA_F32, 64, 2);
+#define SPARDA_PKD(DT_, D_)                       \
+    do {                                          \
+        if (wide) SPARDA_PKD_N(DT_, D_, 2);       \
+        else SPARDA_PKD_N(DT_, D_, 1);            \
+    } while (0)
+        // Wider windows read K and V for more columns, narrow ones are more workgroups. us of 16 / 32 columns, fp32, 12/4
+        // heads of 64: N=512 12.7 / 16.2, 3 x 500 22.0 / 26.7, N=1501 42.8 / 52.8, N=4000 232 / 225; 8/2 of 128:
+        // N=2000 93 / 109, 4 x 750 75 / 76, N=4000 335 / 294, N=8000 1274 / 1081; 12/4 of 32: N=1000 15.3 / 20.1,
+        // N=2000 45.9 / 41.6; bf16 heads of 16: N=1000 7.8 / 8.9, N=2000 20.3 / 16.7, N=16384 761 / 579
+        const bool wide = N * Hq > 16 * 1536 || (D <= 32 && N * Hq > 16 * 1024);
+        if (f32) {
+            if (D == 16) SPARDA_PKD(SPARDA_F32, 16);
+            else if (D == 32) SPARDA_PKD(SPARDA_F32, 32);
+            else if (D == 64) SPARDA_PKD(SPARDA_F32, 64);
+            else SPARDA_PKD(SPARDA_F32, 128);
+        } else {
+            if (D == 16) SPARDA_PKD(SPARDA_BF16, 16);
+            else if (D == 32) SPARDA_PKD_N(SPARDA_BF16, 32, 1);
+            else if (D == 64) SPARDA_PKD_N(SPARDA_BF16, 64, 1);
+            else SPARDA_PKD_N(SPARDA_BF16, 128, 1);
+        }
 #undef SPARDA_PKD
+#undef SPARDA_PKD_N
         return check_hip(hipGetLastError(), "prefill_packed_direct_kernel");
     }
-    if (cores) {
-        PackedPrefill a{static_cast<const uint16_t*>(q), q_st, q_sh, static_cast<const uint16_t*>(k),
-                        static_cast<const uint16_t*>(v), kv_st, kv_sh, cu, static_cast<int>(n), N, static_cast<int>(Hkv),
-                        static_cast<int>(R), causal, 0, sl, static_cast<uint16_t*>(out), out_st, status};
+    PackedPrefill a{static_cast<const uint16_t*>(q), q_st, q_sh, static_cast<const uint16_t*>(k),
+                    static_cast<const uint16_t*>(v), kv_st, kv_sh, cu, static_cast<int>(n), N, static_cast<int>(Hkv),
+                    static_cast<int>(R), causal, 0, sl, static_cast<uint16_t*>(out), out_st, status};
 #define SPARDA_PKM(D_, NT_, CW_, KG_, KB_)                                                                        \
     do {                                                                                                          \
         a.slots = packed_slots(N, n, R, 32 * NT_ * CW_);                                                          \
@@ -912,46 +870,35 @@ int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void*
         hipLaunchKernelGGL((prefill_packed_kernel<D_, NT_, CW_, KG_, KB_>), dim3(static_cast<unsigned>(a.slots * Hkv)), \
                            dim3(CW_ * KG_ * kWave), 0, stream, a);                                                \
     } while (0)
-        // W: windows of 128 columns, NB: 64-key blocks of a mean sequence. Wide windows
-        // stage a block for the most columns; key groups and small windows cut a
-        // window's serial walk where windows are few against the 256 CUs (a group's sums
-        // cost a merge, so that short walks are not cut). us of (tiles a wavefront, wavefronts,
-        // key groups) = (2,4,1) / (1,4,1) / (1,4,2) / (1,2,2) / (1,1,4), 12/4 heads of 64, causal:
-        //   N=64 7.8 / 6.0 / 7.4 / 5.8 / 5.8   N=1000 22.8 / 15.2 / 14.3 / 11.1 / 10.8
-        //   N=2048 38.8 / 25.0 / 23.1 / 19.4 / 21.1   N=4096 70.2 / 49.0 / 42.8 / 44.7 / 56.1
-        //   4 x 1024 38.1 / 25.8 / 22.8 / 23.0 / 30.1   16 x 256 15.6 / 13.3 / 16.3 / 16.2 / 21.8
-        //   N=8192 152 / 129 / 136 / 138 / 173   16 x 1024 67.2 / 59.5 / 72.8 / 72.9 / 105
-        //   N=16384 433 / 433 / 479 / 507 / 622   N=32768 1550 / 1627   8 x 8192 847 / 879
-        // and of (1,4,1) / (1,4,2) / (1,2,2 of 32 keys), heads of 128:
-        //   32/8: N=512 14.7 / 15.9 / 12.4   N=1000 23.2 / 22.9 / 22.2   N=2048 50.5 / 51.3 / 56.2
-        //   8 x 250 21.7 / 31.9 / 25.9   8 x 2000 385 / 459 / 507   8/1: N=8192 169 / 149 / 164
-        const int64_t W = cdiv(N * Hq, 128), NB = cdiv(cdiv(N, n), 64), cus = 256;
-        if (D == 32) {
-            SPARDA_PKM(32, 1, 4, 1, 64);
-        } else if (D == 64) {
-            if (2 * W <= cus) SPARDA_PKM(64, 1, 1, 4, 32);
-            else if (W <= cus && NB >= 8) SPARDA_PKM(64, 1, 2, 2, 64);
-            else if (W <= 2 * cus && NB >= 16) SPARDA_PKM(64, 1, 4, 2, 64);
-            else if (W <= 8 * cus || NB < 32) SPARDA_PKM(64, 1, 4, 1, 64);
-            else SPARDA_PKM(64, 2, 4, 1, 64);
-        } else {
-            if (2 * W <= cus || (W <= cus && NB >= 8)) SPARDA_PKM(128, 1, 2, 2, 32);
-            else if (W <= 2 * cus && NB >= 64) SPARDA_PKM(128, 1, 4, 2, 64);
-            else SPARDA_PKM(128, 1, 4, 1, 64);
-        }
-#undef SPARDA_PKM
-        return check_hip(hipGetLastError(), "prefill_packed_kernel");
+    // W: windows of 128 columns, NB: 64-key blocks of a mean sequence. Wide windows
+    // stage a block for the most columns; key groups and small windows cut a
+    // window's serial walk where windows are few against the 256 CUs (a group's sums
+    // cost a merge, so that short walks are not cut). us of (tiles a wavefront, wavefronts,
+    // key groups) = (2,4,1) / (1,4,1) / (1,4,2) / (1,2,2) / (1,1,4), 12/4 heads of 64, causal:
+    //   N=64 7.8 / 6.0 / 7.4 / 5.8 / 5.8   N=1000 22.8 / 15.2 / 14.3 / 11.1 / 10.8
+    //   N=2048 38.8 / 25.0 / 23.1 / 19.4 / 21.1   N=4096 70.2 / 49.0 / 42.8 / 44.7 / 56.1
+    //   4 x 1024 38.1 / 25.8 / 22.8 / 23.0 / 30.1   16 x 256 15.6 / 13.3 / 16.3 / 16.2 / 21.8
+    //   N=8192 152 / 129 / 136 / 138 / 173   16 x 1024 67.2 / 59.5 / 72.8 / 72.9 / 105
+    //   N=16384 433 / 433 / 479 / 507 / 622   N=32768 1550 / 1627   8 x 8192 847 / 879
+    // and of (1,4,1) / (1,4,2) / (1,2,2 of 32 keys), heads of 128:
+    //   32/8: N=512 14.7 / 15.9 / 12.4   N=1000 23.2 / 22.9 / 22.2   N=2048 50.5 / 51.3 / 56.2
+    //   8 x 250 21.7 / 31.9 / 25.9   8 x 2000 385 / 459 / 507   8/1: N=8192 169 / 149 / 164
+    const int64_t W = cdiv(N * Hq, 128), NB = cdiv(cdiv(N, n), 64), cus = 256;
+    if (D == 32) {
+        SPARDA_PKM(32, 1, 4, 1, 64);
+    } else if (D == 64) {
+        if (2 * W <= cus) SPARDA_PKM(64, 1, 1, 4, 32);
+        else if (W <= cus && NB >= 8) SPARDA_PKM(64, 1, 2, 2, 64);
+        else if (W <= 2 * cus && NB >= 16) SPARDA_PKM(64, 1, 4, 2, 64);
+        else if (W <= 8 * cus || NB < 32) SPARDA_PKM(64, 1, 4, 1, 64);
+        else SPARDA_PKM(64, 2, 4, 1, 64);
+    } else {
+        if (2 * W <= cus || (W <= cus && NB >= 8)) SPARDA_PKM(128, 1, 2, 2, 32);
+        else if (W <= 2 * cus && NB >= 64) SPARDA_PKM(128, 1, 4, 2, 64);
+        else SPARDA_PKM(128, 1, 4, 1, 64);
     }
-    const int64_t groups = cdiv(packed_slots(N, n, 1, 1) * Hq, 4);
-    if (groups >= (int64_t(1) << 31)) return set_error(SPARDA_ERR_SHAPE, "prefill_packed: too many rows and heads");
-#define SPARDA_PKG(DT_)                                                                                            \
-    hipLaunchKernelGGL((prefill_packed_general_kernel<DT_>), dim3(static_cast<unsigned>(groups)), dim3(256), 0,    \
-                       stream, q, q_st, q_sh, k, v, kv_st, kv_sh, cu, static_cast<int>(n), N, static_cast<int>(Hq), \
-                       static_cast<int>(R), static_cast<int>(D), causal, sl, out, out_st, status)
-    if (dtype == SPARDA_F32) SPARDA_PKG(SPARDA_F32);
-    else SPARDA_PKG(SPARDA_BF16);
-#undef SPARDA_PKG
-    return check_hip(hipGetLastError(), "prefill_packed_general_kernel");
+#undef SPARDA_PKM
+    return check_hip(hipGetLastError(), "prefill_packed_kernel");
 }
 
 }  // namespace sparda

@@ -1193,9 +1193,10 @@ def prefill_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
     if cu.numel() < 1:
         raise ValueError("sparda: cu_seqlens holds one offset more than there are sequences")
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    if k.stride() != v.stride():
+    if k.stride() != v.stride() or k.stride(0) >= 1 << 24:
         k, v = k.contiguous(), v.contiguous()
     N, Hq, D = q.shape
+    kv_st = k.stride(0) if N > 1 else k.shape[1] * D
     if scale is None:
         scale = default_scale(D)
     if out is None:
@@ -1204,10 +1205,13 @@ def prefill_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
         _check_out(out, (N, Hq * D), q.dtype)
     if N == 0 or cu.numel() == 1:
         return out
+    to = _rows16(out)                 # (a copy holds the rows that no sequence writes)
     with torch.cuda.device(dev):
-        call("sparda_prefill_packed", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(), k.stride(0),
+        call("sparda_prefill_packed", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(), kv_st,
              k.stride(1), code, cu.data_ptr(), cu.numel() - 1, N, Hq, k.shape[1], D, int(causal), float(scale),
-             out.data_ptr(), out.stride(0), _stream(dev))
+             to.data_ptr(), to.stride(0), _stream(dev))
+        if to is not out:
+            out.copy_(to)
     return out
 
 

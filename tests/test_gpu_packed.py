@@ -186,6 +186,23 @@ def test_packed_strides_and_alignment(dtype):
     assert (wide[:, Hq * D:] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_packed_rows_far_apart_and_an_output_off_16_bytes(dtype):
+    print(f"[case] packed far rows {dtype}", flush=True)
+    cu = offsets([3, 0, 4], start=1)
+    N, D = 9, 64
+    q, k, v = inputs(N, 6, 2, D, dtype, seed=21)
+    far = torch.zeros(N, 1 << 24, dtype=dtype, device=DEV)     # rows 2^24 elements apart
+    kd, vd = (far[:, i * 128:(i + 1) * 128].view(N, 2, D) for i in range(2))
+    kd.copy_(k), vd.copy_(v)
+    out = torch.full((N, 6 * D + 3), 7.0, dtype=dtype, device=DEV)[:, 1:6 * D + 1]
+    got = sparda.prefill_packed(q.to(DEV), kd, vd, torch.from_numpy(cu).to(DEV), out=out)
+    assert got is out and (out[:1] == 7).all() and (out[8:] == 7).all()
+    check(out, q, k, v, cu)
+    one = sparda.prefill_packed(q[:1].to(DEV), kd[1:2], vd[1:2], torch.tensor([0, 1], dtype=torch.int32, device=DEV))
+    check(one, q[:1], k[1:2], v[1:2], [0, 1])                  # one row: its stride has no meaning
+
+
 def test_many_sequences():
     print("[case] packed 300 sequences", flush=True)
     r = np.random.default_rng(2)
@@ -258,7 +275,8 @@ def test_packed_captured_and_replayed_with_other_offsets(dtype):
 CUTS = [(BF, 12, 4, 64, [500]), (BF, 12, 4, 64, [2000]), (BF, 12, 4, 64, [4200]), (BF, 12, 4, 64, [700] * 8),
         (BF, 12, 4, 64, [9000, 13001]), (BF, 16, 16, 64, [1500, 600]), (BF, 32, 8, 128, [400]), (BF, 12, 4, 32, [900, 77]), (BF, 6, 2, 16, [300, 40]), (F32, 6, 2, 32, [300, 40]), (BF, 8, 2, 128, [4300]),
         (BF, 32, 8, 128, [150] * 10), (BF, 32, 8, 128, [3000, 2000]), (F32, 12, 4, 64, [3000]), (F32, 8, 1, 128, [1000, 700]),
-        (BF, 12, 4, 64, [300, 41]), (BF, 8, 2, 128, [260, 33]), (BF, 8, 4, 32, [380, 100]), (F32, 6, 2, 32, [2000])]
+        (BF, 12, 4, 64, [300, 41]), (BF, 8, 2, 128, [260, 33]), (BF, 8, 4, 32, [380, 100]), (F32, 6, 2, 32, [2000]),
+        (F32, 6, 2, 32, [3000, 200]), (BF, 8, 2, 16, [2500, 33]), (F32, 8, 2, 16, [2500, 33]), (F32, 8, 2, 128, [3500])]
 
 
 @pytest.mark.parametrize("causal", [True, False])

@@ -17,14 +17,18 @@ def _expect(code, name, *args):
     assert sparda.load().sparda_last_error()
 
 
-def packed(q=P, k=P, v=P, dtype=1, cu=P, n=2, N=100, Hq=12, Hkv=4, D=64, out=P, out_st=768):
-    return (q, 768, 64, k, v, 256, 64, dtype, cu, n, N, Hq, Hkv, D, 1, 0.125, out, out_st, None)
+def packed(q=P, k=P, v=P, dtype=1, cu=P, n=2, N=100, Hq=12, Hkv=4, D=64, out=P, out_st=768, q_st=768, q_sh=64, kv_st=256,
+           kv_sh=64):
+    return (q, q_st, q_sh, k, v, kv_st, kv_sh, dtype, cu, n, N, Hq, Hkv, D, 1, 0.125, out, out_st, None)
 
 
 @pytest.mark.parametrize("code,bad", [
     (-1, dict(q=None)), (-1, dict(k=None)), (-1, dict(v=None)), (-1, dict(cu=None)), (-1, dict(out=None)),
     (-3, dict(dtype=2)), (-2, dict(n=0)), (-2, dict(N=0)), (-2, dict(Hq=0)), (-2, dict(Hkv=0)), (-2, dict(D=48)),
-    (-2, dict(Hq=13)), (-2, dict(N=1 << 31)), (-2, dict(Hq=1 << 17)), (-5, dict(out_st=767))], ids=str)
+    (-2, dict(Hq=13)), (-2, dict(N=1 << 31)), (-2, dict(Hq=1 << 17)), (-5, dict(out_st=767)),
+    (-2, dict(n=(1 << 30) + 1)), (-2, dict(N=1 << 30, out_st=1 << 20)), (-5, dict(q=P + 8)), (-5, dict(k=P + 2)),
+    (-5, dict(v=P + 4)), (-5, dict(out=P + 8)), (-5, dict(out_st=772)), (-5, dict(q_st=772)), (-5, dict(q_sh=66)),
+    (-5, dict(kv_sh=65)), (-5, dict(kv_st=260)), (-5, dict(kv_st=-256)), (-5, dict(kv_st=1 << 24))], ids=str)
 def test_prefill_packed_argument_errors(code, bad):
     _expect(code, "sparda_prefill_packed", *packed(**bad))
 
@@ -44,7 +48,7 @@ PAGES = [
 
 @pytest.mark.parametrize("code,bad", PAGES + [
     (-1, dict(k=None)), (-1, dict(v=None)), (-1, dict(table=None)), (-1, dict(pos=None)), (-1, dict(kn=None)),
-    (-1, dict(vn=None)), (-2, dict(n=0, N=0)), (-2, dict(N=5)), (-2, dict(cu=P, N=0)), (-5, dict(kn=P + 8)),
+    (-1, dict(vn=None)), (-2, dict(n=0, N=0)), (-2, dict(N=5)), (-2, dict(cu=P, n=(1 << 30) + 1)), (-2, dict(cu=P, N=0)), (-5, dict(kn=P + 8)),
     (-5, dict(new_st=252)), (-5, dict(new_sh=63))], ids=str)
 def test_append_paged_argument_errors(code, bad):
     _expect(code, "sparda_append_paged", *append(**bad))
