@@ -29,32 +29,52 @@ __device__ __forceinline__ int64_t packed_first(int c, int i, int64_t N, int R, 
     return k * R / BM + i;
 }
 
-// The window of a slot, found by every wave for itself: 64 sequences' first
-// slots at a time, the last sequence whose first slot is not past `slot`. Offsets
-// that fall or leave [0, N] set bad (every pair is looked at by slot 0, a slot's
-// own pair by the slot, which then has nothing to do). Wave-uniform results.
-__device__ __forceinline__ PackedWindow packed_window(const int32_t* __restrict__ cu, int n, int64_t N, int R, int BM,
-                                                      int64_t slot, bool& bad) {
+// The last of n sequences whose offset passes `before`, of those that can be the
+// answer where offsets rise: 64 evenly spaced ones first, then 64 at a time behind the
+// last of those that pass (two rounds up to 4096 sequences). -1: none. c0, c1: the
+// sequence's offsets. Wave-uniform results.
+template <class Before>
+__device__ __forceinline__ int packed_find(const int32_t* __restrict__ cu, int n, Before before, int& c0, int& c1) {
     const int lane = threadIdx.x % kWave;
-    int seq = 0, c0 = 0, c1 = 0;
-    for (int i0 = 0; i0 < n; i0 += kWave) {
-        const int i = i0 + lane < n ? i0 + lane : n - 1;
+    int from = 0, to = n;
+    if (n > kWave) {
+        const int step = (n + kWave - 1) / kWave, i = lane * step < n ? lane * step : n - 1;
+        const uint64_t m = __ballot(lane * step < n && before(cu[i], i));
+        from = m == 0 ? 0 : (63 - __builtin_clzll(m)) * step;
+        to = from + step < n ? from + step : n;
+    }
+    int seq = -1;
+    c0 = c1 = 0;
+    for (int i0 = from; i0 < to; i0 += kWave) {
+        const int i = i0 + lane < to ? i0 + lane : to - 1;
         const int a0 = cu[i], a1 = cu[i + 1];   // (both at once: no second load behind the search)
-        const uint64_t m = __ballot(i0 + lane < n && packed_first(a0, i, N, R, BM) <= slot);
-        if (m == 0 && i0 > 0) break;            // (offsets that rise: no later sequence either)
-        const int at = m == 0 ? 0 : 63 - __builtin_clzll(m);
+        const uint64_t m = __ballot(i0 + lane < to && before(a0, i));
+        if (m == 0) break;                      // (no later sequence either)
+        const int at = 63 - __builtin_clzll(m);
         seq = i0 + at;
         c0 = __builtin_amdgcn_readlane(a0, at);
         c1 = __builtin_amdgcn_readlane(a1, at);
         if (m != ~0ull) break;
     }
+    return seq;
+}
+
+// The window of a slot, found by every wave for itself: the last sequence whose
+// first slot is not past `slot`. Offsets that fall or leave [0, N] set bad (every pair
+// is looked at by slot 0, a slot's own pair by the slot, which then has nothing to
+// do). Wave-uniform results.
+__device__ __forceinline__ PackedWindow packed_window(const int32_t* __restrict__ cu, int n, int64_t N, int R, int BM,
+                                                      int64_t slot, bool& bad) {
+    const int lane = threadIdx.x % kWave;
+    int c0, c1;
+    const int seq = packed_find(cu, n, [&](int c, int i) { return packed_first(c, i, N, R, BM) <= slot; }, c0, c1);
     bad = c0 < 0 || c1 < c0 || c1 > N;
     PackedWindow w{-1, 0, 0, 0};
     const bool own = bad;
     if (slot == 0)
         for (int i = lane; i < n; i += kWave) bad = bad || cu[i] < 0 || cu[i + 1] < cu[i] || cu[i + 1] > N;
     bad = __ballot(bad) != 0;
-    if (own) return w;
+    if (own || seq < 0) return w;
     const int64_t win = slot - packed_first(c0, seq, N, R, BM);
     if (win < 0 || win * BM >= static_cast<int64_t>(c1 - c0) * R) return w;
     w.seq = seq;

@@ -4,6 +4,7 @@
 #include "common.h"
 #include "kernels.h"
 #include "mfma.h"
+#include "packed.h"
 
 namespace sparda {
 
@@ -26,8 +27,9 @@ struct Pages {
 // append
 // ---------------------------------------------------------------------------
 
-// One wavefront per new row: its sequence (64 offsets at a time), its page, then
-// the row's heads in 16-byte pieces.
+// One wavefront per new row: its sequence, its page, then the row's heads in 16-byte
+// pieces. Bound by memory, a row read and a row written: 16000 rows of 8 heads of 128
+// take 21.5 us = 6.1 TB/s; 64 rows 2.6 us, a launch and three dependent loads.
 __global__ void __launch_bounds__(256)
 append_paged_kernel(char* __restrict__ k, char* __restrict__ v, Pages pg, int ps, const int32_t* __restrict__ positions,
                     const int32_t* __restrict__ cu, int n, const char* __restrict__ k_new,
@@ -36,7 +38,7 @@ append_paged_kernel(char* __restrict__ k, char* __restrict__ v, Pages pg, int ps
     const int lane = threadIdx.x % kWave;
     const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (t >= N) return;
-    int seq = -1;
+    int seq;
     int64_t at = 0;                               // the row's place among its sequence's new rows
     if (cu == nullptr) {
         seq = static_cast<int>(t);
@@ -47,16 +49,9 @@ append_paged_kernel(char* __restrict__ k, char* __restrict__ v, Pages pg, int ps
             if (__ballot(wrong) != 0 && lane == 0) atomicOr(status, static_cast<uint32_t>(SPARDA_STATUS_SEQUENCE_RANGE));
         }
         // the last sequence that starts at or before t, when t is one of its rows
-        for (int i0 = 0; i0 < n; i0 += kWave) {
-            const int i = i0 + lane;
-            const uint64_t m = __ballot(i < n && cu[i < n ? i : n] <= t);
-            if (m == 0) break;
-            seq = i0 + 63 - __builtin_clzll(m);
-            if (m != ~0ull) break;
-        }
-        seq = __builtin_amdgcn_readfirstlane(seq);
+        int c0, c1;
+        seq = packed_find(cu, n, [&](int c, int) { return c <= t; }, c0, c1);
         if (seq < 0) return;
-        const int c0 = __builtin_amdgcn_readfirstlane(cu[seq]), c1 = __builtin_amdgcn_readfirstlane(cu[seq + 1]);
         if (t >= c1) return;                      // behind the last sequence
         at = t - c0;
     }
@@ -213,6 +208,7 @@ struct PagedDecode {
     int B, cap;
     int Hq, Hkv, R, head_tiles;   // head tiles of 16 query heads per KV head
     int target, least;
+    int whole;                    // every sequence is one item
     int lds_heads;                // heads of the largest tile
     float scale_log2;
     void* out;
@@ -250,7 +246,10 @@ __device__ __forceinline__ void paged_store(const PagedDecode& a, const Share& s
 // step's under the present one's arithmetic, and S^T's layout is already that of the
 // P operand, so nothing passes through LDS before the wavefronts are joined. A
 // tile's 16 keys lie in one page (pages hold a multiple of 16 rows), so that its
-// base address is a scalar.
+// base address is a scalar. Bound by memory where the cache is long: 32 sequences of up to
+// 16384 positions, 32/8 heads of 128, 1.43 GB in 246 us = 5.8 TB/s; 131000 positions of 12/4
+// heads of 64 25.4 us = 5.3 TB/s, of which a launch and the chain lengths, table, keys
+// are 4.
 template <int DT, int D, int HG, int KW>
 __global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : DT == SPARDA_F32 ? 3 : 4) decode_paged_kernel(PagedDecode a) {
     typedef PagedStep<DT, D> Step;
@@ -264,7 +263,13 @@ __global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : DT == SPARDA_F32
     const int item = blockIdx.x / groups, gt = blockIdx.x % groups * HG + wv % HG;
     const int g = gt / a.head_tiles, h0 = gt % a.head_tiles * 16;
     const int nh = a.R - h0 < 16 ? a.R - h0 : 16;           // query heads of the tile
-    const Share sh = paged_item(a.len, a.B, a.cap, kStep, a.target, a.least, true, item);
+    Share sh;
+    if (a.whole) {
+        const int l = __builtin_amdgcn_readfirstlane(a.len[item]), n = l < 0 ? 0 : l > a.cap ? a.cap : l;
+        sh = Share{item, 0, 1, item, paged_steps(l, a.cap, kStep), n, l < 0 || l > a.cap};
+    } else {
+        sh = paged_item(a.len, a.B, a.cap, kStep, a.target, a.least, true, item);
+    }
     if (sh.seq < 0) return;                                 // workgroup-uniform
     const int b = sh.seq, len = sh.len;
     const int steps = paged_steps(len, a.cap, kStep);
@@ -534,7 +539,9 @@ __global__ void __launch_bounds__(kPgJoin) decode_paged_join_kernel(PagedDecode 
     store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d0 + tid, O / den);
 }
 
-// The same for few items a sequence: one thread per (query head, dim), items in order.
+// The same for few items a sequence: one thread per (query head, dim), items in
+// order. Bound by the launch and two dependent loads: 3.0 us for 1000 positions of 12
+// heads of 64.
 template <int DT, int D>
 __global__ void __launch_bounds__(256) decode_paged_join_few_kernel(PagedDecode a) {
     constexpr int kStep = 16 * PagedType<DT>::kTiles;
@@ -577,9 +584,10 @@ namespace {
 // How a launch is cut. us, 12/4 heads of 64 and 32/8 of 128 where named:
 //  - A table whose sequences are short, or a batch that gives every CU a workgroup:
 //    one item a sequence, written straight to the output, no second launch
-//    (B=1, 300 positions 6.3 against 8.2 in shares; B=64, 1000: 12.5 / 15.3; B=128,
-//    300: 8.7 / 12.6). Fewer and longer sequences are faster in shares (B=1, 1000:
-//    10.3 / 8.3).
+//    (B=1, 300 positions 5.1 against 8.2 in shares, 700 7.1 / 8.3, 500 of 32/8 heads
+//    8.3 / 9.2; B=64, 1000: 11.3 / 15.3; B=128, 300: 7.5 / 12.6; B=1000, 2000: 256 / 274).
+//    Fewer and longer sequences are faster in shares (B=1, 1000: 8.7 / 8.2, of 32/8
+//    heads 13.1 / 9.3; B=128, 4000: 75.9 / 69.0).
 //  - Many (sequence, head) pairs: workgroups of 2 or 4 neighbouring heads, which
 //    fetch whole rows of a page at a time (B=32, 16384, 32/8 heads of 128: 257
 //    against 290 with one head a workgroup; 8/8 heads of 64: 137 / 180).
@@ -598,7 +606,7 @@ PagedPlan paged_plan(int64_t B, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D,
     const int even = heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
     const bool eight = (R < 16 ? R : 16) * (D + 4) + 33 <= 2048;  // eight wavefronts' partials fit 64 KB of LDS
     PagedPlan p{1, 4, 1, 4, 0, 0, false};
-    if (steps <= 16 || (steps <= 64 && B * heads >= 128)) {
+    if (steps <= (D == 128 ? 16 : 24) || (steps <= 64 && B * heads >= 128)) {
         p.least = steps;
         if (eight && steps > 8 && B * heads < 512) p.kw = 8;
     } else if (eight && B * heads >= 128 && even > 1) {
@@ -641,6 +649,7 @@ int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k
     a.Hq = static_cast<int>(Hq), a.Hkv = static_cast<int>(Hkv), a.R = static_cast<int>(R);
     a.head_tiles = static_cast<int>(cdiv(R, 16));
     a.target = static_cast<int>(p.target), a.least = static_cast<int>(p.least);
+    a.whole = p.items <= B;
     a.lds_heads = static_cast<int>(R < 16 ? R : 16);
     a.scale_log2 = scale * kPgLog2e, a.out = out, a.out_sb = out_sb;
     a.part_o = static_cast<float*>(workspace);

@@ -360,3 +360,19 @@ def test_packed_short_sequences_in_a_large_batch(dtype, Hq, Hkv, D, causal):
         want, bf, f32 = attend(qn[t, :R], kn[a + 40:e, 0], vn[a + 40:e, 0], D ** -0.5)
         ok = ~nan[t, :R].numpy()
         assert (np.abs(got[t, :R].numpy() - want)[ok] <= (bf if dtype == BF else f32)[ok]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("n", [63, 64, 65, 128, 1000, 4097])
+def test_packed_search_over_many_offsets(dtype, n):
+    print(f"[case] packed {n} sequences {dtype}", flush=True)
+    r = np.random.default_rng(n)
+    lengths = np.where(r.random(n) < 0.3, 0, r.integers(1, 5, n))
+    lengths[-1] = 3
+    cu = offsets(lengths, start=2)
+    N = int(cu[-1]) + 1
+    q, k, v = inputs(N, 3, 1, 64, dtype, seed=n)
+    out = torch.full((N, 192), 7.0, dtype=dtype, device=DEV)
+    sparda.prefill_packed(q.to(DEV), k.to(DEV), v.to(DEV), torch.from_numpy(cu).to(DEV), out=out)
+    assert (out[:2] == 7).all() and (out[N - 1] == 7).all()
+    check(out, q, k, v, cu, rows=range(0, N, 1 + N // 500))

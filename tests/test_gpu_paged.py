@@ -85,6 +85,40 @@ def test_paged_decode_over_many_shares(dtype, Hq, Hkv, D, lengths):
     check(got, q, ks, vs)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("Hq,Hkv,D", [(6, 2, 16), (3, 3, 32), (34, 1, 128)])
+def test_paged_decode_shares_of_other_heads(dtype, Hq, Hkv, D):
+    print(f"[case] paged shares {dtype} {Hq}/{Hkv}x{D}", flush=True)
+    lengths = [4100, 0, 1, 2999]
+    kp, vp, table, ks, vs = cache(lengths, 32, Hkv, D, dtype, seed=D)
+    q = queries(len(lengths), Hq, D, dtype, seed=10) * 2
+    got = sparda.decode_paged(q.to(DEV), kp.to(DEV), vp.to(DEV), table.to(DEV),
+                              torch.tensor(lengths, dtype=torch.int32, device=DEV))
+    check(got, q, ks, vs)
+
+
+@pytest.mark.parametrize("n", [64, 65, 1000, 4097])
+def test_paged_append_of_many_sequences(n):
+    print(f"[case] paged append {n} sequences", flush=True)
+    r = np.random.default_rng(n)
+    lengths = np.where(r.random(n) < 0.3, 0, r.integers(1, 5, n))
+    cu = np.concatenate(([0], np.cumsum(lengths))).astype(np.int32)
+    N, ps = int(cu[-1]), 16
+    pos = r.integers(-1, 28, n).astype(np.int32)
+    table = r.permutation(2 * n).reshape(n, 2).astype(np.int32)
+    kn, vn = (torch.randn(N + 3, 2, 16, generator=torch.Generator().manual_seed(i)).to(BF) for i in (1, 2))
+    kp, vp = (torch.full((2 * n, ps, 2, 16), 7.0, dtype=BF) for _ in range(2))
+    kd, vd = kp.to(DEV), vp.to(DEV)
+    dev = lambda x: torch.from_numpy(x).to(DEV)
+    sparda.append_paged(kd, vd, dev(table), dev(pos), kn.to(DEV), vn.to(DEV), cu_seqlens=dev(cu))
+    for b in range(n):
+        for j in range(lengths[b]):
+            p = int(pos[b]) + j
+            if pos[b] >= 0:
+                kp[table[b, p // ps], p % ps], vp[table[b, p // ps], p % ps] = kn[cu[b] + j], vn[cu[b] + j]
+    assert torch.equal(kd.cpu(), kp) and torch.equal(vd.cpu(), vp) and sparda.status() == 0
+
+
 def test_paged_decode_of_many_sequences():
     print("[case] paged 200 sequences", flush=True)
     r = np.random.default_rng(3)
