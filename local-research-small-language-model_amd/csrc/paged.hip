@@ -118,58 +118,53 @@ __device__ __forceinline__ int paged_steps(int len, int cap, int step) {
     return static_cast<int>((static_cast<int64_t>(c) + step - 1) / step);
 }
 
-__device__ __forceinline__ int wave_sum_i32(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+// Inclusive sums over the lanes: within rows of 16 by shifts, then the rows' totals.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int add_dpp(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan_i32(int v) {
+    v = add_dpp<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+    v = add_dpp<0x112, 0xf>(v);
+    v = add_dpp<0x114, 0xf>(v);
+    v = add_dpp<0x118, 0xf>(v);
+    v = add_dpp<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+    v = add_dpp<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
     return v;
 }
-__device__ __forceinline__ int wave_scan_i32(int v) {  // inclusive
-    const int lane = threadIdx.x % kWave;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const int w = __shfl_up(v, o, kWave);
-        if (lane >= o) v += w;
-    }
-    return v;
-}
+__device__ __forceinline__ int wave_last(int v) { return __builtin_amdgcn_readlane(v, kWave - 1); }
 
-// Steps of an item. The total stays below 2^31 (checked by the host against the capacity).
-__device__ __forceinline__ int paged_share(const int32_t* __restrict__ len, int B, int cap, int step, int target,
-                                           int least) {
-    const int lane = threadIdx.x % kWave;
-    int total = 0;
-    for (int b0 = 0; b0 < B; b0 += kWave) total += b0 + lane < B ? paged_steps(len[b0 + lane], cap, step) : 0;
-    total = __builtin_amdgcn_readfirstlane(wave_sum_i32(total));
-    const int share = (total + target - 1) / target;
-    return share > least ? share : least;
-}
-
-// The item's sequence (by_item), or sequence `want`'s items. Wave-uniform.
+// The item's sequence (by_item), or sequence `want`'s items. Wave-uniform. The total
+// of the steps stays below 2^31 (checked by the host against the capacity).
 __device__ __forceinline__ Share paged_item(const int32_t* __restrict__ len, int B, int cap, int step, int target,
                                             int least, bool by_item, int want) {
     const int lane = threadIdx.x % kWave;
-    Share r{-1, 0, 0, 0, paged_share(len, B, cap, step, target, least), 0, false};
+    auto at_least = [&](int total) { return max(least, (total + target - 1) / target); };
+    auto found = [&](int seq, int l, int parts, int first) {
+        return Share{seq, by_item ? want - first : 0, parts, first, (paged_steps(l, cap, step) + parts - 1) / parts,
+                     l < 0 ? 0 : l > cap ? cap : l, l < 0 || l > cap};
+    };
+    if (B == 1) {
+        const int l = __builtin_amdgcn_readfirstlane(len[0]), steps = paged_steps(l, cap, step), share = at_least(steps);
+        const int parts = max(1, (steps + share - 1) / share);
+        return by_item && want >= parts ? Share{-1} : found(0, l, parts, 0);
+    }
+    int total = 0;
+    for (int b0 = 0; b0 < B; b0 += kWave) total += wave_last(wave_scan_i32(b0 + lane < B ? paged_steps(len[b0 + lane], cap, step) : 0));
+    const int share = at_least(total);
     int before = 0;
     for (int b0 = 0; b0 < B; b0 += kWave) {
-        const int b = b0 + lane;
-        const int n = b < B ? max(1, (paged_steps(len[b], cap, step) + r.share - 1) / r.share) : 0;
+        const int b = b0 + lane, l = b < B ? len[b] : 0;
+        const int n = b < B ? max(1, (paged_steps(l, cap, step) + share - 1) / share) : 0;
         const int end = before + wave_scan_i32(n);      // items of sequences 0 .. b
         const uint64_t m = __ballot(b < B && (by_item ? end > want : b == want));
         if (m != 0) {
-            const int at = __builtin_ctzll(m);
-            r.seq = b0 + at;
-            r.parts = __builtin_amdgcn_readfirstlane(__shfl(n, at, kWave));
-            r.first = __builtin_amdgcn_readfirstlane(__shfl(end, at, kWave)) - r.parts;
-            r.part = by_item ? want - r.first : 0;
-            const int l = __builtin_amdgcn_readfirstlane(len[r.seq]);
-            r.share = (paged_steps(l, cap, step) + r.parts - 1) / r.parts;
-            r.bad = l < 0 || l > cap;
-            r.len = l < 0 ? 0 : l > cap ? cap : l;
-            return r;
+            const int at = __builtin_ctzll(m), parts = __builtin_amdgcn_readlane(n, at);
+            return found(b0 + at, __builtin_amdgcn_readlane(l, at), parts, __builtin_amdgcn_readlane(end, at) - parts);
         }
-        before = __builtin_amdgcn_readfirstlane(__shfl(end, kWave - 1, kWave));
+        before = wave_last(end);
     }
-    return r;
+    return Share{-1};
 }
 
 template <int DT>
