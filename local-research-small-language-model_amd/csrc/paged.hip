@@ -579,17 +579,20 @@ namespace {
 // How a launch is cut. us, 12/4 heads of 64 and 32/8 of 128 where named:
 //  - A table whose sequences are short, or a batch that gives every CU a workgroup:
 //    one item a sequence, written straight to the output, no second launch
-//    (B=1, 300 positions 5.1 against 8.2 in shares, 700 7.1 / 8.3, 500 of 32/8 heads
-//    8.3 / 9.2; B=64, 1000: 11.3 / 15.3; B=128, 300: 7.5 / 12.6; B=1000, 2000: 256 / 274).
-//    Fewer and longer sequences are faster in shares (B=1, 1000: 8.7 / 8.2, of 32/8
-//    heads 13.1 / 9.3; B=128, 4000: 75.9 / 69.0).
+//    (B=1, 200 positions 4.6 against 6.3 in shares, 500 6.2 / 6.4; B=4, 600: 6.7 / 7.4; B=16,
+//    300: 5.3 / 7.5; 200 of 32/8 heads 5.8 / 7.3; B=64, 1000: 11.3 / 15.0; B=1000, 2000:
+//    253 / 269). Fewer and longer sequences are faster in shares (B=1, 1000: 8.7 / 6.4;
+//    500 of 32/8 heads 8.3 / 7.5; B=128, 4000: 75.0 / 68.6).
 //  - Many (sequence, head) pairs: workgroups of 2 or 4 neighbouring heads, which
 //    fetch whole rows of a page at a time (B=32, 16384, 32/8 heads of 128: 257
 //    against 290 with one head a workgroup; 8/8 heads of 64: 137 / 180).
 //  - Otherwise one head a workgroup: four wavefronts on its keys make four times
-//    fewer partials for the join (B=1, 131000: 31.4 / 35). About as many
-//    workgroups as the chip holds: shares of half the length cost a longer join
-//    (B=1, 131000: 34), twice the length a longer walk (B=8, 16384: 26.2 / 25.4).
+//    fewer partials for the join (B=1, 131000: 31.4 / 35). A workgroup on every CU where
+//    sequences are few: more of them cost a longer join (256 / 512 / 1024, B=1, 40000:
+//    12.9 / 13.4 / 15.3, in fp32 131000 44.4 / 49.2 / 47.7; B=16, 4000: 14.6 / 14.7 / 15.3);
+//    with more sequences the shares come out uneven, and more of them even that out
+//    (B=80, 8000, 8/1 heads 28.7 / 24.6 / 25.1; B=22, 10000: 32.3 / 35.0 / 31.8). Heads of 128, two
+//    a CU (B=1, 50000, 32/8 heads 47.8 / 37.7; B=2, 40000: 59.6 / 45.7).
 struct PagedPlan {
     int hg, kw;              // head tiles, and wavefronts for each, of a workgroup
     int64_t target, least;   // items aimed at, steps of the smallest item
@@ -601,7 +604,7 @@ PagedPlan paged_plan(int64_t B, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D,
     const int even = heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
     const bool eight = (R < 16 ? R : 16) * (D + 4) + 33 <= 2048;  // eight wavefronts' partials fit 64 KB of LDS
     PagedPlan p{1, 4, 1, 4, 0, 0, false};
-    if (steps <= (D == 128 ? 16 : 24) || (steps <= 64 && B * heads >= 128)) {
+    if (steps <= (D == 128 ? 12 : B == 1 ? 16 : 20) || (steps <= 64 && B * heads >= 128)) {
         p.least = steps;
         if (eight && steps > 8 && B * heads < 512) p.kw = 8;
     } else if (eight && B * heads >= 128 && even > 1) {
@@ -611,7 +614,7 @@ PagedPlan paged_plan(int64_t B, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D,
         const int64_t round = cdiv(512, heads / even);
         p.target = cdiv(B + round / 2, round) * round - B;
     } else {
-        p.target = (D == 128 ? 512 : 1024) / heads - B / 2;
+        p.target = (D == 128 ? 512 : B * heads <= 64 ? 256 : 1024) / heads - B / 2;
     }
     if (p.target < 1) p.target = 1;
     p.groups = heads / p.hg;
