@@ -14,6 +14,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/Allocator.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -558,13 +559,13 @@ PyObject* decode_paged(PyObject* const* a) {
     const float scale = scale_or(a[5], p.D);
     x.on_current();
     const size_t bytes = g.decode_paged_workspace_bytes(p.B, p.width, p.ps, Hq, p.Hkv, p.D, code(q));
-    at::Tensor part;  // the shares' partials, held until the launch is enqueued
-    if (bytes > 0) part = x.empty({static_cast<int64_t>(bytes)}, at::kByte);
+    at::DataPtr part;  // the shares' partials, held until the launches are enqueued
+    if (bytes > 0) part = c10::GetAllocator(at::kCUDA)->allocate(bytes);
     const at::Tensor out = x.empty({p.B, Hq * p.D}, q.scalar_type());
     return result(run(g.decode_paged, q.data_ptr(), q.stride(0), q.stride(1), p.k.data_ptr(), p.v.data_ptr(), code(q),
                       p.P, p.ps, p.k.stride(0), p.k.stride(1), p.k.stride(2),
                       static_cast<const int32_t*>(p.table.data_ptr()), p.table.stride(0), p.width, len, p.B, Hq, p.Hkv,
-                      p.D, scale, out.data_ptr(), out.stride(0), bytes > 0 ? part.data_ptr() : nullptr, bytes,
+                      p.D, scale, out.data_ptr(), out.stride(0), part.get(), bytes,
                       x.stream()),
                   out);
 }
