@@ -86,9 +86,10 @@ struct PackedPrefill {
 // group has it and nothing is rescaled. A sum past 2^64, or a first tile of -inf
 // alone, sends the workgroup over its keys twice more: for the exact maxima, then
 // against them. Bound by the matrix cores and the exponentials, which share the
-// issue slots: 16384 tokens of 12/4 heads of 64 take 407-430 us = 960-1010 TFLOP/s of
-// the 1210 that a large library product reaches (matrix cores busy 50% of the time by the
-// counters), 8 sequences of 16000 in all, 32/8 heads of 128, 376 us = 900 TFLOP/s.
+// issue slots, at the clock that the card holds under them (about 1.9 GHz): 16384 tokens of
+// 12/4 heads of 64 take 407-430 us = 960-1010 TFLOP/s of the 1210 that a large library
+// product reaches, the matrix cores busy in half of the cycles; 8 sequences of 16000 in all,
+// 32/8 heads of 128, 376 us = 900 TFLOP/s.
 template <int D, int NT, int CW, int KG, int KB>
 __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(PackedPrefill a) {
     constexpr int kCols = 32 * NT, kBM = CW * kCols;
