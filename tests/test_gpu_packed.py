@@ -376,3 +376,16 @@ def test_packed_search_over_many_offsets(dtype, n):
     sparda.prefill_packed(q.to(DEV), k.to(DEV), v.to(DEV), torch.from_numpy(cu).to(DEV), out=out)
     assert (out[:2] == 7).all() and (out[N - 1] == 7).all()
     check(out, q, k, v, cu, rows=range(0, N, 1 + N // 500))
+
+
+@pytest.mark.parametrize("dtype,N,Hq,Hkv,D", [(BF, 600_000, 32, 8, 128), (F32, 300_000, 32, 8, 64)], ids=str)
+def test_packed_rows_past_32_bit_offsets(dtype, N, Hq, Hkv, D):
+    # q and out beyond 2^31 bytes (bf16: 2^31 elements), sequences of 100 rows
+    print(f"[case] packed 64-bit offsets {dtype}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(17)
+    q, k, v = (torch.randn(N, h, D, generator=g, device=DEV, dtype=dtype) for h in (Hq, Hkv, Hkv))
+    cu = torch.arange(0, N + 1, 100, dtype=torch.int32, device=DEV)
+    out = sparda.prefill_packed(q, k, v, cu)
+    for a in (0, N // 2, N - 100):
+        part = [x[a:a + 100].cpu() for x in (q, k, v)]
+        check(out[a:a + 100], *part, [0, 100], rows=(0, 1, 50, 99))

@@ -495,3 +495,78 @@ def test_refusals_of_tensors_that_do_not_fit():
             call()
     with torch.no_grad():
         assert sparda.decode_paged(grad, pages, pages, table, n).shape == (4, 128)
+
+
+def test_pages_past_32_bit_offsets():
+    # 70,000 pages of 64 rows of 8 heads of 128: 4.6e9 elements, the sequences in the last pages
+    print("[case] paged 64-bit offsets", flush=True)
+    P, ps, Hkv, D = 70000, 64, 8, 128
+    kp, vp = (torch.empty(P, ps, Hkv, D, dtype=BF, device=DEV) for _ in range(2))
+    lengths = [130, 1, 64]
+    table = torch.tensor([[P - 1, P - 5, P - 2], [P - 3, 0, 0], [P - 4, 0, 0]], dtype=torch.int32, device=DEV)
+    g = torch.Generator().manual_seed(31)
+    ks, vs = ([torch.randn(n, Hkv, D, generator=g).to(BF) for n in lengths] for _ in range(2))
+    cu = torch.tensor([0, 130, 131, 195], dtype=torch.int32, device=DEV)
+    sparda.append_paged(kp, vp, table, torch.zeros(3, dtype=torch.int32, device=DEV), torch.cat(ks).to(DEV),
+                        torch.cat(vs).to(DEV), cu_seqlens=cu)
+    q = queries(3, 32, D, BF, seed=32)
+    got = sparda.decode_paged(q.to(DEV), kp, vp, table, torch.tensor(lengths, dtype=torch.int32, device=DEV))
+    check(got, q, ks, vs)
+    assert sparda.status() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_sequences_that_share_pages(dtype):
+    print(f"[case] paged shared pages {dtype}", flush=True)
+    lengths = [700, 480, 700, 1]
+    kp, vp, table, ks, vs = cache([700], 16, 2, 64, dtype, seed=12)
+    q = queries(4, 6, 64, dtype, seed=13)
+    got = sparda.decode_paged(q.to(DEV), kp.to(DEV), vp.to(DEV), table.to(DEV).expand(4, -1),
+                              torch.tensor(lengths, dtype=torch.int32, device=DEV))
+    check(got, q, [ks[0][:n] for n in lengths], [vs[0][:n] for n in lengths])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("width", [None, 512])
+def test_paged_values_that_are_not_finite(dtype, width):
+    """Scores of -inf at a sequence's first keys, at all of another's; an infinite
+    value at one position of a third: in one share a sequence, and in several."""
+    print(f"[case] paged not finite {dtype} {width}", flush=True)
+    lengths, D = [300, 90, 300, 300], 64
+    kp, vp, table, ks, vs = cache(lengths, 32, 1, D, dtype, seed=14, width=width)
+    q = queries(4, 2, D, dtype, seed=15)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    for b, upto in ((0, 200), (1, 90)):
+        for p in range(upto):
+            kp[table[b, p // 32], p % 32, 0, 0] = -float("inf")
+    vp[table[2, 100 // 32], 100 % 32, 0, 5] = float("inf")
+    got = sparda.decode_paged(q.to(DEV), kp.to(DEV), vp.to(DEV), table.to(DEV),
+                              torch.tensor(lengths, dtype=torch.int32, device=DEV)).cpu()
+    assert torch.isnan(got[1].float()).all()             # no key with a weight: 0 / 0
+    assert (got[2].view(2, D)[:, 5] == float("inf")).all()
+    check(got[3:], q[3:], ks[3:], vs[3:])
+    check(got[:1], q[:1], [ks[0][200:]], [vs[0][200:]])
+    got[2].view(2, D)[:, 5] = 0                          # (the cache's own copy of that value is finite)
+    vs[2][:, :, 5] = 0
+    check(got[2:3], q[2:3], ks[2:3], vs[2:3])
+    assert sparda.status() == 0
+
+
+def test_paged_calls_on_two_streams_at_once():
+    print("[case] paged two streams", flush=True)
+    sets = []
+    for seed, lengths in ((1, [9000, 40, 0, 3000]), (2, [5000, 7000, 12, 1])):
+        kp, vp, table, _, _ = cache(lengths, 64, 4, 64, BF, seed=seed)
+        q = queries(4, 12, 64, BF, seed=seed)
+        sets.append([x.to(DEV) for x in (q, kp, vp, table, torch.tensor(lengths, dtype=torch.int32))])
+    want = [sparda.decode_paged(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(sparda.decode_paged(*sets[i]))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(w, o) for o in outs)
