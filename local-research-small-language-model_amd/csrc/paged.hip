@@ -124,6 +124,7 @@ __device__ __forceinline__ int add_dpp(int v) {
     return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
 }
 __device__ __forceinline__ int wave_scan_i32(int v) {
+    asm volatile("s_nop 1" : "+v"(v));  // the wait states of the first DPP, on every way here
     v = add_dpp<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
     v = add_dpp<0x112, 0xf>(v);
     v = add_dpp<0x114, 0xf>(v);

@@ -82,8 +82,9 @@ struct PackedPrefill {
 //     P = exp2(S scale log2 e - ref[col])
 //     O^T[d, col] += V^T[d, key] . P^T[key, col]
 // ref[col] is the column's maximum over the sequence's first 32 keys (key 0 is
-// allowed to every column), taken before the walk from memory, so that every key
-// group has it and nothing is rescaled. A sum past 2^64, or a first tile of -inf
+// allowed to every column), which every key group takes from group 0's first block
+// before the walk, so that nothing is rescaled (each wavefront reading those keys from
+// memory again: 16 x 256 tokens 13.3 against 10.2 us). A sum past 2^64, or a first tile of -inf
 // alone, sends the workgroup over its keys twice more: for the exact maxima, then
 // against them. Bound by the matrix cores and the exponentials, which share the
 // issue slots, at the clock that the card holds under them (about 1.9 GHz): 16384 tokens of
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
         }
     };
 
-    // the columns' maxima over the keys [0, upto), straight from memory
+    // the columns' maxima over the keys [0, upto), straight from memory (second pass)
     float ref[NT], l[NT];
     auto take_refs = [&](int upto) __attribute__((always_inline)) {
 #pragma unroll
@@ -386,9 +387,29 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
     for (int pass = 0;; ++pass) {
         if (threadIdx.x == 0) flag = 0;
         if (kg < nblk) stage(kg, 0);
-        take_refs(pass == 0 && w_end > 32 ? 32 : w_end);
         clear();
-        staged_barrier();
+        if (pass == 0) {
+            staged_barrier();
+            // (group 0's first buffer is written again behind the first step's barrier at the earliest)
+            bf16x8 ka[kKS];
+#pragma unroll
+            for (int kk = 0; kk < kKS; ++kk) ka[kk] = lds_read8(&sm.st.k[0][0][0] + k_at[kk]);
+#pragma unroll
+            for (int tt = 0; tt < NT; ++tt) {
+                f32x16 s{};
+#pragma unroll
+                for (int kk = 0; kk < kKS; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[kk], qreg[tt][kk], s, 0, 0, 0);
+                const int mine = lim[tt] - 4 * hf;
+                ref[tt] = -__builtin_inff();
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    ref[tt] = fmaxf(ref[tt], 8 * (i / 4) + i % 4 <= mine ? s[i] * a.scale_log2 : -__builtin_inff());
+                ref[tt] = pair32_max(ref[tt]);
+            }
+        } else {
+            take_refs(w_end);
+            staged_barrier();
+        }
         int i = 0;
         for (; i < whole; ++i) {
             const int j = i * KG + kg;
@@ -823,9 +844,8 @@ int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void*
     const bool f32 = dtype == SPARDA_F32;
     // bf16 without staging: where 16-column windows leave every CU at most one workgroup and sequences are short, the
     // walk's latency is all there is. us of this form / the staged ones below, causal: 12/4 heads of 64: N=1
-    // 4.0 / 5.1, 37 4.2 / 5.6, 256 5.7 / 6.2, 350 6.5 / 6.7, 512 8.8 / 7.3, 4 x 128 6.7 / 6.3, 16 x 32 4.8 / 5.6;
-    // 4/4 heads: N=384 6.3 / 6.6, 512 7.0 / 7.1; 8/1 heads of 128: N=400 9.2 / 10.9, 4 x 200 11.2 / 9.4; 32/8: N=128
-    // 6.8 / 8.0, 256 10.3 / 9.4
+    // 4.0 / 5.4, 37 4.2 / 5.5, 256 5.8 / 6.0, 350 6.5 / 6.5, 512 8.8 / 7.0, 4 x 128 6.7 / 6.1, 16 x 32 5.0 / 5.6;
+    // 8/1 heads of 128: N=200 7.4 / 8.4, 400 9.2 / 10.3; 32/8: N=128 6.8 / 7.4, 256 10.3 / 9.3
     if (f32 || D == 16 || (N * Hq <= 16 * 256 && N <= 384 * n)) {
         PackedDirect a{q, q_st, q_sh, k, v, kv_st, kv_sh, cu, static_cast<int>(n), N, static_cast<int>(Hkv),
                        static_cast<int>(R), causal, 0, sl, out, out_st, status};
@@ -876,14 +896,14 @@ int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void*
     // window's serial walk where windows are few against the 256 CUs (a group's sums
     // cost a merge, so that short walks are not cut). us of (tiles a wavefront, wavefronts,
     // key groups) = (2,4,1) / (1,4,1) / (1,4,2) / (1,2,2) / (1,1,4), 12/4 heads of 64, causal:
-    //   N=64 7.8 / 6.0 / 7.4 / 5.8 / 5.8   N=1000 22.8 / 15.2 / 14.3 / 11.1 / 10.8
-    //   N=2048 38.8 / 25.0 / 23.1 / 19.4 / 21.1   N=4096 70.2 / 49.0 / 42.8 / 44.7 / 56.1
-    //   4 x 1024 38.1 / 25.8 / 22.8 / 23.0 / 30.1   16 x 256 15.6 / 13.3 / 16.3 / 16.2 / 21.8
-    //   N=8192 152 / 129 / 136 / 138 / 173   16 x 1024 67.2 / 59.5 / 72.8 / 72.9 / 105
-    //   N=16384 433 / 433 / 479 / 507 / 622   N=32768 1550 / 1627   8 x 8192 847 / 879
+    //   N=400 13.3 / 8.8 / 8.9 / 7.4 / 7.0   N=1000 22.8 / 14.9 / 13.4 / 10.7 / 10.1
+    //   N=2048 38.7 / 24.9 / 22.4 / 18.3 / 19.5   N=4096 70.5 / 48.5 / 41.0 / 42.0 / 53.1
+    //   4 x 1024 24.6 / 20.1 / 20.8 / 20.7 / 24.7   16 x 256 12.7 / 10.2 / 13.7 / 13.2 / 17.8
+    //   N=8192 152 / 127 / 131 / 133 / 165   16 x 1024 55.5 / 47.7 / 60.3 / 59.5 / 90.4
+    //   N=16384 428 / 425 / 480 / 486 / 626   N=32768 1555 / 1630   8 x 8192 847 / 889
     // and of (1,4,1) / (1,4,2) / (1,2,2 of 32 keys), heads of 128:
-    //   32/8: N=512 14.7 / 15.9 / 12.4   N=1000 23.2 / 22.9 / 22.2   N=2048 50.5 / 51.3 / 56.2
-    //   8 x 250 21.7 / 31.9 / 25.9   8 x 2000 385 / 459 / 507   8/1: N=8192 169 / 149 / 164
+    //   32/8: N=512 14.5 / 15.1 / 11.8   N=1000 23.1 / 22.2 / 20.9   N=2048 49.2 / 48.9 / 53.4
+    //   8 x 250 17.1 / 22.8 / 21.1   8 x 2000 305 / 370 / 400   8/1: N=8192 171 / 144 / 158
     const int64_t W = cdiv(N * Hq, 128), NB = cdiv(cdiv(N, n), 64), cus = 256;
     if (D == 32) {
         SPARDA_PKM(32, 1, 4, 1, 64);
