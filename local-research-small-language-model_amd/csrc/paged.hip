@@ -584,16 +584,17 @@ namespace {
 //    300: 5.3 / 7.5; 200 of 32/8 heads 5.8 / 7.3; B=64, 1000: 11.3 / 15.0; B=1000, 2000:
 //    253 / 269). Fewer and longer sequences are faster in shares (B=1, 1000: 8.7 / 6.4;
 //    500 of 32/8 heads 8.3 / 7.5; B=128, 4000: 75.0 / 68.6).
-//  - Many (sequence, head) pairs: workgroups of 2 or 4 neighbouring heads, which
-//    fetch whole rows of a page at a time (B=32, 16384, 32/8 heads of 128: 257
-//    against 290 with one head a workgroup; 8/8 heads of 64: 137 / 180).
+//  - Many (sequence, head) pairs, or several of long sequences: workgroups of 2 or 4
+//    neighbouring heads, which fetch whole rows of a page at a time (B=32, 16384, 32/8
+//    heads of 128: 257 against 290 with one head a workgroup; 8/8 heads of 64: 137 / 180;
+//    caches read from memory, B=8, 16384: 28.3 / 30.4, B=2, 100000: 45.9 / 48.1; but
+//    8 x 4000 13.5 / 13.1, 2 x 10000 13.3 / 11.6, 1 x 131000 36.0 / 35.0).
 //  - Otherwise one head a workgroup: four wavefronts on its keys make four times
-//    fewer partials for the join (B=1, 131000: 31.4 / 35). A workgroup on every CU where
-//    sequences are few: more of them cost a longer join (256 / 512 / 1024, B=1, 40000:
-//    12.9 / 13.4 / 15.3, in fp32 131000 44.4 / 49.2 / 47.7; B=16, 4000: 14.6 / 14.7 / 15.3);
-//    with more sequences the shares come out uneven, and more of them even that out
-//    (B=80, 8000, 8/1 heads 28.7 / 24.6 / 25.1; B=22, 10000: 32.3 / 35.0 / 31.8). Heads of 128, two
-//    a CU (B=1, 50000, 32/8 heads 47.8 / 37.7; B=2, 40000: 59.6 / 45.7).
+//    fewer partials for the join (B=1, 131000: 31.4 / 35). Two workgroups a CU: fewer do
+//    not keep the memory busy, more cost a longer join (256 / 512 / 1024 / 2048 with the
+//    caches read from memory, B=1, 131000: 41.9 / 35.2 / 36.0 / 37.6, 40000: 17.8 / 16.9 / 18.5 /
+//    18.2; B=16, 4000: 20.6 / 18.2 / 18.8 / 19.6; B=1, 50000, 32/8 heads of 128 49.4 / 49.2 /
+//    50.9 / 54.2). (Caches that the last-level cache holds would have 256, by 5%.)
 struct PagedPlan {
     int hg, kw;              // head tiles, and wavefronts for each, of a workgroup
     int64_t target, least;   // items aimed at, steps of the smallest item
@@ -608,14 +609,14 @@ PagedPlan paged_plan(int64_t B, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D,
     if (steps <= (D == 128 ? 12 : B == 1 ? 16 : 20) || (steps <= 64 && B * heads >= 128)) {
         p.least = steps;
         if (eight && steps > 8 && B * heads < 512) p.kw = 8;
-    } else if (eight && B * heads >= 128 && even > 1) {
+    } else if (eight && even > 1 && (B * heads >= 128 || (B * heads >= 8 && B * heads * steps >= 7168))) {
         p.hg = even;
         p.kw = 8 / even;
-        // (items are target + B at most: whole rounds of 512 workgroups, half of one at least beside the B)
-        const int64_t round = cdiv(512, heads / even);
+        // (items are target + B at most: whole rounds of 512 or 256 workgroups, half of one at least beside the B)
+        const int64_t round = cdiv(B * heads >= 128 ? 512 : 256, heads / even);
         p.target = cdiv(B + round / 2, round) * round - B;
     } else {
-        p.target = (D == 128 ? 512 : B * heads <= 64 ? 256 : 1024) / heads - B / 2;
+        p.target = 512 / heads - B / 2;
     }
     if (p.target < 1) p.target = 1;
     p.groups = heads / p.hg;
