@@ -88,9 +88,9 @@ struct PackedPrefill {
 // alone, sends the workgroup over its keys twice more: for the exact maxima, then
 // against them. Bound by the matrix cores and the exponentials, which share the
 // issue slots, at the clock that the card holds under them (about 1.9 GHz): 16384 tokens of
-// 12/4 heads of 64 take 407-430 us = 960-1010 TFLOP/s of the 1210 that a large library
+// 12/4 heads of 64 take 407-437 us = 940-1010 TFLOP/s of the 1210 that a large library
 // product reaches, the matrix cores busy in half of the cycles; 8 sequences of 16000 in all,
-// 32/8 heads of 128, 376 us = 900 TFLOP/s.
+// 32/8 heads of 128, 354-387 us = 880-960 TFLOP/s.
 template <int D, int NT, int CW, int KG, int KB>
 __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(PackedPrefill a) {
     constexpr int kCols = 32 * NT, kBM = CW * kCols;
