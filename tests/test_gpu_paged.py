@@ -570,3 +570,20 @@ def test_paged_calls_on_two_streams_at_once():
     torch.cuda.synchronize()
     for w, outs in zip(want, got):
         assert all(torch.equal(w, o) for o in outs)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("B,Hq,Hkv,D", [(4, 40, 2, 64), (4, 128, 1, 64), (70, 12, 4, 64), (130, 6, 2, 128), (70, 5, 1, 32)])
+def test_paged_decode_in_a_wide_table(dtype, B, Hq, Hkv, D):
+    """A table far wider than the sequences: many heads a KV head, neighbouring
+    heads together, more sequences than lanes."""
+    print(f"[case] paged wide table {dtype} {B} {Hq}/{Hkv}x{D}", flush=True)
+    r = np.random.default_rng(B + Hq)
+    lengths = [int(x) for x in r.integers(0, 1500 if B < 10 else 300, B)]
+    lengths[1], lengths[-1] = 0, 1200
+    kp, vp, table, ks, vs = cache(lengths, 32, Hkv, D, dtype, seed=B, width=512)
+    q = queries(B, Hq, D, dtype, seed=16) * 2
+    args = [x.to(DEV) for x in (q, kp, vp, table, torch.tensor(lengths, dtype=torch.int32))]
+    got = sparda.decode_paged(*args)
+    check(got, q, ks, vs)
+    assert torch.equal(got, sparda.decode_paged(*args)) and sparda.status() == 0
