@@ -899,22 +899,24 @@ int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void*
     //   N=400 13.3 / 8.8 / 8.9 / 7.4 / 7.0   N=1000 22.8 / 14.9 / 13.4 / 10.7 / 10.1
     //   N=2048 38.7 / 24.9 / 22.4 / 18.3 / 19.5   N=4096 70.5 / 48.5 / 41.0 / 42.0 / 53.1
     //   4 x 1024 24.6 / 20.1 / 20.8 / 20.7 / 24.7   16 x 256 12.7 / 10.2 / 13.7 / 13.2 / 17.8
+    //   N=1600 31.1 / 20.2 / 18.6 / 15.6 / 14.4   2 x 700 19.0 / 11.6 / 11.5 / 9.7 / 10.2
+    //   2 x 2800 53.0 / 48.0 / 38.6 / 39.1 / 50.8   4 x 1400 32.5 / 27.5 / 28.7 / 25.5 / 37.1
     //   N=8192 152 / 127 / 131 / 133 / 165   16 x 1024 55.5 / 47.7 / 60.3 / 59.5 / 90.4
     //   N=16384 428 / 425 / 480 / 486 / 626   N=32768 1555 / 1630   8 x 8192 847 / 889
     // and of (1,4,1) / (1,4,2) / (1,2,2 of 32 keys), heads of 128:
-    //   32/8: N=512 14.5 / 15.1 / 11.8   N=1000 23.1 / 22.2 / 20.9   N=2048 49.2 / 48.9 / 53.4
+    //   32/8: N=512 14.5 / 15.1 / 11.8   N=1100 25.0 / 23.7 / 21.6   N=2048 49.2 / 48.9 / 53.4
     //   8 x 250 17.1 / 22.8 / 21.1   8 x 2000 305 / 370 / 400   8/1: N=8192 171 / 144 / 158
     const int64_t W = cdiv(N * Hq, 128), NB = cdiv(cdiv(N, n), 64), cus = 256;
     if (D == 32) {
         SPARDA_PKM(32, 1, 4, 1, 64);
     } else if (D == 64) {
-        if (2 * W <= cus) SPARDA_PKM(64, 1, 1, 4, 32);
+        if (2 * W <= cus || (8 * W <= 5 * cus && NB >= 20)) SPARDA_PKM(64, 1, 1, 4, 32);
         else if (W <= cus && NB >= 8) SPARDA_PKM(64, 1, 2, 2, 64);
-        else if (W <= 2 * cus && NB >= 16) SPARDA_PKM(64, 1, 4, 2, 64);
+        else if ((W <= 2 * cus && NB >= 16) || (5 * W <= 12 * cus && NB >= 32)) SPARDA_PKM(64, 1, 4, 2, 64);
         else if (W <= 8 * cus || NB < 32) SPARDA_PKM(64, 1, 4, 1, 64);
         else SPARDA_PKM(64, 2, 4, 1, 64);
     } else {
-        if (2 * W <= cus || (W <= cus && NB >= 8)) SPARDA_PKM(128, 1, 2, 2, 32);
+        if (2 * W <= cus || (W <= cus && NB >= 8) || (3 * W <= 4 * cus && NB >= 16)) SPARDA_PKM(128, 1, 2, 2, 32);
         else if (W <= 2 * cus && NB >= 64) SPARDA_PKM(128, 1, 4, 2, 64);
         else SPARDA_PKM(128, 1, 4, 1, 64);
     }

@@ -272,7 +272,7 @@ def test_packed_captured_and_replayed_with_other_offsets(dtype):
 
 
 # sizes on either side of the limits at which the work is cut differently
-CUTS = [(BF, 12, 4, 64, [500]), (BF, 12, 4, 64, [2000]), (BF, 12, 4, 64, [4200]), (BF, 12, 4, 64, [700] * 8),
+CUTS = [(BF, 12, 4, 64, [500]), (BF, 12, 4, 64, [2000]), (BF, 12, 4, 64, [1600]), (BF, 12, 4, 64, [2800, 2850]), (BF, 32, 8, 128, [1200]), (BF, 12, 4, 64, [4200]), (BF, 12, 4, 64, [700] * 8),
         (BF, 12, 4, 64, [9000, 13001]), (BF, 16, 16, 64, [1500, 600]), (BF, 32, 8, 128, [400]), (BF, 12, 4, 32, [900, 77]), (BF, 6, 2, 16, [300, 40]), (F32, 6, 2, 32, [300, 40]), (BF, 8, 2, 128, [4300]),
         (BF, 32, 8, 128, [150] * 10), (BF, 32, 8, 128, [3000, 2000]), (F32, 12, 4, 64, [3000]), (F32, 8, 1, 128, [1000, 700]),
         (BF, 12, 4, 64, [300, 41]), (BF, 8, 2, 128, [260, 33]), (BF, 8, 4, 32, [380, 100]), (F32, 6, 2, 32, [2000]),
