@@ -878,7 +878,8 @@ SPARDA_API int sparda_offload_fetch(sparda_offload_t h, const int32_t* sel, cons
  *   kv_sh, 1); out: [N,Hq*D] of dtype, stride out_st; all rows 16-byte aligned,
  *   0 <= kv_st < 2^24; D in {16, 32, 64, 128}, any Hq that Hkv divides,
  *   N * Hq / Hkv < 2^31 - 256, n_seqs <= 2^30. A row outside A(t) has no part in out[t], whatever
- *   it holds. cu_seqlens: n_seqs + 1 offsets.
+ *   it holds. cu_seqlens: n_seqs + 1 offsets. Whatever the scores, no sum
+ *   overflows where |v| < 2^112 and the rows of A(t) times |v| stay below 2^125.
  */
 SPARDA_API int sparda_prefill_packed(const void* q, int64_t q_st, int64_t q_sh,
                                      const void* k, const void* v, int64_t kv_st, int64_t kv_sh,

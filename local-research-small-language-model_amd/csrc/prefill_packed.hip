@@ -21,7 +21,11 @@ constexpr float kPkLog2e = 1.4426950408889634f;
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-constexpr float kPkGuard = 18446744073709551616.0f;  // 2^64
+constexpr float kPkGuard = 18446744073709551616.0f;  // 2^64: a sum of weights past it means a score far above the reference
+constexpr float kPkOutGuard = 1329227995784915872903807060280344576.0f;  // 2^120: below it the key groups' outputs add up without overflow
+// 2^12: outputs are looked at where a lane's sum of weights passes it. Smaller sums (short prompts of ordinary
+// scores) take values below 2^112 nowhere near overflow; looking at all outputs took 0.2-0.3 us of 11-17.
+constexpr float kPkFar = 4096.0f;
 
 // 16-byte piece `c` of row `r` in an LDS tile of D-element rows: pieces are
 // exchanged within a row so that both reads of a tile are spread over the banks:
@@ -84,9 +88,10 @@ struct PackedPrefill {
 // ref[col] is the column's maximum over the sequence's first 32 keys (key 0 is
 // allowed to every column), which every key group takes from group 0's first block
 // before the walk, so that nothing is rescaled (each wavefront reading those keys from
-// memory again: 16 x 256 tokens 13.3 against 10.2 us). A sum past 2^64, or a first tile of -inf
-// alone, sends the workgroup over its keys twice more: for the exact maxima, then
-// against them. Bound by the matrix cores and the exponentials, which share the
+// memory again: 16 x 256 tokens 13.3 against 10.2 us). A sum past 2^64, an output past 2^120
+// (weights far above 1 times large values), or a first tile of -inf alone sends the
+// workgroup over its keys twice more: for the exact maxima, then against them, where
+// no weight passes 1. Bound by the matrix cores and the exponentials, which share the
 // issue slots, at the clock that the card holds under them (about 1.9 GHz): 16384 tokens of
 // 12/4 heads of 64 take 407-437 us = 940-1010 TFLOP/s of the 1210 that a large library
 // product reaches, the matrix cores busy in half of the cycles; 8 sequences of 16000 in all,
@@ -384,11 +389,15 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
     // step i: group kg computes block i KG + kg from buffer i & 1 while its next is loaded
     // (first the steps whose blocks every column of the workgroup attends)
     const int steps = (nblk + KG - 1) / KG, whole = (a.causal ? col0 / a.R + 1 : len) / KB / KG;
+    // pass 0: against the first block's maxima; 1, after a sum or an output past its guard:
+    // against the exact ones; 2, after an output past its guard that 1 did not bring back
+    // (a value that is not finite): as 0, so that such a value changes no other output
+    int why = 0, past = 0;
     for (int pass = 0;; ++pass) {
         if (threadIdx.x == 0) flag = 0;
         if (kg < nblk) stage(kg, 0);
         clear();
-        if (pass == 0) {
+        if (pass != 1) {
             staged_barrier();
             // (group 0's first buffer is written again behind the first step's barrier at the earliest)
             bf16x8 ka[kKS];
@@ -424,13 +433,41 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
                 if (key0 + 32 * hh < w_end) compute(buf, hh, key0 + 32 * hh);
             staged_barrier();
         }
-        if (pass == 1) break;
-        bool over = false;
+        if (pass == 2) break;
+        bool over = false, far = false;
 #pragma unroll
-        for (int tt = 0; tt < NT; ++tt) over = over || (live && (!(l[tt] <= kPkGuard) || ref[tt] == -__builtin_inff()));
-        if (__ballot(over) != 0 && lane == 0) atomicOr(&flag, 1);
+        for (int tt = 0; tt < NT; ++tt) {
+            over = over || (live && (!(l[tt] <= kPkGuard) || ref[tt] == -__builtin_inff()));
+            far = far || (live && !(l[tt] <= kPkFar));
+        }
+        int now = 0;                                          // outputs past the guard (wave-uniform)
+        if (pass == 1 || __ballot(far) != 0) {
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};          // (infinities and NaN stay in it)
+#pragma unroll
+            for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+                for (int dt = 0; dt < kDT; ++dt)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) sum[x & 3] += __builtin_fabsf(o[tt][dt][x]);
+            const float guard = pass == 0 ? kPkOutGuard : 32.0f * kPkOutGuard;  // (2^125 against the exact maxima)
+            far = live && !((sum[0] + sum[1]) + (sum[2] + sum[3]) <= guard);
+            if (__ballot(far) != 0) {
+#pragma unroll
+                for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+                    for (int dt = 0; dt < kDT; ++dt)
+#pragma unroll
+                        for (int x = 0; x < 16; ++x)
+                            now += __builtin_popcountll(__ballot(far && !(__builtin_fabsf(o[tt][dt][x]) <= guard)));
+            }
+        }
+        const int mine = pass == 0 ? (__ballot(over) != 0 ? 1 : 0) | (now != 0 ? 2 : 0) : now < past ? 1 : 0;
+        if (mine != 0 && lane == 0) atomicOr(&flag, mine);
+        past = now;
         __syncthreads();
-        if (flag == 0) break;                                 // workgroup-uniform
+        const int all = flag;                                 // workgroup-uniform
+        if (pass == 0 ? all == 0 : why != 2 || all != 0) break;
+        why = all;
         __syncthreads();                                      // (read by all before it is cleared)
     }
     if (__ballot(odd) != 0) {                                 // wave-uniform
