@@ -107,8 +107,9 @@ enum {
      * limit (never expected: waits end when earlier tiles commit). Its query
      * window's output rows were written as NaN. */
     SPARDA_STATUS_PREFILL_WAIT_TIMEOUT = 1,
-    /* Offsets of packed sequences that fall or leave [0, N]. Rows of such a
-     * sequence may not have been written. */
+    /* Offsets of packed sequences that fall or leave [0, N]. Such a sequence is
+     * left out; rows of an earlier one that lie at or behind a later sequence's
+     * start may be too. */
     SPARDA_STATUS_SEQUENCE_RANGE = 2,
     /* A page index outside [0, n_pages), or a length or position outside the
      * page table's row. The sequence's output rows were written as NaN

@@ -51,8 +51,8 @@ append_paged_kernel(char* __restrict__ k, char* __restrict__ v, Pages pg, int ps
         // the last sequence that starts at or before t, when t is one of its rows
         int c0, c1;
         seq = packed_find(cu, n, [&](int c, int) { return c <= t; }, c0, c1);
-        if (seq < 0) return;
-        if (t >= c1) return;                      // behind the last sequence
+        if (seq < 0 || t >= c1) return;           // before the first sequence, behind the last
+        if (c0 < 0 || c1 > N) return;             // (offsets out of range: the sequence is left out)
         at = t - c0;
     }
     const int p0 = __builtin_amdgcn_readfirstlane(positions[seq]);

@@ -1175,7 +1175,8 @@ def prefill_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
     h reads KV head h // (Hq // Hkv). Sequences may be empty; rows of `out`
     outside every sequence keep what they hold (with out=None: anything).
     Returns out [N,Hq*D]. Offsets that fall or leave [0, N]: that sequence's
-    rows are not written and status() has STATUS_SEQUENCE_RANGE.
+    rows are not written and status() has STATUS_SEQUENCE_RANGE (rows of an
+    earlier sequence at or behind a later one's start may be left out too).
     """
     if out is None:
         r = _host.prefill_packed(q, k, v, cu_seqlens, causal, scale)
@@ -1236,7 +1237,8 @@ def append_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch
     k_new/v_new [N,Hkv,D] are packed, and row j of sequence b goes to
     positions[b] + j. A sequence with a negative position takes no part; a row
     whose page is missing or outside the cache is dropped and status() has
-    STATUS_PAGE_RANGE (STATUS_SEQUENCE_RANGE for offsets that fall or leave [0, N]).
+    STATUS_PAGE_RANGE. A sequence whose offsets fall or leave [0, N] is left out
+    as in ``prefill_packed``, and status() has STATUS_SEQUENCE_RANGE.
     """
     r = _host.append_paged(k_pages, v_pages, page_table, positions, k_new, v_new, cu_seqlens)
     if r is not None:
