@@ -912,7 +912,8 @@ SPARDA_API size_t sparda_decode_paged_workspace_bytes(int64_t B, int64_t width, 
  *   out[b,h*D+d] = sum_{p < lengths[b]} softmax_p(q[b,h].k[p,g] * scale) v[p,g,d];
  * zeros where lengths[b] is 0.
  *   q: [B,Hq,D] of dtype, strides (q_sb, q_sh, 1), rows 16-byte aligned; B, Hq
- *   <= 65535; lengths: [B]; out: [B,Hq*D] of dtype, stride out_sb. The keys of the whole
+ *   <= 65535, width * page_size <= 2^31 - 64, B * ceil(width * page_size / 16) <
+ *   2^30; lengths: [B]; out: [B,Hq*D] of dtype, stride out_sb. The keys of the whole
  *   batch are cut into equal shares over the workgroups; the shares of a
  *   sequence are joined by a second launch through the workspace (written and
  *   read within the call; calls that share one must be ordered on one stream).

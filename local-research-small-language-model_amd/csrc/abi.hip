@@ -1008,7 +1008,9 @@ SPARDA_API int sparda_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, co
     SPARDA_REQUIRE(B > 0 && B <= 65535 && Hq > 0 && Hq <= 65535, SPARDA_ERR_SHAPE,
                    "decode_paged: sequences and query heads must be in [1, 65535]");
     SPARDA_REQUIRE(Hq % Hkv == 0, SPARDA_ERR_SHAPE, "decode_paged: Hq must be a multiple of Hkv");
-    SPARDA_REQUIRE(B * cdiv(width * page_size, 16) < (1ll << 31), SPARDA_ERR_SHAPE, "decode_paged: too many positions");
+    // (the kernels add steps of the whole batch and shares of it, and positions and a step, in 32 bits)
+    SPARDA_REQUIRE(width * page_size <= (1ll << 31) - 64 && B * cdiv(width * page_size, 16) < (1ll << 30), SPARDA_ERR_SHAPE,
+                   "decode_paged: too many positions");
     const int64_t ve = 16 / (dtype == SPARDA_F32 ? 4 : 2);
     SPARDA_REQUIRE(aligned16(q) && q_sb % ve == 0 && q_sh % ve == 0, SPARDA_ERR_STRIDE,
                    "decode_paged: the rows of q must be 16-byte aligned");

@@ -136,7 +136,8 @@ __device__ __forceinline__ int wave_scan_i32(int v) {
 __device__ __forceinline__ int wave_last(int v) { return __builtin_amdgcn_readlane(v, kWave - 1); }
 
 // The item's sequence (by_item), or sequence `want`'s items. Wave-uniform. The total
-// of the steps stays below 2^31 (checked by the host against the capacity).
+// of the steps stays below 2^30 (checked by the host against the capacity), so that
+// the sums with the target or a share stay in 32 bits.
 __device__ __forceinline__ Share paged_item(const int32_t* __restrict__ len, int B, int cap, int step, int target,
                                             int least, bool by_item, int want) {
     const int lane = threadIdx.x % kWave;
