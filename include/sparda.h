@@ -878,7 +878,8 @@ SPARDA_API int sparda_offload_fetch(sparda_offload_t h, const int32_t* sel, cons
  *   q: [N,Hq,D] strides (q_st, q_sh, 1); k, v: [N,Hkv,D] strides (kv_st,
  *   kv_sh, 1); out: [N,Hq*D] of dtype, stride out_st; all rows 16-byte aligned,
  *   0 <= kv_st < 2^24; D in {16, 32, 64, 128}, any Hq that Hkv divides,
- *   N * Hq / Hkv < 2^31 - 256, n_seqs <= 2^30. A row outside A(t) has no part in out[t], whatever
+ *   N * Hq / Hkv < 2^31 - 256, n_seqs <= 2^30; a launch of 2^32 threads is refused
+ *   (N * Hq / 16 + n_seqs * Hkv < 2^24 always stays below). A row outside A(t) has no part in out[t], whatever
  *   it holds. cu_seqlens: n_seqs + 1 offsets. Whatever the scores, no sum
  *   overflows where |v| < 2^112 and the rows of A(t) times |v| stay below 2^125.
  */
@@ -893,7 +894,7 @@ SPARDA_API int sparda_prefill_packed(const void* q, int64_t q_st, int64_t q_sh,
  * position positions[i] + j.
  *   k_new, v_new: [N,Hkv,D] of dtype, strides (new_st, new_sh, 1), rows 16-byte
  *   aligned; cu_seqlens: the sequences' rows, or NULL: one row per sequence,
- *   N = n_seqs. A sequence with a negative position takes no part. Two rows for
+ *   N = n_seqs; N <= 2^26 - 4. A sequence with a negative position takes no part. Two rows for
  *   the same page row in one call leave either of them there.
  */
 SPARDA_API int sparda_append_paged(void* k_pages, void* v_pages, int dtype, int64_t n_pages, int64_t page_size,
@@ -913,7 +914,8 @@ SPARDA_API size_t sparda_decode_paged_workspace_bytes(int64_t B, int64_t width, 
  * zeros where lengths[b] is 0.
  *   q: [B,Hq,D] of dtype, strides (q_sb, q_sh, 1), rows 16-byte aligned; B, Hq
  *   <= 65535, width * page_size <= 2^31 - 64, B * ceil(width * page_size / 16) <
- *   2^30; lengths: [B]; out: [B,Hq*D] of dtype, stride out_sb. The keys of the whole
+ *   2^30; a launch of 2^32 threads is refused (B * Hkv * ceil(Hq / Hkv / 16) < 2^22
+ *   always stays below); lengths: [B]; out: [B,Hq*D] of dtype, stride out_sb. The keys of the whole
  *   batch are cut into equal shares over the workgroups; the shares of a
  *   sequence are joined by a second launch through the workspace (written and
  *   read within the call; calls that share one must be ordered on one stream).

@@ -38,6 +38,8 @@ int launch_prefill_routed(const void* q, int64_t q_sb, int64_t q_st, int64_t q_s
 
 // copy the device's status word (SPARDA_STATUS_* bits) to out, clearing it when asked
 int launch_read_status(uint32_t* out, int clear, hipStream_t stream);
+// a launch counts its threads in 32 bits
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks < (int64_t(1) << 32) && blocks * threads < (int64_t(1) << 32); }
 // the current device's status word, for kernels of other sources
 int status_word(uint32_t** word);
 

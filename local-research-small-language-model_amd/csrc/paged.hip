@@ -80,6 +80,7 @@ int launch_append_paged(void* k, void* v, int64_t n_pages, int64_t ps, int64_t p
                         int dtype, const int32_t* table, int64_t t_st, int64_t width, const int32_t* positions,
                         const int32_t* cu, int64_t n, const void* k_new, const void* v_new, int64_t N, int64_t new_st,
                         int64_t new_sh, int64_t Hkv, int64_t D, hipStream_t stream) {
+    if (!grid_fits(cdiv(N, 4), 256)) return set_error(SPARDA_ERR_SHAPE, "append_paged: grid too large");
     uint32_t* status;
     if (const int rc = status_word(&status)) return rc;
     const Pages pg{p_st, s_st, h_st, table, t_st, static_cast<int>(width), static_cast<int>(n_pages)};
@@ -641,9 +642,10 @@ int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k
                         int64_t t_st, int64_t width, const int32_t* len, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
                         float scale, void* out, int64_t out_sb, void* workspace, hipStream_t stream) {
     PagedDecode a{};
-    if (const int rc = status_word(&a.status)) return rc;
     const int64_t cap = width * ps, R = Hq / Hkv;
     const PagedPlan p = paged_plan(B, cap, Hq, Hkv, D, dtype);
+    if (!grid_fits(p.items * p.groups, p.hg * p.kw * kWave)) return set_error(SPARDA_ERR_SHAPE, "decode_paged: grid too large");
+    if (const int rc = status_word(&a.status)) return rc;
     a.q = q, a.q_sb = q_sb, a.q_sh = q_sh, a.k = k, a.v = v;
     a.pg = Pages{p_st, s_st, h_st, table, t_st, static_cast<int>(width), static_cast<int>(n_pages)};
     a.ps16 = static_cast<int>(ps / 16), a.len = len, a.B = static_cast<int>(B), a.cap = static_cast<int>(cap);
@@ -655,7 +657,6 @@ int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k
     a.scale_log2 = scale * kPgLog2e, a.out = out, a.out_sb = out_sb;
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = workspace ? a.part_o + p.items * Hq * D : nullptr;
-    if (p.items * p.groups >= (int64_t(1) << 31)) return set_error(SPARDA_ERR_SHAPE, "decode_paged: grid too large");
     const dim3 grid(static_cast<unsigned>(p.items * p.groups));
 #define SPARDA_PGD_W(DT_, D_, HG_, KW_)                                                                           \
     hipLaunchKernelGGL((decode_paged_kernel<DT_, D_, HG_, KW_>), grid, dim3(HG_ * KW_ * kWave),                   \

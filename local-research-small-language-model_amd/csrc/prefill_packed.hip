@@ -874,8 +874,6 @@ __global__ void __launch_bounds__(kPdWaves* kWave, 2) prefill_packed_direct_kern
 int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void* k, const void* v, int64_t kv_st,
                           int64_t kv_sh, int dtype, const int32_t* cu, int64_t n, int64_t N, int64_t Hq, int64_t Hkv,
                           int64_t D, int causal, float scale, void* out, int64_t out_st, hipStream_t stream) {
-    uint32_t* status;
-    if (const int rc = status_word(&status)) return rc;
     const int64_t R = Hq / Hkv;
     const float sl = scale * kPkLog2e;
     const bool f32 = dtype == SPARDA_F32;
@@ -885,11 +883,12 @@ int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void*
     // 8/1 heads of 128: N=200 7.4 / 8.4, 400 9.2 / 10.3; 32/8: N=128 6.8 / 7.4, 256 10.3 / 9.3
     if (f32 || D == 16 || (N * Hq <= 16 * 256 && N <= 384 * n)) {
         PackedDirect a{q, q_st, q_sh, k, v, kv_st, kv_sh, cu, static_cast<int>(n), N, static_cast<int>(Hkv),
-                       static_cast<int>(R), causal, 0, sl, out, out_st, status};
+                       static_cast<int>(R), causal, 0, sl, out, out_st, nullptr};
 #define SPARDA_PKD_N(DT_, D_, NT_)                                                                                \
     do {                                                                                                          \
         a.slots = packed_slots(N, n, R, 16 * NT_);                                                                \
-        if (a.slots * Hkv >= (int64_t(1) << 31)) return set_error(SPARDA_ERR_SHAPE, "prefill_packed: grid too large"); \
+        if (!grid_fits(a.slots * Hkv, kPdWaves * kWave)) return set_error(SPARDA_ERR_SHAPE, "prefill_packed: grid too large"); \
+        if (const int rc = status_word(&a.status)) return rc;                                                     \
         hipLaunchKernelGGL((prefill_packed_direct_kernel<DT_, D_, NT_>), dim3(static_cast<unsigned>(a.slots * Hkv)), \
                            dim3(kPdWaves * kWave), 0, stream, a);                                                 \
     } while (0)
@@ -920,11 +919,12 @@ int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void*
     }
     PackedPrefill a{static_cast<const uint16_t*>(q), q_st, q_sh, static_cast<const uint16_t*>(k),
                     static_cast<const uint16_t*>(v), kv_st, kv_sh, cu, static_cast<int>(n), N, static_cast<int>(Hkv),
-                    static_cast<int>(R), causal, 0, sl, static_cast<uint16_t*>(out), out_st, status};
+                    static_cast<int>(R), causal, 0, sl, static_cast<uint16_t*>(out), out_st, nullptr};
 #define SPARDA_PKM(D_, NT_, CW_, KG_, KB_)                                                                        \
     do {                                                                                                          \
         a.slots = packed_slots(N, n, R, 32 * NT_ * CW_);                                                          \
-        if (a.slots * Hkv >= (int64_t(1) << 31)) return set_error(SPARDA_ERR_SHAPE, "prefill_packed: grid too large"); \
+        if (!grid_fits(a.slots * Hkv, CW_ * KG_ * kWave)) return set_error(SPARDA_ERR_SHAPE, "prefill_packed: grid too large"); \
+        if (const int rc = status_word(&a.status)) return rc;                                                     \
         hipLaunchKernelGGL((prefill_packed_kernel<D_, NT_, CW_, KG_, KB_>), dim3(static_cast<unsigned>(a.slots * Hkv)), \
                            dim3(CW_ * KG_ * kWave), 0, stream, a);                                                \
     } while (0)
