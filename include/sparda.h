@@ -874,14 +874,16 @@ SPARDA_API int sparda_offload_fetch(sparda_offload_t h, const int32_t* sel, cons
  *   out[t,h*D+d] = sum_{s in A(t)} softmax_s(q[t,h].k[s,g] * scale) v[s,g,d],
  *   g = h / (Hq/Hkv), A(t) = the rows of t's sequence, those up to t if causal.
  * Sums and softmax statistics in fp32; for bf16 the weights are rounded to
- * bf16 for the product with v.
+ * bf16 for the product with v, and where whole blocks of keys are attended
+ * their sum adds the rounded ones.
  *   q: [N,Hq,D] strides (q_st, q_sh, 1); k, v: [N,Hkv,D] strides (kv_st,
  *   kv_sh, 1); out: [N,Hq*D] of dtype, stride out_st; all rows 16-byte aligned,
  *   0 <= kv_st < 2^24; D in {16, 32, 64, 128}, any Hq that Hkv divides,
  *   N * Hq / Hkv < 2^31 - 256, n_seqs <= 2^30; a launch of 2^32 threads is refused
- *   (N * Hq / 16 + n_seqs * Hkv < 2^24 always stays below). A row outside A(t) has no part in out[t], whatever
- *   it holds. cu_seqlens: n_seqs + 1 offsets. Whatever the scores, no sum
- *   overflows where |v| < 2^112 and the rows of A(t) times |v| stay below 2^125.
+ *   (N * Hq / 16 + n_seqs * Hkv < 2^24 always stays below). A row outside A(t) has
+ *   no part in out[t], whatever it holds. cu_seqlens: n_seqs + 1 offsets. Whatever
+ *   the scores, no sum overflows where |v| < 2^112 and the rows of A(t) times |v|
+ *   stay below 2^125.
  */
 SPARDA_API int sparda_prefill_packed(const void* q, int64_t q_st, int64_t q_sh,
                                      const void* k, const void* v, int64_t kv_st, int64_t kv_sh,
@@ -894,8 +896,9 @@ SPARDA_API int sparda_prefill_packed(const void* q, int64_t q_st, int64_t q_sh,
  * position positions[i] + j.
  *   k_new, v_new: [N,Hkv,D] of dtype, strides (new_st, new_sh, 1), rows 16-byte
  *   aligned; cu_seqlens: the sequences' rows, or NULL: one row per sequence,
- *   N = n_seqs; N <= 2^26 - 4. A sequence with a negative position takes no part. Two rows for
- *   the same page row in one call leave either of them there.
+ *   N = n_seqs; N <= 2^26 - 4. A sequence with a negative position takes no
+ *   part. Two rows for the same page row in one call leave 16-byte pieces of
+ *   either there.
  */
 SPARDA_API int sparda_append_paged(void* k_pages, void* v_pages, int dtype, int64_t n_pages, int64_t page_size,
                                    int64_t p_st, int64_t s_st, int64_t h_st, const int32_t* page_table,
@@ -911,14 +914,16 @@ SPARDA_API size_t sparda_decode_paged_workspace_bytes(int64_t B, int64_t width, 
 /*
  * Attention of one token per sequence over the paged cache:
  *   out[b,h*D+d] = sum_{p < lengths[b]} softmax_p(q[b,h].k[p,g] * scale) v[p,g,d];
- * zeros where lengths[b] is 0.
+ * zeros where lengths[b] is 0. Sums and softmax statistics in fp32; for bf16 the
+ * weights are rounded to bf16 for the product with v.
  *   q: [B,Hq,D] of dtype, strides (q_sb, q_sh, 1), rows 16-byte aligned; B, Hq
  *   <= 65535, width * page_size <= 2^31 - 64, B * ceil(width * page_size / 16) <
- *   2^30; a launch of 2^32 threads is refused (B * Hkv * ceil(Hq / Hkv / 16) < 2^22
- *   always stays below); lengths: [B]; out: [B,Hq*D] of dtype, stride out_sb. The keys of the whole
- *   batch are cut into equal shares over the workgroups; the shares of a
- *   sequence are joined by a second launch through the workspace (written and
- *   read within the call; calls that share one must be ordered on one stream).
+ *   2^30; a launch of 2^32 threads is refused (B * Hkv * ceil(Hq / Hkv / 16) <
+ *   2^22 always stays below); lengths: [B]; out: [B,Hq*D] of dtype, stride
+ *   out_sb. The keys of the whole batch are cut into equal shares over the
+ *   workgroups; the shares of a sequence are joined by a second launch through
+ *   the workspace (written and read within the call; calls that share one must
+ *   be ordered on one stream).
  *   The result depends on the batch's lengths through the order of summation.
  */
 SPARDA_API int sparda_decode_paged(const void* q, int64_t q_sb, int64_t q_sh,

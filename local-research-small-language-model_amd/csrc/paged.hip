@@ -29,7 +29,8 @@ struct Pages {
 
 // One wavefront per new row: its sequence, its page, then the row's heads in 16-byte
 // pieces. Bound by memory, a row read and a row written: 16000 rows of 8 heads of 128
-// take 21.5 us = 6.1 TB/s; 64 rows 2.6 us, a launch and three dependent loads.
+// take 27.7 us a call = 4.7 TB/s where rows and pages change from call to call, 21.5 us =
+// 6.1 TB/s where the last-level cache holds them; 64 rows 2.6 us, a launch and three dependent loads.
 __global__ void __launch_bounds__(256)
 append_paged_kernel(char* __restrict__ k, char* __restrict__ v, Pages pg, int ps, const int32_t* __restrict__ positions,
                     const int32_t* __restrict__ cu, int n, const char* __restrict__ k_new,
@@ -245,9 +246,9 @@ __device__ __forceinline__ void paged_store(const PagedDecode& a, const Share& s
 // P operand, so nothing passes through LDS before the wavefronts are joined. A
 // tile's 16 keys lie in one page (pages hold a multiple of 16 rows), so that its
 // base address is a scalar. Bound by memory where the cache is long: 32 sequences of up to
-// 16384 positions, 32/8 heads of 128, 1.43 GB in 246 us = 5.8 TB/s; 131000 positions of 12/4
-// heads of 64 25.4 us = 5.3 TB/s, of which a launch and the chain lengths, table, keys
-// are 4.
+// 16384 positions, 32/8 heads of 128, 1.43 GB in 246 us = 5.8 TB/s. 131000 positions of 12/4
+// heads of 64, 134 MB, take 25.4 us from the last-level cache, of which a launch and the
+// chain lengths, table, keys are 4; a call whose cache comes from memory takes 32.0 with the join.
 template <int DT, int D, int HG, int KW>
 __global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : DT == SPARDA_F32 ? 3 : 4) decode_paged_kernel(PagedDecode a) {
     typedef PagedStep<DT, D> Step;
@@ -537,8 +538,8 @@ __global__ void __launch_bounds__(kPgJoin) decode_paged_join_kernel(PagedDecode 
     store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d0 + tid, O / den);
 }
 
-// The same for few items a sequence: one thread per (query head, dim), items in
-// order. Bound by the launch and two dependent loads: 3.0 us for 1000 positions of 12
+// The same where sequences have few items in the mean: one thread per (query head,
+// dim), items in order, eight in flight. Bound by the launch and two dependent loads: 3.0 us for 1000 positions of 12
 // heads of 64.
 template <int DT, int D>
 __global__ void __launch_bounds__(256) decode_paged_join_few_kernel(PagedDecode a) {
@@ -590,18 +591,28 @@ namespace {
 //    neighbouring heads, which fetch whole rows of a page at a time (B=32, 16384, 32/8
 //    heads of 128: 257 against 290 with one head a workgroup; 8/8 heads of 64: 137 / 180;
 //    caches read from memory, B=8, 16384: 28.3 / 30.4, B=2, 100000: 45.9 / 48.1; but
-//    8 x 4000 13.5 / 13.1, 2 x 10000 13.3 / 11.6, 1 x 131000 36.0 / 35.0).
+//    8 x 4000 13.5 / 13.1, 2 x 10000 13.3 / 11.6, 1 x 131000 36.0 / 35.0: lengths from a
+//    quarter of the longest up. Where all are as long as the table, neighbouring heads lead
+//    from below the limit on: B=8, 4000: 15.3 / 16.5, 6000: 19.5 / 20.4, 8000: 21.9 / 23.3, 12000:
+//    27.8 / 29.9; B=2, 20000: 17.1 / 17.8, 50000: 28.4 / 30.5).
 //  - Otherwise one head a workgroup: four wavefronts on its keys make four times
 //    fewer partials for the join (B=1, 131000: 31.4 / 35). Two workgroups a CU: fewer do
 //    not keep the memory busy, more cost a longer join (256 / 512 / 1024 / 2048 with the
 //    caches read from memory, B=1, 131000: 41.9 / 35.2 / 36.0 / 37.6, 40000: 17.8 / 16.9 / 18.5 /
 //    18.2; B=16, 4000: 20.6 / 18.2 / 18.8 / 19.6; B=1, 50000, 32/8 heads of 128 49.4 / 49.2 /
 //    50.9 / 54.2). (Caches that the last-level cache holds would have 256, by 5%.)
+//  - The join: one thread a dim where a sequence has 16 items in the mean, items over thread
+//    groups where it has more. us of the first / the second, caches read from memory: B=1, 1000:
+//    7.1 / 7.9; B=16, 4000: 21.7 / 22.3; B=32 of 16384, 32/8 heads of 128 381 / 395; B=32 of 300 in a
+//    table of 131072 12.3 / 14.2; B=4, 3000: 12.1 / 11.4. The host knows the mean alone: one
+//    sequence among many short ones gets nearly all items, and one thread a dim then walks
+//    hundreds of them (131000 and 31 of 300: 68.0 / 38.0; 32768 and 31 of 200, 32/8 heads of 128
+//    57.7 / 56.4).
 struct PagedPlan {
     int hg, kw;              // head tiles, and wavefronts for each, of a workgroup
     int64_t target, least;   // items aimed at, steps of the smallest item
     int64_t items, groups;   // items at most, workgroups an item
-    bool few;                // a sequence has few items
+    bool few;                // a sequence has few items in the mean
 };
 PagedPlan paged_plan(int64_t B, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D, int dtype) {
     const int64_t R = Hq / Hkv, heads = Hkv * cdiv(R, 16), steps = cdiv(cap, dtype == SPARDA_F32 ? 16 : 32);

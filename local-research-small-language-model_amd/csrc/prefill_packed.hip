@@ -85,6 +85,7 @@ struct PackedPrefill {
 //     S^T[key, col] = K[key, :] . Q[col, :]
 //     P = exp2(S scale log2 e - ref[col])
 //     O^T[d, col] += V^T[d, key] . P^T[key, col]
+// P is rounded to bf16 for the second product (half a step, 2^-8 of sum p |v| at most);
 // ref[col] is the column's maximum over the sequence's first 32 keys (key 0 is
 // allowed to every column), which every key group takes from group 0's first block
 // before the walk, so that nothing is rescaled (each wavefront reading those keys from
@@ -361,6 +362,8 @@ __global__ void __launch_bounds__(CW* KG* kWave, 2) prefill_packed_kernel(Packed
                 pv(u - 1);
                 if (NT > 1 && u % NT == 0) read_v(u / NT, va[0]);
             }
+            // the sum takes the rounded weights, two an instruction: the weights of the product are those
+            // that it is divided by
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -928,7 +931,9 @@ int launch_prefill_packed(const void* q, int64_t q_st, int64_t q_sh, const void*
         hipLaunchKernelGGL((prefill_packed_kernel<D_, NT_, CW_, KG_, KB_>), dim3(static_cast<unsigned>(a.slots * Hkv)), \
                            dim3(CW_ * KG_ * kWave), 0, stream, a);                                                \
     } while (0)
-    // W: windows of 128 columns, NB: 64-key blocks of a mean sequence. Wide windows
+    // W: windows of 128 columns, NB: 64-key blocks of a mean sequence (the host does not know
+    // the lengths: a long sequence among short ones goes with the short). Heads of 32 have one
+    // form, other calls than causal ones follow the same rule; neither was measured against others. Wide windows
     // stage a block for the most columns; key groups and small windows cut a
     // window's serial walk where windows are few against the 256 CUs (a group's sums
     // cost a merge, so that short walks are not cut). us of (tiles a wavefront, wavefronts,
