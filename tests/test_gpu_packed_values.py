@@ -85,3 +85,30 @@ def test_large_values_beside_an_infinite_one(Hq, Hkv, D, lengths, causal):
         for h in range(Hkv):
             want, bf, _ = attend(qn[t, h * R:(h + 1) * R], kn[a:e, h], vn[a:e, h][:, keep], SCALE)
             assert (np.abs(gn[t, h * R:(h + 1) * R][:, keep] - want) <= bf).all()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("Hq,Hkv,D,lengths", [f[1:] for f in FORMS if f[0] == BF], ids=str)
+def test_a_value_that_is_not_finite_changes_no_other_bit(Hq, Hkv, D, lengths, bad, causal):
+    # under weights of 2^20 against the first keys, and ordinary values
+    print(f"[case] packed {bad} alone {Hq}/{Hkv}x{D} {lengths} causal={causal}", flush=True)
+    cu = offsets(lengths)
+    N, R = int(cu[-1]), Hq // Hkv
+    a, b = int(cu[-2]), int(cu[-1])
+    g = torch.Generator().manual_seed(N + 1)
+    q, k, v = (torch.randn(N, h, D, generator=g) for h in (Hq, Hkv, Hkv))
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    k[a + 40:b:19, :, 0] = 20.0
+    q, k, v = q.to(BF).to(DEV), k.to(BF).to(DEV), v.to(BF).to(DEV)
+    cud = torch.from_numpy(cu).to(DEV)
+    clean = sparda.prefill_packed(q, k, v, cud, causal=causal, scale=SCALE).view(N, Hq, D)
+    assert torch.isfinite(clean).all()
+    for at in (a + 2, a + 40):
+        v2 = v.clone()
+        v2[at, Hkv - 1, 5] = bad
+        got = sparda.prefill_packed(q, k, v2, cud, causal=causal, scale=SCALE).view(N, Hq, D)
+        hit = torch.zeros(N, Hq, D, dtype=torch.bool, device=DEV)
+        hit[(at if causal else a):b, Hq - R:, 5] = True
+        assert torch.equal(~torch.isfinite(got), hit)
+        assert torch.equal(got[~hit], clean[~hit])
