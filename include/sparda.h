@@ -115,6 +115,10 @@ enum {
      * page table's row. The sequence's output rows were written as NaN
      * (sparda_decode_paged); the new row was dropped (sparda_append_paged). */
     SPARDA_STATUS_PAGE_RANGE = 4,
+    /* A position behind the tables of the rotation's angles
+     * (sparda_rotate_append_paged, sparda_append_paged_q4). The row was dropped, its
+     * rotated query written as NaN. */
+    SPARDA_STATUS_POSITION_RANGE = 8,
 };
 
 /*
@@ -933,6 +937,114 @@ SPARDA_API int sparda_decode_paged(const void* q, int64_t q_sb, int64_t q_sh,
                                    const int32_t* lengths, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
                                    float scale, void* out, int64_t out_sb,
                                    void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * sparda_append_paged with the rotation by position applied on the way: key row j
+ * of sequence i, at position p = positions[i] + j, is written as
+ *   y[d] = x[d] cos[p,d] - x[d+D/2] sin[p,d],  y[d+D/2] = x[d+D/2] cos[p,d] + x[d] sin[p,d]
+ * (d < D/2; in fp32, every operation rounded by itself, once to dtype at the end),
+ * the value row as it is, and the rows of q, [N,Hq,D] with strides (q_st, q_sh,
+ * 1), are rotated in the same way into q_out, strides (qo_st, qo_sh, 1); q_out may
+ * be q itself, and Hq = 0 with both NULL rotates keys alone. cos, sin: fp32
+ * [rows, D/2], rows cs_st apart. Rows of q and of the tables 16-byte aligned; Hq <=
+ * 65535, otherwise as sparda_append_paged. Rows that no sequence holds, or whose sequence
+ * has a negative position, leave q_out as it was; a row without a page is rotated in q_out
+ * and dropped in the cache; a position of `rows` or more gives NaN in
+ * q_out, a dropped row, and SPARDA_STATUS_POSITION_RANGE.
+ */
+SPARDA_API int sparda_rotate_append_paged(void* k_pages, void* v_pages, int dtype, int64_t n_pages, int64_t page_size,
+                                          int64_t p_st, int64_t s_st, int64_t h_st, const int32_t* page_table,
+                                          int64_t t_st, int64_t width, const int32_t* positions,
+                                          const int32_t* cu_seqlens, int64_t n_seqs, const void* q, int64_t q_st,
+                                          int64_t q_sh, int64_t Hq, const void* k_new, const void* v_new, int64_t N,
+                                          int64_t new_st, int64_t new_sh, int64_t Hkv, int64_t D, const float* cos,
+                                          const float* sin, int64_t cs_st, int64_t rows, void* q_out, int64_t qo_st,
+                                          int64_t qo_sh, void* stream);
+
+/*
+ * Pages of 4-bit codes. Dims are taken in groups of 32 (a head of 16 dims is half of one);
+ * G = ceil(D / 32). A group of a row x, rounded to bf16, is held as
+ *   h (2 c[d] - 15),  h = fp16(max|x| / 15),  c[d] = floor(x[d] / 2h) + 8 in 0 .. 15
+ * (4.5 bits a dim). A group with a value that is not finite is held as NaN; magnitudes
+ * above 15 * 65504 are cut off there, groups below 15 * 2^-25 are zeros.
+ * pages: [n_pages, Hkv, page_size / 16, 576 G] bytes, strides (p_st, h_st, 576 G, 1) in
+ * bytes, 16-byte aligned: 16 positions of a head (a tile) lie together,
+ *   keys' codes    byte 16 G i + 4 G p + 4 g + b of position i: dims 32 g + 8 p + e, e = 0 .. 7,
+ *                  dim e in nibble e/2 + 4 (e % 2) of the four bytes, the low one first
+ *   values' codes  byte 256 G + 4 G (16 (i / 4) + w) + 4 g + {0, 2, 1, 3}[i % 4]: dims 32 g + 2 w (low nibble), + 1
+ *   keys' h        [16][G] fp16 at 512 G, the values' behind them at 544 G.
+ * Tables, positions and offsets as for the other pages.
+ */
+
+/* sparda_append_paged into pages of 4-bit codes; with cos and sin (not NULL) the keys
+ * are rotated first and the rows of q into q_out, as sparda_rotate_append_paged does (q, q_out
+ * NULL and Hq = 0 otherwise). dtype: of q, k_new, v_new. Two rows for the same page row
+ * in one call leave a mixture of both there. */
+SPARDA_API int sparda_append_paged_q4(void* pages, int64_t n_pages, int64_t page_size, int64_t p_st, int64_t h_st,
+                                      const int32_t* page_table, int64_t t_st, int64_t width, const int32_t* positions,
+                                      const int32_t* cu_seqlens, int64_t n_seqs, const void* q, int64_t q_st,
+                                      int64_t q_sh, int64_t Hq, const void* k_new, const void* v_new, int dtype,
+                                      int64_t N, int64_t new_st, int64_t new_sh, int64_t Hkv, int64_t D,
+                                      const float* cos, const float* sin, int64_t cs_st, int64_t rows, void* q_out,
+                                      int64_t qo_st, int64_t qo_sh, void* stream);
+
+/* The values that rows of 4-bit pages stand for: k, v [N,Hkv,D] of dtype (rounded to
+ * it once), strides (st, sh, 1), rows 16-byte aligned; row j of sequence i is position
+ * positions[i] + j, cu_seqlens NULL: one row per sequence. Rows without a page are NaN; rows
+ * of no sequence, or of one with a negative position, are left as they were. */
+SPARDA_API int sparda_gather_paged_q4(const void* pages, int64_t n_pages, int64_t page_size, int64_t p_st, int64_t h_st,
+                                      const int32_t* page_table, int64_t t_st, int64_t width, const int32_t* positions,
+                                      const int32_t* cu_seqlens, int64_t n_seqs, void* k, void* v, int dtype, int64_t N,
+                                      int64_t st, int64_t sh, int64_t Hkv, int64_t D, void* stream);
+
+/* Workspace bytes sparda_decode_paged_q4 needs for these sizes (0: none). */
+SPARDA_API size_t sparda_decode_paged_q4_workspace_bytes(int64_t B, int64_t T, int64_t width, int64_t page_size,
+                                                         int64_t Hq, int64_t Hkv, int64_t D);
+
+/*
+ * sparda_decode_paged over pages of 4-bit codes, for the last T tokens of every sequence:
+ * token t of sequence b attends to positions [0, lengths[b] - T + 1 + t), zeros
+ * where that is empty.
+ *   q: [B,T,Hq,D] of dtype, strides (q_sb, q_st, q_sh, 1), rows 16-byte aligned; out: [B,T,Hq*D] of dtype,
+ *   sequences out_sb apart, tokens Hq*D; 1 <= T <= 64, T * Hq <= 65535, B <= 65535,
+ *   otherwise as sparda_decode_paged. Scores, statistics and sums in fp32. bf16: the weights
+ *   times h are rounded to bf16 for the product with the codes; fp32: taken in
+ *   three bf16 terms, as q is. A row at or behind a token's last position has no part in
+ *   its output, whatever it holds.
+ */
+SPARDA_API int sparda_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype,
+                                      const void* pages, int64_t n_pages, int64_t page_size, int64_t p_st, int64_t h_st,
+                                      const int32_t* page_table, int64_t t_st, int64_t width, const int32_t* lengths,
+                                      int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, float scale, void* out,
+                                      int64_t out_sb, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace bytes sparda_verify_drafts needs for these sizes. */
+SPARDA_API size_t sparda_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V, int dtype);
+
+/*
+ * Verification of drafted tokens (no counterpart in the reference, whose sampling loop
+ * draws one token a forward, model/model.py:159-195). p_i = softmax(logits[b,i] / temperature), q_i =
+ * draft_probs[b,i] (NULL: all on the draft). Draft i is accepted while
+ *   uniform[b,i] q_i(draft_i) < p_i(draft_i);
+ * behind n accepted drafts the token is the lowest one at which the cumulated sum of r
+ * passes uniform[b,K] times its total, r = max(p_n - q_n, 0) after a rejection (p_n where that is
+ * zero everywhere), r = p_n behind the last draft; sums that decide the token in fp64. A
+ * temperature that is not above 0: draft i is accepted if it is the lowest index of
+ * row i's largest logit, and the token is that of row n. A row without a distribution (no logit above
+ * -inf, or NaN or +inf among them) accepts nothing and gives token -1; so does a
+ * draft outside [0, V) accept nothing.
+ *   logits: [B,K+1,V] of dtype, strides (l_sb, l_st, 1); drafts: [B,K] int32, stride d_sb; uniform: fp32
+ *   [B,K+1] in [0, 1), stride u_sb; draft_probs: fp32 [B,K,V], strides (p_sb, p_st, 1); n_drafts: int32 [B]
+ *   (NULL: K each), taken into [0, K]; temperatures: fp32 [B] (NULL: `temperature` for all).
+ *   tokens: int32 [B,K+1], the accepted drafts, the token, then -1; n_accepted: int32 [B].
+ *   0 <= K <= 64, B (K+1) <= 65535, V <= 2^21 - 8. Workspace 16-byte aligned; calls that share one must be
+ *   ordered on one stream.
+ */
+SPARDA_API int sparda_verify_drafts(const void* logits, int dtype, int64_t l_sb, int64_t l_st, const int32_t* drafts,
+                                    int64_t d_sb, const float* uniform, int64_t u_sb, const float* draft_probs,
+                                    int64_t p_sb, int64_t p_st, const int32_t* n_drafts, const float* temperatures,
+                                    float temperature, int64_t B, int64_t K, int64_t V, int32_t* tokens,
+                                    int32_t* n_accepted, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

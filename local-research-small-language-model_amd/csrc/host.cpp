@@ -49,6 +49,13 @@ struct Entries {
     decltype(&sparda_append_paged) append_paged;
     decltype(&sparda_decode_paged) decode_paged;
     decltype(&sparda_decode_paged_workspace_bytes) decode_paged_workspace_bytes;
+    decltype(&sparda_rotate_append_paged) rotate_append_paged;
+    decltype(&sparda_append_paged_q4) append_paged_q4;
+    decltype(&sparda_gather_paged_q4) gather_paged_q4;
+    decltype(&sparda_decode_paged_q4) decode_paged_q4;
+    decltype(&sparda_decode_paged_q4_workspace_bytes) decode_paged_q4_workspace_bytes;
+    decltype(&sparda_verify_drafts) verify_drafts;
+    decltype(&sparda_verify_drafts_workspace_bytes) verify_drafts_workspace_bytes;
 } g;
 
 // the call is not of the common form: the Python operator takes it
@@ -570,6 +577,174 @@ PyObject* decode_paged(PyObject* const* a) {
                   out);
 }
 
+// new rows and their sequences: [N,Hkv,D] of one type, a position and an offset each
+struct NewRows {
+    const at::Tensor &k, &v;
+    const int32_t *pos, *cu;
+    int64_t N;
+    NewRows(Args& x, PyObject* k_, PyObject* v_, PyObject* pos_, PyObject* cu_, int64_t B, int64_t Hkv, int64_t D)
+        : k(x.operand(k_, 3)), v(x.operand(v_, 3)), pos(x.ints(pos_, B)), cu(cu_ != Py_None ? x.ints(cu_, B + 1) : nullptr),
+          N(k.size(0)) {
+        need(k.scalar_type() == v.scalar_type() && k.sizes() == v.sizes() && k.size(1) == Hkv && k.size(2) == D);
+        need(N > 0 && same_strides(k, v) && rows16(k) && rows16(v) && (cu != nullptr || N == B));
+    }
+};
+// the rotation's tables and queries
+struct Rotation {
+    const at::Tensor &q, &cos, &sin;
+    Rotation(Args& x, PyObject* q_, PyObject* cos_, PyObject* sin_, const NewRows& n, int64_t D)
+        : q(x.operand(q_, 3)), cos(x.f32(cos_, 2)), sin(x.f32(sin_, 2)) {
+        need(q.scalar_type() == n.k.scalar_type() && q.size(0) == n.N && q.size(1) > 0 && q.size(2) == D && rows16(q));
+        need(cos.sizes() == sin.sizes() && cos.size(0) > 0 && cos.size(1) * 2 == D && aligned(cos, 16) && aligned(sin, 16));
+    }
+};
+
+// rotate_append_paged(k_pages, v_pages, page_table, positions, q, k_new, v_new, cos, sin, cu_seqlens)
+PyObject* rotate_append_paged(PyObject* const* a) {
+    Args x;
+    const PagesArg p(x, a);
+    const NewRows n(x, a[5], a[6], a[3], a[9], p.B, p.Hkv, p.D);
+    const Rotation r(x, a[4], a[7], a[8], n, p.D);
+    need(n.k.scalar_type() == p.k.scalar_type());
+    x.on_current();
+    const at::Tensor out = x.empty(r.q.sizes(), r.q.scalar_type());
+    return result(run(g.rotate_append_paged, p.k.data_ptr(), p.v.data_ptr(), code(p.k), p.P, p.ps, p.k.stride(0),
+                      p.k.stride(1), p.k.stride(2), static_cast<const int32_t*>(p.table.data_ptr()), p.table.stride(0),
+                      p.width, n.pos, n.cu, p.B, r.q.data_ptr(), r.q.stride(0), r.q.stride(1), r.q.size(1),
+                      n.k.data_ptr(), n.v.data_ptr(), n.N, n.k.stride(0), n.k.stride(1), p.Hkv, p.D,
+                      static_cast<const float*>(r.cos.data_ptr()), static_cast<const float*>(r.sin.data_ptr()),
+                      r.cos.stride(0), r.cos.size(0), out.data_ptr(), out.stride(0), out.stride(1), x.stream()),
+                  out);
+}
+
+// pages of 4-bit codes and their table; D -1: what a tile holds
+struct Q4Arg {
+    const at::Tensor &pages, &table;
+    int64_t P, ps, Hkv, D, B, width;
+    Q4Arg(Args& x, PyObject* pages_, PyObject* table_, int64_t D_)
+        : pages(x.tensor(pages_, 4)), table(x.tensor(table_, 2)), P(pages.size(0)), ps(pages.size(2) * 16),
+          Hkv(pages.size(1)), D(D_ < 0 ? pages.size(3) / 18 : D_), B(table.size(0)), width(table.size(1)) {
+        need(pages.scalar_type() == at::kByte && pages.size(3) > 0 && pages.size(3) == (D + 31) / 32 * 576 && ps > 0);
+        need(pages.stride(3) == 1 && (pages.size(2) == 1 || pages.stride(2) == pages.size(3)));
+        need(table.scalar_type() == at::kInt && B > 0 && (width == 1 || table.stride(1) == 1));
+    }
+    const int32_t* rows() const { return static_cast<const int32_t*>(table.data_ptr()); }
+};
+
+// append_paged_q4(pages, page_table, positions, k_new, v_new, cu_seqlens, q, cos, sin): the rotated queries, or a status
+PyObject* append_paged_q4(PyObject* const* a) {
+    Args x;
+    const at::Tensor& k = x.operand(a[3], 3);
+    const Q4Arg p(x, a[0], a[1], k.size(2));
+    const NewRows n(x, a[3], a[4], a[2], a[5], p.B, p.Hkv, p.D);
+    if (a[6] == Py_None) {
+        need(a[7] == Py_None && a[8] == Py_None);
+        x.on_current();
+        return PyLong_FromLong(run(g.append_paged_q4, p.pages.data_ptr(), p.P, p.ps, p.pages.stride(0), p.pages.stride(1),
+                                   p.rows(), p.table.stride(0), p.width, n.pos, n.cu, p.B, nullptr, 0, 0, 0,
+                                   n.k.data_ptr(), n.v.data_ptr(), code(n.k), n.N, n.k.stride(0), n.k.stride(1), p.Hkv, p.D,
+                                   nullptr, nullptr, 0, 0, nullptr, 0, 0, x.stream()));
+    }
+    const Rotation r(x, a[6], a[7], a[8], n, p.D);
+    x.on_current();
+    const at::Tensor out = x.empty(r.q.sizes(), r.q.scalar_type());
+    return result(run(g.append_paged_q4, p.pages.data_ptr(), p.P, p.ps, p.pages.stride(0), p.pages.stride(1), p.rows(),
+                      p.table.stride(0), p.width, n.pos, n.cu, p.B, r.q.data_ptr(), r.q.stride(0), r.q.stride(1),
+                      r.q.size(1), n.k.data_ptr(), n.v.data_ptr(), code(n.k), n.N, n.k.stride(0), n.k.stride(1), p.Hkv, p.D,
+                      static_cast<const float*>(r.cos.data_ptr()), static_cast<const float*>(r.sin.data_ptr()),
+                      r.cos.stride(0), r.cos.size(0), out.data_ptr(), out.stride(0), out.stride(1), x.stream()),
+                  out);
+}
+
+PyObject* pair(int rc, const at::Tensor& a, const at::Tensor& b) {
+    if (rc != 0) return PyLong_FromLong(rc);
+    PyObject* t = PyTuple_New(2);
+    if (t == nullptr) throw Decline{};
+    PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(a));
+    PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(b));
+    return t;
+}
+
+// gather_paged_q4(pages, page_table, positions, rows, cu_seqlens, head_dim, float32)
+PyObject* gather_paged_q4(PyObject* const* a) {
+    Args x;
+    const Q4Arg p(x, a[0], a[1], a[5] == Py_None ? -1 : as_int(a[5]));
+    const int32_t* pos = x.ints(a[2], p.B);
+    const int64_t N = as_int(a[3]);
+    const int32_t* cu = a[4] != Py_None ? x.ints(a[4], p.B + 1) : nullptr;
+    const at::ScalarType dt = as_bool(a[6]) ? at::kFloat : at::kBFloat16;
+    need(N > 0 && (cu != nullptr || N == p.B));
+    x.on_current();
+    const at::Tensor k = x.empty({N, p.Hkv, p.D}, dt), v = x.empty({N, p.Hkv, p.D}, dt);
+    return pair(run(g.gather_paged_q4, p.pages.data_ptr(), p.P, p.ps, p.pages.stride(0), p.pages.stride(1), p.rows(),
+                    p.table.stride(0), p.width, pos, cu, p.B, k.data_ptr(), v.data_ptr(), code(k), N, k.stride(0),
+                    k.stride(1), p.Hkv, p.D, x.stream()),
+                k, v);
+}
+
+// decode_paged_q4(q, pages, page_table, lengths, scale)
+PyObject* decode_paged_q4(PyObject* const* a) {
+    Args x;
+    need(THPVariable_CheckExact(a[0]));
+    const int64_t dim = THPVariable_Unpack(a[0]).dim();
+    need(dim == 3 || dim == 4);
+    const at::Tensor& q = x.operand(a[0], dim);
+    const int64_t T = dim == 4 ? q.size(1) : 1, Hq = q.size(dim - 2), D = q.size(dim - 1);
+    const Q4Arg p(x, a[1], a[2], D);
+    const int32_t* len = x.ints(a[3], p.B);
+    need(q.size(0) == p.B && T > 0 && rows16(q));
+    const float scale = scale_or(a[4], D);
+    x.on_current();
+    const size_t bytes = g.decode_paged_q4_workspace_bytes(p.B, T, p.width, p.ps, Hq, p.Hkv, D);
+    at::DataPtr part;  // the shares' partials, held until the launches are enqueued
+    if (bytes > 0) part = c10::GetAllocator(at::kCUDA)->allocate(bytes);
+    const at::Tensor out = dim == 4 ? x.empty({p.B, T, Hq * D}, q.scalar_type()) : x.empty({p.B, Hq * D}, q.scalar_type());
+    return result(run(g.decode_paged_q4, q.data_ptr(), q.stride(0), dim == 4 ? q.stride(1) : 0, q.stride(dim - 2), code(q),
+                      p.pages.data_ptr(), p.P, p.ps, p.pages.stride(0), p.pages.stride(1), p.rows(), p.table.stride(0),
+                      p.width, len, p.B, T, Hq, p.Hkv, D, scale, out.data_ptr(), out.stride(0), part.get(), bytes,
+                      x.stream()),
+                  out);
+}
+
+// verify_drafts(logits, drafts, uniform, draft_probs, n_drafts, temperature): (tokens, n_accepted)
+PyObject* verify_drafts(PyObject* const* a) {
+    Args x;
+    const at::Tensor& logits = x.operand(a[0], 3);
+    const int64_t B = logits.size(0), K = logits.size(1) - 1, V = logits.size(2);
+    const at::Tensor& drafts = x.tensor(a[1], 2);
+    const at::Tensor& uniform = x.tensor(a[2], 2);
+    need(B > 0 && K >= 0 && drafts.scalar_type() == at::kInt && drafts.size(0) == B && drafts.size(1) == K);
+    need(uniform.scalar_type() == at::kFloat && uniform.size(0) == B && uniform.size(1) == K + 1);
+    need((K <= 1 || drafts.stride(1) == 1) && (K == 0 || uniform.stride(1) == 1));
+    const at::Tensor* probs = nullptr;
+    if (a[3] != Py_None) {
+        probs = &x.operand(a[3], 3);
+        need(probs->scalar_type() == at::kFloat && probs->size(0) == B && probs->size(1) == K && probs->size(2) == V);
+        if (K == 0) probs = nullptr;
+    }
+    const int32_t* counts = a[4] != Py_None ? x.ints(a[4], B) : nullptr;
+    const float* each = nullptr;
+    float all = 0.0f;
+    if (THPVariable_Check(a[5])) {
+        each = static_cast<const float*>(x.f32(a[5], 1).data_ptr());
+        need(THPVariable_Unpack(a[5]).numel() == B);
+    } else {
+        all = static_cast<float>(as_float(a[5]));
+    }
+    x.on_current();
+    const size_t bytes = g.verify_drafts_workspace_bytes(B, K, V, code(logits));
+    need(bytes > 0);
+    const at::DataPtr ws = c10::GetAllocator(at::kCUDA)->allocate(bytes);
+    const at::Tensor tokens = x.empty({B, K + 1}, at::kInt), accepted = x.empty({B}, at::kInt);
+    return pair(run(g.verify_drafts, logits.data_ptr(), code(logits), logits.stride(0), logits.stride(1),
+                    K > 0 ? static_cast<const int32_t*>(drafts.data_ptr()) : nullptr, K > 0 ? drafts.stride(0) : 0,
+                    static_cast<const float*>(uniform.data_ptr()), uniform.stride(0),
+                    probs ? static_cast<const float*>(probs->data_ptr()) : nullptr, probs ? probs->stride(0) : 0,
+                    probs ? probs->stride(1) : 0, counts, each, all, B, K, V, static_cast<int32_t*>(tokens.data_ptr()),
+                    static_cast<int32_t*>(accepted.data_ptr()), ws.get(), bytes, x.stream()),
+                tokens, accepted);
+}
+
 // bind(raw_stream, addresses): the current-stream query and the entry points' addresses, in Entries' order
 PyObject* bind(PyObject*, PyObject* args) {
     PyObject *raw, *list;
@@ -612,6 +787,11 @@ PyMethodDef kMethods[] = {
     SPARDA_FAST(prefill_packed, 6),
     SPARDA_FAST(append_paged, 7),
     SPARDA_FAST(decode_paged, 6),
+    SPARDA_FAST(rotate_append_paged, 10),
+    SPARDA_FAST(append_paged_q4, 9),
+    SPARDA_FAST(gather_paged_q4, 7),
+    SPARDA_FAST(decode_paged_q4, 5),
+    SPARDA_FAST(verify_drafts, 6),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -5,23 +5,9 @@
 #include "kernels.h"
 #include "mfma.h"
 #include "packed.h"
+#include "paged.h"
 
 namespace sparda {
-
-namespace {
-
-constexpr float kPgLog2e = 1.4426950408889634f;
-
-// the pages and the table, as both kernels read them (strides in elements)
-struct Pages {
-    int64_t p_st, s_st, h_st;      // page, row, head
-    const int32_t* table;
-    int64_t t_st;                  // between the sequences' rows of the table
-    int width;                     // entries of a row
-    int n_pages;
-};
-
-}  // namespace
 
 // ---------------------------------------------------------------------------
 // append
@@ -39,34 +25,9 @@ append_paged_kernel(char* __restrict__ k, char* __restrict__ v, Pages pg, int ps
     const int lane = threadIdx.x % kWave;
     const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (t >= N) return;
-    int seq;
-    int64_t at = 0;                               // the row's place among its sequence's new rows
-    if (cu == nullptr) {
-        seq = static_cast<int>(t);
-    } else {
-        if (t == 0) {                             // the first row's wavefront looks at every pair of offsets
-            bool wrong = false;
-            for (int i = lane; i < n; i += kWave) wrong = wrong || cu[i] < 0 || cu[i + 1] < cu[i] || cu[i + 1] > N;
-            if (__ballot(wrong) != 0 && lane == 0) atomicOr(status, static_cast<uint32_t>(SPARDA_STATUS_SEQUENCE_RANGE));
-        }
-        // the last sequence that starts at or before t, when t is one of its rows
-        int c0, c1;
-        seq = packed_find(cu, n, [&](int c, int) { return c <= t; }, c0, c1);
-        if (seq < 0 || t >= c1) return;           // before the first sequence, behind the last
-        if (c0 < 0 || c1 > N) return;             // (offsets out of range: the sequence is left out)
-        at = t - c0;
-    }
-    const int p0 = __builtin_amdgcn_readfirstlane(positions[seq]);
-    if (p0 < 0) return;                           // a sequence that takes no part
-    const int64_t pos = p0 + at;
-    const int64_t slot = pos / ps;
-    int page = -1;
-    if (slot < pg.width) page = __builtin_amdgcn_readfirstlane(pg.table[seq * pg.t_st + slot]);
-    if (page < 0 || page >= pg.n_pages) {         // the row is dropped
-        if (lane == 0) atomicOr(status, static_cast<uint32_t>(SPARDA_STATUS_PAGE_RANGE));
-        return;
-    }
-    const int64_t to = (page * pg.p_st + (pos - slot * ps) * pg.s_st) * es;
+    const PagedRow r = paged_row(pg, ps, positions, cu, n, N, t, status);
+    if (!r.takes || r.page < 0) return;           // (without a page the row is dropped)
+    const int64_t to = (r.page * pg.p_st + r.row * pg.s_st) * es;
     const int64_t from = t * new_st * es;
     const int per = row_bytes / 16;               // pieces of a head's row
     for (int c = lane; c < Hkv * per; c += kWave) {
@@ -99,78 +60,6 @@ int launch_append_paged(void* k, void* v, int64_t n_pages, int64_t ps, int64_t p
 
 namespace {
 
-// Shares of a launch. A sequence's keys are walked in steps of 16 kTiles keys.
-// All steps of the batch are cut into shares of the same number of steps, so
-// that long and short sequences load the workgroups alike: the share length is
-// the total over `target`, at least `least`, and sequence b takes
-// n_b = max(1, ceil(steps_b / share)) consecutive items of about equal length, at
-// most target + B of them in all. Every workgroup derives this from the lengths
-// for itself.
-struct Share {
-    int seq;         // -1: no sequence has this item
-    int part, parts; // the item's place among its sequence's
-    int first;       // the sequence's first item
-    int share;       // steps of each of them
-    int len;         // the sequence's length, cut to the table's capacity
-    bool bad;        // the length is out of range
-};
-
-__device__ __forceinline__ int paged_steps(int len, int cap, int step) {
-    const int c = len < 0 ? 0 : len > cap ? cap : len;
-    return static_cast<int>((static_cast<int64_t>(c) + step - 1) / step);
-}
-
-// Inclusive sums over the lanes: within rows of 16 by shifts, then the rows' totals.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int add_dpp(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ int wave_scan_i32(int v) {
-    asm volatile("s_nop 1" : "+v"(v));  // the wait states of the first DPP, on every way here
-    v = add_dpp<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
-    v = add_dpp<0x112, 0xf>(v);
-    v = add_dpp<0x114, 0xf>(v);
-    v = add_dpp<0x118, 0xf>(v);
-    v = add_dpp<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
-    v = add_dpp<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
-    return v;
-}
-__device__ __forceinline__ int wave_last(int v) { return __builtin_amdgcn_readlane(v, kWave - 1); }
-
-// The item's sequence (by_item), or sequence `want`'s items. Wave-uniform. The total
-// of the steps stays below 2^30 (checked by the host against the capacity), so that
-// the sums with the target or a share stay in 32 bits.
-__device__ __forceinline__ Share paged_item(const int32_t* __restrict__ len, int B, int cap, int step, int target,
-                                            int least, bool by_item, int want) {
-    const int lane = threadIdx.x % kWave;
-    auto at_least = [&](int total) { return max(least, (total + target - 1) / target); };
-    auto found = [&](int seq, int l, int parts, int first) {
-        return Share{seq, by_item ? want - first : 0, parts, first, (paged_steps(l, cap, step) + parts - 1) / parts,
-                     l < 0 ? 0 : l > cap ? cap : l, l < 0 || l > cap};
-    };
-    if (B == 1) {
-        const int l = __builtin_amdgcn_readfirstlane(len[0]), steps = paged_steps(l, cap, step), share = at_least(steps);
-        const int parts = max(1, (steps + share - 1) / share);
-        return by_item && want >= parts ? Share{-1} : found(0, l, parts, 0);
-    }
-    int total = 0;
-    for (int b0 = 0; b0 < B; b0 += kWave) total += wave_last(wave_scan_i32(b0 + lane < B ? paged_steps(len[b0 + lane], cap, step) : 0));
-    const int share = at_least(total);
-    int before = 0;
-    for (int b0 = 0; b0 < B; b0 += kWave) {
-        const int b = b0 + lane, l = b < B ? len[b] : 0;
-        const int n = b < B ? max(1, (paged_steps(l, cap, step) + share - 1) / share) : 0;
-        const int end = before + wave_scan_i32(n);      // items of sequences 0 .. b
-        const uint64_t m = __ballot(b < B && (by_item ? end > want : b == want));
-        if (m != 0) {
-            const int at = __builtin_ctzll(m), parts = __builtin_amdgcn_readlane(n, at);
-            return found(b0 + at, __builtin_amdgcn_readlane(l, at), parts, __builtin_amdgcn_readlane(end, at) - parts);
-        }
-        before = wave_last(end);
-    }
-    return Share{-1};
-}
-
 template <int DT>
 struct PagedType;
 template <>
@@ -195,26 +84,6 @@ struct PagedStep {
     VRow v[kTiles][4];
 };
 
-constexpr int kPgJoin = 512;        // threads of a join
-
-struct PagedDecode {
-    const void* q;
-    int64_t q_sb, q_sh;
-    const void *k, *v;
-    Pages pg;
-    int ps16;                     // 16-key tiles of a page
-    const int32_t* len;
-    int B, cap;
-    int Hq, Hkv, R, head_tiles;   // head tiles of 16 query heads per KV head
-    int target, least;
-    int whole;                    // every sequence is one item
-    int lds_heads;                // heads of the largest tile
-    float scale_log2;
-    void* out;
-    int64_t out_sb;
-    float *part_o, *part_ml;      // [items, Hq, D], [items, Hq, 2]
-    uint32_t* status;
-};
 
 }  // namespace
 
@@ -469,6 +338,13 @@ __global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : DT == SPARDA_F32
     }
 }
 
+// A joined output; zeros for a token that comes before the sequence's first position (of a
+// bad sequence, whose sums are NaN: NaN)
+__device__ __forceinline__ float paged_join_out(const PagedDecode& a, const Share& sh, int h, float O, float L) {
+    const bool none = a.T > 1 && sh.len - a.T + 1 + h / a.heads <= 0;
+    return none && O == O ? 0.0f : O / L;
+}
+
 // Joins the items of a sequence, one workgroup per (32 dims of a query head, sequence):
 //     M = max m_i, out = sum exp2(m_i - M) O_i / sum exp2(m_i - M) l_i.
 // The items' weights once into LDS, then dims over the lanes and the items over the
@@ -479,10 +355,10 @@ __global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : DT == SPARDA_F32
 template <int DT, int D>
 __global__ void __launch_bounds__(kPgJoin) decode_paged_join_kernel(PagedDecode a) {
     constexpr int JD = D < 32 ? D : 32;                       // dims of a workgroup
-    constexpr int kStep = 16 * PagedType<DT>::kTiles, kG = kPgJoin / JD, kChunk = 1024, kJW = kPgJoin / kWave;
+    constexpr int kG = kPgJoin / JD, kChunk = 1024, kJW = kPgJoin / kWave;
     __shared__ float red[kPgJoin], wts[kChunk], rm[kJW], rl[kJW];
     const int b = blockIdx.y, h = blockIdx.x / (D / JD), d0 = blockIdx.x % (D / JD) * JD, tid = threadIdx.x, wave = tid / kWave;
-    const Share sh = paged_item(a.len, a.B, a.cap, kStep, a.target, a.least, false, b);
+    const Share sh = paged_item(a.len, a.B, a.cap, a.step, a.target, a.least, false, b);
     if (sh.parts <= 1) return;                                // written by its one item
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + static_cast<int64_t>(sh.first) * a.Hq + h;
     const float* po = a.part_o + (static_cast<int64_t>(sh.first) * a.Hq + h) * D + d0 + tid % JD;
@@ -535,7 +411,7 @@ __global__ void __launch_bounds__(kPgJoin) decode_paged_join_kernel(PagedDecode 
     for (int w = 0; w < kJW; ++w) den += rl[w];
 #pragma unroll
     for (int i = 1; i < kG; ++i) O += red[i * JD + tid];
-    store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d0 + tid, O / den);
+    store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d0 + tid, paged_join_out(a, sh, h, O, den));
 }
 
 // The same where sequences have few items in the mean: one thread per (query head,
@@ -543,9 +419,8 @@ __global__ void __launch_bounds__(kPgJoin) decode_paged_join_kernel(PagedDecode 
 // heads of 64.
 template <int DT, int D>
 __global__ void __launch_bounds__(256) decode_paged_join_few_kernel(PagedDecode a) {
-    constexpr int kStep = 16 * PagedType<DT>::kTiles;
     const int b = blockIdx.y, h = blockIdx.x * (256 / D) + threadIdx.x / D, d = threadIdx.x % D;
-    const Share sh = paged_item(a.len, a.B, a.cap, kStep, a.target, a.least, false, b);
+    const Share sh = paged_item(a.len, a.B, a.cap, a.step, a.target, a.least, false, b);
     if (sh.parts <= 1 || h >= a.Hq) return;                   // written by its one item
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + static_cast<int64_t>(sh.first) * a.Hq + h;
     const float* po = a.part_o + (static_cast<int64_t>(sh.first) * a.Hq + h) * D + d;
@@ -575,7 +450,7 @@ __global__ void __launch_bounds__(256) decode_paged_join_few_kernel(PagedDecode 
                 O = __builtin_fmaf(wt, y[e], O);
             }
     }
-    store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d, O / L);
+    store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d, paged_join_out(a, sh, h, O, L));
 }
 
 namespace {
@@ -648,6 +523,27 @@ size_t decode_paged_workspace_bytes(int64_t B, int64_t cap, int64_t Hq, int64_t 
     return p.items <= B ? 0 : static_cast<size_t>(p.items * Hq * (D + 2)) * sizeof(float);
 }
 
+void launch_paged_join(const PagedDecode& a, int64_t D, int dtype, bool few, hipStream_t stream) {
+#define SPARDA_PGJ(DT_, D_)                                                                                       \
+    if (few)                                                                                                      \
+        hipLaunchKernelGGL((decode_paged_join_few_kernel<DT_, D_>),                                               \
+                           dim3(static_cast<unsigned>(cdiv(a.Hq, 256 / D_)), static_cast<unsigned>(a.B)), dim3(256), 0, stream, a); \
+    else                                                                                                          \
+        hipLaunchKernelGGL((decode_paged_join_kernel<DT_, D_>),                                                   \
+                           dim3(static_cast<unsigned>(a.Hq * (D_ < 32 ? 1 : D_ / 32)), static_cast<unsigned>(a.B)), dim3(kPgJoin), 0, stream, a)
+#define SPARDA_PGJ_D(DT_)                     \
+    switch (D) {                              \
+        case 16: SPARDA_PGJ(DT_, 16); break;  \
+        case 32: SPARDA_PGJ(DT_, 32); break;  \
+        case 64: SPARDA_PGJ(DT_, 64); break;  \
+        default: SPARDA_PGJ(DT_, 128); break; \
+    }
+    if (dtype == SPARDA_F32) SPARDA_PGJ_D(SPARDA_F32)
+    else SPARDA_PGJ_D(SPARDA_BF16)
+#undef SPARDA_PGJ_D
+#undef SPARDA_PGJ
+}
+
 int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k, const void* v, int64_t n_pages,
                         int64_t ps, int64_t p_st, int64_t s_st, int64_t h_st, int dtype, const int32_t* table,
                         int64_t t_st, int64_t width, const int32_t* len, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
@@ -659,6 +555,7 @@ int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k
     if (const int rc = status_word(&a.status)) return rc;
     a.q = q, a.q_sb = q_sb, a.q_sh = q_sh, a.k = k, a.v = v;
     a.pg = Pages{p_st, s_st, h_st, table, t_st, static_cast<int>(width), static_cast<int>(n_pages)};
+    a.T = 1, a.heads = static_cast<int>(Hq), a.step = dtype == SPARDA_F32 ? 16 : 32;
     a.ps16 = static_cast<int>(ps / 16), a.len = len, a.B = static_cast<int>(B), a.cap = static_cast<int>(cap);
     a.Hq = static_cast<int>(Hq), a.Hkv = static_cast<int>(Hkv), a.R = static_cast<int>(R);
     a.head_tiles = static_cast<int>(cdiv(R, 16));
@@ -677,13 +574,7 @@ int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k
         if (p.hg == 4) SPARDA_PGD_W(DT_, D_, 4, 2);                                                               \
         else if (p.hg == 2) SPARDA_PGD_W(DT_, D_, 2, 4);                                                          \
         else if (p.kw == 4) SPARDA_PGD_W(DT_, D_, 1, 4);                                                          \
-        else SPARDA_PGD_W(DT_, D_, 1, 8);                                                                         \
-        if (p.items > B && p.few)                                                                                 \
-            hipLaunchKernelGGL((decode_paged_join_few_kernel<DT_, D_>),                                           \
-                               dim3(static_cast<unsigned>(cdiv(Hq, 256 / D_)), static_cast<unsigned>(B)), dim3(256), 0, stream, a); \
-        else if (p.items > B)                                                                                     \
-            hipLaunchKernelGGL((decode_paged_join_kernel<DT_, D_>),                                               \
-                               dim3(static_cast<unsigned>(Hq * (D_ < 32 ? 1 : D_ / 32)), static_cast<unsigned>(B)), dim3(kPgJoin), 0, stream, a); \
+        else SPARDA_PGD_W(DT_, D_, 1, 8);                                                          \
     } while (0)
 #define SPARDA_PGD_D(DT_)                     \
     switch (D) {                              \
@@ -697,6 +588,7 @@ int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k
 #undef SPARDA_PGD_D
 #undef SPARDA_PGD_W
 #undef SPARDA_PGD
+    if (p.items > B) launch_paged_join(a, D, dtype, p.few, stream);
     return check_hip(hipGetLastError(), "decode_paged_kernel");
 }
 

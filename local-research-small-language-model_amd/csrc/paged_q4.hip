@@ -1,0 +1,657 @@
+// A key-value cache in pages of 4-bit codes (sparda_append_paged_q4,
+// sparda_gather_paged_q4, sparda_decode_paged_q4).
+//
+// Dims are taken in groups of 32 (a head of 16 dims is half a group). A group of
+// a row x, in bf16, is held as h (2 c - 15), c in 0 .. 15 a dim and h = max|x| / 15 in
+// fp16: the odd multiples of h, of which the nearest to x is that of
+// c = floor(x / 2h) + 8. 4.5 bits a dim; a row of N(0,1) comes back with a relative error
+// of 9%. One number a group (no offset) costs the products no second sum: the
+// levels' middle, 7.5, is the same for all.
+//
+// 16 positions of a head (a tile) lie together, 576 bytes a group, G groups a head:
+//   keys' codes    [16 positions][4 quarters][G][4 bytes]: quarter p of group i holds dims
+//                  32 i + 8 p + e, e = 0 .. 7, in nibble e/2 + 4 (e % 2), so that nibbles four apart
+//                  are neighbouring dims
+//   values' codes  [4 fours of positions][16 pairs w][G][4 bytes]: byte s is position
+//                  {0, 2, 1, 3}[s] of the four, its nibbles dims 32 g + 2 w and + 1
+//   keys' h        [16 positions][G], then the values' h
+// Both are what a lane of the matrix products takes (decode below), and a wavefront reads
+// a tile's codes as one block of memory.
+#include "common.h"
+#include "kernels.h"
+#include "mfma.h"
+#include "paged.h"
+#include "rotate.h"
+
+namespace sparda {
+
+namespace {
+
+constexpr int q4_groups(int D) { return D < 32 ? 1 : D / 32; }
+
+// h of a group from the bits of its largest magnitude. A value that is not finite makes the
+// group NaN; magnitudes above 15 * 65504 are cut off.
+__device__ __forceinline__ _Float16 q4_scale(uint32_t top) {
+    if (top >= 0x7f800000u) return __builtin_bit_cast(_Float16, static_cast<uint16_t>(0x7e00));
+    const float h = __uint_as_float(top) / 15.0f;
+    return static_cast<_Float16>(h < 65504.0f ? h : 65504.0f);
+}
+
+// floor(x / 2h) + 8 in 0 .. 15, exactly: the rounded quotient is within half of the
+// true one, so that one of its neighbours is the floor, and x - n 2h, on a grid of
+// at most 14 bits, has no rounding to hide its sign.
+__device__ __forceinline__ uint32_t q4_code(float x, float h2, float inv) {
+    const float n = fminf(fmaxf(__builtin_rintf(x * inv), -9.0f), 8.0f);   // (where h is cut off, x / 2h may be any number)
+    const float e = __builtin_fmaf(-n, h2, x);
+    const int c = static_cast<int>(n) - (e < 0.0f ? 1 : 0) + 8;
+    return static_cast<uint32_t>(c < 0 ? 0 : c > 15 ? 15 : c);
+}
+
+// Eight codes of a group of one number h.
+__device__ __forceinline__ void q4_codes(const float (&x)[8], _Float16 h, uint32_t (&c)[8]) {
+    const float h2 = 2.0f * static_cast<float>(h);
+    if (!(h2 > 0.0f)) {                            // zeros, or NaN: any code
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[e] = 8;
+        return;
+    }
+    const float inv = 1.0f / h2;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = q4_code(x[e], h2, inv);
+}
+
+// Eight elements of a row, as bf16 values in fp32 (round: fp32 rows are rounded)
+template <int DT>
+__device__ __forceinline__ void q4_load8(const char* p, float (&x)[8]) {
+    if constexpr (DT == SPARDA_F32) {
+        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 16);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[2 * e] = __uint_as_float(w[e] << 16), x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+    }
+}
+template <int DT>
+__device__ __forceinline__ void q4_store8(char* p, const float (&x)[8]) {
+    if constexpr (DT == SPARDA_F32) {
+        *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(p + 16) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+__device__ __forceinline__ uint32_t q4_top(float (&x)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        x[e] = static_cast<float>(static_cast<__bf16>(x[e]));
+        m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
+    }
+    return m;
+}
+// the largest over neighbouring lanes: 2 or 4 of them
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u32_max(uint32_t v) {
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false)));
+}
+template <int LANES>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+    if constexpr (LANES >= 2) asm volatile("s_nop 1" : "+v"(v));  // the wait states of the first DPP, on every way here
+    if constexpr (LANES >= 2) v = dpp_u32_max<kDppXor1>(v);
+    if constexpr (LANES >= 4) v = dpp_u32_max<kDppXor2>(v);
+    return v;
+}
+
+// byte offsets in a tile
+template <int G>
+__device__ __forceinline__ int q4_key_word(int key, int dim) { return key * 16 * G + dim % 32 / 8 * 4 * G + dim / 32 * 4; }
+template <int G>
+__device__ __forceinline__ int q4_value_byte(int key, int dim) {
+    const int i = key % 4, slot = i == 1 ? 2 : i == 2 ? 1 : i;
+    return 256 * G + (key / 4 * 16 + dim % 32 / 2) * 4 * G + dim / 32 * 4 + slot;
+}
+template <int G>
+__device__ __forceinline__ int q4_scale_at(int which, int key, int group) { return 512 * G + which * 32 * G + (key * G + group) * 2; }
+
+__device__ __forceinline__ uint32_t q4_key_pack(const uint32_t (&c)[8]) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w |= c[e] << (4 * (e / 2 + 4 * (e % 2)));
+    return w;
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+
+// One wavefront per new row. A lane takes eight dims and the eight that they are paired
+// with; the largest magnitude of a group comes from up to four neighbouring lanes.
+template <int DT, int D, bool ROT>
+__global__ void __launch_bounds__(256) append_paged_q4_kernel(RotateAppend a, char* __restrict__ pages) {
+    constexpr int G = q4_groups(D), kEs = DT == SPARDA_F32 ? 4 : 2, kPer = D / 16;
+    const int lane = threadIdx.x % kWave;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if (t >= a.N) return;
+    const PagedRow r = paged_row(a.pg, a.ps, a.positions, a.cu, a.n, a.N, t, a.status);
+    if (!r.takes) return;
+    const bool off_table = ROT && r.pos >= a.rows;
+    if (off_table && lane == 0) atomicOr(a.status, static_cast<uint32_t>(SPARDA_STATUS_POSITION_RANGE));
+    const bool keep = r.page >= 0 && !off_table;
+    const int c = lane % kPer;
+    float cs[8], sn[8];
+    if constexpr (ROT) {
+        load_angles<8>(a, r.pos, c * 8, off_table, cs, sn);
+        for (int h = lane / kPer; h < a.Hq; h += kWave / kPer) {
+            const char* from = static_cast<const char*>(a.q) + (t * a.q_st + h * a.q_sh + c * 8) * kEs;
+            char* to = static_cast<char*>(a.q_out) + (t * a.qo_st + h * a.qo_sh + c * 8) * kEs;
+            float x[8], y[8];
+            q4_load8<DT>(from, x);
+            q4_load8<DT>(from + D / 2 * kEs, y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) turn(x[e], y[e], cs[e], sn[e]);
+            q4_store8<DT>(to, x);
+            q4_store8<DT>(to + D / 2 * kEs, y);
+        }
+    }
+    if (!keep) return;
+    const int key = static_cast<int>(r.row % 16);
+    char* tiles = pages + r.page * a.pg.p_st + r.row / 16 * (576 * G);
+    for (int h = lane / kPer; h < a.Hkv; h += kWave / kPer) {
+        const char* from = static_cast<const char*>(a.k_new) + (t * a.new_st + h * a.new_sh + c * 8) * kEs;
+        char* tile = tiles + h * a.pg.h_st;
+        float x[2][8];
+        q4_load8<DT>(from, x[0]);
+        q4_load8<DT>(from + D / 2 * kEs, x[1]);
+        if constexpr (ROT) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) turn(x[0][e], x[1][e], cs[e], sn[e]);
+        }
+        uint32_t top[2] = {q4_top(x[0]), q4_top(x[1])};
+        if constexpr (D < 64) top[0] = top[1] = max(top[0], top[1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const _Float16 hh = q4_scale(lanes_max<(D >= 64 ? 4 : D == 32 ? 2 : 1)>(top[i]));
+            const int dim = i * (D / 2) + c * 8;
+            uint32_t code[8];
+            q4_codes(x[i], hh, code);
+            *reinterpret_cast<uint32_t*>(tile + q4_key_word<G>(key, dim)) = q4_key_pack(code);
+            if (dim % 32 == 0) *reinterpret_cast<_Float16*>(tile + q4_scale_at<G>(0, key, dim / 32)) = hh;
+        }
+    }
+    for (int i = lane; i < a.Hkv * 2 * kPer; i += kWave) {
+        const int h = i / (2 * kPer), dim = i % (2 * kPer) * 8;
+        char* tile = tiles + h * a.pg.h_st;
+        float x[8];
+        q4_load8<DT>(static_cast<const char*>(a.v_new) + (t * a.new_st + h * a.new_sh + dim) * kEs, x);
+        const _Float16 hh = q4_scale(lanes_max<(D >= 32 ? 4 : 2)>(q4_top(x)));
+        uint32_t code[8];
+        q4_codes(x, hh, code);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2)
+            *reinterpret_cast<uint8_t*>(tile + q4_value_byte<G>(key, dim + e)) = static_cast<uint8_t>(code[e] | code[e + 1] << 4);
+        if (dim % 32 == 0) *reinterpret_cast<_Float16*>(tile + q4_scale_at<G>(1, key, dim / 32)) = hh;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// gather
+// ---------------------------------------------------------------------------
+
+// One wavefront per row, eight dims a lane: the values that the codes stand for.
+template <int DT, int D>
+__global__ void __launch_bounds__(256)
+gather_paged_q4_kernel(RotateAppend a, const char* __restrict__ pages, char* __restrict__ k, char* __restrict__ v) {
+    constexpr int G = q4_groups(D), kEs = DT == SPARDA_F32 ? 4 : 2, kPer = D / 8;
+    const int lane = threadIdx.x % kWave;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if (t >= a.N) return;
+    const PagedRow r = paged_row(a.pg, a.ps, a.positions, a.cu, a.n, a.N, t, a.status);
+    if (!r.takes) return;
+    const int key = static_cast<int>(r.row % 16);
+    const char* tiles = pages + r.page * a.pg.p_st + r.row / 16 * (576 * G);
+    for (int i = lane; i < a.Hkv * kPer; i += kWave) {
+        const int h = i / kPer, dim = i % kPer * 8;
+        float x[8], y[8];
+        if (r.page >= 0) {
+            const char* tile = tiles + h * a.pg.h_st;
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + q4_key_word<G>(key, dim));
+            const float hk = *reinterpret_cast<const _Float16*>(tile + q4_scale_at<G>(0, key, dim / 32));
+            const float hv = *reinterpret_cast<const _Float16*>(tile + q4_scale_at<G>(1, key, dim / 32));
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const uint32_t b = *reinterpret_cast<const uint8_t*>(tile + q4_value_byte<G>(key, dim + e));
+                x[e] = hk * static_cast<float>(static_cast<int>(w >> (2 * e) & 15) * 2 - 15);
+                x[e + 1] = hk * static_cast<float>(static_cast<int>(w >> (2 * e + 16) & 15) * 2 - 15);
+                y[e] = hv * static_cast<float>(static_cast<int>(b & 15) * 2 - 15);
+                y[e + 1] = hv * static_cast<float>(static_cast<int>(b >> 4) * 2 - 15);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = y[e] = __builtin_nanf("");
+        }
+        const int64_t at = (t * a.new_st + h * a.new_sh + dim) * kEs;
+        q4_store8<DT>(k + at, x);
+        q4_store8<DT>(v + at, y);
+    }
+}
+
+int launch_append_paged_q4(const RotateAppend& given, void* pages, int dtype, int64_t D, hipStream_t stream) {
+    RotateAppend a = given;
+    if (!grid_fits(cdiv(a.N, 4), 256)) return set_error(SPARDA_ERR_SHAPE, "append_paged_q4: grid too large");
+    if (const int rc = status_word(&a.status)) return rc;
+    const dim3 grid(static_cast<unsigned>(cdiv(a.N, 4)));
+#define SPARDA_AQ(DT_, D_)                                                                                                  \
+    do {                                                                                                                    \
+        if (a.cos) hipLaunchKernelGGL((append_paged_q4_kernel<DT_, D_, true>), grid, dim3(256), 0, stream, a, static_cast<char*>(pages)); \
+        else hipLaunchKernelGGL((append_paged_q4_kernel<DT_, D_, false>), grid, dim3(256), 0, stream, a, static_cast<char*>(pages));      \
+    } while (0)
+#define SPARDA_AQ_D(DT_)                      \
+    switch (D) {                              \
+        case 16: SPARDA_AQ(DT_, 16); break;   \
+        case 32: SPARDA_AQ(DT_, 32); break;   \
+        case 64: SPARDA_AQ(DT_, 64); break;   \
+        default: SPARDA_AQ(DT_, 128); break;  \
+    }
+    if (dtype == SPARDA_F32) SPARDA_AQ_D(SPARDA_F32)
+    else SPARDA_AQ_D(SPARDA_BF16)
+#undef SPARDA_AQ_D
+#undef SPARDA_AQ
+    return check_hip(hipGetLastError(), "append_paged_q4_kernel");
+}
+
+int launch_gather_paged_q4(const RotateAppend& given, const void* pages, int dtype, int64_t D, void* k, void* v,
+                           hipStream_t stream) {
+    RotateAppend a = given;
+    if (!grid_fits(cdiv(a.N, 4), 256)) return set_error(SPARDA_ERR_SHAPE, "gather_paged_q4: grid too large");
+    if (const int rc = status_word(&a.status)) return rc;
+    const dim3 grid(static_cast<unsigned>(cdiv(a.N, 4)));
+#define SPARDA_GQ(DT_, D_)                                                                                            \
+    hipLaunchKernelGGL((gather_paged_q4_kernel<DT_, D_>), grid, dim3(256), 0, stream, a, static_cast<const char*>(pages), \
+                       static_cast<char*>(k), static_cast<char*>(v))
+#define SPARDA_GQ_D(DT_)                      \
+    switch (D) {                              \
+        case 16: SPARDA_GQ(DT_, 16); break;   \
+        case 32: SPARDA_GQ(DT_, 32); break;   \
+        case 64: SPARDA_GQ(DT_, 64); break;   \
+        default: SPARDA_GQ(DT_, 128); break;  \
+    }
+    if (dtype == SPARDA_F32) SPARDA_GQ_D(SPARDA_F32)
+    else SPARDA_GQ_D(SPARDA_BF16)
+#undef SPARDA_GQ_D
+#undef SPARDA_GQ
+    return check_hip(hipGetLastError(), "gather_paged_q4_kernel");
+}
+
+// ---------------------------------------------------------------------------
+// decode
+// ---------------------------------------------------------------------------
+
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// a step's operands of 32 keys (two tiles), as loaded; words of a lane
+template <int D>
+struct Q4Step {
+    static constexpr int G = q4_groups(D);
+    uint32_t k[2][G], v[2][G];
+    _Float16 hk[2][4][G], hv[2][4][G];
+};
+
+template <int N>
+__device__ __forceinline__ void q4_load_words(const char* p, uint32_t (&w)[N]) {
+    if constexpr (N == 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else if constexpr (N == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        w[0] = x.x, w[1] = x.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+}
+// four positions' numbers, [4][G]
+template <int G>
+__device__ __forceinline__ void q4_load_scales(const char* p, _Float16 (&h)[4][G]) {
+    if constexpr (G == 1) {
+        const auto x = __builtin_bit_cast(__attribute__((ext_vector_type(4))) _Float16, *reinterpret_cast<const uint2*>(p));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i][0] = x[i];
+    } else {
+#pragma unroll
+        for (int j = 0; j < G / 2; ++j) {
+            const auto x = __builtin_bit_cast(f16x8, *reinterpret_cast<const uint4*>(p + 16 * j));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[(j * 8 + e) / G][(j * 8 + e) % G] = x[e];
+        }
+    }
+}
+
+// Eight codes of a word as bf16 128 + c: nibbles n and n + 4 are the halves of register n
+__device__ __forceinline__ bf16x8 q4_key_operand(uint32_t w) {
+    uint4 x;
+    x.x = (w & 0x000f000fu) | 0x43004300u;
+    x.y = (w >> 4 & 0x000f000fu) | 0x43004300u;
+    x.z = (w >> 8 & 0x000f000fu) | 0x43004300u;
+    x.w = (w >> 12 & 0x000f000fu) | 0x43004300u;
+    return __builtin_bit_cast(bf16x8, x);
+}
+// nibble j of the eight positions of two tiles' words
+__device__ __forceinline__ bf16x8 q4_value_operand(uint32_t w0, uint32_t w1, int j) {
+    uint4 x;
+    x.x = (w0 >> (4 * j) & 0x000f000fu) | 0x43004300u;
+    x.y = (w0 >> (4 * j + 8) & 0x000f000fu) | 0x43004300u;
+    x.z = (w1 >> (4 * j) & 0x000f000fu) | 0x43004300u;
+    x.w = (w1 >> (4 * j + 8) & 0x000f000fu) | 0x43004300u;
+    return __builtin_bit_cast(bf16x8, x);
+}
+
+// x as a sum of TERMS bf16 values (1: rounded; 3: all 24 bits of it)
+template <int TERMS>
+__device__ __forceinline__ void q4_split(const float (&x)[8], bf16x8 (&out)[TERMS]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float rest = x[e];
+#pragma unroll
+        for (int n = 0; n < TERMS; ++n) {
+            out[n][e] = static_cast<__bf16>(rest);
+            rest -= static_cast<float>(out[n][e]);
+        }
+    }
+}
+
+}  // namespace
+
+// One workgroup of KW wavefronts per (tile of 16 columns, item). The columns are the (token, query
+// head) pairs of a KV head, token-major; token t of T sees the positions below
+// len - T + 1 + t. The codes go to the matrix products as bf16 128 + c, and the
+// numbers h stay outside of them:
+//     S^T[key, col] = 2 sum_g h_g[key] (sum_{d in g} (128 + c) q[d] - 135.5 sum_{d in g} q[d])
+//     O^T[d, col]  += 2 sum_key P_g[key, col] (128 + c) - 135.5 P_g,  P_g = exp2(S - m) h_g[key] in bf16
+// The subtracted sums are products themselves: of q with ones once, the start of every
+// score's accumulator, and of the rounded P_g with ones beside the values', so that
+// their roundings cancel. The levels, odd multiples of h, thereby enter without rounding.
+template <int DT, int D, int KW>
+__global__ void __launch_bounds__(KW* kWave, 2) decode_paged_q4_kernel(PagedDecode a) {
+    constexpr int G = q4_groups(D), kTerms = DT == SPARDA_F32 ? 3 : 1, kStep = 32, kEs = DT == SPARDA_F32 ? 4 : 2;
+    extern __shared__ float lds[];
+    const int lane = threadIdx.x % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int c16 = lane % 16, grp = lane / 16;
+    const int groups = a.Hkv * a.head_tiles;
+    const int item = blockIdx.x / groups, gt = blockIdx.x % groups;
+    const int g = gt / a.head_tiles, col0 = gt % a.head_tiles * 16;
+    const int nh = a.R * a.T - col0 < 16 ? a.R * a.T - col0 : 16;   // columns of the tile
+    Share sh;
+    if (a.whole) {
+        const int l = __builtin_amdgcn_readfirstlane(a.len[item]), n = l < 0 ? 0 : l > a.cap ? a.cap : l;
+        sh = Share{item, 0, 1, item, paged_steps(l, a.cap, kStep), n, l < 0 || l > a.cap};
+    } else {
+        sh = paged_item(a.len, a.B, a.cap, kStep, a.target, a.least, true, item);
+    }
+    if (sh.seq < 0) return;                                 // workgroup-uniform
+    const int b = sh.seq, len = sh.len;
+    const int steps = paged_steps(len, a.cap, kStep);
+    const int s_end = min(steps, (sh.part + 1) * sh.share);
+    bool bad = sh.bad;
+
+    // this lane's column of Q, and what its codes' 135.5 amount to
+    const int col = col0 + (c16 < nh ? c16 : nh - 1), tok = col / a.R, head = g * a.R + col % a.R;
+    const int lim = len - a.T + 1 + tok;                    // positions the column sees
+    bf16x8 qr[G][kTerms];
+    f32x4 less[G];
+    {
+        bf16x8 ones;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ones[e] = static_cast<__bf16>(1.0f);
+        const char* q = static_cast<const char*>(a.q) + (b * a.q_sb + tok * a.q_st + head * a.q_sh) * kEs;
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            float x[8];
+            if (c16 < nh && 32 * i + 8 * grp < D) {
+                q4_load8<DT>(q + (32 * i + 8 * grp) * kEs, x);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+            }
+            q4_split<kTerms>(x, qr[i]);
+            f32x4 s{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int n = 0; n < kTerms; ++n) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, qr[i][n], s, 0, 0, 0);
+            less[i] = s * -135.5f;
+        }
+    }
+
+    const int32_t* row = a.pg.table + b * a.pg.t_st;
+    const char* kv = static_cast<const char*>(a.k) + g * a.pg.h_st;
+    const int last_tile = (len - 1) / 16;
+    const int o_codes = lane * 4 * G, o_scale = 512 * G + grp * 8 * G;
+    auto load = [&](int u, Q4Step<D>& x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            int tile = 2 * u + t;
+            if (tile > last_tile) tile = last_tile;         // past the end: the last tile again, masked
+            const int p = tile / a.ps16, r = tile - p * a.ps16;
+            int id = row[p];
+            if (id < 0 || id >= a.pg.n_pages) bad = true, id = 0;
+            const char* base = kv + id * a.pg.p_st + r * (576 * G);
+            // (keys: position c16, quarter grp; values: four grp, pair c16)
+            q4_load_words<G>(base + (c16 * 4 + grp) * 4 * G, x.k[t]);
+            q4_load_words<G>(base + 256 * G + o_codes, x.v[t]);
+            q4_load_scales<G>(base + o_scale, x.hk[t]);
+            q4_load_scales<G>(base + o_scale + 32 * G, x.hv[t]);
+        }
+    };
+
+    float m = -__builtin_inff(), l = 0.0f;                   // the column's maximum (log2 units), this lane's part of its sum
+    f32x4 o[G][2], op[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) o[i][0] = o[i][1] = op[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    bf16x8 ones;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ones[e] = static_cast<__bf16>(1.0f);
+    auto compute = [&](int u, const Q4Step<D>& x) __attribute__((always_inline)) {
+        f32x4 s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                const bf16x8 ka = q4_key_operand(x.k[t][i]);
+                f32x4 y = less[i];
+#pragma unroll
+                for (int n = 0; n < kTerms; ++n) y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qr[i][n], y, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[t][e] = __builtin_fmaf(y[e], static_cast<float>(x.hk[t][e][i]), s[t][e]);
+            }
+        }
+        const int left = lim - u * kStep - 4 * grp;          // this lane's keys 16 t + e below it are the column's
+        float mx = m;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, 16 * t + e < left ? s[t][e] * a.scale_log2 : -__builtin_inff());
+        mx = pair32_max(pair16_max(mx));
+        const float ref = mx == -__builtin_inff() ? 0.0f : mx;
+        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+        m = mx;
+        l *= alpha;
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool in = 16 * (e / 4) + e % 4 < left;
+            p[e] = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 4][e % 4], a.scale_log2, -ref)) : 0.0f;
+            l += p[e];
+        }
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            float ph[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                // (a number behind the column's positions may be anything)
+                const bool in = 16 * (e / 4) + e % 4 < left;
+                ph[e] = in ? p[e] * static_cast<float>(x.hv[e / 4][e % 4][i]) : 0.0f;
+            }
+            bf16x8 pb[kTerms];
+            q4_split<kTerms>(ph, pb);
+            o[i][0] *= alpha, o[i][1] *= alpha, op[i] *= alpha;
+#pragma unroll
+            for (int n = 0; n < kTerms; ++n) {
+                op[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pb[n], op[i], 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    o[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_value_operand(x.v[0][i], x.v[1][i], j), pb[n], o[i][j], 0, 0, 0);
+            }
+        }
+    };
+
+    int u = sh.part * sh.share + wave;
+    if (u < s_end) {
+        Q4Step<D> x, y;
+        load(u, x);
+        while (true) {                                       // wave-uniform
+            if (u + KW < s_end) load(u + KW, y);
+            compute(u, x);
+            u += KW;
+            if (u >= s_end) break;
+            if (u + KW < s_end) load(u + KW, x);
+            compute(u, y);
+            u += KW;
+            if (u >= s_end) break;
+        }
+    }
+    l = pair32_sum(pair16_sum(l));
+
+    const bool any_bad = __ballot(bad) != 0;                  // wave-uniform
+    // ---- the wavefronts' partials, joined in order: thread -> (column, dim) ----
+    float* lo = lds;                                          // [KW][lds_heads][D + 4]
+    float* lm = lo + KW * a.lds_heads * (D + 4);              // [KW][16][2]
+    int* lbad = reinterpret_cast<int*>(lm + KW * 32);         // [KW]
+    if (c16 < nh) {
+#pragma unroll
+        for (int i = 0; i < G; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = 32 * i + 2 * (4 * grp + e) + j;
+                    if (d < D)
+                        lo[(wave * a.lds_heads + c16) * (D + 4) + d] = 2.0f * __builtin_fmaf(op[i][e], -135.5f, o[i][j][e]);
+                }
+        if (grp == 0) {
+            lm[(wave * 16 + c16) * 2] = m;
+            lm[(wave * 16 + c16) * 2 + 1] = l;
+        }
+    }
+    if (lane == 0) lbad[wave] = any_bad ? 1 : 0;
+    __syncthreads();
+    int bads = 0;
+#pragma unroll
+    for (int w = 0; w < KW; ++w) bads |= lbad[w];
+    if (bads != 0 && wave == 0 && lane == 0) atomicOr(a.status, static_cast<uint32_t>(SPARDA_STATUS_PAGE_RANGE));
+    for (int e = wave * kWave + lane; e < nh * D; e += KW * kWave) {
+        const int c = e / D, d = e % D;
+        float mw[KW], M = -__builtin_inff();
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+            mw[w] = lm[(w * 16 + c) * 2];
+            M = fmaxf(M, mw[w]);
+        }
+        const float ref = M == -__builtin_inff() ? 0.0f : M;
+        float L = 0.0f, O = 0.0f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+            const float wt = __builtin_amdgcn_exp2f(mw[w] - ref);
+            L = __builtin_fmaf(wt, lm[(w * 16 + c) * 2 + 1], L);
+            O = __builtin_fmaf(wt, lo[(w * a.lds_heads + c) * (D + 4) + d], O);
+        }
+        if (bads) O = __builtin_nanf("");
+        const int t = (col0 + c) / a.R, h = t * a.heads + g * a.R + (col0 + c) % a.R;
+        if (sh.parts == 1) {
+            // (a token before the sequence's first position: zeros)
+            store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d,
+                           len - a.T + 1 + t <= 0 && !bads ? 0.0f : O / L);
+        } else {
+            const int64_t at = static_cast<int64_t>(item) * a.Hq + h;
+            a.part_o[at * D + d] = O;
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(M, L);
+        }
+    }
+}
+
+namespace {
+
+struct Q4Plan {
+    int kw;                  // wavefronts of a workgroup
+    int64_t target, least;   // items aimed at, steps of the smallest item
+    int64_t items, groups;   // items at most, workgroups an item
+    bool few;                // a sequence has few items in the mean
+};
+Q4Plan q4_plan(int64_t B, int64_t T, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D) {
+    const int64_t R = Hq / Hkv * T, heads = Hkv * cdiv(R, 16), steps = cdiv(cap, 32);
+    Q4Plan p{4, 1, 4, 0, heads, false};
+    if (steps <= 16 || (steps <= 64 && B * heads >= 128)) p.least = steps;
+    else p.target = 512 / heads - B / 2;
+    if (p.target < 1) p.target = 1;
+    p.items = p.target + B;
+    const int64_t most = B * cdiv(steps, p.least);   // every share the smallest
+    if (p.items > most) p.items = most;
+    p.few = p.items <= 16 * B;
+    return p;
+}
+
+}  // namespace
+
+size_t decode_paged_q4_workspace_bytes(int64_t B, int64_t T, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D) {
+    const Q4Plan p = q4_plan(B, T, cap, Hq, Hkv, D);
+    return p.items <= B ? 0 : static_cast<size_t>(p.items * T * Hq * (D + 2)) * sizeof(float);
+}
+
+int launch_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype, const void* pages,
+                           int64_t n_pages, int64_t ps, int64_t p_st, int64_t h_st, const int32_t* table, int64_t t_st,
+                           int64_t width, const int32_t* len, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                           float scale, void* out, int64_t out_sb, void* workspace, hipStream_t stream) {
+    PagedDecode a{};
+    const int64_t cap = width * ps, R = Hq / Hkv;
+    const Q4Plan p = q4_plan(B, T, cap, Hq, Hkv, D);
+    if (!grid_fits(p.items * p.groups, p.kw * kWave)) return set_error(SPARDA_ERR_SHAPE, "decode_paged_q4: grid too large");
+    if (const int rc = status_word(&a.status)) return rc;
+    a.q = q, a.q_sb = q_sb, a.q_st = q_st, a.q_sh = q_sh, a.k = pages;
+    a.pg = Pages{p_st, 0, h_st, table, t_st, static_cast<int>(width), static_cast<int>(n_pages)};
+    a.T = static_cast<int>(T), a.heads = static_cast<int>(Hq), a.step = 32;
+    a.ps16 = static_cast<int>(ps / 16), a.len = len, a.B = static_cast<int>(B), a.cap = static_cast<int>(cap);
+    a.Hq = static_cast<int>(T * Hq), a.Hkv = static_cast<int>(Hkv), a.R = static_cast<int>(R);
+    a.head_tiles = static_cast<int>(cdiv(R * T, 16));
+    a.target = static_cast<int>(p.target), a.least = static_cast<int>(p.least);
+    a.whole = p.items <= B;
+    a.lds_heads = static_cast<int>(R * T < 16 ? R * T : 16);
+    a.scale_log2 = 2.0f * scale * kPgLog2e, a.out = out, a.out_sb = out_sb;   // (h (2 c - 15) = 2 h (c - 7.5))
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = workspace ? a.part_o + p.items * a.Hq * D : nullptr;
+    const dim3 grid(static_cast<unsigned>(p.items * p.groups));
+#define SPARDA_DQ(DT_, D_)                                                                        \
+    hipLaunchKernelGGL((decode_paged_q4_kernel<DT_, D_, 4>), grid, dim3(4 * kWave),               \
+                       4 * (a.lds_heads * ((D_) + 4) + 33) * sizeof(float), stream, a)
+#define SPARDA_DQ_D(DT_)                      \
+    switch (D) {                              \
+        case 16: SPARDA_DQ(DT_, 16); break;   \
+        case 32: SPARDA_DQ(DT_, 32); break;   \
+        case 64: SPARDA_DQ(DT_, 64); break;   \
+        default: SPARDA_DQ(DT_, 128); break;  \
+    }
+    if (dtype == SPARDA_F32) SPARDA_DQ_D(SPARDA_F32)
+    else SPARDA_DQ_D(SPARDA_BF16)
+#undef SPARDA_DQ_D
+#undef SPARDA_DQ
+    if (p.items > B) launch_paged_join(a, D, dtype, p.few, stream);
+    return check_hip(hipGetLastError(), "decode_paged_q4_kernel");
+}
+
+}  // namespace sparda

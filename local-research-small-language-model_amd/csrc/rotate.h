@@ -1,0 +1,87 @@
+// The rotation of queries and keys by their positions, as the writes into pages
+// apply it (paged_rotate.hip, paged_q4.hip): pairs (i, i + D/2),
+//     y[i] = x[i] cos - x[i + D/2] sin,  y[i + D/2] = x[i + D/2] cos + x[i] sin,
+// products, sum and difference each rounded to fp32 (no fused multiply-add, so that the
+// result is that of the same formula in fp32 torch operations, and the 4-bit codes
+// made from it are the same), and once to the rows' type.
+#pragma once
+
+#include "common.h"
+#include "paged.h"
+
+namespace sparda {
+
+// New rows and their places; strides in elements.
+struct RotateAppend {
+    Pages pg;
+    int ps;
+    const int32_t *positions, *cu;
+    int n;
+    int64_t N;
+    const void* q;                 // [N, Hq, D]; Hq 0: none
+    int64_t q_st, q_sh;
+    const void *k_new, *v_new;     // [N, Hkv, D]
+    int64_t new_st, new_sh;
+    const float *cos, *sin;        // [rows, D/2]
+    int64_t cs_st, rows;
+    int Hq, Hkv;
+    void* q_out;
+    int64_t qo_st, qo_sh;
+    uint32_t* status;
+};
+
+// N angles of position pos from dim `at` on; NaN behind the tables
+template <int N>
+__device__ __forceinline__ void load_angles(const RotateAppend& a, int64_t pos, int at, bool off_table, float (&c)[N], float (&s)[N]) {
+    if (off_table) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) c[e] = s[e] = __builtin_nanf("");
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < N; e += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(a.cos + pos * a.cs_st + at + e);
+        const float4 y = *reinterpret_cast<const float4*>(a.sin + pos * a.cs_st + at + e);
+        c[e] = x.x, c[e + 1] = x.y, c[e + 2] = x.z, c[e + 3] = x.w;
+        s[e] = y.x, s[e + 1] = y.y, s[e + 2] = y.z, s[e + 3] = y.w;
+    }
+}
+
+__device__ __forceinline__ void turn(float& x, float& y, float c, float s) {
+#pragma clang fp contract(off)
+    const float xc = x * c, ys = y * s, yc = y * c, xs = x * s;
+    x = xc - ys;
+    y = yc + xs;
+}
+
+// two fp32 values as bf16, rounded to the nearest even
+__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    bf16x2 v;
+    v[0] = static_cast<__bf16>(x), v[1] = static_cast<__bf16>(y);
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+// 16 bytes of a row's first half and the 16 that they are paired with
+template <int DT, int N>
+__device__ __forceinline__ void turn_pieces(uint4& x, uint4& y, const float (&c)[N], const float (&s)[N]) {
+    uint32_t a[4] = {x.x, x.y, x.z, x.w}, b[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if constexpr (DT == SPARDA_F32) {
+            float u = __uint_as_float(a[w]), v = __uint_as_float(b[w]);
+            turn(u, v, c[w], s[w]);
+            a[w] = __float_as_uint(u), b[w] = __float_as_uint(v);
+        } else {
+            float u0 = __uint_as_float(a[w] << 16), u1 = __uint_as_float(a[w] & 0xffff0000u);
+            float v0 = __uint_as_float(b[w] << 16), v1 = __uint_as_float(b[w] & 0xffff0000u);
+            turn(u0, v0, c[2 * w], s[2 * w]);
+            turn(u1, v1, c[2 * w + 1], s[2 * w + 1]);
+            a[w] = pack_bf16(u0, u1), b[w] = pack_bf16(v0, v1);
+        }
+    }
+    x = make_uint4(a[0], a[1], a[2], a[3]);
+    y = make_uint4(b[0], b[1], b[2], b[3]);
+}
+
+}  // namespace sparda

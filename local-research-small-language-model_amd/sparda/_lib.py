@@ -134,6 +134,19 @@ SIGNATURES = {
     "sparda_decode_paged_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _int]),
     "sparda_decode_paged": (_int, [_p, _i64, _i64, _p, _p, _int, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p,
                                    _i64, _i64, _i64, _i64, _f32, _p, _i64, _p, _size, _p]),
+    "sparda_rotate_append_paged": (_int, [_p, _p, _int, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p,
+                                          _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64,
+                                          _p, _i64, _i64, _p]),
+    "sparda_append_paged_q4": (_int, [_p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _i64, _i64, _i64, _p,
+                                      _p, _int, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _p]),
+    "sparda_gather_paged_q4": (_int, [_p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _p, _int, _i64, _i64,
+                                      _i64, _i64, _i64, _p]),
+    "sparda_decode_paged_q4_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "sparda_decode_paged_q4": (_int, [_p, _i64, _i64, _i64, _int, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64,
+                                      _i64, _i64, _i64, _i64, _f32, _p, _i64, _p, _size, _p]),
+    "sparda_verify_drafts_workspace_bytes": (_size, [_i64, _i64, _i64, _int]),
+    "sparda_verify_drafts": (_int, [_p, _int, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _p, _p, _f32, _i64, _i64,
+                                    _i64, _p, _p, _p, _size, _p]),
 }
 
 _lock = threading.Lock()
@@ -189,7 +202,9 @@ def fail(name: str, rc: int) -> None:
 _HOST_ENTRIES = ("compress", "route", "prefill", "prefill_routed", "prefill_chunked", "decode",
                  "decode_workspace_bytes", "decode_selected", "decode_dense_workspace_bytes", "decode_sums", "produce",
                  "produce_at", "produce_cache_at", "ffn_decode", "rows_residual", "norm_gemv", "teacher_mass",
-                 "prefill_packed", "append_paged", "decode_paged", "decode_paged_workspace_bytes")
+                 "prefill_packed", "append_paged", "decode_paged", "decode_paged_workspace_bytes", "rotate_append_paged",
+                 "append_paged_q4", "gather_paged_q4", "decode_paged_q4", "decode_paged_q4_workspace_bytes",
+                 "verify_drafts", "verify_drafts_workspace_bytes")
 
 
 class _NoHost:

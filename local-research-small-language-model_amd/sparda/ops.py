@@ -481,6 +481,7 @@ class DecodeWorkspace:
 STATUS_PREFILL_WAIT_TIMEOUT = 1
 STATUS_SEQUENCE_RANGE = 2
 STATUS_PAGE_RANGE = 4
+STATUS_POSITION_RANGE = 8
 
 
 def status(device=None, clear: bool = True) -> int:
@@ -1318,6 +1319,309 @@ def decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
              lengths.data_ptr(), B, Hq, Hkv, D, float(scale), out.data_ptr(), out.stride(0),
              ws.data_ptr() if ws is not None else None, nbytes, _stream(dev))
     return out
+
+
+def _check_rotation(q, cos, sin, N: int, D: int, dtype, out):
+    """Queries and angles of a rotated write: q or None, both tables, out or None."""
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise TypeError("sparda: cos and sin must be float32")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] * 2 != D or cos.shape[0] == 0:
+        raise ValueError(f"sparda: cos and sin must be [positions,{D // 2}], got {tuple(cos.shape)}, {tuple(sin.shape)}")
+    if q is None:
+        if out is not None:
+            raise ValueError("sparda: out is the rotated queries', and there are none")
+        return None, cos, sin, None
+    if q.dtype != dtype:
+        raise TypeError("sparda: q and the new rows must share a dtype")
+    if q.dim() != 3 or q.shape[0] != N or q.shape[2] != D:
+        raise ValueError(f"sparda: q must be [{N},Hq,{D}], got {tuple(q.shape)}")
+    if out is not None:
+        _check_out(out, q.shape, dtype)
+    return _rows16(q), cos, sin, out
+
+
+def _tables16(cos, sin):
+    cos, sin = _rows16(cos), _rows16(sin)
+    if cos.stride(0) != sin.stride(0):
+        cos, sin = cos.contiguous(), sin.contiguous()
+    return cos, sin
+
+
+def _new_rows(k_new, v_new, positions, cu_seqlens, B: int, Hkv: int, D: int):
+    """The new rows of an append, as pieces of 16 bytes with the same strides."""
+    if k_new.dtype != v_new.dtype:
+        raise TypeError("sparda: k_new and v_new must share a dtype")
+    if k_new.dim() != 3 or k_new.shape != v_new.shape or tuple(k_new.shape[1:]) != (Hkv, D):
+        raise ValueError(f"sparda: the new rows must be [N,{Hkv},{D}], got {tuple(k_new.shape)}, {tuple(v_new.shape)}")
+    _check_sequences(positions, cu_seqlens, B, k_new.shape[0])
+    k_new, v_new = _rows16(k_new), _rows16(v_new)
+    if k_new.stride() != v_new.stride():
+        k_new, v_new = k_new.contiguous(), v_new.contiguous()
+    return k_new, v_new
+
+
+def _check_sequences(positions, cu_seqlens, B: int, N: int) -> None:
+    if _int32_array(positions, 1, "positions").numel() != B:
+        raise ValueError(f"sparda: {positions.numel()} positions for {B} sequences")
+    if cu_seqlens is None:
+        if N != B:
+            raise ValueError(f"sparda: {N} rows for {B} sequences: give cu_seqlens, or one row for each")
+    elif _int32_array(cu_seqlens, 1, "cu_seqlens").numel() != B + 1:
+        raise ValueError(f"sparda: cu_seqlens must hold {B + 1} offsets")
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return t.data_ptr() if t is not None else None
+
+
+def rotate_append_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                        positions: torch.Tensor, q: Optional[torch.Tensor], k_new: torch.Tensor, v_new: torch.Tensor,
+                        cos: torch.Tensor, sin: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
+                        out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """``append_paged`` with the rotation by position applied on the way.
+
+    q [N,Hq,D] (or None) and k_new [N,Hkv,D] are rotated by their rows' positions
+    (positions[b] + j) with cos, sin fp32 [positions,D/2] (``RotaryEmbedding.tables``): pairs (d, d + D/2), in
+    fp32, rounded once. The keys and, as they are, the values go into the
+    pages; returns the rotated queries [N,Hq,D] (`out`, which may be q itself, or None without
+    q). Rows of no sequence, or of one with a negative position, keep what `out`
+    holds (with out=None: anything). A position behind the tables gives a query of NaN, a dropped
+    row, and STATUS_POSITION_RANGE in status(); the rest as in ``append_paged``.
+    """
+    if out is None and q is not None:
+        r = _host.rotate_append_paged(k_pages, v_pages, page_table, positions, q, k_new, v_new, cos, sin, cu_seqlens)
+        if r is not None:
+            return r if type(r) is not int else _lib.fail("sparda_rotate_append_paged", r)
+    dev = require_device(k_pages, v_pages, page_table, positions, q, k_new, v_new, cos, sin, cu_seqlens, out)
+    _inference_only(k_pages, v_pages, q, k_new, v_new)
+    _check_pages(k_pages, v_pages, page_table)
+    code = _dtype_code(k_pages)
+    if k_new.dtype != k_pages.dtype or v_new.dtype != k_pages.dtype:
+        raise TypeError("sparda: the new rows and the pages must share a dtype")
+    P, ps, Hkv, D = k_pages.shape
+    B, width = page_table.shape
+    k_new, v_new = _new_rows(k_new, v_new, positions, cu_seqlens, B, Hkv, D)
+    N = k_new.shape[0]
+    q, cos, sin, out = _check_rotation(q, cos, sin, N, D, k_pages.dtype, out)
+    if q is not None and out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if N == 0 or B == 0:
+        return out
+    cos, sin = _tables16(cos, sin)
+    to = _rows16(out) if out is not None else None
+    with torch.cuda.device(dev):
+        call("sparda_rotate_append_paged", k_pages.data_ptr(), v_pages.data_ptr(), code, P, ps, *k_pages.stride()[:3],
+             page_table.data_ptr(), page_table.stride(0), width, positions.data_ptr(), _ptr(cu_seqlens), B, _ptr(q),
+             *(q.stride()[:2] if q is not None else (0, 0)), q.shape[1] if q is not None else 0, k_new.data_ptr(),
+             v_new.data_ptr(), N, k_new.stride(0), k_new.stride(1), Hkv, D, cos.data_ptr(), sin.data_ptr(),
+             cos.stride(0), cos.shape[0], _ptr(to), *(to.stride()[:2] if to is not None else (0, 0)), _stream(dev))
+        if to is not out:
+            out.copy_(to)
+    return out
+
+
+def q4_page_shape(n_pages: int, page_size: int, n_kv_heads: int, head_dim: int) -> Tuple[int, int, int, int]:
+    """Shape of a uint8 tensor that holds keys and values as pages of 4-bit codes."""
+    if page_size < 16 or page_size % 16 or head_dim not in (16, 32, 64, 128):
+        raise ValueError(f"sparda: pages of {page_size} rows of {head_dim} dims (a multiple of 16; 16, 32, 64 or 128)")
+    return n_pages, n_kv_heads, page_size // 16, 576 * ((head_dim + 31) // 32)
+
+
+def _check_q4(pages: torch.Tensor, page_table: torch.Tensor, D: int):
+    """Pages, rows of a page, heads; D None: what the tiles hold."""
+    if pages.dtype != torch.uint8:
+        raise TypeError(f"sparda: pages of 4-bit codes are uint8, got {pages.dtype}")
+    if pages.dim() != 4 or pages.shape[3] not in (576, 1152, 2304) or pages.shape[2] == 0:
+        raise ValueError(f"sparda: pages of 4-bit codes are [pages,Hkv,page_size/16,576 G] (q4_page_shape), got "
+                         f"{tuple(pages.shape)}")
+    P, Hkv, tiles, size = pages.shape
+    if pages.stride(3) != 1 or (tiles > 1 and pages.stride(2) != size):
+        raise ValueError("sparda: the tiles of a head of a page must be contiguous")
+    _int32_array(page_table, 2, "page_table")
+    if D is None:
+        D = size // 18
+    if (D + 31) // 32 * 576 != size:
+        raise ValueError(f"sparda: pages with tiles of {size} bytes do not hold heads of {D} dims")
+    return P, tiles * 16, Hkv, D
+
+
+def append_paged_q4(pages: torch.Tensor, page_table: torch.Tensor, positions: torch.Tensor, k_new: torch.Tensor,
+                    v_new: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
+                    cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """``append_paged`` into pages of 4-bit codes, keys and values in one tensor.
+
+    pages uint8 of ``q4_page_shape``: groups of 32 dims, each the odd multiples -15 h .. 15 h of
+    a number of its own (the group's largest magnitude over 15, in fp16), the
+    nearest one to each element; 4.5 bits a dim. With cos and sin the keys
+    are rotated before, and the rows of q, which are returned, as by ``rotate_append_paged``. A group with a value that is not
+    finite is read as NaN.
+    """
+    if out is None:
+        r = _host.append_paged_q4(pages, page_table, positions, k_new, v_new, cu_seqlens, q, cos, sin)
+        if r is not None:
+            return r if type(r) is not int else None if r == 0 else _lib.fail("sparda_append_paged_q4", r)
+    dev = require_device(pages, page_table, positions, k_new, v_new, cu_seqlens, q, cos, sin, out)
+    _inference_only(q, k_new, v_new)
+    code = _dtype_code(k_new)
+    P, ps, Hkv, D = _check_q4(pages, page_table, k_new.shape[-1])
+    B, width = page_table.shape
+    k_new, v_new = _new_rows(k_new, v_new, positions, cu_seqlens, B, Hkv, D)
+    N = k_new.shape[0]
+    if (cos is None) != (sin is None) or (cos is None and (q is not None or out is not None)):
+        raise ValueError("sparda: the rotation takes cos and sin, and queries take the rotation")
+    if cos is not None:
+        q, cos, sin, out = _check_rotation(q, cos, sin, N, D, k_new.dtype, out)
+        cos, sin = _tables16(cos, sin)
+    if q is not None and out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if N == 0 or B == 0:
+        return out
+    to = _rows16(out) if out is not None else None
+    with torch.cuda.device(dev):
+        call("sparda_append_paged_q4", pages.data_ptr(), P, ps, pages.stride(0), pages.stride(1), page_table.data_ptr(),
+             page_table.stride(0), width, positions.data_ptr(), _ptr(cu_seqlens), B, _ptr(q),
+             *(q.stride()[:2] if q is not None else (0, 0)), q.shape[1] if q is not None else 0, k_new.data_ptr(),
+             v_new.data_ptr(), code, N, k_new.stride(0), k_new.stride(1), Hkv, D, _ptr(cos), _ptr(sin),
+             cos.stride(0) if cos is not None else 0, cos.shape[0] if cos is not None else 0, _ptr(to),
+             *(to.stride()[:2] if to is not None else (0, 0)), _stream(dev))
+        if to is not out:
+            out.copy_(to)
+    return out
+
+
+def gather_paged_q4(pages: torch.Tensor, page_table: torch.Tensor, positions: torch.Tensor, rows: int,
+                    cu_seqlens: Optional[torch.Tensor] = None, head_dim: Optional[int] = None,
+                    dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The values that rows of 4-bit pages stand for: k, v [rows,Hkv,head_dim] of dtype.
+
+    The counterpart of ``append_paged_q4``: row j of sequence b is position
+    positions[b] + j, sequences packed by cu_seqlens (int32 [B+1]), or one row each without. A
+    prompt that is prefilled in chunks attends to them with ``prefill_packed``. head_dim: 16 where
+    the heads have 16 dims (32 are taken from the tiles then). Rows without a page are NaN and raise
+    STATUS_PAGE_RANGE; rows of no sequence hold anything.
+    """
+    r = _host.gather_paged_q4(pages, page_table, positions, rows, cu_seqlens, head_dim, dtype is torch.float32) \
+        if dtype in _DT else None
+    if r is not None:
+        return r if type(r) is not int else _lib.fail("sparda_gather_paged_q4", r)
+    dev = require_device(pages, page_table, positions, cu_seqlens)
+    P, ps, Hkv, D = _check_q4(pages, page_table, head_dim)
+    B, width = page_table.shape
+    if rows < 0:
+        raise ValueError(f"sparda: {rows} rows")
+    _check_sequences(positions, cu_seqlens, B, rows)
+    k, v = (torch.empty((rows, Hkv, D), dtype=dtype, device=dev) for _ in range(2))
+    code = _dtype_code(k)
+    if rows == 0 or B == 0:
+        return k, v
+    with torch.cuda.device(dev):
+        call("sparda_gather_paged_q4", pages.data_ptr(), P, ps, pages.stride(0), pages.stride(1), page_table.data_ptr(),
+             page_table.stride(0), width, positions.data_ptr(), _ptr(cu_seqlens), B, k.data_ptr(), v.data_ptr(), code,
+             rows, k.stride(0), k.stride(1), Hkv, D, _stream(dev))
+    return k, v
+
+
+def decode_paged_q4(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                    scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``decode_paged`` over pages of 4-bit codes, for one token or the last T of every sequence.
+
+    q [B,Hq,D], or [B,T,Hq,D] with the T newest tokens (drafted ones, T <= 64); pages and
+    page_table as in ``append_paged_q4``; lengths int32 [B], the T tokens among them: token t attends to
+    positions [0, lengths[b] - T + 1 + t). Returns [B,Hq*D] or [B,T,Hq*D]; zeros, NaN and the
+    status as in ``decode_paged``.
+    """
+    if out is None:
+        r = _host.decode_paged_q4(q, pages, page_table, lengths, scale)
+        if r is not None:
+            return r if type(r) is not int else _lib.fail("sparda_decode_paged_q4", r)
+    dev = require_device(q, pages, page_table, lengths, out)
+    _inference_only(q)
+    code = _dtype_code(q)
+    P, ps, Hkv, D = _check_q4(pages, page_table, q.shape[-1])
+    B, width = page_table.shape
+    if q.dim() not in (3, 4) or q.shape[0] != B:
+        raise ValueError(f"sparda: decode_paged_q4 takes q [{B},Hq,{D}] or [{B},T,Hq,{D}] for this cache, got {tuple(q.shape)}")
+    if _int32_array(lengths, 1, "lengths").numel() != B:
+        raise ValueError(f"sparda: {lengths.numel()} lengths for {B} sequences")
+    T, Hq = (1 if q.dim() == 3 else q.shape[1]), q.shape[-2]
+    q = _rows16(q)
+    shape = (B, Hq * D) if q.dim() == 3 else (B, T, Hq * D)
+    if scale is None:
+        scale = default_scale(D)
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+    else:
+        _check_out(out, shape, q.dtype)
+        if q.dim() == 4 and T > 1 and out.stride(1) != Hq * D:
+            raise ValueError("sparda: out must hold the tokens of a sequence contiguously")
+    if B == 0 or T == 0:
+        return out
+    nbytes = _lib.load().sparda_decode_paged_q4_workspace_bytes(B, T, width, ps, Hq, Hkv, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with torch.cuda.device(dev):
+        call("sparda_decode_paged_q4", q.data_ptr(), q.stride(0), q.stride(1) if q.dim() == 4 else 0, q.stride(-2), code,
+             pages.data_ptr(), P, ps, pages.stride(0), pages.stride(1), page_table.data_ptr(), page_table.stride(0), width,
+             lengths.data_ptr(), B, T, Hq, Hkv, D, float(scale), out.data_ptr(), out.stride(0), _ptr(ws), nbytes,
+             _stream(dev))
+    return out
+
+
+def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, uniform: torch.Tensor,
+                  draft_probs: Optional[torch.Tensor] = None, n_drafts: Optional[torch.Tensor] = None,
+                  temperature=1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Which drafted tokens the target accepts, and the token it draws behind them.
+
+    logits [B,K+1,V] (fp32 or bf16), the target's at every sequence's last token and its K drafts; drafts int32
+    [B,K]; uniform fp32 [B,K+1] in [0, 1); draft_probs fp32 [B,K,V], the
+    distributions that the drafts were drawn from (None: given tokens, as from a
+    lookup); n_drafts int32 [B], the drafts that count (None: K each); temperature: a number, or fp32 [B]. With p_i =
+    softmax(logits[:, i] / temperature), draft i is accepted while uniform[i] q_i(draft) < p_i(draft); behind
+    n accepted ones the token is drawn by uniform[K] from max(p_n - q_n, 0) after a
+    rejection, otherwise from p_n. A temperature of 0 takes the largest logit (the lowest index of equal ones). So the tokens
+    are distributed as if each had been drawn from p.
+
+    Returns tokens int32 [B,K+1] (accepted drafts, the token, then -1) and
+    n_accepted int32 [B]. Filters (top-k and the like) are -inf logits. A row without a
+    distribution (no logit above -inf, or NaN or +inf) accepts nothing and gives -1.
+    """
+    whole = isinstance(temperature, torch.Tensor)
+    r = _host.verify_drafts(logits, drafts, uniform, draft_probs, n_drafts, temperature)
+    if r is not None:
+        return r if type(r) is not int else _lib.fail("sparda_verify_drafts", r)
+    dev = require_device(logits, drafts, uniform, draft_probs, n_drafts, temperature if whole else None)
+    _inference_only(logits, draft_probs)
+    code = _dtype_code(logits)
+    if logits.dim() != 3 or logits.shape[1] < 1:
+        raise ValueError(f"sparda: verify_drafts takes logits [B,K+1,V], got {tuple(logits.shape)}")
+    B, K, V = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+    if drafts.dtype != torch.int32 or (n_drafts is not None and n_drafts.dtype != torch.int32):
+        raise TypeError("sparda: drafts and n_drafts must be int32")
+    if tuple(drafts.shape) != (B, K) or (n_drafts is not None and tuple(n_drafts.shape) != (B,)):
+        raise ValueError(f"sparda: drafts must be [{B},{K}] and n_drafts [{B}] for these logits")
+    if uniform.dtype != torch.float32 or (draft_probs is not None and draft_probs.dtype != torch.float32):
+        raise TypeError("sparda: uniform and draft_probs must be float32")
+    if tuple(uniform.shape) != (B, K + 1) or (draft_probs is not None and tuple(draft_probs.shape) != (B, K, V)):
+        raise ValueError(f"sparda: uniform must be [{B},{K + 1}] and draft_probs [{B},{K},{V}] for these logits")
+    if whole and (temperature.dtype != torch.float32 or tuple(temperature.shape) != (B,)):
+        raise ValueError(f"sparda: temperatures must be float32 [{B}]")
+    tokens = torch.empty((B, K + 1), dtype=torch.int32, device=dev)
+    accepted = torch.empty((B,), dtype=torch.int32, device=dev)
+    if B == 0:
+        return tokens, accepted
+    logits, uniform, drafts = _rowmajor(logits), _rowmajor(uniform), _rowmajor(drafts)
+    probs = _rowmajor(draft_probs) if draft_probs is not None and K > 0 else None
+    n_drafts = n_drafts.contiguous() if n_drafts is not None else None
+    each = temperature.contiguous() if whole else None
+    nbytes = _lib.load().sparda_verify_drafts_workspace_bytes(B, K, V, code)
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        call("sparda_verify_drafts", logits.data_ptr(), code, logits.stride(0), logits.stride(1), _ptr(drafts) if K else None,
+             drafts.stride(0) if K else 0, uniform.data_ptr(), uniform.stride(0), _ptr(probs),
+             *(probs.stride()[:2] if probs is not None else (0, 0)), _ptr(n_drafts), _ptr(each),
+             0.0 if whole else float(temperature), B, K, V, tokens.data_ptr(), accepted.data_ptr(), ws.data_ptr(), nbytes,
+             _stream(dev))
+    return tokens, accepted
 
 
 def block_sums(k: torch.Tensor, pos: int, n: int, block_size: int, sums: torch.Tensor) -> torch.Tensor:
