@@ -153,7 +153,8 @@ struct PagedDecode {
     int target, least;
     int whole;                    // every sequence is one item
     int lds_heads;                // heads of the largest tile
-    float scale_log2;
+    float scale_log2;             // the scores' scale in log2 units
+    int negate;                   // (4-bit pages: scale_log2 is its magnitude, q takes the sign)
     void* out;
     int64_t out_sb;
     float *part_o, *part_ml;      // [items, Hq, D], [items, Hq, 2]

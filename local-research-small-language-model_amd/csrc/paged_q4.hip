@@ -23,6 +23,9 @@
 #include "paged.h"
 #include "rotate.h"
 
+#include <type_traits>
+#include <cstdlib>
+
 namespace sparda {
 
 namespace {
@@ -297,14 +300,6 @@ namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-// a step's operands of 32 keys (two tiles), as loaded; words of a lane
-template <int D>
-struct Q4Step {
-    static constexpr int G = q4_groups(D);
-    uint32_t k[2][G], v[2][G];
-    _Float16 hk[2][4][G], hv[2][4][G];
-};
-
 template <int N>
 __device__ __forceinline__ void q4_load_words(const char* p, uint32_t (&w)[N]) {
     if constexpr (N == 4) {
@@ -334,52 +329,73 @@ __device__ __forceinline__ void q4_load_scales(const char* p, _Float16 (&h)[4][G
     }
 }
 
-// Eight codes of a word as bf16 128 + c: nibbles n and n + 4 are the halves of register n
-__device__ __forceinline__ bf16x8 q4_key_operand(uint32_t w) {
-    uint4 x;
-    x.x = (w & 0x000f000fu) | 0x43004300u;
-    x.y = (w >> 4 & 0x000f000fu) | 0x43004300u;
-    x.z = (w >> 8 & 0x000f000fu) | 0x43004300u;
-    x.w = (w >> 12 & 0x000f000fu) | 0x43004300u;
-    return __builtin_bit_cast(bf16x8, x);
+// Codes go to the matrix products as bf16 16.5 + c: a code at bits 3 .. 6 of the mantissa over a
+// half below it. The middle level is then 24, a bf16 value, and is taken off by a product with the
+// constant -24 (128 + c would need one shift less, and a middle of 135.5, which bf16 does not hold).
+// The masks are held in registers, so that the and and the or of a word are one instruction (of
+// two literals the compiler makes two).
+struct Q4Masks {
+    uint32_t bits, magic;
+};
+__device__ __forceinline__ Q4Masks q4_masks() {
+    Q4Masks m{0x00780078u, 0x41844184u};
+    asm("" : "+s"(m.bits));
+    asm("" : "+v"(m.magic));
+    return m;
 }
-// nibble j of the eight positions of two tiles' words
-__device__ __forceinline__ bf16x8 q4_value_operand(uint32_t w0, uint32_t w1, int j) {
-    uint4 x;
-    x.x = (w0 >> (4 * j) & 0x000f000fu) | 0x43004300u;
-    x.y = (w0 >> (4 * j + 8) & 0x000f000fu) | 0x43004300u;
-    x.z = (w1 >> (4 * j) & 0x000f000fu) | 0x43004300u;
-    x.w = (w1 >> (4 * j + 8) & 0x000f000fu) | 0x43004300u;
-    return __builtin_bit_cast(bf16x8, x);
+// bits n .. n + 3 of both halves of a word
+template <int N>
+__device__ __forceinline__ uint32_t q4_pair(uint32_t w, const Q4Masks& m) {
+    return ((N < 3 ? w << (3 - N) : w >> (N > 3 ? N - 3 : 0)) & m.bits) | m.magic;
+}
+// the eight codes of a key word: nibbles n and n + 4 are the halves of register n
+__device__ __forceinline__ bf16x8 q4_key_operand(uint32_t w, const Q4Masks& m) {
+    return __builtin_bit_cast(bf16x8, make_uint4(q4_pair<0>(w, m), q4_pair<4>(w, m), q4_pair<8>(w, m), q4_pair<12>(w, m)));
+}
+// nibble J of the eight positions of two tiles' words
+template <int J>
+__device__ __forceinline__ bf16x8 q4_value_operand(uint32_t w0, uint32_t w1, const Q4Masks& m) {
+    return __builtin_bit_cast(bf16x8, make_uint4(q4_pair<4 * J>(w0, m), q4_pair<4 * J + 8>(w0, m), q4_pair<4 * J>(w1, m),
+                                                 q4_pair<4 * J + 8>(w1, m)));
 }
 
 // x as a sum of TERMS bf16 values (1: rounded; 3: all 24 bits of it)
 template <int TERMS>
 __device__ __forceinline__ void q4_split(const float (&x)[8], bf16x8 (&out)[TERMS]) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    float rest[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        float rest = x[e];
+    for (int e = 0; e < 8; ++e) rest[e] = x[e];
 #pragma unroll
-        for (int n = 0; n < TERMS; ++n) {
-            out[n][e] = static_cast<__bf16>(rest);
-            rest -= static_cast<float>(out[n][e]);
+    for (int n = 0; n < TERMS; ++n) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            w[e] = pack_bf16(rest[2 * e], rest[2 * e + 1]);
+            if (n + 1 < TERMS) {
+                rest[2 * e] -= __uint_as_float(w[e] << 16);
+                rest[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
+            }
         }
+        out[n] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
     }
 }
+
+// pages and tiles of the two tiles of a step
+struct Q4Place {
+    int id[2], tile[2];
+};
 
 }  // namespace
 
 // One workgroup of KW wavefronts per (tile of 16 columns, item). The columns are the (token, query
 // head) pairs of a KV head, token-major; token t of T sees the positions below
-// len - T + 1 + t. The codes go to the matrix products as bf16 128 + c, and the
-// numbers h stay outside of them:
-//     S^T[key, col] = 2 sum_g h_g[key] (sum_{d in g} (128 + c) q[d] - 135.5 sum_{d in g} q[d])
-//     O^T[d, col]  += 2 sum_key P_g[key, col] (128 + c) - 135.5 P_g,  P_g = exp2(S - m) h_g[key] in bf16
-// The subtracted sums are products themselves: of q with ones once, the start of every
-// score's accumulator, and of the rounded P_g with ones beside the values', so that
-// their roundings cancel. The levels, odd multiples of h, thereby enter without rounding.
+// len - T + 1 + t. The numbers h stay outside of the products with the codes:
+//     S^T[key, col] = 2 sum_g h_g[key] sum_{d in g} ((16.5 + c) - 24) q[d]
+//     O^T[d, col]  += 2 sum_key ((16.5 + c) - 24) P_g[key, col],  P_g = exp2(S - m) h_g[key] in bf16
+// so that the levels, odd multiples of h, enter without rounding.
 template <int DT, int D, int KW>
-__global__ void __launch_bounds__(KW* kWave, 2) decode_paged_q4_kernel(PagedDecode a) {
+__global__ void __launch_bounds__(KW* kWave, (D == 128 ? 3 : 4) - (DT == SPARDA_F32 ? 1 : 0)) decode_paged_q4_kernel(PagedDecode a) {
     constexpr int G = q4_groups(D), kTerms = DT == SPARDA_F32 ? 3 : 1, kStep = 32, kEs = DT == SPARDA_F32 ? 4 : 2;
     extern __shared__ float lds[];
     const int lane = threadIdx.x % kWave;
@@ -402,92 +418,122 @@ __global__ void __launch_bounds__(KW* kWave, 2) decode_paged_q4_kernel(PagedDeco
     const int s_end = min(steps, (sh.part + 1) * sh.share);
     bool bad = sh.bad;
 
-    // this lane's column of Q, and what its codes' 135.5 amount to
+    // this lane's column of Q
     const int col = col0 + (c16 < nh ? c16 : nh - 1), tok = col / a.R, head = g * a.R + col % a.R;
     const int lim = len - a.T + 1 + tok;                    // positions the column sees
     bf16x8 qr[G][kTerms];
-    f32x4 less[G];
     {
-        bf16x8 ones;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ones[e] = static_cast<__bf16>(1.0f);
         const char* q = static_cast<const char*>(a.q) + (b * a.q_sb + tok * a.q_st + head * a.q_sh) * kEs;
 #pragma unroll
         for (int i = 0; i < G; ++i) {
             float x[8];
             if (c16 < nh && 32 * i + 8 * grp < D) {
                 q4_load8<DT>(q + (32 * i + 8 * grp) * kEs, x);
+                if (a.negate) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = -x[e];
+                }
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = 0.0f;
             }
             q4_split<kTerms>(x, qr[i]);
-            f32x4 s{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int n = 0; n < kTerms; ++n) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, qr[i][n], s, 0, 0, 0);
-            less[i] = s * -135.5f;
         }
     }
 
-    const int32_t* row = a.pg.table + b * a.pg.t_st;
+    // The walk over the table: tile 2 u is `rem` tiles into page `page`. The page numbers of a step are
+    // read a step before its codes, through the scalar cache.
+    const auto* row = (const __attribute__((address_space(4))) int32_t*)(a.pg.table + b * a.pg.t_st);
     const char* kv = static_cast<const char*>(a.k) + g * a.pg.h_st;
     const int last_tile = (len - 1) / 16;
-    const int o_codes = lane * 4 * G, o_scale = 512 * G + grp * 8 * G;
-    auto load = [&](int u, Q4Step<D>& x) __attribute__((always_inline)) {
+    const int o_keys = (c16 * 4 + grp) * 4 * G, o_values = 256 * G + lane * 4 * G, o_scales = 512 * G + grp * 8 * G;
+    int u = sh.part * sh.share + wave;
+    int page = 2 * u / a.ps16, rem = 2 * u % a.ps16;
+    const int adv_p = 2 * KW / a.ps16, adv_r = 2 * KW % a.ps16;
+    auto places = [&](int v) __attribute__((always_inline)) {
+        Q4Place at;
+        const bool two = 2 * v + 1 <= last_tile, next = rem + 1 == a.ps16;   // (past the end: the first tile again, masked)
+        at.tile[0] = rem, at.tile[1] = !two ? rem : next ? 0 : rem + 1;
+        at.id[0] = row[page], at.id[1] = row[two && next ? page + 1 : page];
+        rem += adv_r;
+        page += adv_p;
+        if (rem >= a.ps16) rem -= a.ps16, ++page;
+        return at;
+    };
+    uint32_t xk[2][G], xv[2][G];                             // the codes of a step, as loaded
+    _Float16 hk[2][4][G], hv[2][4][G];
+    const char* base[2];
+    auto locate = [&](const Q4Place& at) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            int tile = 2 * u + t;
-            if (tile > last_tile) tile = last_tile;         // past the end: the last tile again, masked
-            const int p = tile / a.ps16, r = tile - p * a.ps16;
-            int id = row[p];
+            int id = at.id[t];
             if (id < 0 || id >= a.pg.n_pages) bad = true, id = 0;
-            const char* base = kv + id * a.pg.p_st + r * (576 * G);
-            // (keys: position c16, quarter grp; values: four grp, pair c16)
-            q4_load_words<G>(base + (c16 * 4 + grp) * 4 * G, x.k[t]);
-            q4_load_words<G>(base + 256 * G + o_codes, x.v[t]);
-            q4_load_scales<G>(base + o_scale, x.hk[t]);
-            q4_load_scales<G>(base + o_scale + 32 * G, x.hv[t]);
+            base[t] = kv + id * a.pg.p_st + at.tile[t] * (576 * G);
         }
     };
+    // (keys: position c16, quarter grp; values: four grp, pair c16)
+    auto load_keys = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) q4_load_words<G>(base[t] + o_keys, xk[t]), q4_load_scales<G>(base[t] + o_scales, hk[t]);
+    };
+    auto load_values = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) q4_load_words<G>(base[t] + o_values, xv[t]), q4_load_scales<G>(base[t] + o_scales + 32 * G, hv[t]);
+    };
 
-    float m = -__builtin_inff(), l = 0.0f;                   // the column's maximum (log2 units), this lane's part of its sum
-    f32x4 o[G][2], op[G];
+    // m: the column's reference, in the scores' own units, l: this lane's part of its sum
+    float m = -__builtin_inff(), ref = 0.0f, l = 0.0f;
+    const float slack = 16.0f / a.scale_log2;
+    f32x4 o[G][2];
 #pragma unroll
-    for (int i = 0; i < G; ++i) o[i][0] = o[i][1] = op[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    bf16x8 ones;
+    for (int i = 0; i < G; ++i) o[i][0] = o[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    bf16x8 middle;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ones[e] = static_cast<__bf16>(1.0f);
-    auto compute = [&](int u, const Q4Step<D>& x) __attribute__((always_inline)) {
-        f32x4 s[2];
+    for (int e = 0; e < 8; ++e) middle[e] = static_cast<__bf16>(-24.0f);
+    const Q4Masks masks = q4_masks();
+    f32x4 s[2];
+    auto scores = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < G; ++i) {
-                const bf16x8 ka = q4_key_operand(x.k[t][i]);
-                f32x4 y = less[i];
+                const bf16x8 ka = q4_key_operand(xk[t][i], masks);
+                f32x4 y{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int n = 0; n < kTerms; ++n) y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, qr[i][n], y, 0, 0, 0);
 #pragma unroll
                 for (int n = 0; n < kTerms; ++n) y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qr[i][n], y, 0, 0, 0);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[t][e] = __builtin_fmaf(y[e], static_cast<float>(x.hk[t][e][i]), s[t][e]);
+                for (int e = 0; e < 4; ++e) s[t][e] = __builtin_fmaf(y[e], static_cast<float>(hk[t][e][i]), s[t][e]);
+                __builtin_amdgcn_sched_barrier(0);           // (operands of one group at a time: registers)
             }
         }
-        const int left = lim - u * kStep - 4 * grp;          // this lane's keys 16 t + e below it are the column's
-        float mx = m;
+    };
+    auto attend = [&](auto masked, int v) __attribute__((always_inline)) {
+        constexpr bool kMask = decltype(masked)::value;
+        const int left = lim - v * kStep - 4 * grp;          // this lane's keys 16 t + e below it are the column's
+        float mx = -__builtin_inff();
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, 16 * t + e < left ? s[t][e] * a.scale_log2 : -__builtin_inff());
-        mx = pair32_max(pair16_max(mx));
-        const float ref = mx == -__builtin_inff() ? 0.0f : mx;
-        const float alpha = __builtin_amdgcn_exp2f(m - ref);
-        m = mx;
-        l *= alpha;
+            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, !kMask || 16 * t + e < left ? s[t][e] : -__builtin_inff());
+        // The reference follows the maximum only where a weight would pass 2^16: weights keep their
+        // relative precision whatever they are measured against, and most steps rescale nothing.
+        if (__ballot(!(mx <= m + slack)) != 0) {             // (scale 0: -inf + inf, no order)
+            const float top = fmaxf(m, pair32_max(pair16_max(mx)));
+            const float to = top == -__builtin_inff() ? 0.0f : top * a.scale_log2;
+            const float alpha = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - to);
+            m = top, ref = to;
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < G; ++i) o[i][0] *= alpha, o[i][1] *= alpha;
+        }
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const bool in = 16 * (e / 4) + e % 4 < left;
-            p[e] = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 4][e % 4], a.scale_log2, -ref)) : 0.0f;
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 4][e % 4], a.scale_log2, -ref));
+            if (kMask) p[e] = 16 * (e / 4) + e % 4 < left ? p[e] : 0.0f;
             l += p[e];
         }
 #pragma unroll
@@ -495,38 +541,48 @@ __global__ void __launch_bounds__(KW* kWave, 2) decode_paged_q4_kernel(PagedDeco
             float ph[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                // (a number behind the column's positions may be anything)
-                const bool in = 16 * (e / 4) + e % 4 < left;
-                ph[e] = in ? p[e] * static_cast<float>(x.hv[e / 4][e % 4][i]) : 0.0f;
+                ph[e] = __builtin_fmaf(p[e], static_cast<float>(hv[e / 4][e % 4][i]), 0.0f);
+                if (kMask) ph[e] = 16 * (e / 4) + e % 4 < left ? ph[e] : 0.0f;   // (a number behind the column's positions may be anything)
             }
             bf16x8 pb[kTerms];
             q4_split<kTerms>(ph, pb);
-            o[i][0] *= alpha, o[i][1] *= alpha, op[i] *= alpha;
 #pragma unroll
             for (int n = 0; n < kTerms; ++n) {
-                op[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pb[n], op[i], 0, 0, 0);
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    o[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_value_operand(x.v[0][i], x.v[1][i], j), pb[n], o[i][j], 0, 0, 0);
+                o[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, pb[n], o[i][0], 0, 0, 0);
+                o[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, pb[n], o[i][1], 0, 0, 0);
+                o[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_value_operand<0>(xv[0][i], xv[1][i], masks), pb[n], o[i][0], 0, 0, 0);
+                o[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_value_operand<1>(xv[0][i], xv[1][i], masks), pb[n], o[i][1], 0, 0, 0);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-
-    int u = sh.part * sh.share + wave;
     if (u < s_end) {
-        Q4Step<D> x, y;
-        load(u, x);
-        while (true) {                                       // wave-uniform
-            if (u + KW < s_end) load(u + KW, y);
-            compute(u, x);
-            u += KW;
-            if (u >= s_end) break;
-            if (u + KW < s_end) load(u + KW, x);
-            compute(u, y);
-            u += KW;
-            if (u >= s_end) break;
-        }
+        locate(places(u));
+        load_keys();
+        load_values();
+        Q4Place at{};
+        if (u + KW < s_end) at = places(u + KW);
+        // The next step's keys go into the registers that the scores leave free, its values behind the
+        // sums. `until`: wave-uniform
+        auto walk = [&](auto masked, int until) __attribute__((always_inline)) {
+            while (u < until) {
+                const bool more = u + KW < s_end;
+                scores();
+                if (more) {
+                    locate(at);
+                    load_keys();
+                    if (u + 2 * KW < s_end) at = places(u + 2 * KW);
+                }
+                attend(masked, u);
+                if (more) load_values();
+                u += KW;
+            }
+        };
+        const int seen = len - a.T + 1;                      // positions that every token sees
+        walk(std::false_type{}, seen < 0 ? 0 : min(s_end, seen / kStep));
+        walk(std::true_type{}, s_end);
     }
+    m = m == -__builtin_inff() ? m : ref;                    // (log2 units from here)
     l = pair32_sum(pair16_sum(l));
 
     const bool any_bad = __ballot(bad) != 0;                  // wave-uniform
@@ -543,7 +599,7 @@ __global__ void __launch_bounds__(KW* kWave, 2) decode_paged_q4_kernel(PagedDeco
                 for (int e = 0; e < 4; ++e) {
                     const int d = 32 * i + 2 * (4 * grp + e) + j;
                     if (d < D)
-                        lo[(wave * a.lds_heads + c16) * (D + 4) + d] = 2.0f * __builtin_fmaf(op[i][e], -135.5f, o[i][j][e]);
+                        lo[(wave * a.lds_heads + c16) * (D + 4) + d] = 2.0f * o[i][j][e];
                 }
         if (grp == 0) {
             lm[(wave * 16 + c16) * 2] = m;
@@ -598,7 +654,9 @@ Q4Plan q4_plan(int64_t B, int64_t T, int64_t cap, int64_t Hq, int64_t Hkv, int64
     const int64_t R = Hq / Hkv * T, heads = Hkv * cdiv(R, 16), steps = cdiv(cap, 32);
     Q4Plan p{4, 1, 4, 0, heads, false};
     if (steps <= 16 || (steps <= 64 && B * heads >= 128)) p.least = steps;
-    else p.target = 512 / heads - B / 2;
+    else p.target = (D == 128 ? 768 : 1280) / heads - B;
+    if (getenv("Q4T")) p.target = atoll(getenv("Q4T"));
+    if (getenv("Q4L")) p.least = atoll(getenv("Q4L"));
     if (p.target < 1) p.target = 1;
     p.items = p.target + B;
     const int64_t most = B * cdiv(steps, p.least);   // every share the smallest
@@ -632,7 +690,8 @@ int launch_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
     a.target = static_cast<int>(p.target), a.least = static_cast<int>(p.least);
     a.whole = p.items <= B;
     a.lds_heads = static_cast<int>(R * T < 16 ? R * T : 16);
-    a.scale_log2 = 2.0f * scale * kPgLog2e, a.out = out, a.out_sb = out_sb;   // (h (2 c - 15) = 2 h (c - 7.5))
+    a.negate = scale < 0.0f;
+    a.scale_log2 = 2.0f * fabsf(scale) * kPgLog2e, a.out = out, a.out_sb = out_sb;   // (h (2 c - 15) = 2 h (c - 7.5))
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = workspace ? a.part_o + p.items * a.Hq * D : nullptr;
     const dim3 grid(static_cast<unsigned>(p.items * p.groups));
