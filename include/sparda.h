@@ -999,7 +999,7 @@ SPARDA_API int sparda_gather_paged_q4(const void* pages, int64_t n_pages, int64_
 
 /* Workspace bytes sparda_decode_paged_q4 needs for these sizes (0: none). */
 SPARDA_API size_t sparda_decode_paged_q4_workspace_bytes(int64_t B, int64_t T, int64_t width, int64_t page_size,
-                                                         int64_t Hq, int64_t Hkv, int64_t D);
+                                                         int64_t Hq, int64_t Hkv, int64_t D, int dtype);
 
 /*
  * sparda_decode_paged over pages of 4-bit codes, for the last T tokens of every sequence:

@@ -12,7 +12,7 @@ namespace sparda {
 int launch_rotate_append_paged(const RotateAppend& a, void* k, void* v, int dtype, int64_t D, hipStream_t stream);
 int launch_append_paged_q4(const RotateAppend& a, void* pages, int dtype, int64_t D, hipStream_t stream);
 int launch_gather_paged_q4(const RotateAppend& a, const void* pages, int dtype, int64_t D, void* k, void* v, hipStream_t stream);
-size_t decode_paged_q4_workspace_bytes(int64_t B, int64_t T, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D);
+size_t decode_paged_q4_workspace_bytes(int64_t B, int64_t T, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D, int dtype);
 int launch_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype, const void* pages,
                            int64_t n_pages, int64_t ps, int64_t p_st, int64_t h_st, const int32_t* table, int64_t t_st,
                            int64_t width, const int32_t* len, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
@@ -158,9 +158,9 @@ SPARDA_API int sparda_gather_paged_q4(const void* pages, int64_t n_pages, int64_
 }
 
 SPARDA_API size_t sparda_decode_paged_q4_workspace_bytes(int64_t B, int64_t T, int64_t width, int64_t page_size,
-                                                         int64_t Hq, int64_t Hkv, int64_t D) {
-    if (B <= 0 || T <= 0 || width <= 0 || page_size <= 0 || Hkv <= 0 || Hq < Hkv || D <= 0) return 0;
-    return decode_paged_q4_workspace_bytes(B, T, width * page_size, Hq, Hkv, D);
+                                                         int64_t Hq, int64_t Hkv, int64_t D, int dtype) {
+    if (B <= 0 || T <= 0 || !dtype_ok(dtype) || width <= 0 || page_size <= 0 || Hkv <= 0 || Hq < Hkv || D <= 0) return 0;
+    return decode_paged_q4_workspace_bytes(B, T, width * page_size, Hq, Hkv, D, dtype);
 }
 
 SPARDA_API int sparda_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype,
@@ -183,7 +183,7 @@ SPARDA_API int sparda_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st,
     SPARDA_REQUIRE(aligned16(q) && q_sb % ve == 0 && q_st % ve == 0 && q_sh % ve == 0, SPARDA_ERR_STRIDE,
                    "%s: the rows of q must be 16-byte aligned", who);
     SPARDA_REQUIRE(B == 1 || out_sb >= T * Hq * D, SPARDA_ERR_STRIDE, "%s: output rows overlap", who);
-    const size_t need = decode_paged_q4_workspace_bytes(B, T, width * page_size, Hq, Hkv, D);
+    const size_t need = decode_paged_q4_workspace_bytes(B, T, width * page_size, Hq, Hkv, D, dtype);
     SPARDA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)), SPARDA_ERR_WORKSPACE,
                    "%s: workspace of %zu bytes needed, 16-byte aligned", who, need);
     return launch_decode_paged_q4(q, q_sb, q_st, q_sh, dtype, pages, n_pages, page_size, p_st, h_st, page_table, t_st, width,

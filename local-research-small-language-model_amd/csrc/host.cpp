@@ -695,7 +695,7 @@ PyObject* decode_paged_q4(PyObject* const* a) {
     need(q.size(0) == p.B && T > 0 && rows16(q));
     const float scale = scale_or(a[4], D);
     x.on_current();
-    const size_t bytes = g.decode_paged_q4_workspace_bytes(p.B, T, p.width, p.ps, Hq, p.Hkv, D);
+    const size_t bytes = g.decode_paged_q4_workspace_bytes(p.B, T, p.width, p.ps, Hq, p.Hkv, D, code(q));
     at::DataPtr part;  // the shares' partials, held until the launches are enqueued
     if (bytes > 0) part = c10::GetAllocator(at::kCUDA)->allocate(bytes);
     const at::Tensor out = dim == 4 ? x.empty({p.B, T, Hq * D}, q.scalar_type()) : x.empty({p.B, Hq * D}, q.scalar_type());

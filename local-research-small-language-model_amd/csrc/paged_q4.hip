@@ -24,7 +24,6 @@
 #include "rotate.h"
 
 #include <type_traits>
-#include <cstdlib>
 
 namespace sparda {
 
@@ -362,7 +361,6 @@ __device__ __forceinline__ bf16x8 q4_value_operand(uint32_t w0, uint32_t w1, con
 // x as a sum of TERMS bf16 values (1: rounded; 3: all 24 bits of it)
 template <int TERMS>
 __device__ __forceinline__ void q4_split(const float (&x)[8], bf16x8 (&out)[TERMS]) {
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
     float rest[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) rest[e] = x[e];
@@ -388,14 +386,15 @@ struct Q4Place {
 
 }  // namespace
 
-// One workgroup of KW wavefronts per (tile of 16 columns, item). The columns are the (token, query
+// One workgroup of KW wavefronts per (16 NC columns, item). The columns are the (token, query
 // head) pairs of a KV head, token-major; token t of T sees the positions below
 // len - T + 1 + t. The numbers h stay outside of the products with the codes:
 //     S^T[key, col] = 2 sum_g h_g[key] sum_{d in g} ((16.5 + c) - 24) q[d]
 //     O^T[d, col]  += 2 sum_key ((16.5 + c) - 24) P_g[key, col],  P_g = exp2(S - m) h_g[key] in bf16
 // so that the levels, odd multiples of h, enter without rounding.
-template <int DT, int D, int KW>
-__global__ void __launch_bounds__(KW* kWave, (D == 128 ? 3 : 4) - (DT == SPARDA_F32 ? 1 : 0)) decode_paged_q4_kernel(PagedDecode a) {
+template <int DT, int D, int KW, int NC>
+__global__ void __launch_bounds__(KW* kWave, (D == 128 ? 3 : 4) - (DT == SPARDA_F32 ? 1 : 0) - (NC > 1 ? 1 : 0))
+decode_paged_q4_kernel(PagedDecode a) {
     constexpr int G = q4_groups(D), kTerms = DT == SPARDA_F32 ? 3 : 1, kStep = 32, kEs = DT == SPARDA_F32 ? 4 : 2;
     extern __shared__ float lds[];
     const int lane = threadIdx.x % kWave;
@@ -403,8 +402,8 @@ __global__ void __launch_bounds__(KW* kWave, (D == 128 ? 3 : 4) - (DT == SPARDA_
     const int c16 = lane % 16, grp = lane / 16;
     const int groups = a.Hkv * a.head_tiles;
     const int item = blockIdx.x / groups, gt = blockIdx.x % groups;
-    const int g = gt / a.head_tiles, col0 = gt % a.head_tiles * 16;
-    const int nh = a.R * a.T - col0 < 16 ? a.R * a.T - col0 : 16;   // columns of the tile
+    const int g = gt / a.head_tiles, col0 = gt % a.head_tiles * (16 * NC);
+    const int ncol = a.R * a.T - col0 < 16 * NC ? a.R * a.T - col0 : 16 * NC;   // columns of the workgroup
     Share sh;
     if (a.whole) {
         const int l = __builtin_amdgcn_readfirstlane(a.len[item]), n = l < 0 ? 0 : l > a.cap ? a.cap : l;
@@ -418,16 +417,18 @@ __global__ void __launch_bounds__(KW* kWave, (D == 128 ? 3 : 4) - (DT == SPARDA_
     const int s_end = min(steps, (sh.part + 1) * sh.share);
     bool bad = sh.bad;
 
-    // this lane's column of Q
-    const int col = col0 + (c16 < nh ? c16 : nh - 1), tok = col / a.R, head = g * a.R + col % a.R;
-    const int lim = len - a.T + 1 + tok;                    // positions the column sees
-    bf16x8 qr[G][kTerms];
-    {
+    // this lane's columns of Q
+    int lim[NC];                                             // positions a column sees
+    bf16x8 qr[NC][G][kTerms];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int at = 16 * c + c16, col = col0 + (at < ncol ? at : ncol - 1), tok = col / a.R, head = g * a.R + col % a.R;
+        lim[c] = len - a.T + 1 + tok;
         const char* q = static_cast<const char*>(a.q) + (b * a.q_sb + tok * a.q_st + head * a.q_sh) * kEs;
 #pragma unroll
         for (int i = 0; i < G; ++i) {
             float x[8];
-            if (c16 < nh && 32 * i + 8 * grp < D) {
+            if (at < ncol && 32 * i + 8 * grp < D) {
                 q4_load8<DT>(q + (32 * i + 8 * grp) * kEs, x);
                 if (a.negate) {
 #pragma unroll
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(KW* kWave, (D == 128 ? 3 : 4) - (DT == SPARDA_
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = 0.0f;
             }
-            q4_split<kTerms>(x, qr[i]);
+            q4_split<kTerms>(x, qr[c][i]);
         }
     }
 
@@ -481,77 +482,93 @@ __global__ void __launch_bounds__(KW* kWave, (D == 128 ? 3 : 4) - (DT == SPARDA_
         for (int t = 0; t < 2; ++t) q4_load_words<G>(base[t] + o_values, xv[t]), q4_load_scales<G>(base[t] + o_scales + 32 * G, hv[t]);
     };
 
-    // m: the column's reference, in the scores' own units, l: this lane's part of its sum
-    float m = -__builtin_inff(), ref = 0.0f, l = 0.0f;
+    // m: the columns' references, in the scores' own units, l: this lane's part of their sums
+    float m[NC], ref[NC], l[NC];
     const float slack = 16.0f / a.scale_log2;
-    f32x4 o[G][2];
+    f32x4 o[NC][G][2];
 #pragma unroll
-    for (int i = 0; i < G; ++i) o[i][0] = o[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < NC; ++c) {
+        m[c] = -__builtin_inff(), ref[c] = l[c] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < G; ++i) o[c][i][0] = o[c][i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     bf16x8 middle;
 #pragma unroll
     for (int e = 0; e < 8; ++e) middle[e] = static_cast<__bf16>(-24.0f);
     const Q4Masks masks = q4_masks();
-    f32x4 s[2];
+    f32x4 s[NC][2];
     auto scores = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < NC; ++c) s[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < G; ++i) {
                 const bf16x8 ka = q4_key_operand(xk[t][i], masks);
-                f32x4 y{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int n = 0; n < kTerms; ++n) y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, qr[i][n], y, 0, 0, 0);
+                for (int c = 0; c < NC; ++c) {
+                    f32x4 y{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int n = 0; n < kTerms; ++n) y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qr[i][n], y, 0, 0, 0);
+                    for (int n = 0; n < kTerms; ++n) y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, qr[c][i][n], y, 0, 0, 0);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[t][e] = __builtin_fmaf(y[e], static_cast<float>(hk[t][e][i]), s[t][e]);
+                    for (int n = 0; n < kTerms; ++n) y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qr[c][i][n], y, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[c][t][e] = __builtin_fmaf(y[e], static_cast<float>(hk[t][e][i]), s[c][t][e]);
+                }
                 __builtin_amdgcn_sched_barrier(0);           // (operands of one group at a time: registers)
             }
         }
     };
     auto attend = [&](auto masked, int v) __attribute__((always_inline)) {
         constexpr bool kMask = decltype(masked)::value;
-        const int left = lim - v * kStep - 4 * grp;          // this lane's keys 16 t + e below it are the column's
-        float mx = -__builtin_inff();
+        float p[NC][8];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int c = 0; c < NC; ++c) {
+            const int left = lim[c] - v * kStep - 4 * grp;   // this lane's keys 16 t + e below it are the column's
+            float mx = -__builtin_inff();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, !kMask || 16 * t + e < left ? s[t][e] : -__builtin_inff());
-        // The reference follows the maximum only where a weight would pass 2^16: weights keep their
-        // relative precision whatever they are measured against, and most steps rescale nothing.
-        if (__ballot(!(mx <= m + slack)) != 0) {             // (scale 0: -inf + inf, no order)
-            const float top = fmaxf(m, pair32_max(pair16_max(mx)));
-            const float to = top == -__builtin_inff() ? 0.0f : top * a.scale_log2;
-            const float alpha = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - to);
-            m = top, ref = to;
-            l *= alpha;
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int i = 0; i < G; ++i) o[i][0] *= alpha, o[i][1] *= alpha;
-        }
-        float p[8];
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, !kMask || 16 * t + e < left ? s[c][t][e] : -__builtin_inff());
+            // The reference follows the maximum only where a weight would pass 2^16: weights keep their
+            // relative precision whatever they are measured against, and most steps rescale nothing.
+            if (__ballot(!(mx <= m[c] + slack)) != 0) {      // (scale 0: -inf + inf, no order)
+                const float top = fmaxf(m[c], pair32_max(pair16_max(mx)));
+                const float to = top == -__builtin_inff() ? 0.0f : top * a.scale_log2;
+                const float alpha = m[c] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref[c] - to);
+                m[c] = top, ref[c] = to;
+                l[c] *= alpha;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 4][e % 4], a.scale_log2, -ref));
-            if (kMask) p[e] = 16 * (e / 4) + e % 4 < left ? p[e] : 0.0f;
-            l += p[e];
+                for (int i = 0; i < G; ++i) o[c][i][0] *= alpha, o[c][i][1] *= alpha;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                p[c][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][e / 4][e % 4], a.scale_log2, -ref[c]));
+                if (kMask) p[c][e] = 16 * (e / 4) + e % 4 < left ? p[c][e] : 0.0f;
+                l[c] += p[c][e];
+            }
         }
 #pragma unroll
         for (int i = 0; i < G; ++i) {
-            float ph[8];
+            const bf16x8 v0 = q4_value_operand<0>(xv[0][i], xv[1][i], masks), v1 = q4_value_operand<1>(xv[0][i], xv[1][i], masks);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                ph[e] = __builtin_fmaf(p[e], static_cast<float>(hv[e / 4][e % 4][i]), 0.0f);
-                if (kMask) ph[e] = 16 * (e / 4) + e % 4 < left ? ph[e] : 0.0f;   // (a number behind the column's positions may be anything)
-            }
-            bf16x8 pb[kTerms];
-            q4_split<kTerms>(ph, pb);
+            for (int c = 0; c < NC; ++c) {
+                const int left = lim[c] - v * kStep - 4 * grp;
+                float ph[8];
 #pragma unroll
-            for (int n = 0; n < kTerms; ++n) {
-                o[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, pb[n], o[i][0], 0, 0, 0);
-                o[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, pb[n], o[i][1], 0, 0, 0);
-                o[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_value_operand<0>(xv[0][i], xv[1][i], masks), pb[n], o[i][0], 0, 0, 0);
-                o[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_value_operand<1>(xv[0][i], xv[1][i], masks), pb[n], o[i][1], 0, 0, 0);
+                for (int e = 0; e < 8; ++e) {
+                    ph[e] = __builtin_fmaf(p[c][e], static_cast<float>(hv[e / 4][e % 4][i]), 0.0f);
+                    if (kMask) ph[e] = 16 * (e / 4) + e % 4 < left ? ph[e] : 0.0f;   // (a number behind the column's positions may be anything)
+                }
+                bf16x8 pb[kTerms];
+                q4_split<kTerms>(ph, pb);
+#pragma unroll
+                for (int n = 0; n < kTerms; ++n) {
+                    o[c][i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, pb[n], o[c][i][0], 0, 0, 0);
+                    o[c][i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, pb[n], o[c][i][1], 0, 0, 0);
+                    o[c][i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pb[n], o[c][i][0], 0, 0, 0);
+                    o[c][i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pb[n], o[c][i][1], 0, 0, 0);
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -582,62 +599,66 @@ __global__ void __launch_bounds__(KW* kWave, (D == 128 ? 3 : 4) - (DT == SPARDA_
         walk(std::false_type{}, seen < 0 ? 0 : min(s_end, seen / kStep));
         walk(std::true_type{}, s_end);
     }
-    m = m == -__builtin_inff() ? m : ref;                    // (log2 units from here)
-    l = pair32_sum(pair16_sum(l));
 
     const bool any_bad = __ballot(bad) != 0;                  // wave-uniform
-    // ---- the wavefronts' partials, joined in order: thread -> (column, dim) ----
+    // ---- the wavefronts' partials, joined in order: thread -> (column, dim), 16 columns at a time ----
     float* lo = lds;                                          // [KW][lds_heads][D + 4]
     float* lm = lo + KW * a.lds_heads * (D + 4);              // [KW][16][2]
     int* lbad = reinterpret_cast<int*>(lm + KW * 32);         // [KW]
-    if (c16 < nh) {
-#pragma unroll
-        for (int i = 0; i < G; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int d = 32 * i + 2 * (4 * grp + e) + j;
-                    if (d < D)
-                        lo[(wave * a.lds_heads + c16) * (D + 4) + d] = 2.0f * o[i][j][e];
-                }
-        if (grp == 0) {
-            lm[(wave * 16 + c16) * 2] = m;
-            lm[(wave * 16 + c16) * 2 + 1] = l;
-        }
-    }
     if (lane == 0) lbad[wave] = any_bad ? 1 : 0;
-    __syncthreads();
-    int bads = 0;
 #pragma unroll
-    for (int w = 0; w < KW; ++w) bads |= lbad[w];
-    if (bads != 0 && wave == 0 && lane == 0) atomicOr(a.status, static_cast<uint32_t>(SPARDA_STATUS_PAGE_RANGE));
-    for (int e = wave * kWave + lane; e < nh * D; e += KW * kWave) {
-        const int c = e / D, d = e % D;
-        float mw[KW], M = -__builtin_inff();
+    for (int c = 0; c < NC; ++c) {
+        const int nh = ncol - 16 * c < 16 ? ncol - 16 * c : 16;
+        if (nh <= 0) break;                                   // workgroup-uniform
+        if (c > 0) __syncthreads();                           // the last ones have been read
+        l[c] = pair32_sum(pair16_sum(l[c]));
+        if (c16 < nh) {
 #pragma unroll
-        for (int w = 0; w < KW; ++w) {
-            mw[w] = lm[(w * 16 + c) * 2];
-            M = fmaxf(M, mw[w]);
+            for (int i = 0; i < G; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int d = 32 * i + 2 * (4 * grp + e) + j;
+                        if (d < D) lo[(wave * a.lds_heads + c16) * (D + 4) + d] = 2.0f * o[c][i][j][e];
+                    }
+            if (grp == 0) {
+                lm[(wave * 16 + c16) * 2] = m[c] == -__builtin_inff() ? m[c] : ref[c];   // (log2 units from here)
+                lm[(wave * 16 + c16) * 2 + 1] = l[c];
+            }
         }
-        const float ref = M == -__builtin_inff() ? 0.0f : M;
-        float L = 0.0f, O = 0.0f;
+        __syncthreads();
+        int bads = 0;
 #pragma unroll
-        for (int w = 0; w < KW; ++w) {
-            const float wt = __builtin_amdgcn_exp2f(mw[w] - ref);
-            L = __builtin_fmaf(wt, lm[(w * 16 + c) * 2 + 1], L);
-            O = __builtin_fmaf(wt, lo[(w * a.lds_heads + c) * (D + 4) + d], O);
-        }
-        if (bads) O = __builtin_nanf("");
-        const int t = (col0 + c) / a.R, h = t * a.heads + g * a.R + (col0 + c) % a.R;
-        if (sh.parts == 1) {
-            // (a token before the sequence's first position: zeros)
-            store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d,
-                           len - a.T + 1 + t <= 0 && !bads ? 0.0f : O / L);
-        } else {
-            const int64_t at = static_cast<int64_t>(item) * a.Hq + h;
-            a.part_o[at * D + d] = O;
-            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(M, L);
+        for (int w = 0; w < KW; ++w) bads |= lbad[w];
+        if (c == 0 && bads != 0 && wave == 0 && lane == 0) atomicOr(a.status, static_cast<uint32_t>(SPARDA_STATUS_PAGE_RANGE));
+        for (int e = wave * kWave + lane; e < nh * D; e += KW * kWave) {
+            const int cc = e / D, d = e % D;
+            float mw[KW], M = -__builtin_inff();
+#pragma unroll
+            for (int w = 0; w < KW; ++w) {
+                mw[w] = lm[(w * 16 + cc) * 2];
+                M = fmaxf(M, mw[w]);
+            }
+            const float top = M == -__builtin_inff() ? 0.0f : M;
+            float L = 0.0f, O = 0.0f;
+#pragma unroll
+            for (int w = 0; w < KW; ++w) {
+                const float wt = __builtin_amdgcn_exp2f(mw[w] - top);
+                L = __builtin_fmaf(wt, lm[(w * 16 + cc) * 2 + 1], L);
+                O = __builtin_fmaf(wt, lo[(w * a.lds_heads + cc) * (D + 4) + d], O);
+            }
+            if (bads) O = __builtin_nanf("");
+            const int col = col0 + 16 * c + cc, t = col / a.R, h = t * a.heads + g * a.R + col % a.R;
+            if (sh.parts == 1) {
+                // (a token before the sequence's first position: zeros)
+                store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d,
+                               len - a.T + 1 + t <= 0 && !bads ? 0.0f : O / L);
+            } else {
+                const int64_t to = static_cast<int64_t>(item) * a.Hq + h;
+                a.part_o[to * D + d] = O;
+                if (d == 0) *reinterpret_cast<float2*>(a.part_ml + to * 2) = make_float2(M, L);
+            }
         }
     }
 }
@@ -645,18 +666,22 @@ __global__ void __launch_bounds__(KW* kWave, (D == 128 ? 3 : 4) - (DT == SPARDA_
 namespace {
 
 struct Q4Plan {
-    int kw;                  // wavefronts of a workgroup
+    int nc;                  // column tiles of a workgroup
     int64_t target, least;   // items aimed at, steps of the smallest item
     int64_t items, groups;   // items at most, workgroups an item
     bool few;                // a sequence has few items in the mean
 };
-Q4Plan q4_plan(int64_t B, int64_t T, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D) {
-    const int64_t R = Hq / Hkv * T, heads = Hkv * cdiv(R, 16), steps = cdiv(cap, 32);
-    Q4Plan p{4, 1, 4, 0, heads, false};
-    if (steps <= 16 || (steps <= 64 && B * heads >= 128)) p.least = steps;
-    else p.target = (D == 128 ? 768 : 1280) / heads - B;
-    if (getenv("Q4T")) p.target = atoll(getenv("Q4T"));
-    if (getenv("Q4L")) p.least = atoll(getenv("Q4L"));
+Q4Plan q4_plan(int64_t B, int64_t T, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D, int dtype) {
+    const int64_t cols = Hq / Hkv * T, steps = cdiv(cap, 32);
+    Q4Plan p{dtype == SPARDA_BF16 && cols > 16 ? 2 : 1, 1, 4, 0, 0, false};
+    p.groups = Hkv * cdiv(cols, 16 * p.nc);
+    if (steps <= 16 || (steps <= 64 && B * p.groups >= 128)) {
+        p.least = steps;
+    } else {
+        // (items are target + B at most, target + B / 2 in the mean)
+        const int64_t slots = 256 * ((D == 128 ? 3 : 4) - (p.nc > 1 ? 1 : 0));
+        p.target = slots / p.groups - B / 2;
+    }
     if (p.target < 1) p.target = 1;
     p.items = p.target + B;
     const int64_t most = B * cdiv(steps, p.least);   // every share the smallest
@@ -667,8 +692,8 @@ Q4Plan q4_plan(int64_t B, int64_t T, int64_t cap, int64_t Hq, int64_t Hkv, int64
 
 }  // namespace
 
-size_t decode_paged_q4_workspace_bytes(int64_t B, int64_t T, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D) {
-    const Q4Plan p = q4_plan(B, T, cap, Hq, Hkv, D);
+size_t decode_paged_q4_workspace_bytes(int64_t B, int64_t T, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D, int dtype) {
+    const Q4Plan p = q4_plan(B, T, cap, Hq, Hkv, D, dtype);
     return p.items <= B ? 0 : static_cast<size_t>(p.items * T * Hq * (D + 2)) * sizeof(float);
 }
 
@@ -678,15 +703,15 @@ int launch_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
                            float scale, void* out, int64_t out_sb, void* workspace, hipStream_t stream) {
     PagedDecode a{};
     const int64_t cap = width * ps, R = Hq / Hkv;
-    const Q4Plan p = q4_plan(B, T, cap, Hq, Hkv, D);
-    if (!grid_fits(p.items * p.groups, p.kw * kWave)) return set_error(SPARDA_ERR_SHAPE, "decode_paged_q4: grid too large");
+    const Q4Plan p = q4_plan(B, T, cap, Hq, Hkv, D, dtype);
+    if (!grid_fits(p.items * p.groups, 4 * kWave)) return set_error(SPARDA_ERR_SHAPE, "decode_paged_q4: grid too large");
     if (const int rc = status_word(&a.status)) return rc;
     a.q = q, a.q_sb = q_sb, a.q_st = q_st, a.q_sh = q_sh, a.k = pages;
     a.pg = Pages{p_st, 0, h_st, table, t_st, static_cast<int>(width), static_cast<int>(n_pages)};
     a.T = static_cast<int>(T), a.heads = static_cast<int>(Hq), a.step = 32;
     a.ps16 = static_cast<int>(ps / 16), a.len = len, a.B = static_cast<int>(B), a.cap = static_cast<int>(cap);
     a.Hq = static_cast<int>(T * Hq), a.Hkv = static_cast<int>(Hkv), a.R = static_cast<int>(R);
-    a.head_tiles = static_cast<int>(cdiv(R * T, 16));
+    a.head_tiles = static_cast<int>(cdiv(R * T, 16 * p.nc));
     a.target = static_cast<int>(p.target), a.least = static_cast<int>(p.least);
     a.whole = p.items <= B;
     a.lds_heads = static_cast<int>(R * T < 16 ? R * T : 16);
@@ -695,9 +720,18 @@ int launch_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = workspace ? a.part_o + p.items * a.Hq * D : nullptr;
     const dim3 grid(static_cast<unsigned>(p.items * p.groups));
-#define SPARDA_DQ(DT_, D_)                                                                        \
-    hipLaunchKernelGGL((decode_paged_q4_kernel<DT_, D_, 4>), grid, dim3(4 * kWave),               \
+#define SPARDA_DQ_C(DT_, D_, NC_)                                                                 \
+    hipLaunchKernelGGL((decode_paged_q4_kernel<DT_, D_, 4, NC_>), grid, dim3(4 * kWave),          \
                        4 * (a.lds_heads * ((D_) + 4) + 33) * sizeof(float), stream, a)
+#define SPARDA_DQ(DT_, D_)                                                                        \
+    do {                                                                                          \
+        if constexpr (DT_ == SPARDA_BF16) {                                                       \
+            if (p.nc == 2) SPARDA_DQ_C(DT_, D_, 2);                                               \
+            else SPARDA_DQ_C(DT_, D_, 1);                                                         \
+        } else {                                                                                  \
+            SPARDA_DQ_C(DT_, D_, 1);                                                              \
+        }                                                                                         \
+    } while (0)
 #define SPARDA_DQ_D(DT_)                      \
     switch (D) {                              \
         case 16: SPARDA_DQ(DT_, 16); break;   \
@@ -709,6 +743,7 @@ int launch_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
     else SPARDA_DQ_D(SPARDA_BF16)
 #undef SPARDA_DQ_D
 #undef SPARDA_DQ
+#undef SPARDA_DQ_C
     if (p.items > B) launch_paged_join(a, D, dtype, p.few, stream);
     return check_hip(hipGetLastError(), "decode_paged_q4_kernel");
 }

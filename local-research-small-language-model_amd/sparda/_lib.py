@@ -141,7 +141,7 @@ SIGNATURES = {
                                       _p, _int, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _p]),
     "sparda_gather_paged_q4": (_int, [_p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _p, _int, _i64, _i64,
                                       _i64, _i64, _i64, _p]),
-    "sparda_decode_paged_q4_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "sparda_decode_paged_q4_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int]),
     "sparda_decode_paged_q4": (_int, [_p, _i64, _i64, _i64, _int, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64,
                                       _i64, _i64, _i64, _i64, _f32, _p, _i64, _p, _size, _p]),
     "sparda_verify_drafts_workspace_bytes": (_size, [_i64, _i64, _i64, _int]),

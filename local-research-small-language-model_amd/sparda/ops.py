@@ -1557,7 +1557,7 @@ def decode_paged_q4(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tens
             raise ValueError("sparda: out must hold the tokens of a sequence contiguously")
     if B == 0 or T == 0:
         return out
-    nbytes = _lib.load().sparda_decode_paged_q4_workspace_bytes(B, T, width, ps, Hq, Hkv, D)
+    nbytes = _lib.load().sparda_decode_paged_q4_workspace_bytes(B, T, width, ps, Hq, Hkv, D, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with torch.cuda.device(dev):
         call("sparda_decode_paged_q4", q.data_ptr(), q.stride(0), q.stride(1) if q.dim() == 4 else 0, q.stride(-2), code,

@@ -102,10 +102,10 @@ def test_verify_argument_errors(code, bad):
 
 def test_workspace_sizes():
     ws = sparda.load().sparda_decode_paged_q4_workspace_bytes
-    assert ws(1, 1, 1, 16, 12, 4, 64) == 0            # one share a sequence: no partials
-    some = ws(8, 1, 256, 64, 12, 4, 64)
+    assert ws(1, 1, 1, 16, 12, 4, 64, 1) == 0            # one share a sequence: no partials
+    some = ws(8, 1, 256, 64, 12, 4, 64, 1)
     assert some > 0 and some % (12 * 66 * 4) == 0     # (m, l, o[D]) fp32 for each item and head
-    assert ws(0, 1, 256, 64, 12, 4, 64) == 0 and ws(8, 0, 256, 64, 12, 4, 64) == 0 and ws(8, 1, 256, 64, 2, 4, 64) == 0
+    assert ws(0, 1, 256, 64, 12, 4, 64, 1) == 0 and ws(8, 0, 256, 64, 12, 4, 64, 1) == 0 and ws(8, 1, 256, 64, 2, 4, 64, 1) == 0
     ws = sparda.load().sparda_verify_drafts_workspace_bytes
     assert ws(1, 4, 32000, 1) > 0 and ws(1, 65, 32000, 1) == 0 and ws(0, 4, 32000, 1) == 0 and ws(1, 4, 1 << 21, 1) == 0
 
