@@ -22,7 +22,7 @@ namespace sparda {
 namespace {
 
 constexpr int kVdThreads = 256;
-constexpr int kVdChunks = 256;        // chunks of a row in either launch, at most
+constexpr int kVdChunks = 256;        // chunks of a row in the first launch, at most
 constexpr int kVdRows = 65;           // rows of a sequence (drafts + 1), at most
 constexpr float kVdLog2e = 1.4426950408889634f;
 
@@ -168,8 +168,8 @@ __global__ void __launch_bounds__(kVdThreads) verify_stats_kernel(Verify a) {
                 if (x[k][e] == m) arg = static_cast<int>(first + (tid + k * kVdThreads) * kVe + e);
         arg = wave_min_i32(arg);
     }
-    const double d = wave_sum_f64(static_cast<double>(s));
-    if (tid % kWave == 0) rs[wave] = d, ra[wave] = arg;
+    s = wave_sum(s);
+    if (tid % kWave == 0) rs[wave] = s, ra[wave] = arg;
     __syncthreads();
     if (tid == 0) {
         ChunkStat st{m, ra[0], rs[0]};
@@ -187,7 +187,7 @@ struct VdRow {
     const float* q;       // mode kVdResidual
     int without;          // mode kVdWithout
     int mode;
-    double m, inv_t, total;   // total: the sum of p's weights (kVdResidual)
+    double m, inv_t, inv_total;   // inv_total: one over the sum of p's weights (kVdResidual)
 };
 
 // r of eight or four elements; w: p's weights, not divided by their total
@@ -202,7 +202,7 @@ __device__ __forceinline__ void vd_weights(const VdRow& r, int64_t at, int64_t V
         if (r.mode == kVdWithout && at + e == r.without) w[e] = 0.0;
         if (residual) {
             const double q = at + e >= 0 && at + e < V ? static_cast<double>(r.q[at + e]) : 0.0;
-            const double d = w[e] / r.total - q;
+            const double d = w[e] * r.inv_total - q;
             w[e] = d > 0.0 ? d : 0.0;
         }
     }
@@ -220,36 +220,25 @@ __device__ __forceinline__ double block_sum_f64(double v, double* red) {
     return s;
 }
 
-// The token of the sums in LDS: the chunk where they pass, then the token in it. All threads of the workgroup.
+// The token of the chunks' sums (lane c of every wavefront holds chunk c's): the chunk where they pass
+// u times their total, then the token in it. All threads of the workgroup.
 template <int DT>
-__device__ int vd_draw(const VdRow& r, const double* sums, int chunks, int64_t len, int64_t V, bool residual, float u,
-                       double* red, int* found) {
+__device__ __forceinline__ int vd_draw(const VdRow& r, double mine_of_all, int64_t len, int64_t V, bool residual, float u, double* red,
+                                       int* found) {
     constexpr int kVe = VdType<DT>::kVe, kW = kVdThreads / kWave;
     const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
-    double total = 0.0;
-    for (int c = 0; c < chunks; ++c) total += sums[c];
-    const double target = static_cast<double>(u) * total;
-    double before = 0.0, base = 0.0;
-    int chunk = -1, last = 0;
-    for (int c = 0; c < chunks; ++c) {
-        if (chunk < 0 && before + sums[c] > target) chunk = c, base = before;
-        if (sums[c] > 0.0) last = c;
-        before += sums[c];
-    }
-    const bool passed = chunk >= 0;
-    if (!passed) chunk = last;                    // the last token that weighs anything
-    const int shift = vd_shift<DT>(r.row);
-    const int64_t first = chunk * len - shift;
+    const double upto_chunk = wave_scan_f64(mine_of_all);
+    const double target = static_cast<double>(u) * __shfl(upto_chunk, kWave - 1, kWave);
+    const uint64_t pass = __ballot(upto_chunk > target), some = __ballot(mine_of_all > 0.0);
+    // (none passes where u is 1, or the last by a rounding: the last token that weighs anything)
+    const int chunk = pass != 0 ? __builtin_ctzll(pass) : 63 - __builtin_clzll(some | 1);
+    double base = __shfl(upto_chunk - mine_of_all, chunk, kWave);
+    const int64_t first = chunk * len - vd_shift<DT>(r.row);
     int best = -1;                                // the last token with a weight so far
     for (int64_t p0 = 0; p0 < len; p0 += kVdThreads * kVe) {
         const int64_t at = first + p0 + tid * kVe;
         double w[kVe], mine = 0.0;
-        if (p0 + tid * kVe < len) {
-            vd_weights<DT>(r, at, V, residual, w);
-        } else {
-#pragma unroll
-            for (int e = 0; e < kVe; ++e) w[e] = 0.0;
-        }
+        vd_weights<DT>(r, at, V, residual, w);
         int top = -1;
 #pragma unroll
         for (int e = 0; e < kVe; ++e) {
@@ -260,27 +249,26 @@ __device__ int vd_draw(const VdRow& r, const double* sums, int chunks, int64_t l
         __syncthreads();                          // (the arrays' last use)
         if (lane == kWave - 1) red[wave] = upto;
         if (tid == 0) found[0] = 0x7fffffff;
-        if (tid < kW) found[1 + tid] = -1;
-        __syncthreads();
-        double mybase = base;
-        for (int v = 0; v < wave; ++v) mybase += red[v];
-        if (passed && mybase + upto > target) {
-            double acc = mybase + upto - mine;
-            int e0 = kVe - 1;                     // (rounding may leave the piece's own sums below: its last weight)
-#pragma unroll
-            for (int e = kVe - 1; e >= 0; --e)
-                if (w[e] > 0.0) { e0 = e; break; }
-            bool hit = false;
-#pragma unroll
-            for (int e = 0; e < kVe; ++e) {
-                acc += w[e];
-                if (!hit && w[e] > 0.0 && acc > target) hit = true, e0 = e;
-            }
-            if (w[e0] > 0.0) atomicMin(&found[0], static_cast<int>(at + e0));
-        }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, kWave));
         if (lane == 0) found[1 + wave] = top;
+        __syncthreads();
+        double before = base;
+        for (int v = 0; v < wave; ++v) before += red[v];
+        if (pass != 0 && mine > 0.0 && before + upto > target) {
+            // (rounding may leave the piece's own sums below: its last weight)
+            double acc = before + upto - mine;
+            int hit = -1, last = -1;
+#pragma unroll
+            for (int e = 0; e < kVe; ++e) {
+                acc += w[e];
+                if (w[e] > 0.0) {
+                    last = e;
+                    if (hit < 0 && acc > target) hit = e;
+                }
+            }
+            atomicMin(&found[0], static_cast<int>(at + (hit >= 0 ? hit : last)));
+        }
         __syncthreads();
         if (found[0] != 0x7fffffff) return found[0];
 #pragma unroll
@@ -291,21 +279,21 @@ __device__ int vd_draw(const VdRow& r, const double* sums, int chunks, int64_t l
     return best;
 }
 
-// true in the workgroup that is the last of `all` to come here; what the others wrote before is visible to it
-__device__ __forceinline__ bool vd_last(uint32_t* done, uint32_t all, int* flag) {
-    __syncthreads();
+// What workgroups of a launch hand to the last of them goes through stores and loads at the device's
+// scope, which pass the caches that they do not share; a store is waited for before its
+// workgroup is counted. (A release or acquire at that scope would write back and drop whole caches instead, once a workgroup.)
+__device__ __forceinline__ double vd_read(const double* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// writes the workgroup's number and counts it; true in the last of `all`
+__device__ __forceinline__ bool vd_last(double* to, double v, uint32_t* done, uint32_t all, int* flag) {
     if (threadIdx.x == 0) {
-        __threadfence();
-        const uint32_t n = __hip_atomic_fetch_add(done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-        *flag = n + 1 == all;
+        __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __builtin_amdgcn_s_waitcnt(0x0f70);       // vmcnt(0): the store has arrived
+        asm volatile("" ::: "memory");
+        *flag = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == all;
     }
     __syncthreads();
-    const bool last = *flag != 0;
-    if (last) __threadfence();
-    return last;
+    return *flag != 0;
 }
-__device__ __forceinline__ double vd_read(const double* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ void vd_write(double* p, double v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 // the sum of a chunk's weights, by all threads
 template <int DT>
@@ -330,7 +318,7 @@ __device__ __forceinline__ double vd_chunk_sum(const VdRow& r, int chunk, int64_
 template <int DT>
 __global__ void __launch_bounds__(kVdThreads) verify_accept_kernel(Verify a) {
     constexpr int kEs = VdType<DT>::kEs, kW = kVdThreads / kWave;
-    __shared__ double red[kW], sums[kVdChunks], rz[kVdRows];
+    __shared__ double red[kW];
     __shared__ float rmax[kVdRows];
     __shared__ int rarg[kVdRows], ok[kVdRows], found[1 + kW], flag;
     const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, chunk = blockIdx.x, b = blockIdx.y;
@@ -340,33 +328,38 @@ __global__ void __launch_bounds__(kVdThreads) verify_accept_kernel(Verify a) {
     const double inv_t = greedy ? 1.0 : 1.0 / static_cast<double>(T);
     for (int i = wave; i <= count; i += kW) {                 // a wavefront a row
         const ChunkStat* st = a.stats + (static_cast<int64_t>(b) * (a.K + 1) + i) * a.chunks1;
-        float m = -__builtin_inff();
-        for (int c = lane; c < a.chunks1; c += kWave) m = fmaxf(m, st[c].m);
+        // (the draft's own numbers under the chunks')
+        int d = -1;
+        float x = -__builtin_inff(), u = 0.0f, q = 1.0f;
+        if (i < count) {
+            d = a.drafts[b * a.d_sb + i];
+            if (d >= 0 && d < a.V) {
+                x = load_elem<DT>(a.logits, b * a.l_sb + i * a.l_st + d);
+                u = a.uniform[b * a.u_sb + i];
+                if (a.probs) q = a.probs[b * a.p_sb + i * a.p_st + d];
+            }
+        }
+        ChunkStat own{-__builtin_inff(), 0x7fffffff, 0.0};
+        if (lane < a.chunks1) own = st[lane];
+        float m = own.m;
+        for (int c = lane + kWave; c < a.chunks1; c += kWave) m = fmaxf(m, st[c].m);
         m = wave_max(m);
         double z = 0.0;
         int arg = 0x7fffffff;
-        for (int c = lane; c < a.chunks1; c += kWave) {
-            const ChunkStat x = st[c];
-            // (a chunk without a finite logit: nothing, NaN among them stays)
-            z += x.m == -__builtin_inff() ? x.sum : x.sum * exp((static_cast<double>(x.m) - m) * inv_t);
-            if (x.m == m) arg = min(arg, x.arg);
-        }
+        auto add = [&](const ChunkStat& s) {
+            // (a chunk without a finite logit: nothing; NaN among them stays)
+            z += s.m == -__builtin_inff() ? s.sum : s.sum * exp((static_cast<double>(s.m) - m) * inv_t);
+            if (s.m == m) arg = min(arg, s.arg);
+        };
+        add(own);
+        for (int c = lane + kWave; c < a.chunks1; c += kWave) add(st[c]);
         z = wave_sum_f64(z);
-        arg = wave_min_i32(arg);
+        if (greedy) arg = wave_min_i32(arg);
         if (lane == 0) {
             const bool valid = m > -__builtin_inff() && m < __builtin_inff() && z < __builtin_inf();
-            bool accept = false;
-            if (valid && i < count) {
-                const int d = a.drafts[b * a.d_sb + i];
-                if (greedy) {
-                    accept = d == arg;
-                } else if (d >= 0 && d < a.V) {
-                    const float x = load_elem<DT>(a.logits, b * a.l_sb + i * a.l_st + d);
-                    const double q = a.probs ? static_cast<double>(a.probs[b * a.p_sb + i * a.p_st + d]) : 1.0;
-                    accept = static_cast<double>(a.uniform[b * a.u_sb + i]) * q < exp((static_cast<double>(x) - m) * inv_t) / z;
-                }
-            }
-            rmax[i] = m, rz[i] = z, rarg[i] = valid ? arg : -1, ok[i] = accept ? 1 : 0;
+            const bool accept = greedy ? d == arg
+                                       : d >= 0 && d < a.V && static_cast<double>(u) * q < exp((static_cast<double>(x) - m) * inv_t) / z;
+            rmax[i] = m, rarg[i] = valid ? (greedy ? arg : 0) : -1, ok[i] = valid && i < count && accept ? 1 : 0;
         }
     }
     __syncthreads();
@@ -389,28 +382,27 @@ __global__ void __launch_bounds__(kVdThreads) verify_accept_kernel(Verify a) {
         return;
     }
     const double s = vd_chunk_sum<DT>(r, chunk, a.len2, a.V, false, red);
-    if (tid == 0) vd_write(&a.sums[static_cast<int64_t>(b) * a.chunks2 + chunk].p, s);
-    if (r.mode == kVdResidual) return;
-    if (!vd_last(&a.state[b].done[0], static_cast<uint32_t>(a.chunks2), &flag)) return;
-    bool any = false;
-    for (int c = tid; c < a.chunks2; c += kVdThreads) sums[c] = vd_read(&a.sums[static_cast<int64_t>(b) * a.chunks2 + c].p);
-    __syncthreads();
-    for (int c = 0; c < a.chunks2; ++c) any = any || sums[c] > 0.0;
-    if (!any) {                                               // p is all on the draft that was rejected: p
-        r.mode = kVdPlain;
+    ChunkSum* sums = a.sums + static_cast<int64_t>(b) * a.chunks2;
+    if (r.mode == kVdResidual) {
+        if (tid == 0) sums[chunk].p = s;                      // the third launch goes on
+        return;
+    }
+    if (!vd_last(&sums[chunk].p, s, &a.state[b].done[0], static_cast<uint32_t>(a.chunks2), &flag)) return;
+    const double mine = lane < a.chunks2 ? vd_read(&sums[lane].p) : 0.0;
+    if (__ballot(mine > 0.0) == 0) {                          // p is all on the draft that was rejected: p
         write(d);
         return;
     }
-    write(vd_draw<DT>(r, sums, a.chunks2, a.len2, a.V, false, a.uniform[b * a.u_sb + a.K], red, found));
+    write(vd_draw<DT>(r, mine, a.len2, a.V, false, a.uniform[b * a.u_sb + a.K], red, found));
 }
 
 // The same for max(p - q, 0), p's total known.
 template <int DT>
 __global__ void __launch_bounds__(kVdThreads) verify_residual_kernel(Verify a) {
     constexpr int kEs = VdType<DT>::kEs, kW = kVdThreads / kWave;
-    __shared__ double red[kW], sums[kVdChunks];
+    __shared__ double red[kW];
     __shared__ int found[1 + kW], flag;
-    const int tid = threadIdx.x, chunk = blockIdx.x, b = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid % kWave, chunk = blockIdx.x, b = blockIdx.y;
     if (a.state[b].mode != kVdResidual) return;
     const int n = a.state[b].n;
     VdRow r{};
@@ -418,24 +410,14 @@ __global__ void __launch_bounds__(kVdThreads) verify_residual_kernel(Verify a) {
     r.q = a.probs + b * a.p_sb + n * a.p_st;
     r.mode = kVdResidual;
     r.m = a.state[b].m, r.inv_t = 1.0 / static_cast<double>(vd_temperature(a, b));
-    ChunkSum* mine = a.sums + static_cast<int64_t>(b) * a.chunks2;
-    for (int c = tid; c < a.chunks2; c += kVdThreads) sums[c] = mine[c].p;
-    __syncthreads();
-    double total = 0.0;
-    for (int c = 0; c < a.chunks2; ++c) total += sums[c];
-    r.total = total;
+    ChunkSum* sums = a.sums + static_cast<int64_t>(b) * a.chunks2;
+    const double plain = lane < a.chunks2 ? sums[lane].p : 0.0;
+    r.inv_total = 1.0 / wave_sum_f64(plain);
     const double s = vd_chunk_sum<DT>(r, chunk, a.len2, a.V, true, red);
-    if (tid == 0) vd_write(&mine[chunk].r, s);
-    if (!vd_last(&a.state[b].done[1], static_cast<uint32_t>(a.chunks2), &flag)) return;
-    double left = 0.0;
-    for (int c = 0; c < a.chunks2; ++c) left += vd_read(&mine[c].r);
-    const bool residual = left > 0.0;                         // otherwise from p
-    __syncthreads();
-    if (residual) {
-        for (int c = tid; c < a.chunks2; c += kVdThreads) sums[c] = vd_read(&mine[c].r);
-        __syncthreads();
-    }
-    const int token = vd_draw<DT>(r, sums, a.chunks2, a.len2, a.V, residual, a.uniform[b * a.u_sb + a.K], red, found);
+    if (!vd_last(&sums[chunk].r, s, &a.state[b].done[1], static_cast<uint32_t>(a.chunks2), &flag)) return;
+    const double less = lane < a.chunks2 ? vd_read(&sums[lane].r) : 0.0;
+    const bool residual = __ballot(less > 0.0) != 0;          // otherwise from p
+    const int token = vd_draw<DT>(r, residual ? less : plain, a.len2, a.V, residual, a.uniform[b * a.u_sb + a.K], red, found);
     for (int i = tid; i <= a.K; i += kVdThreads)
         a.tokens[static_cast<int64_t>(b) * (a.K + 1) + i] = i < n ? a.drafts[b * a.d_sb + i] : i == n ? token : -1;
     if (tid == 0) a.accepted[b] = n;
@@ -457,8 +439,7 @@ VerifyPlan verify_plan(int64_t B, int64_t K, int64_t V, int dtype) {
     p.len1 = round * p.pieces;
     p.chunks1 = static_cast<int>(cdiv(all, p.len1));
     p.len2 = round;
-    while (B * cdiv(all, p.len2) > 1024 && cdiv(all, p.len2) > 1) p.len2 += round;
-    while (cdiv(all, p.len2) > kVdChunks) p.len2 += round;
+    while (cdiv(all, p.len2) > kWave) p.len2 += round;
     p.chunks2 = static_cast<int>(cdiv(all, p.len2));
     p.stats = 0;
     p.sums = p.stats + static_cast<size_t>(B * (K + 1) * p.chunks1) * sizeof(ChunkStat);
