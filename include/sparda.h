@@ -1037,7 +1037,7 @@ SPARDA_API size_t sparda_verify_drafts_workspace_bytes(int64_t B, int64_t K, int
  *   [B,K+1] in [0, 1), stride u_sb; draft_probs: fp32 [B,K,V], strides (p_sb, p_st, 1); n_drafts: int32 [B]
  *   (NULL: K each), taken into [0, K]; temperatures: fp32 [B] (NULL: `temperature` for all).
  *   tokens: int32 [B,K+1], the accepted drafts, the token, then -1; n_accepted: int32 [B].
- *   0 <= K <= 64, B (K+1) <= 65535, V <= 2^21 - 8. Workspace 16-byte aligned; calls that share one must be
+ *   0 <= K <= 64, B (K+1) <= 65535, V <= 2^20 - 8. Workspace 16-byte aligned; calls that share one must be
  *   ordered on one stream.
  */
 SPARDA_API int sparda_verify_drafts(const void* logits, int dtype, int64_t l_sb, int64_t l_st, const int32_t* drafts,

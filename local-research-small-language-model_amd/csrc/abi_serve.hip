@@ -193,7 +193,7 @@ SPARDA_API int sparda_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st,
 
 namespace {
 bool verify_sizes_ok(int64_t B, int64_t K, int64_t V) {
-    return B > 0 && K >= 0 && K <= 64 && B <= 65535 / (K + 1) && V > 0 && V <= (1ll << 21) - 8;
+    return B > 0 && K >= 0 && K <= 64 && B <= 65535 / (K + 1) && V > 0 && V <= (1ll << 20) - 8;
 }
 }  // namespace
 
@@ -210,7 +210,7 @@ SPARDA_API int sparda_verify_drafts(const void* logits, int dtype, int64_t l_sb,
     SPARDA_REQUIRE(logits && uniform && tokens && n_accepted && (drafts || K == 0), SPARDA_ERR_NULL, "%s: null pointer", who);
     SPARDA_REQUIRE(dtype_ok(dtype), SPARDA_ERR_DTYPE, "%s: dtype %d unsupported", who, dtype);
     SPARDA_REQUIRE(verify_sizes_ok(B, K, V), SPARDA_ERR_SHAPE,
-                   "%s: %lld sequences of %lld drafts of a vocabulary of %lld: at most 64 drafts, 65535 rows, 2^21 - 8 tokens", who,
+                   "%s: %lld sequences of %lld drafts of a vocabulary of %lld: at most 64 drafts, 65535 rows, 2^20 - 8 tokens", who,
                    (long long)B, (long long)K, (long long)V);
     SPARDA_REQUIRE(temperatures || (temperature >= 0.0f && temperature <= 3.4e38f), SPARDA_ERR_SHAPE,
                    "%s: the temperature must be finite and not negative", who);

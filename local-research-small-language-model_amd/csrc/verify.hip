@@ -1,19 +1,23 @@
 // Verification of drafted tokens (sparda_verify_drafts): which of a sequence's
 // drafts its target distributions accept, and the token drawn behind them.
 //
-//   p_i = softmax(logits[b, i] / temperature[b]), q_i the draft's distribution of draft i
-//   (all of it on the draft where none is given). Draft d_i is accepted while u_i q_i(d_i) < p_i(d_i). Behind n
+//   p_i = softmax(logits[b, i] / temperature[b]), q_i the draft's distribution of draft i (all of it on
+//   the draft where none is given). Draft d_i is accepted while u_i q_i(d_i) < p_i(d_i). Behind n
 //   accepted ones the token is the first at which the cumulated sum of r passes u_K times
-//   its total: r = max(p_n - q_n, 0) after a rejection (p_n where that leaves nothing),
-//   r = p_n where no draft is left. Temperature 0: the drafts are compared with
-//   the largest logits' lowest indexes.
+//   its total: r = max(p_n - q_n, 0) after a rejection (p_n where that leaves nothing), r = p_n
+//   where no draft is left. Temperature 0: the drafts are compared with the largest logits' lowest indexes.
 //
-// The first launch reads all logits once, in fp32: maximum and sum of every chunk of
-// every row. The test of a draft needs no more. The token is where a long sum
-// passes a number, and which token that is must not hang on how fp32 rounds, so the one row
-// it is drawn from is summed again in fp64: a second launch over (chunk, sequence),
-// and after rejections against given distributions a third, which needs the row's total.
-// The workgroup that comes last among a sequence's draws the token from the chunks' sums.
+// Which token a long sum passes must not hang on how fp32 rounds, so the row that it is drawn from is
+// summed in fp64. Two launches. One reads all logits once and leaves the maximum and the sum of every chunk of
+// every row, for calls of up to 2^21 logits in fp64, in fp32 beyond, where fp64 would take longer than the
+// memory (64 x 8 x 50257: 24.5 us against 12). In the other, workgroups of a (chunk, sequence) find
+// the accepted drafts, which the sums in fp32 decide well enough; each sums its chunk
+// of the row again, and the last one that comes draws. A token from p over sums in fp64 is drawn
+// by the first workgroup alone.
+//
+// The sums of max(p - q, 0) need p's total Z, which no workgroup has. They are taken apart: over the tokens
+// where w / Z' > q, w = p Z and Z' the total in fp32, sum (w / Z - q) = A / Z - Q with
+// A = sum w, Q = sum q, and the last workgroup has Z. Tokens between the two borders weigh 10^-7 of themselves.
 #include "common.h"
 #include "kernels.h"
 
@@ -21,25 +25,22 @@ namespace sparda {
 
 namespace {
 
-constexpr int kVdThreads = 256;
-constexpr int kVdChunks = 256;        // chunks of a row in the first launch, at most
+constexpr int kVdThreads = 256, kVdWaves = kVdThreads / kWave;
 constexpr int kVdRows = 65;           // rows of a sequence (drafts + 1), at most
-constexpr float kVdLog2e = 1.4426950408889634f;
+constexpr int kVdRounds = 16;         // rounds of a chunk (one 16-byte piece a thread), at most; a row has at most 64 chunks
+constexpr double kVdLog2e = 1.4426950408889634074;
 
 struct alignas(16) ChunkStat {
     float m;         // largest logit of the chunk
     int32_t arg;     // its lowest index (greedy sequences)
-    double sum;      // of exp((x - m) / temperature)
+    double sum;      // of 2^((x - m) log2 e / temperature)
 };
-struct alignas(16) ChunkSum {
-    double p, r;     // sums of p's weights and of r's
+struct ChunkSum {
+    double w, above, q;  // of the weights, those above q, q there
 };
 struct SequenceState {
-    uint32_t done[2];    // workgroups of the second and third launch that are through
-    int32_t n, mode;     // drafts accepted, how the token is drawn
-    double m;            // the row's largest logit
+    uint32_t done, pad;  // workgroups of the second launch that are through
 };
-enum { kVdNone = 0, kVdPlain = 1, kVdWithout = 2, kVdResidual = 3 };  // modes: nothing to draw, p, p without the draft, max(p - q, 0)
 
 struct Verify {
     const void* logits;
@@ -55,10 +56,11 @@ struct Verify {
     float all_temperature;
     int K;
     int64_t V;
-    int64_t len1, len2;          // elements of a chunk in the first launch, in the others
+    int rounds1, rounds2;        // rounds of a chunk in either launch
     int chunks1, chunks2;
     ChunkStat* stats;            // [B, K + 1, chunks1]
     ChunkSum* sums;              // [B, chunks2]
+    int exact;                   // the statistics' sums are fp64's
     SequenceState* state;        // [B]
     int32_t *tokens, *accepted;  // [B, K + 1], [B]
 };
@@ -72,32 +74,64 @@ __device__ __forceinline__ float vd_temperature(const Verify& a, int b) {
     return a.temperature != nullptr ? a.temperature[b] : a.all_temperature;
 }
 
+// 2^t for -1020 <= t <= 0: t = n + f, |f| <= 1/2, and the Taylor series of 2^f up to f^10, whose
+// rest is below 3 10^-13. n is rounded by the addition of 1.5 2^52, whose low word then holds it, and goes
+// into the exponent as an integer (the conversions and the scaling of fp64 run at a
+// quarter of the rate: 50257 x 512 logits 31.5 us with them, @@ without).
+__device__ __forceinline__ double vd_exp2(double t) {
+    constexpr double kShift = 6755399441055744.0;
+    const double y = t + kShift, f = t - (y - kShift);
+    double p = 7.0549116208011209e-09;            // (ln 2)^k / k!, k = 10 .. 0
+    p = __builtin_fma(p, f, 1.0178086009239696e-07);
+    p = __builtin_fma(p, f, 1.3215486790144305e-06);
+    p = __builtin_fma(p, f, 1.5252733804059838e-05);
+    p = __builtin_fma(p, f, 1.5403530393381606e-04);
+    p = __builtin_fma(p, f, 1.3333558146428441e-03);
+    p = __builtin_fma(p, f, 9.6181291076284769e-03);
+    p = __builtin_fma(p, f, 5.5504108664821576e-02);
+    p = __builtin_fma(p, f, 2.4022650695910069e-01);
+    p = __builtin_fma(p, f, 6.9314718055994529e-01);
+    p = __builtin_fma(p, f, 1.0);
+    const uint64_t u = __builtin_bit_cast(uint64_t, p);
+    const uint32_t n = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, y));
+    return __builtin_bit_cast(double, (static_cast<uint64_t>(static_cast<uint32_t>(u >> 32) + (n << 20)) << 32) | static_cast<uint32_t>(u));
+}
+// for every t <= 0: 0 below -1020, which leaves -inf no weight
+__device__ __forceinline__ double vd_weight(double t) {
+    const double w = vd_exp2(fmax(t, -1020.0));
+    return t > -1020.0 ? w : 0.0;
+}
+
 template <int DT>
 struct VdType {
     static constexpr int kEs = DT == SPARDA_F32 ? 4 : 2, kVe = 16 / kEs;   // bytes of an element, elements of a piece
+    static constexpr int kRound = kVdThreads * kVe;                        // elements of a round
 };
 
-// Elements [at, at + kVe) of a row of V in aligned pieces of 16 bytes; those outside [0, V) are
-// -inf. A piece that leaves the row is read element by element.
+// A piece of 16 bytes of a row, elements [at, at + kVe); those outside [0, V) are -inf. A piece
+// that leaves the row is read element by element.
 template <int DT>
-__device__ __forceinline__ void vd_load(const char* row, int64_t at, int64_t V, float (&x)[VdType<DT>::kVe]) {
+__device__ __forceinline__ uint4 vd_load(const char* row, int64_t at, int64_t V) {
     constexpr int kVe = VdType<DT>::kVe, kEs = VdType<DT>::kEs;
-    if (at >= 0 && at + kVe <= V) {
-        const uint4 w = *reinterpret_cast<const uint4*>(row + at * kEs);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    if (at >= 0 && at + kVe <= V) return *reinterpret_cast<const uint4*>(row + at * kEs);
+    uint32_t w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if constexpr (DT == SPARDA_F32) {
-                x[e] = __uint_as_float(u[e]);
-            } else {
-                x[2 * e] = __uint_as_float(u[e] << 16);
-                x[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
-            }
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == SPARDA_F32) {
+            w[i] = at + i >= 0 && at + i < V ? reinterpret_cast<const uint32_t*>(row)[at + i] : 0xff800000u;
+        } else {
+            const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+            const int64_t e = at + 2 * i;
+            w[i] = (e >= 0 && e < V ? p[e] : 0xff80u) | static_cast<uint32_t>(e + 1 >= 0 && e + 1 < V ? p[e + 1] : 0xff80u) << 16;
         }
-    } else {
-#pragma unroll
-        for (int e = 0; e < kVe; ++e) x[e] = at + e >= 0 && at + e < V ? load_elem<DT>(row, at + e) : -__builtin_inff();
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <int DT>
+__device__ __forceinline__ float vd_element(const uint4& x, int e) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    if constexpr (DT == SPARDA_F32) return __uint_as_float(w[e]);
+    else return __uint_as_float(e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
 }
 
 // elements before a row's start in its first aligned piece
@@ -106,158 +140,223 @@ __device__ __forceinline__ int vd_shift(const char* row) {
     return static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16) / VdType<DT>::kEs;
 }
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
-    return v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, ROWS, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
-// inclusive sums over the lanes
+// inclusive sums over the lanes: within rows of 16 by shifts, then the rows' totals
 __device__ __forceinline__ double wave_scan_f64(double v) {
-    const int lane = threadIdx.x % kWave;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const double w = __shfl_up(v, o, kWave);
-        if (lane >= o) v += w;
-    }
+    v += dpp_f64<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+    v += dpp_f64<0x112, 0xf>(v);
+    v += dpp_f64<0x114, 0xf>(v);
+    v += dpp_f64<0x118, 0xf>(v);
+    v += dpp_f64<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+    v += dpp_f64<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
     return v;
 }
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(u), lane);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(u >> 32), lane);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum_f64(double v) { return lane_f64(wave_scan_f64(v), kWave - 1); }
 
 }  // namespace
 
-// Maximum and sum of a chunk of a row, in one read: the chunk's pieces stay in registers.
-template <int DT, int PIECES>
+// Maximum and sum of a chunk of a row, in one read: the chunk's pieces stay in registers. Every
+// wavefront measures its exponentials against its own maximum, so that the wavefronts meet once.
+template <int DT, int ROUNDS, bool EXACT>
 __global__ void __launch_bounds__(kVdThreads) verify_stats_kernel(Verify a) {
     constexpr int kVe = VdType<DT>::kVe, kEs = VdType<DT>::kEs;
-    __shared__ float rm[kVdThreads / kWave];
-    __shared__ double rs[kVdThreads / kWave];
-    __shared__ int ra[kVdThreads / kWave];
+    __shared__ float rm[kVdWaves];
+    __shared__ double rs[kVdWaves];
+    __shared__ int ra[kVdWaves];
     const int tid = threadIdx.x, wave = tid / kWave, chunk = blockIdx.x;
     const int b = blockIdx.y / (a.K + 1), i = blockIdx.y % (a.K + 1);
-    if (chunk == 0 && i == 0 && tid == 0) a.state[b].done[0] = a.state[b].done[1] = 0;
+    if (chunk == 0 && i == 0 && tid == 0) a.state[b].done = 0;
+    const char* row = static_cast<const char*>(a.logits) + (b * a.l_sb + i * a.l_st) * kEs;
+    const int64_t first = static_cast<int64_t>(chunk) * ROUNDS * VdType<DT>::kRound - vd_shift<DT>(row);
     if (i > vd_count(a, b)) return;                           // no draft's row
+    uint4 x[ROUNDS];
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k) x[k] = vd_load<DT>(row, first + (tid + k * kVdThreads) * kVe, a.V);
     const float T = vd_temperature(a, b);
     const bool greedy = !(T > 0.0f);
-    const float c = greedy ? kVdLog2e : fminf(kVdLog2e / T, 3e38f);
-    const char* row = static_cast<const char*>(a.logits) + (b * a.l_sb + i * a.l_st) * kEs;
-    const int64_t first = chunk * a.len1 - vd_shift<DT>(row);
-    float x[PIECES][kVe];
-#pragma unroll
-    for (int k = 0; k < PIECES; ++k) vd_load<DT>(row, first + (tid + k * kVdThreads) * kVe, a.V, x[k]);
+    const double c = greedy ? kVdLog2e : kVdLog2e / static_cast<double>(T);
     float m = -__builtin_inff();
 #pragma unroll
-    for (int k = 0; k < PIECES; ++k)
+    for (int k = 0; k < ROUNDS; ++k)
 #pragma unroll
-        for (int e = 0; e < kVe; ++e) m = fmaxf(m, x[k][e]);
+        for (int e = 0; e < kVe; ++e) m = fmaxf(m, vd_element<DT>(x[k], e));
     m = wave_max(m);
-    if (tid % kWave == 0) rm[wave] = m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kVdThreads / kWave; ++w) m = fmaxf(m, rm[w]);
-    const float ref = m == -__builtin_inff() ? 0.0f : m;
-    float s = 0.0f;
+    double s = 0.0;
     int arg = 0x7fffffff;
+    // a NaN comes back in every sum in fp32, the masked and the greedy ones' too
+    if constexpr (!EXACT) {
+        const float c32 = static_cast<float>(fmin(c, 3e38)), ref = m == -__builtin_inff() ? 0.0f : m;
+        float s32 = 0.0f;
 #pragma unroll
-    for (int k = 0; k < PIECES; ++k)
+        for (int k = 0; k < ROUNDS; ++k)
 #pragma unroll
-        for (int e = 0; e < kVe; ++e) s += __builtin_amdgcn_exp2f((x[k][e] - ref) * c);
+            for (int e = 0; e < kVe; ++e) s32 += __builtin_amdgcn_exp2f((vd_element<DT>(x[k], e) - ref) * c32);
+        s = wave_sum(s32);
+    } else {
+        float nan = 0.0f;                                     // NaN or 0, one operation a logit
+#pragma unroll
+        for (int k = 0; k < ROUNDS; ++k)
+#pragma unroll
+            for (int e = 0; e < kVe; ++e) nan = __builtin_fmaf(vd_element<DT>(x[k], e) == -__builtin_inff() ? 0.0f : vd_element<DT>(x[k], e), 0.0f, nan);
+        if (!greedy && m > -__builtin_inff()) {               // (wave-uniform)
+#pragma unroll
+            for (int k = 0; k < ROUNDS; ++k)
+#pragma unroll
+                for (int e = 0; e < kVe; ++e)
+                    s += vd_exp2(fmax((static_cast<double>(vd_element<DT>(x[k], e)) - static_cast<double>(m)) * c, -1020.0));
+        }
+        s = wave_sum_f64(s);
+        if (__ballot(nan != nan) != 0) s = __builtin_nan("");
+    }
     if (greedy) {
 #pragma unroll
-        for (int k = PIECES - 1; k >= 0; --k)
+        for (int k = ROUNDS - 1; k >= 0; --k)
 #pragma unroll
             for (int e = kVe - 1; e >= 0; --e)
-                if (x[k][e] == m) arg = static_cast<int>(first + (tid + k * kVdThreads) * kVe + e);
+                if (vd_element<DT>(x[k], e) == m) arg = static_cast<int>(first + (tid + k * kVdThreads) * kVe + e);
         arg = wave_min_i32(arg);
     }
-    s = wave_sum(s);
-    if (tid % kWave == 0) rs[wave] = s, ra[wave] = arg;
+    if (tid % kWave == 0) rm[wave] = m, rs[wave] = s, ra[wave] = arg;
     __syncthreads();
     if (tid == 0) {
-        ChunkStat st{m, ra[0], rs[0]};
+        ChunkStat st{rm[0], 0x7fffffff, 0.0};
 #pragma unroll
-        for (int w = 1; w < kVdThreads / kWave; ++w) st.sum += rs[w], st.arg = min(st.arg, ra[w]);
+        for (int w = 1; w < kVdWaves; ++w) st.m = fmaxf(st.m, rm[w]);
+#pragma unroll
+        for (int w = 0; w < kVdWaves; ++w) {
+            // (a wavefront without a finite logit adds nothing, NaN among them stays)
+            st.sum += rm[w] == -__builtin_inff() ? rs[w] : rs[w] * vd_weight((static_cast<double>(rm[w]) - st.m) * c);
+            if (rm[w] == st.m) st.arg = min(st.arg, ra[w]);
+        }
         a.stats[static_cast<int64_t>(blockIdx.y) * a.chunks1 + chunk] = st;
     }
 }
 
 namespace {
 
-// What a token is drawn from: row, and what is taken off its weights.
+// What a token is drawn from, and what is taken off its weights.
 struct VdRow {
     const char* row;
-    const float* q;       // mode kVdResidual
-    int without;          // mode kVdWithout
-    int mode;
-    double m, inv_t, inv_total;   // inv_total: one over the sum of p's weights (kVdResidual)
+    const float* q;          // nullptr, or the weights are max(p - q, 0)
+    int64_t without;         // no weight for this token (-1: none)
+    double c, m;             // a weight is 2^((x - m) c): 1 for every x of m, whatever they are
+    double inv_total;        // one over p's weights (with q)
 };
 
-// r of eight or four elements; w: p's weights, not divided by their total
+// weights of a piece, not yet against q, and q
 template <int DT>
-__device__ __forceinline__ void vd_weights(const VdRow& r, int64_t at, int64_t V, bool residual, double (&w)[VdType<DT>::kVe]) {
+__device__ __forceinline__ void vd_piece(const VdRow& r, int64_t at, int64_t V, double (&w)[VdType<DT>::kVe], float (&q)[VdType<DT>::kVe]) {
     constexpr int kVe = VdType<DT>::kVe;
-    float x[kVe];
-    vd_load<DT>(r.row, at, V, x);
+    const uint4 x = vd_load<DT>(r.row, at, V);
+    if (r.q != nullptr) {
+        if (at >= 0 && at + kVe <= V) {
+#pragma unroll
+            for (int e = 0; e < kVe; ++e) q[e] = r.q[at + e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < kVe; ++e) q[e] = at + e >= 0 && at + e < V ? r.q[at + e] : 0.0f;
+        }
+    }
 #pragma unroll
     for (int e = 0; e < kVe; ++e) {
-        w[e] = exp((static_cast<double>(x[e]) - r.m) * r.inv_t);
-        if (r.mode == kVdWithout && at + e == r.without) w[e] = 0.0;
-        if (residual) {
-            const double q = at + e >= 0 && at + e < V ? static_cast<double>(r.q[at + e]) : 0.0;
-            const double d = w[e] * r.inv_total - q;
-            w[e] = d > 0.0 ? d : 0.0;
-        }
+        w[e] = vd_weight((static_cast<double>(vd_element<DT>(x, e)) - r.m) * r.c);
+        if (at + e == r.without) w[e] = 0.0;
+    }
+}
+template <int DT>
+__device__ __forceinline__ void vd_weights(const VdRow& r, int64_t at, int64_t V, double (&w)[VdType<DT>::kVe]) {
+    constexpr int kVe = VdType<DT>::kVe;
+    float q[kVe];
+    vd_piece<DT>(r, at, V, w, q);
+    if (r.q == nullptr) return;
+#pragma unroll
+    for (int e = 0; e < kVe; ++e) {
+        const double d = __builtin_fma(w[e], r.inv_total, -static_cast<double>(q[e]));
+        w[e] = d > 0.0 ? d : 0.0;
     }
 }
 
-__device__ __forceinline__ double block_sum_f64(double v, double* red) {
-    const int wave = threadIdx.x / kWave;
-    v = wave_sum_f64(v);
-    __syncthreads();                              // (the array's last use)
-    if (threadIdx.x % kWave == 0) red[wave] = v;
-    __syncthreads();
-    double s = red[0];
+// the sums of a chunk's weights, by all threads; the result in every one
+template <int DT>
+__device__ __forceinline__ ChunkSum vd_chunk_sum(const VdRow& r, int64_t first, int rounds, int64_t V, double* red) {
+    constexpr int kVe = VdType<DT>::kVe;
+    ChunkSum s{0.0, 0.0, 0.0};
+    for (int k = 0; k < rounds; ++k) {
+        double w[kVe];
+        float q[kVe];
+        vd_piece<DT>(r, first + (threadIdx.x + k * kVdThreads) * kVe, V, w, q);
 #pragma unroll
-    for (int w = 1; w < kVdThreads / kWave; ++w) s += red[w];
+        for (int e = 0; e < kVe; ++e) {
+            s.w += w[e];
+            if (r.q != nullptr && __builtin_fma(w[e], r.inv_total, -static_cast<double>(q[e])) > 0.0) s.above += w[e], s.q += q[e];
+        }
+    }
+    s.w = wave_sum_f64(s.w);
+    if (r.q != nullptr) s.above = wave_sum_f64(s.above), s.q = wave_sum_f64(s.q);
+    const int wave = threadIdx.x / kWave;
+    __syncthreads();                              // (the array's last use)
+    if (threadIdx.x % kWave == 0) red[3 * wave] = s.w, red[3 * wave + 1] = s.above, red[3 * wave + 2] = s.q;
+    __syncthreads();
+    s = ChunkSum{red[0], red[1], red[2]};
+#pragma unroll
+    for (int w = 1; w < kVdWaves; ++w) s.w += red[3 * w], s.above += red[3 * w + 1], s.q += red[3 * w + 2];
     return s;
 }
 
 // The token of the chunks' sums (lane c of every wavefront holds chunk c's): the chunk where they pass
-// u times their total, then the token in it. All threads of the workgroup.
+// u times their total, the round and the wavefront in it, then the token. All threads of the workgroup; red: one
+// number a round and wavefront.
 template <int DT>
-__device__ __forceinline__ int vd_draw(const VdRow& r, double mine_of_all, int64_t len, int64_t V, bool residual, float u, double* red,
-                                       int* found) {
-    constexpr int kVe = VdType<DT>::kVe, kW = kVdThreads / kWave;
+__device__ __forceinline__ int vd_draw(const VdRow& r, double of_lane, int rounds, int64_t V, float u, double* red, int* found) {
+    constexpr int kVe = VdType<DT>::kVe;
     const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
-    const double upto_chunk = wave_scan_f64(mine_of_all);
-    const double target = static_cast<double>(u) * __shfl(upto_chunk, kWave - 1, kWave);
-    const uint64_t pass = __ballot(upto_chunk > target), some = __ballot(mine_of_all > 0.0);
+    const double upto_chunk = wave_scan_f64(of_lane);
+    const double target = static_cast<double>(u) * lane_f64(upto_chunk, kWave - 1);
+    const uint64_t pass = __ballot(upto_chunk > target), some = __ballot(of_lane > 0.0);
     // (none passes where u is 1, or the last by a rounding: the last token that weighs anything)
     const int chunk = pass != 0 ? __builtin_ctzll(pass) : 63 - __builtin_clzll(some | 1);
-    double base = __shfl(upto_chunk - mine_of_all, chunk, kWave);
-    const int64_t first = chunk * len - vd_shift<DT>(r.row);
-    int best = -1;                                // the last token with a weight so far
-    for (int64_t p0 = 0; p0 < len; p0 += kVdThreads * kVe) {
-        const int64_t at = first + p0 + tid * kVe;
-        double w[kVe], mine = 0.0;
-        vd_weights<DT>(r, at, V, residual, w);
-        int top = -1;
+    const double base = lane_f64(upto_chunk, chunk) - lane_f64(of_lane, chunk);
+    const int64_t first = static_cast<int64_t>(chunk) * rounds * VdType<DT>::kRound - vd_shift<DT>(r.row);
+    double w[kVe];
+    __syncthreads();                              // (the arrays' last use)
+    for (int k = 0; k < rounds; ++k) {
+        vd_weights<DT>(r, first + (tid + k * kVdThreads) * kVe, V, w);
+        double s = 0.0;
 #pragma unroll
-        for (int e = 0; e < kVe; ++e) {
-            mine += w[e];
-            if (w[e] > 0.0) top = static_cast<int>(at + e);
-        }
-        const double upto = wave_scan_f64(mine);
-        __syncthreads();                          // (the arrays' last use)
-        if (lane == kWave - 1) red[wave] = upto;
-        if (tid == 0) found[0] = 0x7fffffff;
+        for (int e = 0; e < kVe; ++e) s += w[e];
+        s = wave_sum_f64(s);
+        if (lane == 0) red[k * kVdWaves + wave] = s;
+    }
+    if (tid == 0) *found = -1;
+    __syncthreads();
+    // lane: a (round, wavefront), in the order of the row
+    const double part = lane < rounds * kVdWaves ? red[lane] : 0.0, upto = wave_scan_f64(part);
+    const uint64_t here = __ballot(base + upto > target), any = __ballot(part > 0.0);
+    const int at_part = pass != 0 && here != 0 ? __builtin_ctzll(here) : 63 - __builtin_clzll(any | 1);
+    if (wave == at_part % kVdWaves) {             // the wavefront whose pieces they are
+        const int64_t at = first + (tid + at_part / kVdWaves * kVdThreads) * kVe;
+        vd_weights<DT>(r, at, V, w);
+        double mine = 0.0;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, kWave));
-        if (lane == 0) found[1 + wave] = top;
-        __syncthreads();
-        double before = base;
-        for (int v = 0; v < wave; ++v) before += red[v];
-        if (pass != 0 && mine > 0.0 && before + upto > target) {
-            // (rounding may leave the piece's own sums below: its last weight)
-            double acc = before + upto - mine;
+        for (int e = 0; e < kVe; ++e) mine += w[e];
+        const double scan = wave_scan_f64(mine), before = base + (lane_f64(upto, at_part) - lane_f64(part, at_part));
+        const uint64_t over = __ballot(mine > 0.0 && before + scan > target), have = __ballot(mine > 0.0);
+        // (rounding may leave these sums below the parts': the last that weighs anything)
+        const bool passes = pass != 0 && here != 0 && over != 0;
+        if (lane == (passes ? __builtin_ctzll(over) : 63 - __builtin_clzll(have | 1))) {
+            double acc = before + (scan - mine);
             int hit = -1, last = -1;
 #pragma unroll
             for (int e = 0; e < kVe; ++e) {
@@ -267,27 +366,26 @@ __device__ __forceinline__ int vd_draw(const VdRow& r, double mine_of_all, int64
                     if (hit < 0 && acc > target) hit = e;
                 }
             }
-            atomicMin(&found[0], static_cast<int>(at + (hit >= 0 ? hit : last)));
+            *found = last < 0 ? -1 : static_cast<int>(at + (passes && hit >= 0 ? hit : last));
         }
-        __syncthreads();
-        if (found[0] != 0x7fffffff) return found[0];
-#pragma unroll
-        for (int v = 0; v < kW; ++v) best = max(best, found[1 + v]);
-#pragma unroll
-        for (int v = 0; v < kW; ++v) base += red[v];
     }
-    return best;
+    __syncthreads();
+    return *found;
 }
 
 // What workgroups of a launch hand to the last of them goes through stores and loads at the device's
-// scope, which pass the caches that they do not share; a store is waited for before its
-// workgroup is counted. (A release or acquire at that scope would write back and drop whole caches instead, once a workgroup.)
+// scope, which pass the caches that they do not share; a store is waited for before its workgroup
+// is counted. (A release or acquire at that scope would write back and drop whole caches instead, once a
+// workgroup: 35 us a launch of 1024.)
 __device__ __forceinline__ double vd_read(const double* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-// writes the workgroup's number and counts it; true in the last of `all`
-__device__ __forceinline__ bool vd_last(double* to, double v, uint32_t* done, uint32_t all, int* flag) {
+__device__ __forceinline__ void vd_write(double* p, double v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// writes the workgroup's sums and counts it; true in the last of `all`
+__device__ __forceinline__ bool vd_last(ChunkSum* to, const ChunkSum& s, uint32_t* done, uint32_t all, int* flag) {
     if (threadIdx.x == 0) {
-        __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __builtin_amdgcn_s_waitcnt(0x0f70);       // vmcnt(0): the store has arrived
+        vd_write(&to->w, s.w);
+        vd_write(&to->above, s.above);
+        vd_write(&to->q, s.q);
+        __builtin_amdgcn_s_waitcnt(0x0f70);       // vmcnt(0): the stores have arrived
         asm volatile("" ::: "memory");
         *flag = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == all;
     }
@@ -295,152 +393,118 @@ __device__ __forceinline__ bool vd_last(double* to, double v, uint32_t* done, ui
     return *flag != 0;
 }
 
-// the sum of a chunk's weights, by all threads
-template <int DT>
-__device__ __forceinline__ double vd_chunk_sum(const VdRow& r, int chunk, int64_t len, int64_t V, bool residual, double* red) {
-    constexpr int kVe = VdType<DT>::kVe;
-    const int64_t first = chunk * len - vd_shift<DT>(r.row);
-    double s = 0.0;
-    for (int64_t p0 = threadIdx.x * kVe; p0 < len; p0 += kVdThreads * kVe) {
-        double w[kVe];
-        vd_weights<DT>(r, first + p0, V, residual, w);
-#pragma unroll
-        for (int e = 0; e < kVe; ++e) s += w[e];
-    }
-    return block_sum_f64(s, red);
-}
-
 }  // namespace
 
-// One workgroup per (chunk, sequence). Every one finds the accepted drafts for itself, from the
-// chunks' statistics; then the chunk's sum of the row behind them, and the last one the token,
-// unless it is drawn from max(p - q, 0), which takes p's total.
+// One workgroup per (chunk, sequence), or per sequence where all sums are there and no distributions are given.
 template <int DT>
-__global__ void __launch_bounds__(kVdThreads) verify_accept_kernel(Verify a) {
-    constexpr int kEs = VdType<DT>::kEs, kW = kVdThreads / kWave;
-    __shared__ double red[kW];
+__global__ void __launch_bounds__(kVdThreads, 4) verify_draw_kernel(Verify a) {
+    constexpr int kEs = VdType<DT>::kEs;
+    __shared__ double red[kVdRounds * kVdWaves], rz[kVdRows];   // (red: a number a round and wavefront, three a wavefront)
     __shared__ float rmax[kVdRows];
-    __shared__ int rarg[kVdRows], ok[kVdRows], found[1 + kW], flag;
+    __shared__ int rarg[kVdRows], ok[kVdRows], found, flag;
     const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, chunk = blockIdx.x, b = blockIdx.y;
     const int count = vd_count(a, b);
     const float T = vd_temperature(a, b);
     const bool greedy = !(T > 0.0f);
-    const double inv_t = greedy ? 1.0 : 1.0 / static_cast<double>(T);
-    for (int i = wave; i <= count; i += kW) {                 // a wavefront a row
-        const ChunkStat* st = a.stats + (static_cast<int64_t>(b) * (a.K + 1) + i) * a.chunks1;
+    const double c = greedy ? kVdLog2e : kVdLog2e / static_cast<double>(T);
+    const ChunkStat* stats = a.stats + static_cast<int64_t>(b) * (a.K + 1) * a.chunks1;
+    // a chunk's sum, measured against the row's maximum
+    auto in_row = [&](const ChunkStat& s, float m) {
+        return s.m == -__builtin_inff() ? s.sum : s.sum * vd_weight((static_cast<double>(s.m) - m) * c);
+    };
+    for (int i = wave; i <= count; i += kVdWaves) {           // a wavefront a row
+        ChunkStat own{-__builtin_inff(), 0x7fffffff, 0.0};
+        if (lane < a.chunks1) own = stats[i * a.chunks1 + lane];
         // (the draft's own numbers under the chunks')
         int d = -1;
         float x = -__builtin_inff(), u = 0.0f, q = 1.0f;
         if (i < count) {
             d = a.drafts[b * a.d_sb + i];
+            u = a.uniform[b * a.u_sb + i];
             if (d >= 0 && d < a.V) {
                 x = load_elem<DT>(a.logits, b * a.l_sb + i * a.l_st + d);
-                u = a.uniform[b * a.u_sb + i];
                 if (a.probs) q = a.probs[b * a.p_sb + i * a.p_st + d];
             }
         }
-        ChunkStat own{-__builtin_inff(), 0x7fffffff, 0.0};
-        if (lane < a.chunks1) own = st[lane];
-        float m = own.m;
-        for (int c = lane + kWave; c < a.chunks1; c += kWave) m = fmaxf(m, st[c].m);
-        m = wave_max(m);
-        double z = 0.0;
-        int arg = 0x7fffffff;
-        auto add = [&](const ChunkStat& s) {
-            // (a chunk without a finite logit: nothing; NaN among them stays)
-            z += s.m == -__builtin_inff() ? s.sum : s.sum * exp((static_cast<double>(s.m) - m) * inv_t);
-            if (s.m == m) arg = min(arg, s.arg);
-        };
-        add(own);
-        for (int c = lane + kWave; c < a.chunks1; c += kWave) add(st[c]);
-        z = wave_sum_f64(z);
-        if (greedy) arg = wave_min_i32(arg);
+        const float m = wave_max(own.m);
+        const bool finite = m > -__builtin_inff() && m < __builtin_inff();
+        const double z = wave_sum_f64(finite ? in_row(own, m) : 0.0);
+        const int arg = greedy ? wave_min_i32(own.m == m ? own.arg : 0x7fffffff) : 0;
         if (lane == 0) {
-            const bool valid = m > -__builtin_inff() && m < __builtin_inff() && z < __builtin_inf();
-            const bool accept = greedy ? d == arg
-                                       : d >= 0 && d < a.V && static_cast<double>(u) * q < exp((static_cast<double>(x) - m) * inv_t) / z;
-            rmax[i] = m, rarg[i] = valid ? (greedy ? arg : 0) : -1, ok[i] = valid && i < count && accept ? 1 : 0;
+            const bool valid = finite && z < __builtin_inf();
+            const bool inside = d >= 0 && d < a.V;
+            const double p = valid && inside ? vd_weight((static_cast<double>(x) - m) * c) : 0.0;
+            rmax[i] = m, rz[i] = z, rarg[i] = valid ? arg : -1;
+            ok[i] = valid && inside && (greedy ? d == arg : static_cast<double>(u) * q < p / z) ? 1 : 0;
         }
     }
     __syncthreads();
     int n = 0;
     while (n < count && ok[n] != 0) ++n;
-    VdRow r{};
-    r.row = static_cast<const char*>(a.logits) + (b * a.l_sb + n * a.l_st) * kEs;
-    r.m = rmax[n], r.inv_t = inv_t;
-    const int d = n < count ? a.drafts[b * a.d_sb + n] : -1;
-    r.mode = rarg[n] < 0 || greedy ? kVdNone : n == count ? kVdPlain : a.probs ? kVdResidual : kVdWithout;
-    r.without = d;
     auto write = [&](int token) {
         for (int i = tid; i <= a.K; i += kVdThreads)
             a.tokens[static_cast<int64_t>(b) * (a.K + 1) + i] = i < n ? a.drafts[b * a.d_sb + i] : i == n ? token : -1;
         if (tid == 0) a.accepted[b] = n;
     };
-    if (chunk == 0 && tid == 0) a.state[b].n = n, a.state[b].mode = r.mode, a.state[b].m = r.m;
-    if (r.mode == kVdNone) {
+    if (rarg[n] < 0 || greedy) {
         if (chunk == 0) write(rarg[n]);
         return;
     }
-    const double s = vd_chunk_sum<DT>(r, chunk, a.len2, a.V, false, red);
-    ChunkSum* sums = a.sums + static_cast<int64_t>(b) * a.chunks2;
-    if (r.mode == kVdResidual) {
-        if (tid == 0) sums[chunk].p = s;                      // the third launch goes on
-        return;
-    }
-    if (!vd_last(&sums[chunk].p, s, &a.state[b].done[0], static_cast<uint32_t>(a.chunks2), &flag)) return;
-    const double mine = lane < a.chunks2 ? vd_read(&sums[lane].p) : 0.0;
-    if (__ballot(mine > 0.0) == 0) {                          // p is all on the draft that was rejected: p
-        write(d);
-        return;
-    }
-    write(vd_draw<DT>(r, mine, a.len2, a.V, false, a.uniform[b * a.u_sb + a.K], red, found));
-}
-
-// The same for max(p - q, 0), p's total known.
-template <int DT>
-__global__ void __launch_bounds__(kVdThreads) verify_residual_kernel(Verify a) {
-    constexpr int kEs = VdType<DT>::kEs, kW = kVdThreads / kWave;
-    __shared__ double red[kW];
-    __shared__ int found[1 + kW], flag;
-    const int tid = threadIdx.x, lane = tid % kWave, chunk = blockIdx.x, b = blockIdx.y;
-    if (a.state[b].mode != kVdResidual) return;
-    const int n = a.state[b].n;
+    const float u = a.uniform[b * a.u_sb + a.K];
     VdRow r{};
     r.row = static_cast<const char*>(a.logits) + (b * a.l_sb + n * a.l_st) * kEs;
-    r.q = a.probs + b * a.p_sb + n * a.p_st;
-    r.mode = kVdResidual;
-    r.m = a.state[b].m, r.inv_t = 1.0 / static_cast<double>(vd_temperature(a, b));
-    ChunkSum* sums = a.sums + static_cast<int64_t>(b) * a.chunks2;
-    const double plain = lane < a.chunks2 ? sums[lane].p : 0.0;
-    r.inv_total = 1.0 / wave_sum_f64(plain);
-    const double s = vd_chunk_sum<DT>(r, chunk, a.len2, a.V, true, red);
-    if (!vd_last(&sums[chunk].r, s, &a.state[b].done[1], static_cast<uint32_t>(a.chunks2), &flag)) return;
-    const double less = lane < a.chunks2 ? vd_read(&sums[lane].r) : 0.0;
-    const bool residual = __ballot(less > 0.0) != 0;          // otherwise from p
-    const int token = vd_draw<DT>(r, residual ? less : plain, a.len2, a.V, residual, a.uniform[b * a.u_sb + a.K], red, found);
-    for (int i = tid; i <= a.K; i += kVdThreads)
-        a.tokens[static_cast<int64_t>(b) * (a.K + 1) + i] = i < n ? a.drafts[b * a.d_sb + i] : i == n ? token : -1;
-    if (tid == 0) a.accepted[b] = n;
+    r.c = c, r.m = rmax[n], r.inv_total = 1.0 / rz[n], r.without = -1;
+    const bool rejected = n < count, against = rejected && a.probs != nullptr;
+    const int64_t d = rejected && !against ? a.drafts[b * a.d_sb + n] : -1;   // the rejected draft weighs nothing
+    if (d >= 0 && d < a.V) r.without = d;
+    const int64_t shift = vd_shift<DT>(r.row);
+    double of_lane;                                           // a chunk's weight
+    int rounds = a.rounds2, token = -1;
+    VdRow less = r;
+    if (against) less.q = a.probs + b * a.p_sb + n * a.p_st;
+    if (!a.exact || against) {
+        ChunkSum* sums = a.sums + static_cast<int64_t>(b) * a.chunks2;
+        const ChunkSum s = vd_chunk_sum<DT>(less, static_cast<int64_t>(chunk) * rounds * VdType<DT>::kRound - shift, rounds, a.V, red);
+        if (!vd_last(&sums[chunk], s, &a.state[b].done, static_cast<uint32_t>(a.chunks2), &flag)) return;
+        of_lane = lane < a.chunks2 ? vd_read(&sums[lane].w) : 0.0;
+        if (against) {
+            less.inv_total = 1.0 / wave_sum_f64(of_lane);
+            const double left = lane < a.chunks2 ? __builtin_fma(vd_read(&sums[lane].above), less.inv_total, -vd_read(&sums[lane].q)) : 0.0;
+            const double of_less = left > 0.0 ? left : 0.0;
+            if (__ballot(of_less > 0.0) != 0) token = vd_draw<DT>(less, of_less, rounds, a.V, u, red, &found);
+        }
+    } else {
+        if (chunk != 0) return;
+        rounds = a.rounds1;
+        of_lane = lane < a.chunks1 ? in_row(stats[n * a.chunks1 + lane], rmax[n]) : 0.0;
+        if (r.without >= 0) {
+            const int at = static_cast<int>((r.without + shift) / (static_cast<int64_t>(rounds) * VdType<DT>::kRound));
+            const ChunkSum s = vd_chunk_sum<DT>(r, static_cast<int64_t>(at) * rounds * VdType<DT>::kRound - shift, rounds, a.V, red);
+            of_lane = lane == at ? s.w : of_lane;
+        }
+    }
+    // from p (without the draft, which holds all of it where nothing is left)
+    if (token < 0) token = __ballot(of_lane > 0.0) != 0 ? vd_draw<DT>(r, of_lane, rounds, a.V, u, red, &found) : static_cast<int>(r.without);
+    write(token);
 }
 
 namespace {
 
 struct VerifyPlan {
-    int pieces;                  // 16-byte pieces of a thread in the first launch
-    int64_t len1, len2;
-    int chunks1, chunks2;
+    bool exact;
+    int rounds1, rounds2, chunks1, chunks2;
     size_t stats, sums, state, bytes;   // offsets, and all
 };
 VerifyPlan verify_plan(int64_t B, int64_t K, int64_t V, int dtype) {
     VerifyPlan p{};
-    const int64_t ve = dtype == SPARDA_F32 ? 4 : 8, round = kVdThreads * ve, all = V + ve;   // (a row may start inside a piece)
-    p.pieces = 1;
-    while (p.pieces < 8 && (B * (K + 1) * cdiv(all, round * p.pieces) > 2048 || cdiv(all, round * p.pieces) > kVdChunks)) p.pieces *= 2;
-    p.len1 = round * p.pieces;
-    p.chunks1 = static_cast<int>(cdiv(all, p.len1));
-    p.len2 = round;
-    while (cdiv(all, p.len2) > kWave) p.len2 += round;
-    p.chunks2 = static_cast<int>(cdiv(all, p.len2));
+    const int64_t ve = dtype == SPARDA_F32 ? 4 : 8, round = kVdThreads * ve, all = V + ve - 1;   // (a row may start inside a piece)
+    p.exact = B * (K + 1) * V <= (1 << 21);
+    p.rounds1 = 1;
+    while (p.rounds1 < kVdRounds && ((p.rounds1 < 8 && B * (K + 1) * cdiv(all, round * p.rounds1) > 4096) || cdiv(all, round * p.rounds1) > kWave)) p.rounds1 *= 2;
+    p.chunks1 = static_cast<int>(cdiv(all, round * p.rounds1));
+    p.rounds2 = static_cast<int>(cdiv(all, round * kWave));
+    while (p.rounds2 < kVdRounds && B * cdiv(all, round * p.rounds2) > 1024) ++p.rounds2;
+    p.chunks2 = static_cast<int>(cdiv(all, round * p.rounds2));
     p.stats = 0;
     p.sums = p.stats + static_cast<size_t>(B * (K + 1) * p.chunks1) * sizeof(ChunkStat);
     p.state = p.sums + static_cast<size_t>(B * p.chunks2) * sizeof(ChunkSum);
@@ -459,25 +523,33 @@ int launch_verify_drafts(const void* logits, int dtype, int64_t l_sb, int64_t l_
     const VerifyPlan p = verify_plan(B, K, V, dtype);
     char* ws = static_cast<char*>(workspace);
     const Verify a{logits, l_sb, l_st, drafts, d_sb, uniform, u_sb, probs, p_sb, p_st, counts, temperature, all_temperature,
-                   static_cast<int>(K), V, p.len1, p.len2, p.chunks1, p.chunks2,
-                   reinterpret_cast<ChunkStat*>(ws + p.stats), reinterpret_cast<ChunkSum*>(ws + p.sums),
+                   static_cast<int>(K), V, p.rounds1, p.rounds2, p.chunks1, p.chunks2,
+                   reinterpret_cast<ChunkStat*>(ws + p.stats), reinterpret_cast<ChunkSum*>(ws + p.sums), p.exact ? 1 : 0,
                    reinterpret_cast<SequenceState*>(ws + p.state), tokens, accepted};
     if (!grid_fits(static_cast<int64_t>(p.chunks1) * B * (K + 1), kVdThreads) || !grid_fits(static_cast<int64_t>(p.chunks2) * B, kVdThreads))
         return set_error(SPARDA_ERR_SHAPE, "verify_drafts: grid too large");
-    const dim3 grid1(static_cast<unsigned>(p.chunks1), static_cast<unsigned>(B * (K + 1)));
-    const dim3 grid2(static_cast<unsigned>(p.chunks2), static_cast<unsigned>(B)), threads(kVdThreads);
-#define SPARDA_VD(DT_)                                                                                       \
-    do {                                                                                                     \
-        if (p.pieces == 1) hipLaunchKernelGGL((verify_stats_kernel<DT_, 1>), grid1, threads, 0, stream, a);   \
-        else if (p.pieces == 2) hipLaunchKernelGGL((verify_stats_kernel<DT_, 2>), grid1, threads, 0, stream, a); \
-        else if (p.pieces == 4) hipLaunchKernelGGL((verify_stats_kernel<DT_, 4>), grid1, threads, 0, stream, a); \
-        else hipLaunchKernelGGL((verify_stats_kernel<DT_, 8>), grid1, threads, 0, stream, a);                 \
-        hipLaunchKernelGGL((verify_accept_kernel<DT_>), grid2, threads, 0, stream, a);                        \
-        if (probs && K > 0) hipLaunchKernelGGL((verify_residual_kernel<DT_>), grid2, threads, 0, stream, a);  \
+    const dim3 grid1(static_cast<unsigned>(p.chunks1), static_cast<unsigned>(B * (K + 1))), threads(kVdThreads);
+    const dim3 grid2(static_cast<unsigned>(probs || !p.exact ? p.chunks2 : 1), static_cast<unsigned>(B));
+#define SPARDA_VD_R(DT_, R_)                                                                             \
+    do {                                                                                                 \
+        if (p.exact) hipLaunchKernelGGL((verify_stats_kernel<DT_, R_, true>), grid1, threads, 0, stream, a); \
+        else hipLaunchKernelGGL((verify_stats_kernel<DT_, R_, false>), grid1, threads, 0, stream, a);    \
+    } while (0)
+#define SPARDA_VD(DT_)                                                                       \
+    do {                                                                                     \
+        switch (p.rounds1) {                                                                 \
+            case 1: SPARDA_VD_R(DT_, 1); break;                                              \
+            case 2: SPARDA_VD_R(DT_, 2); break;                                              \
+            case 4: SPARDA_VD_R(DT_, 4); break;                                              \
+            case 8: SPARDA_VD_R(DT_, 8); break;                                              \
+            default: SPARDA_VD_R(DT_, 16); break;                                            \
+        }                                                                                    \
+        hipLaunchKernelGGL((verify_draw_kernel<DT_>), grid2, threads, 0, stream, a);         \
     } while (0)
     if (dtype == SPARDA_F32) SPARDA_VD(SPARDA_F32);
     else SPARDA_VD(SPARDA_BF16);
 #undef SPARDA_VD
+#undef SPARDA_VD_R
     return check_hip(hipGetLastError(), "verify_drafts");
 }
 

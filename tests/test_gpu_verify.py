@@ -99,6 +99,36 @@ def test_tokens_and_counts(B, K, V, dtype, sampled):
     same((logits, drafts, uniform), dict(draft_probs=q, temperature=0.0))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("sampled", [False, True], ids=["given", "sampled"])
+@pytest.mark.parametrize("B,K,V", [(11, 4, 50257), (70, 1, 15001), (5, 0, 524289), (2, 1, 1048568)])
+def test_calls_of_more_than_two_million_logits(B, K, V, dtype, sampled):
+    """The statistics are in fp32 there, the drawn row's sums still in fp64."""
+    print(f"[case] verify {B}x{K} of {V} {dtype} sampled={sampled}", flush=True)
+    logits, drafts, uniform, q = inputs(B, K, V, dtype, sampled, seed=B + K)
+    each = torch.tensor([0.8, 1.3, 0.0, 0.25])[torch.arange(B) % 4]
+    same((logits, drafts, uniform), dict(draft_probs=q, temperature=each))
+
+
+@pytest.mark.parametrize("sampled", [False, True], ids=["given", "sampled"])
+def test_masks_in_calls_of_more_than_two_million_logits(sampled):
+    print(f"[case] verify masks, many logits, sampled={sampled}", flush=True)
+    inf, B, K, V = float("inf"), 12, 3, 50003
+    logits, drafts, uniform, q = inputs(B, K, V, F32, sampled, seed=6)
+    logits[0, :, 100:] = -inf
+    logits[1, 0] = -inf
+    logits[2, 0, 7] = float("nan")
+    logits[3, 1, V - 1] = inf
+    logits[4, 0] = torch.finfo(F32).min
+    drafts[6, 0], drafts[7, 0] = V, -1
+    logits[8, :, drafts[8, 0]] = 80.0                             # all of p on one token, and drafts beside it
+    drafts[9, 0] = (int(logits[9, 0].argmin()))
+    uniform[9, 0] = 0.5
+    tokens, n = same((logits, drafts, uniform), dict(draft_probs=q))
+    assert tokens[1, 0] == -1 and tokens[2, 0] == -1 and n[6] == 0 and n[7] == 0
+    same((logits, drafts, uniform), dict(draft_probs=q, temperature=1e-30))
+
+
 def test_every_count_of_accepted_drafts():
     """Drafts that are accepted up to a place and not there, each place of a row of 70 sequences."""
     print("[case] verify every place", flush=True)
