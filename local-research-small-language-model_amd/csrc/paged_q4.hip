@@ -146,25 +146,17 @@ __global__ void __launch_bounds__(256) append_paged_q4_kernel(RotateAppend a, ch
     const bool off_table = ROT && r.pos >= a.rows;
     if (off_table && lane == 0) atomicOr(a.status, static_cast<uint32_t>(SPARDA_STATUS_POSITION_RANGE));
     const bool keep = r.page >= 0 && !off_table;
-    const int c = lane % kPer;
-    float cs[8], sn[8];
     if constexpr (ROT) {
-        load_angles<8>(a, r.pos, c * 8, off_table, cs, sn);
-        for (int h = lane / kPer; h < a.Hq; h += kWave / kPer) {
-            const char* from = static_cast<const char*>(a.q) + (t * a.q_st + h * a.q_sh + c * 8) * kEs;
-            char* to = static_cast<char*>(a.q_out) + (t * a.qo_st + h * a.qo_sh + c * 8) * kEs;
-            float x[8], y[8];
-            q4_load8<DT>(from, x);
-            q4_load8<DT>(from + D / 2 * kEs, y);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) turn(x[e], y[e], cs[e], sn[e]);
-            q4_store8<DT>(to, x);
-            q4_store8<DT>(to + D / 2 * kEs, y);
-        }
+        const char* q = static_cast<const char*>(a.q) + t * a.q_st * kEs;
+        char* qo = static_cast<char*>(a.q_out) + t * a.qo_st * kEs;
+        turn_heads<DT, D>(a, r.pos, off_table, a.Hq, [&](int h) { return q + h * a.q_sh * kEs; }, [&](int h) { return qo + h * a.qo_sh * kEs; });
     }
     if (!keep) return;
     const int key = static_cast<int>(r.row % 16);
     char* tiles = pages + r.page * a.pg.p_st + r.row / 16 * (576 * G);
+    const int c = lane % kPer;
+    float cs[8], sn[8];
+    if constexpr (ROT) load_angles<8>(a, r.pos, c * 8, false, cs, sn);
     for (int h = lane / kPer; h < a.Hkv; h += kWave / kPer) {
         const char* from = static_cast<const char*>(a.k_new) + (t * a.new_st + h * a.new_sh + c * 8) * kEs;
         char* tile = tiles + h * a.pg.h_st;

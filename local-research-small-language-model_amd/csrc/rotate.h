@@ -84,4 +84,37 @@ __device__ __forceinline__ void turn_pieces(uint4& x, uint4& y, const float (&c)
     y = make_uint4(b[0], b[1], b[2], b[3]);
 }
 
+// Rotates `heads` heads of row t: head h from from(h) to to(h), both at its first element. A lane takes 16
+// bytes and the 16 that they are paired with, of four heads at a time; D/2 holds 1 to 16
+// such pieces, so that a lane's piece of the angles is the same for every head and is loaded once.
+template <int DT, int D, class From, class To>
+__device__ __forceinline__ void turn_heads(const RotateAppend& a, int64_t pos, bool off_table, int heads, From from, To to) {
+    constexpr int kEs = DT == SPARDA_F32 ? 4 : 2, kVe = 16 / kEs, kPer = D / 2 / kVe, kAtOnce = kWave / kPer, kBatch = 4;
+    const int lane = threadIdx.x % kWave, c = lane % kPer;
+    float cs[kVe], sn[kVe];
+    load_angles<kVe>(a, pos, c * kVe, off_table, cs, sn);
+    for (int h0 = lane / kPer; h0 < heads; h0 += kBatch * kAtOnce) {
+        uint4 x[kBatch], y[kBatch];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+            const int h = h0 + e * kAtOnce;
+            if (h < heads) {
+                const char* p = from(h) + c * 16;
+                x[e] = *reinterpret_cast<const uint4*>(p);
+                y[e] = *reinterpret_cast<const uint4*>(p + D / 2 * kEs);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+            const int h = h0 + e * kAtOnce;
+            if (h < heads) {
+                char* p = to(h) + c * 16;
+                turn_pieces<DT>(x[e], y[e], cs, sn);
+                *reinterpret_cast<uint4*>(p) = x[e];
+                *reinterpret_cast<uint4*>(p + D / 2 * kEs) = y[e];
+            }
+        }
+    }
+}
+
 }  // namespace sparda
