@@ -163,6 +163,24 @@ __device__ __forceinline__ double lane_f64(double v, int lane) {
     const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(u >> 32), lane);
     return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
+// over the 16 lanes of a row, the result in every one
+__device__ __forceinline__ float row16_max(float v) {
+    v = fmaxf(v, dpp_f32<kDppXor1>(v));
+    v = fmaxf(v, dpp_f32<kDppXor2>(v));
+    v = fmaxf(v, dpp_f32<kDppHalfMirror>(v));
+    return fmaxf(v, dpp_f32<kDppMirror>(v));
+}
+__device__ __forceinline__ double row16_sum_f64(double v) {
+    v += dpp_f64<kDppXor1, 0xf>(v);
+    v += dpp_f64<kDppXor2, 0xf>(v);
+    v += dpp_f64<kDppHalfMirror, 0xf>(v);
+    return v + dpp_f64<kDppMirror, 0xf>(v);
+}
+__device__ __forceinline__ int row16_min(int v) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 16));
+    return v;
+}
 __device__ __forceinline__ double wave_sum_f64(double v) { return lane_f64(wave_scan_f64(v), kWave - 1); }
 
 }  // namespace
@@ -347,7 +365,7 @@ __device__ __forceinline__ int vd_draw(const VdRow& r, double of_lane, int round
     const int at_part = pass != 0 && here != 0 ? __builtin_ctzll(here) : 63 - __builtin_clzll(any | 1);
     if (wave == at_part % kVdWaves) {             // the wavefront whose pieces they are
         const int64_t at = first + (tid + at_part / kVdWaves * kVdThreads) * kVe;
-        vd_weights<DT>(r, at, V, w);
+        if (at_part / kVdWaves != rounds - 1) vd_weights<DT>(r, at, V, w);   // (the last round's are there)
         double mine = 0.0;
 #pragma unroll
         for (int e = 0; e < kVe; ++e) mine += w[e];
@@ -402,7 +420,7 @@ __global__ void __launch_bounds__(kVdThreads, 4) verify_draw_kernel(Verify a) {
     __shared__ double red[kVdRounds * kVdWaves], rz[kVdRows];   // (red: a number a round and wavefront, three a wavefront)
     __shared__ float rmax[kVdRows];
     __shared__ int rarg[kVdRows], ok[kVdRows], found, flag;
-    const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, chunk = blockIdx.x, b = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid % kWave, chunk = blockIdx.x, b = blockIdx.y;
     const int count = vd_count(a, b);
     const float T = vd_temperature(a, b);
     const bool greedy = !(T > 0.0f);
@@ -412,13 +430,18 @@ __global__ void __launch_bounds__(kVdThreads, 4) verify_draw_kernel(Verify a) {
     auto in_row = [&](const ChunkStat& s, float m) {
         return s.m == -__builtin_inff() ? s.sum : s.sum * vd_weight((static_cast<double>(s.m) - m) * c);
     };
-    for (int i = wave; i <= count; i += kVdWaves) {           // a wavefront a row
-        ChunkStat own{-__builtin_inff(), 0x7fffffff, 0.0};
-        if (lane < a.chunks1) own = stats[i * a.chunks1 + lane];
-        // (the draft's own numbers under the chunks')
+    for (int i = tid / 16; i <= a.K; i += kVdThreads / 16) {  // 16 lanes a row
+        const int l16 = tid % 16;
+        ChunkStat own[4];                                     // chunks l16, l16 + 16 ..
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            own[j] = ChunkStat{-__builtin_inff(), 0x7fffffff, 0.0};
+            if (l16 + 16 * j < a.chunks1) own[j] = stats[i * a.chunks1 + l16 + 16 * j];
+        }
+        // (the draft's own numbers under the chunks'; of a row behind the last draft nothing is used)
         int d = -1;
         float x = -__builtin_inff(), u = 0.0f, q = 1.0f;
-        if (i < count) {
+        if (i < a.K) {
             d = a.drafts[b * a.d_sb + i];
             u = a.uniform[b * a.u_sb + i];
             if (d >= 0 && d < a.V) {
@@ -426,15 +449,22 @@ __global__ void __launch_bounds__(kVdThreads, 4) verify_draw_kernel(Verify a) {
                 if (a.probs) q = a.probs[b * a.p_sb + i * a.p_st + d];
             }
         }
-        const float m = wave_max(own.m);
+        const float m = row16_max(fmaxf(fmaxf(own[0].m, own[1].m), fmaxf(own[2].m, own[3].m)));
         const bool finite = m > -__builtin_inff() && m < __builtin_inff();
-        const double z = wave_sum_f64(finite ? in_row(own, m) : 0.0);
-        const int arg = greedy ? wave_min_i32(own.m == m ? own.arg : 0x7fffffff) : 0;
-        if (lane == 0) {
+        double z = 0.0;
+        int arg = 0x7fffffff;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (16 * j < a.chunks1) z += finite ? in_row(own[j], m) : 0.0;
+            arg = own[j].m == m ? min(arg, own[j].arg) : arg;
+        }
+        z = row16_sum_f64(z);
+        if (greedy) arg = row16_min(arg);
+        if (l16 == 0) {
             const bool valid = finite && z < __builtin_inf();
             const bool inside = d >= 0 && d < a.V;
             const double p = valid && inside ? vd_weight((static_cast<double>(x) - m) * c) : 0.0;
-            rmax[i] = m, rz[i] = z, rarg[i] = valid ? arg : -1;
+            rmax[i] = m, rz[i] = z, rarg[i] = valid ? (greedy ? arg : 0) : -1;
             ok[i] = valid && inside && (greedy ? d == arg : static_cast<double>(u) * q < p / z) ? 1 : 0;
         }
     }
@@ -503,7 +533,7 @@ VerifyPlan verify_plan(int64_t B, int64_t K, int64_t V, int dtype) {
     while (p.rounds1 < kVdRounds && ((p.rounds1 < 8 && B * (K + 1) * cdiv(all, round * p.rounds1) > 4096) || cdiv(all, round * p.rounds1) > kWave)) p.rounds1 *= 2;
     p.chunks1 = static_cast<int>(cdiv(all, round * p.rounds1));
     p.rounds2 = static_cast<int>(cdiv(all, round * kWave));
-    while (p.rounds2 < kVdRounds && B * cdiv(all, round * p.rounds2) > 1024) ++p.rounds2;
+    while (p.rounds2 < kVdRounds && B * cdiv(all, round * p.rounds2) > 2048) ++p.rounds2;
     p.chunks2 = static_cast<int>(cdiv(all, round * p.rounds2));
     p.stats = 0;
     p.sums = p.stats + static_cast<size_t>(B * (K + 1) * p.chunks1) * sizeof(ChunkStat);
