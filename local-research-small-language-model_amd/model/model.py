@@ -109,12 +109,19 @@ class SparDAResearchModel(nn.Module):
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int = 50, temperature: float = 0.8,
                  top_k: int = 50, eos_token_id: Optional[int] = None,
-                 kv_caches: Optional[List] = None) -> torch.Tensor:
+                 kv_caches: Optional[List] = None, draft_model: Optional["SparDAResearchModel"] = None,
+                 num_drafts: int = 4) -> torch.Tensor:
         """Sampling loop (model/model.py:159-195). With ``kv_caches`` (one per
         layer, empty) the prompt is prefilled once and each new token runs one
         cached decode step; without, every step re-runs the full forward as
-        the reference does."""
+        the reference does. With ``draft_model`` (a smaller model of the same
+        vocabulary; one sequence, no caches) it drafts ``num_drafts`` tokens, one forward of this
+        model scores them all, and ``sparda.verify_drafts`` keeps those that this model's
+        distribution accepts and draws the next, as if every token had been drawn from it."""
         self.eval()
+        if draft_model is not None:
+            return self._generate_drafted(input_ids, max_new_tokens, temperature, top_k, eos_token_id, kv_caches,
+                                          draft_model.eval(), num_drafts)
         if kv_caches is not None:
             logits = self.forward(input_ids, kv_caches=kv_caches)["logits"][:, -1, :]
         for step in range(max_new_tokens):
@@ -135,4 +142,46 @@ class SparDAResearchModel(nn.Module):
                 break
             if kv_caches is not None and step + 1 < max_new_tokens:
                 logits = self.forward(nxt, kv_caches=kv_caches)["logits"][:, -1, :]
+        return input_ids
+
+    def _generate_drafted(self, input_ids, max_new_tokens, temperature, top_k, eos_token_id, kv_caches, draft_model,
+                          num_drafts) -> torch.Tensor:
+        if input_ids.shape[0] != 1 or kv_caches is not None:
+            raise ValueError("drafted generation takes one sequence, without caches")
+        if draft_model.config.vocab_size != self.config.vocab_size:
+            raise ValueError(f"the draft model's vocabulary has {draft_model.config.vocab_size} tokens, this one's "
+                             f"{self.config.vocab_size}")
+        if not 0 <= num_drafts <= 64:
+            raise ValueError(f"num_drafts must be in [0, 64], got {num_drafts}")
+
+        def logits(model, ids, n):
+            return model(ids[:, -model.config.context_length:])["logits"][:, -n:].float()
+
+        def kept(x):
+            if top_k is None or top_k <= 0 or temperature <= 0.0:
+                return x
+            v, _ = torch.topk(x, min(top_k, x.size(-1)))
+            return x.masked_fill(x < v[..., [-1]], -float("inf"))
+
+        end = input_ids.shape[1] + max_new_tokens
+        while input_ids.shape[1] < end:
+            K = min(num_drafts, end - input_ids.shape[1] - 1, self.config.context_length - 1)
+            ids, probs = input_ids, []
+            for _ in range(K):
+                x = kept(logits(draft_model, ids, 1))[:, 0]
+                if temperature > 0.0:
+                    probs.append(F.softmax(x / temperature, dim=-1))
+                    nxt = torch.multinomial(probs[-1], num_samples=1)
+                else:
+                    nxt = torch.argmax(x, dim=-1, keepdim=True)
+                ids = torch.cat((ids, nxt), dim=1)
+            tokens, n = sparda.verify_drafts(kept(logits(self, ids, K + 1)), ids[:, input_ids.shape[1]:].int(),
+                                             torch.rand(1, K + 1, device=ids.device),
+                                             draft_probs=torch.stack(probs, 1) if probs else None,
+                                             temperature=max(float(temperature), 0.0))
+            new = tokens[:, :int(n) + 1].long()
+            if eos_token_id is not None and (new == eos_token_id).any():
+                stop = int((new[0] == eos_token_id).nonzero()[0])
+                return torch.cat((input_ids, new[:, :stop + 1]), dim=1)
+            input_ids = torch.cat((input_ids, new), dim=1)
         return input_ids
