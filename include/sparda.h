@@ -1030,7 +1030,7 @@ SPARDA_API size_t sparda_verify_drafts_workspace_bytes(int64_t B, int64_t K, int
  * passes uniform[b,K] times its total, r = max(p_n - q_n, 0) after a rejection (p_n where that is
  * zero everywhere), r = p_n behind the last draft; sums that decide the token in fp64. A
  * temperature that is not above 0: draft i is accepted if it is the lowest index of
- * row i's largest logit, and the token is that of row n. A row without a distribution (no logit above
+ * row i's largest logit, and the token is that of row n; +inf counts as 3.4e38. A row without a distribution (no logit above
  * -inf, or NaN or +inf among them) accepts nothing and gives token -1; so does a
  * draft outside [0, V) accept nothing.
  *   logits: [B,K+1,V] of dtype, strides (l_sb, l_st, 1); drafts: [B,K] int32, stride d_sb; uniform: fp32

@@ -461,7 +461,7 @@ decode_paged_q4_kernel(PagedDecode a) {
         for (int t = 0; t < 2; ++t) {
             int id = at.id[t];
             if (id < 0 || id >= a.pg.n_pages) bad = true, id = 0;
-            base[t] = kv + id * a.pg.p_st + at.tile[t] * (576 * G);
+            base[t] = kv + id * a.pg.p_st + static_cast<int64_t>(at.tile[t]) * (576 * G);
         }
     };
     // (keys: position c16, quarter grp; values: four grp, pair c16)

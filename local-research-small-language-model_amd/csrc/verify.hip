@@ -71,13 +71,14 @@ __device__ __forceinline__ int vd_count(const Verify& a, int b) {
     return n < 0 ? 0 : n > a.K ? a.K : n;
 }
 __device__ __forceinline__ float vd_temperature(const Verify& a, int b) {
-    return a.temperature != nullptr ? a.temperature[b] : a.all_temperature;
+    const float T = a.temperature != nullptr ? a.temperature[b] : a.all_temperature;
+    return T > 3.4e38f ? 3.4e38f : T;             // (inf: -inf logits keep their weight of 0)
 }
 
 // 2^t for -1020 <= t <= 0: t = n + f, |f| <= 1/2, and the Taylor series of 2^f up to f^10, whose
 // rest is below 3 10^-13. n is rounded by the addition of 1.5 2^52, whose low word then holds it, and goes
 // into the exponent as an integer (the conversions and the scaling of fp64 run at a
-// quarter of the rate: 50257 x 512 logits 31.5 us with them, @@ without).
+// quarter of the rate: 50257 x 512 logits 31.5 us with them, 28 without).
 __device__ __forceinline__ double vd_exp2(double t) {
     constexpr double kShift = 6755399441055744.0;
     const double y = t + kShift, f = t - (y - kShift);
@@ -480,7 +481,7 @@ __global__ void __launch_bounds__(kVdThreads, 4) verify_draw_kernel(Verify a) {
         if (chunk == 0) write(rarg[n]);
         return;
     }
-    const float u = a.uniform[b * a.u_sb + a.K];
+    const float u01 = a.uniform[b * a.u_sb + a.K], u = u01 < 0.0f ? 0.0f : u01;
     VdRow r{};
     r.row = static_cast<const char*>(a.logits) + (b * a.l_sb + n * a.l_st) * kEs;
     r.c = c, r.m = rmax[n], r.inv_total = 1.0 / rz[n], r.without = -1;

@@ -312,6 +312,33 @@ def test_pages_past_32_bit_offsets():
     assert sparda.status() == 0
 
 
+def test_a_page_of_more_than_two_gibibytes():
+    """Offsets inside one page pass 32 bits: rows before and behind that place are written, read and attended to."""
+    print("[case] q4 page of 2.1 GB", flush=True)
+    D, ps = 128, 16 * 932_300                                     # 932068 tiles of 2304 bytes are 2^31
+    pages = torch.zeros(sparda.q4_page_shape(1, ps, 1, D), dtype=torch.uint8, device=DEV)
+    table, n = dev([[0]]), 40
+    at = [5, 16 * 932_060, ps - n]
+    k, v = randn(n, 1, D, dtype=BF, seed=1), randn(n, 1, D, dtype=BF, seed=2)
+    for p in at:
+        sparda.append_paged_q4(pages, table, dev([p]), dev(k), dev(v), dev([0, n]))
+    kh, vh = held(np32(k)), held(np32(v))
+    for p in at:
+        got = sparda.gather_paged_q4(pages, table, dev([p]), n, dev([0, n]), dtype=F32)
+        assert np.array_equal(got[0].cpu().numpy(), kh.astype(np.float32)) and np.array_equal(got[1].cpu().numpy(), vh.astype(np.float32))
+    # (the other rows are zeros: a score of 0 each and no value)
+    q = (dev(k[:2]) * 3).view(1, 2, D)
+    for length in (ps, ps - n // 2, 16 * 932_060 + n):
+        out = sparda.decode_paged_q4(q, pages, table, dev([length]))[0].view(2, D).cpu().double().numpy()
+        rows = [r for p in at for r in range(n) if p + r < length]
+        s = np32(q.cpu()).astype(np.float64)[0] @ kh[rows, 0].T / D ** 0.5
+        w = np.exp(s - s.max(-1, keepdims=True))
+        rest = (length - len(rows)) * np.exp(-s.max(-1, keepdims=True))
+        want = w @ vh[rows, 0] / (w.sum(-1, keepdims=True) + rest)
+        # (outputs are of the size of 1: the weights' and the result's rounding to bf16, 2^-8 each of a sum's terms)
+        assert np.abs(out - want).max() <= 2 * 2.0 ** -8 * np.abs(vh).max() and np.abs(want).max() > 0.5
+
+
 def test_refusals_of_tensors_that_do_not_fit():
     print("[case] q4 refusals", flush=True)
     q, kn = randn(3, 4, 64, dtype=BF, seed=1).to(DEV), randn(3, 2, 64, dtype=BF, seed=2).to(DEV)

@@ -270,6 +270,25 @@ def test_captured_and_replayed():
         assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
 
 
+@pytest.mark.parametrize("B,V", [(4, 700), (60, 50257)])
+def test_an_infinite_temperature_and_numbers_below_zero(B, V):
+    """All tokens with a logit are alike at a temperature of +inf, one with -inf keeps its weight of zero; a number
+    below zero draws as zero does."""
+    print(f"[case] verify infinite temperature {B} of {V}", flush=True)
+    logits, drafts, uniform, q = inputs(B, 1, V, F32, True, seed=12)
+    logits[:, :, ::3] = -float("inf")
+    drafts[1, 0] = 3
+    call = lambda T, u: [t.cpu() for t in sparda.verify_drafts(logits.to(DEV), drafts.to(DEV), u.to(DEV), draft_probs=q.to(DEV),
+                                                               temperature=torch.full((B,), T, device=DEV))]
+    want = oracle(logits, drafts, uniform, q, temperature=3.4e38)
+    got = call(float("inf"), uniform)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and (got[0][:, 0] >= 0).all()
+    uniform[:, 1] = 0.0
+    want = call(0.9, uniform)
+    uniform[:, 1] = -0.5
+    assert all(torch.equal(a, b) for a, b in zip(call(0.9, uniform), want))
+
+
 def test_refusals():
     print("[case] verify refusals", flush=True)
     logits, drafts, uniform, q = (t.to(DEV) for t in inputs(3, 2, 100, BF, True, seed=1))
