@@ -134,7 +134,11 @@ __device__ __forceinline__ uint32_t q4_key_pack(const uint32_t (&c)[8]) {
 // ---------------------------------------------------------------------------
 
 // One wavefront per new row. A lane takes eight dims and the eight that they are paired
-// with; the largest magnitude of a group comes from up to four neighbouring lanes.
+// with; the largest magnitude of a group comes from up to four neighbouring lanes. The queries are rotated
+// as for 16-bit pages, four heads at a time. Bound by memory: 16000 rows of 32/8 heads of 128 (196.6 MB read,
+// 149.4 written) take 75-79 us = 4.4-4.6 TB/s where a large copy reaches 5.1; the rest is the values' bytes, of
+// which a row holds every fourth of a word (counted: 171 MB written, 210 read). 64 rows of 12/4 heads of
+// 64 take 5.3 us, a chain of five dependent loads. Neighbouring rows on one XCD: 77.5 against 78.2 us, not taken.
 template <int DT, int D, bool ROT>
 __global__ void __launch_bounds__(256) append_paged_q4_kernel(RotateAppend a, char* __restrict__ pages) {
     constexpr int G = q4_groups(D), kEs = DT == SPARDA_F32 ? 4 : 2, kPer = D / 16;
@@ -198,7 +202,9 @@ __global__ void __launch_bounds__(256) append_paged_q4_kernel(RotateAppend a, ch
 // gather
 // ---------------------------------------------------------------------------
 
-// One wavefront per row, eight dims a lane: the values that the codes stand for.
+// One wavefront per row, eight dims a lane: the values that the codes stand for. Bound by memory: 17486
+// rows of 8 heads of 128 (20.1 MB of codes, 71.6 written) take 21.8-23.1 us = 4.0-4.2 TB/s; the codes of a row
+// lie in a third of a tile's lines, and other rows read the same lines again (counted: 37 MB read).
 template <int DT, int D>
 __global__ void __launch_bounds__(256)
 gather_paged_q4_kernel(RotateAppend a, const char* __restrict__ pages, char* __restrict__ k, char* __restrict__ v) {
@@ -383,7 +389,18 @@ struct Q4Place {
 // len - T + 1 + t. The numbers h stay outside of the products with the codes:
 //     S^T[key, col] = 2 sum_g h_g[key] sum_{d in g} ((16.5 + c) - 24) q[d]
 //     O^T[d, col]  += 2 sum_key ((16.5 + c) - 24) P_g[key, col],  P_g = exp2(S - m) h_g[key] in bf16
-// so that the levels, odd multiples of h, enter without rounding.
+// so that the levels, odd multiples of h, enter without rounding. The rounding of P_g, half a step of 2^-8 as that
+// of the weights over 16-bit pages, keeps the product on the bf16 matrix cores; fp32 calls take P_g and q in three
+// bf16 terms each.
+//
+// A lane's keys of a step (positions 4 grp .. 4 grp + 3 of two tiles) are the same in S^T's rows and in
+// the operand that P^T becomes, so P never leaves its lanes, and the order of the codes in memory is that
+// of the operands: no LDS but for the join of the wavefronts. What a step spends is vector issue, about 300
+// instructions of 32 keys with D = 128: 60 unpack, 130 apply h to scores and weights, the rest is softmax and
+// addresses. 32 sequences of up to 16384, 32/8 heads of 128 (401 MB): 83 us = 4.8 TB/s, with loads alone
+// 74.5 and with arithmetic alone 72.9; 8 x 16384, 12/4 heads of 64 (29 MB): 12.3; 16 x 5 tokens at up
+// to 8000, 32/8 of 128: 34.9, arithmetic alone 35.8; 1 x 1000: 4.9, a launch and four dependent loads. The steps
+// staged through LDS one or two ahead took 97 and 105 us where this took 95; four wavefronts a SIMD 96.
 template <int DT, int D, int KW, int NC>
 __global__ void __launch_bounds__(KW* kWave, (D == 128 ? 3 : 4) - (DT == SPARDA_F32 ? 1 : 0) - (NC > 1 ? 1 : 0))
 decode_paged_q4_kernel(PagedDecode a) {
@@ -657,6 +674,17 @@ decode_paged_q4_kernel(PagedDecode a) {
 
 namespace {
 
+// How the work is cut, and what was measured on either side of each rule:
+// - Two tiles of 16 columns share the unpacked codes where there are more than 16 columns and the products
+//   are single: 16 x 5 tokens of 32/8 heads of 128 at 8000 (20 columns) 41 us, 47 with a tile a workgroup. In
+//   fp32 the terms of two tiles do not fit the registers.
+// - A sequence is one item, with no join, up to 16 steps of 32 keys, or up to 64 where the sequences fill
+//   half of the chip by themselves; otherwise there are as many items as workgroups run at a time (256 CUs
+//   times the wavefronts that a SIMD holds), and B / 2 fewer asked for, since a sequence's last share is half
+//   empty in the mean: all shares are then done in one round. 32 x 16384 of 32/8 heads of 128 (slots 96 a
+//   KV head): 64 / 80 / 96 / 128 items 101.5 / 89.1 / 104.4 / 99.9 us; 8 x 16384 of 12/4 of 64 (256): 100 /
+//   256 / 312 items 16.4 / 15.9 / 18.1; 16 x 5 tokens (64): 32 / 48 / 56 / 64 items 54.7 / 42.9 / 41.1 / 53.1.
+// - A share is four steps at least, one for each wavefront.
 struct Q4Plan {
     int nc;                  // column tiles of a workgroup
     int64_t target, least;   // items aimed at, steps of the smallest item

@@ -187,7 +187,9 @@ __device__ __forceinline__ double wave_sum_f64(double v) { return lane_f64(wave_
 }  // namespace
 
 // Maximum and sum of a chunk of a row, in one read: the chunk's pieces stay in registers. Every
-// wavefront measures its exponentials against its own maximum, so that the wavefronts meet once.
+// wavefront measures its exponentials against its own maximum, so that the wavefronts meet once. Bound by memory in
+// large calls: 64 x 8 rows of 50257 in bf16 (51.5 MB) take 13.3 us = 3.9 TB/s, 32 x 6 of 32000 in fp32
+// (24.6 MB) 7.2-8.9; 5 rows of 32000 take 4.0, a launch, a load and a reduction.
 template <int DT, int ROUNDS, bool EXACT>
 __global__ void __launch_bounds__(kVdThreads) verify_stats_kernel(Verify a) {
     constexpr int kVe = VdType<DT>::kVe, kEs = VdType<DT>::kEs;
@@ -415,6 +417,11 @@ __device__ __forceinline__ bool vd_last(ChunkSum* to, const ChunkSum& s, uint32_
 }  // namespace
 
 // One workgroup per (chunk, sequence), or per sequence where all sums are there and no distributions are given.
+// Bound by its chain: the statistics, the row (a load that waits for what was accepted), a reduction,
+// the sums' way through memory, the last workgroup's loads of them and of its chunk again. 64 rows of 50257 with
+// q (19 MB) 15.2 us, of which the last workgroups' draw is 2.2 and the exponentials in fp64 1.7 (measured
+// without each); 32 of 32000 11.7; one sequence 6.0. Drafts' logits and q fetched by the first launch instead of
+// here: no difference in a call (28.5 / 28.3, 20.1 / 20.1 us).
 template <int DT>
 __global__ void __launch_bounds__(kVdThreads, 4) verify_draw_kernel(Verify a) {
     constexpr int kEs = VdType<DT>::kEs;
@@ -521,6 +528,14 @@ __global__ void __launch_bounds__(kVdThreads, 4) verify_draw_kernel(Verify a) {
 
 namespace {
 
+// Sizes, with what was measured on either side (us a call):
+// - fp64 statistics up to 2^21 logits, where the launch and the loads hide them (5 x 32000: 10.1 either way) and
+//   a token from p needs no second pass; beyond, 64 x 8 x 50257 31.5 with them, 28.3 without.
+// - The first launch's chunks grow from one round (256 pieces of 16 bytes) to eight while there are more than
+//   4096 of them: two / four / eight rounds at 64 x 8 x 50257 32.3 / 31.4 / 34.5 (then; four is the rule's).
+// - The second launch's grow while there are more than 2048: limits of 256 / 512 / 1024 / 2048 / 4096 at 64 x
+//   50257 38.0 / 32.8 / 29.8 / 28.4 / 28.4, at 32 x 32000 in fp32 21.0 / 19.2 / 20.0 / 20.4 / 20.0.
+// - A row has at most 64 chunks, a lane each.
 struct VerifyPlan {
     bool exact;
     int rounds1, rounds2, chunks1, chunks2;
