@@ -297,17 +297,15 @@ namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-template <int N>
+// N words of codes; STREAM: read once, not to stay in the caches
+template <int N, bool STREAM>
 __device__ __forceinline__ void q4_load_words(const char* p, uint32_t (&w)[N]) {
-    if constexpr (N == 4) {
-        const uint4 x = *reinterpret_cast<const uint4*>(p);
-        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-    } else if constexpr (N == 2) {
-        const uint2 x = *reinterpret_cast<const uint2*>(p);
-        w[0] = x.x, w[1] = x.y;
-    } else {
-        w[0] = *reinterpret_cast<const uint32_t*>(p);
-    }
+    typedef uint32_t words __attribute__((ext_vector_type(N)));
+    words x;
+    if constexpr (STREAM) x = __builtin_nontemporal_load(reinterpret_cast<const words*>(p));
+    else x = *reinterpret_cast<const words*>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = x[i];
 }
 // four positions' numbers, [4][G]
 template <int G>
@@ -377,10 +375,35 @@ __device__ __forceinline__ void q4_split(const float (&x)[8], bf16x8 (&out)[TERM
     }
 }
 
+// a lane permutation without lanes outside (bound_ctrl, so that it is taken into the operation that uses it)
+template <int CTRL>
+__device__ __forceinline__ float q4_dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+// x times lane E of the quad's h
+template <int E>
+__device__ __forceinline__ float q4_by_quad(float x, float h) {
+    return x * q4_dpp<E * 0x55>(h);
+}
+// sums over the lanes 16 / G apart in a row of 16, in an order and with roundings (no fused multiply-add)
+// that make them equal in all of those
+template <int G>
+__device__ __forceinline__ float q4_group_sum(float v) {
+#pragma clang fp contract(off)
+    if constexpr (G >= 2) v = v + q4_dpp<0x128>(v);   // row_ror:8
+    if constexpr (G >= 4) v = v + q4_dpp<0x124>(v);   // row_ror:4
+    return v;
+}
+
 // pages and tiles of the two tiles of a step
 struct Q4Place {
     int id[2], tile[2];
 };
+
+// wavefronts of a SIMD
+constexpr int q4_waves(int DT, int D, int NC, bool REP) {
+    return (D == 128 && !REP ? 3 : 4) - (DT == SPARDA_F32 ? 1 : 0) - (NC > 1 ? 1 : 0);
+}
 
 }  // namespace
 
@@ -395,16 +418,26 @@ struct Q4Place {
 //
 // A lane's keys of a step (positions 4 grp .. 4 grp + 3 of two tiles) are the same in S^T's rows and in
 // the operand that P^T becomes, so P never leaves its lanes, and the order of the codes in memory is that
-// of the operands: no LDS but for the join of the wavefronts. What a step spends is vector issue, about 300
-// instructions of 32 keys with D = 128: 60 unpack, 130 apply h to scores and weights, the rest is softmax and
-// addresses. 32 sequences of up to 16384, 32/8 heads of 128 (401 MB): 83 us = 4.8 TB/s, with loads alone
-// 74.5 and with arithmetic alone 72.9; 8 x 16384, 12/4 heads of 64 (29 MB): 12.3; 16 x 5 tokens at up
-// to 8000, 32/8 of 128: 34.9, arithmetic alone 35.8; 1 x 1000: 4.9, a launch and four dependent loads. The steps
-// staged through LDS one or two ahead took 97 and 105 us where this took 95; four wavefronts a SIMD 96.
-template <int DT, int D, int KW, int NC>
-__global__ void __launch_bounds__(KW* kWave, (D == 128 ? 3 : 4) - (DT == SPARDA_F32 ? 1 : 0) - (NC > 1 ? 1 : 0))
+// of the operands: no LDS but for the join of the wavefronts.
+//
+// Where the columns fit 16 / G of a tile's 16 (REP), every column stands in it once for each of its G groups: column
+// h + kCols g takes the scores of group g alone (Q's operand is zero elsewhere) and carries the weights of
+// group g alone. The products of all groups then go into one accumulator, which starts at the
+// middle's share of the column (a constant), h is one number a lane and key, and the groups' sums are added
+// across lanes: 16 products a step of 32 keys instead of 32, and 210 vector instructions instead of 307 (D =
+// 128). Unpacking is 128 of them.
+//
+// 32 sequences of up to 16384, 32/8 heads of 128 (401 MB): 74.7 us a call = 5.4 TB/s; without REP and STREAM
+// 87.6, with REP 84.2. Loads alone took 74.5, arithmetic alone 72.9 without REP. 8 x 16384, 12/4 heads of 64 (29
+// MB): 12.3 of 15.5 us a call, a chain of three steps' reads under load; 16 x 5 tokens at up to 8000, 32/8 of
+// 128 (20 columns in two tiles): 35.5 of 41, where arithmetic alone is 35.8; 1 x 1000: 4.9 of 8, a launch and
+// four dependent loads. Steps staged through LDS one or two ahead took 97 and 105 us where this took 95.
+template <int DT, int D, int KW, int NC, bool REP, bool STREAM>
+__global__ void __launch_bounds__(KW* kWave, q4_waves(DT, D, NC, REP))
 decode_paged_q4_kernel(PagedDecode a) {
     constexpr int G = q4_groups(D), kTerms = DT == SPARDA_F32 ? 3 : 1, kStep = 32, kEs = DT == SPARDA_F32 ? 4 : 2;
+    constexpr int kCols = REP ? 16 / G : 16;                 // columns of a tile
+    static_assert(!REP || (NC == 1 && G > 1), "one tile, of several groups");
     extern __shared__ float lds[];
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
@@ -426,18 +459,23 @@ decode_paged_q4_kernel(PagedDecode a) {
     const int s_end = min(steps, (sh.part + 1) * sh.share);
     bool bad = sh.bad;
 
-    // this lane's columns of Q
+    bf16x8 middle;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) middle[e] = static_cast<__bf16>(-24.0f);
+    // this lane's columns of Q (REP: column h of group g in lane h + kCols g, in the product with that group's codes alone)
+    const int mine = c16 / kCols;
     int lim[NC];                                             // positions a column sees
     bf16x8 qr[NC][G][kTerms];
+    f32x4 start{0.f, 0.f, 0.f, 0.f};                         // REP: -24 times the sum of the column's q in its group
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const int at = 16 * c + c16, col = col0 + (at < ncol ? at : ncol - 1), tok = col / a.R, head = g * a.R + col % a.R;
+        const int at = 16 * c + c16 % kCols, col = col0 + (at < ncol ? at : ncol - 1), tok = col / a.R, head = g * a.R + col % a.R;
         lim[c] = len - a.T + 1 + tok;
         const char* q = static_cast<const char*>(a.q) + (b * a.q_sb + tok * a.q_st + head * a.q_sh) * kEs;
 #pragma unroll
         for (int i = 0; i < G; ++i) {
             float x[8];
-            if (at < ncol && 32 * i + 8 * grp < D) {
+            if (at < ncol && 32 * i + 8 * grp < D && (!REP || mine == i)) {
                 q4_load8<DT>(q + (32 * i + 8 * grp) * kEs, x);
                 if (a.negate) {
 #pragma unroll
@@ -448,6 +486,10 @@ decode_paged_q4_kernel(PagedDecode a) {
                 for (int e = 0; e < 8; ++e) x[e] = 0.0f;
             }
             q4_split<kTerms>(x, qr[c][i]);
+            if constexpr (REP) {
+#pragma unroll
+                for (int n = 0; n < kTerms; ++n) start = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, qr[c][i][n], start, 0, 0, 0);
+            }
         }
     }
 
@@ -456,7 +498,8 @@ decode_paged_q4_kernel(PagedDecode a) {
     const auto* row = (const __attribute__((address_space(4))) int32_t*)(a.pg.table + b * a.pg.t_st);
     const char* kv = static_cast<const char*>(a.k) + g * a.pg.h_st;
     const int last_tile = (len - 1) / 16;
-    const int o_keys = (c16 * 4 + grp) * 4 * G, o_values = 256 * G + lane * 4 * G, o_scales = 512 * G + grp * 8 * G;
+    const int o_keys = (c16 * 4 + grp) * 4 * G, o_values = 256 * G + lane * 4 * G;
+    const int o_scales = 512 * G + grp * 8 * G + (REP ? (c16 % 4 * G + mine) * 2 : 0);
     int u = sh.part * sh.share + wave;
     int page = 2 * u / a.ps16, rem = 2 * u % a.ps16;
     const int adv_p = 2 * KW / a.ps16, adv_r = 2 * KW % a.ps16;
@@ -471,7 +514,7 @@ decode_paged_q4_kernel(PagedDecode a) {
         return at;
     };
     uint32_t xk[2][G], xv[2][G];                             // the codes of a step, as loaded
-    _Float16 hk[2][4][G], hv[2][4][G];
+    _Float16 hk[2][REP ? 1 : 4][REP ? 1 : G], hv[2][REP ? 1 : 4][REP ? 1 : G];   // REP: position 4 grp + c16 % 4 and the lane's group
     const char* base[2];
     auto locate = [&](const Q4Place& at) __attribute__((always_inline)) {
 #pragma unroll
@@ -484,31 +527,51 @@ decode_paged_q4_kernel(PagedDecode a) {
     // (keys: position c16, quarter grp; values: four grp, pair c16)
     auto load_keys = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) q4_load_words<G>(base[t] + o_keys, xk[t]), q4_load_scales<G>(base[t] + o_scales, hk[t]);
+        for (int t = 0; t < 2; ++t) {
+            q4_load_words<G, STREAM>(base[t] + o_keys, xk[t]);
+            if constexpr (REP) hk[t][0][0] = *reinterpret_cast<const _Float16*>(base[t] + o_scales);
+            else q4_load_scales<G>(base[t] + o_scales, hk[t]);
+        }
     };
     auto load_values = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) q4_load_words<G>(base[t] + o_values, xv[t]), q4_load_scales<G>(base[t] + o_scales + 32 * G, hv[t]);
+        for (int t = 0; t < 2; ++t) {
+            q4_load_words<G, STREAM>(base[t] + o_values, xv[t]);
+            if constexpr (REP) hv[t][0][0] = *reinterpret_cast<const _Float16*>(base[t] + o_scales + 32 * G);
+            else q4_load_scales<G>(base[t] + o_scales + 32 * G, hv[t]);
+        }
     };
 
     // m: the columns' references, in the scores' own units, l: this lane's part of their sums
     float m[NC], ref[NC], l[NC];
     const float slack = 16.0f / a.scale_log2;
-    f32x4 o[NC][G][2];
+    f32x4 o[NC][G][2], less{0.f, 0.f, 0.f, 0.f};             // less: REP: -24 times the sum of the column's weights
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         m[c] = -__builtin_inff(), ref[c] = l[c] = 0.0f;
 #pragma unroll
         for (int i = 0; i < G; ++i) o[c][i][0] = o[c][i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    bf16x8 middle;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) middle[e] = static_cast<__bf16>(-24.0f);
     const Q4Masks masks = q4_masks();
     f32x4 s[NC][2];
     auto scores = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+            if constexpr (REP) {
+                f32x4 y = start;
+#pragma unroll
+                for (int i = 0; i < G; ++i) {
+                    const bf16x8 ka = q4_key_operand(xk[t][i], masks);
+#pragma unroll
+                    for (int n = 0; n < kTerms; ++n) y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qr[0][i][n], y, 0, 0, 0);
+                }
+                const float h = static_cast<float>(hk[t][0][0]);
+                s[0][t][0] = q4_group_sum<G>(q4_by_quad<0>(y[0], h));
+                s[0][t][1] = q4_group_sum<G>(q4_by_quad<1>(y[1], h));
+                s[0][t][2] = q4_group_sum<G>(q4_by_quad<2>(y[2], h));
+                s[0][t][3] = q4_group_sum<G>(q4_by_quad<3>(y[3], h));
+                continue;
+            }
 #pragma unroll
             for (int c = 0; c < NC; ++c) s[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -522,7 +585,7 @@ decode_paged_q4_kernel(PagedDecode a) {
 #pragma unroll
                     for (int n = 0; n < kTerms; ++n) y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qr[c][i][n], y, 0, 0, 0);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[c][t][e] = __builtin_fmaf(y[e], static_cast<float>(hk[t][e][i]), s[c][t][e]);
+                    for (int e = 0; e < 4; ++e) s[c][t][e] = __builtin_fmaf(y[e], static_cast<float>(hk[t][REP ? 0 : e][REP ? 0 : i]), s[c][t][e]);
                 }
                 __builtin_amdgcn_sched_barrier(0);           // (operands of one group at a time: registers)
             }
@@ -549,6 +612,7 @@ decode_paged_q4_kernel(PagedDecode a) {
                 l[c] *= alpha;
 #pragma unroll
                 for (int i = 0; i < G; ++i) o[c][i][0] *= alpha, o[c][i][1] *= alpha;
+                if constexpr (REP) less *= alpha;
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -556,6 +620,36 @@ decode_paged_q4_kernel(PagedDecode a) {
                 if (kMask) p[c][e] = 16 * (e / 4) + e % 4 < left ? p[c][e] : 0.0f;
                 l[c] += p[c][e];
             }
+        }
+        if constexpr (REP) {
+            const int left = lim[0] - v * kStep - 4 * grp;
+            float ph[8];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const float h = static_cast<float>(hv[t][0][0]);
+                ph[4 * t] = q4_by_quad<0>(p[0][4 * t], h);
+                ph[4 * t + 1] = q4_by_quad<1>(p[0][4 * t + 1], h);
+                ph[4 * t + 2] = q4_by_quad<2>(p[0][4 * t + 2], h);
+                ph[4 * t + 3] = q4_by_quad<3>(p[0][4 * t + 3], h);
+            }
+            if constexpr (kMask) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ph[e] = 16 * (e / 4) + e % 4 < left ? ph[e] : 0.0f;   // (as below)
+            }
+            bf16x8 pb[kTerms];
+            q4_split<kTerms>(ph, pb);
+#pragma unroll
+            for (int n = 0; n < kTerms; ++n) less = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, pb[n], less, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                const bf16x8 v0 = q4_value_operand<0>(xv[0][i], xv[1][i], masks), v1 = q4_value_operand<1>(xv[0][i], xv[1][i], masks);
+#pragma unroll
+                for (int n = 0; n < kTerms; ++n) {
+                    o[0][i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pb[n], o[0][i][0], 0, 0, 0);
+                    o[0][i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pb[n], o[0][i][1], 0, 0, 0);
+                }
+            }
+            return;
         }
 #pragma unroll
         for (int i = 0; i < G; ++i) {
@@ -566,7 +660,7 @@ decode_paged_q4_kernel(PagedDecode a) {
                 float ph[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    ph[e] = __builtin_fmaf(p[c][e], static_cast<float>(hv[e / 4][e % 4][i]), 0.0f);
+                    ph[e] = __builtin_fmaf(p[c][e], static_cast<float>(hv[e / 4][REP ? 0 : e % 4][REP ? 0 : i]), 0.0f);
                     if (kMask) ph[e] = 16 * (e / 4) + e % 4 < left ? ph[e] : 0.0f;   // (a number behind the column's positions may be anything)
                 }
                 bf16x8 pb[kTerms];
@@ -621,17 +715,19 @@ decode_paged_q4_kernel(PagedDecode a) {
         if (nh <= 0) break;                                   // workgroup-uniform
         if (c > 0) __syncthreads();                           // the last ones have been read
         l[c] = pair32_sum(pair16_sum(l[c]));
-        if (c16 < nh) {
+        if (c16 % kCols < nh) {
 #pragma unroll
-            for (int i = 0; i < G; ++i)
+            for (int i = 0; i < G; ++i) {
+                if (REP && mine != i) continue;               // (other groups' weights)
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int d = 32 * i + 2 * (4 * grp + e) + j;
-                        if (d < D) lo[(wave * a.lds_heads + c16) * (D + 4) + d] = 2.0f * o[c][i][j][e];
+                        if (d < D) lo[(wave * a.lds_heads + c16 % kCols) * (D + 4) + d] = 2.0f * (o[c][i][j][e] + less[e]);
                     }
-            if (grp == 0) {
+            }
+            if (grp == 0 && mine == 0) {
                 lm[(wave * 16 + c16) * 2] = m[c] == -__builtin_inff() ? m[c] : ref[c];   // (log2 units from here)
                 lm[(wave * 16 + c16) * 2 + 1] = l[c];
             }
@@ -678,35 +774,45 @@ namespace {
 // - Two tiles of 16 columns share the unpacked codes where there are more than 16 columns and the products
 //   are single: 16 x 5 tokens of 32/8 heads of 128 at 8000 (20 columns) 41 us, 47 with a tile a workgroup. In
 //   fp32 the terms of two tiles do not fit the registers.
+// - Columns that fit 16 / G of a tile stand in it G times (REP above); a call of 20 columns would take five such tiles.
 // - A sequence is one item, with no join, up to 16 steps of 32 keys, or up to 64 where the sequences fill
 //   half of the chip by themselves; otherwise there are as many items as workgroups run at a time (256 CUs
-//   times the wavefronts that a SIMD holds), and B / 2 fewer asked for, since a sequence's last share is half
-//   empty in the mean: all shares are then done in one round. 32 x 16384 of 32/8 heads of 128 (slots 96 a
-//   KV head): 64 / 80 / 96 / 128 items 101.5 / 89.1 / 104.4 / 99.9 us; 8 x 16384 of 12/4 of 64 (256): 100 /
-//   256 / 312 items 16.4 / 15.9 / 18.1; 16 x 5 tokens (64): 32 / 48 / 56 / 64 items 54.7 / 42.9 / 41.1 / 53.1.
+//   times the wavefronts that a SIMD holds), so that all shares are done in one round: one too many
+//   costs a second. The target is below that by B / 2, since ceil adds half an item a sequence in the mean, and
+//   by two standard deviations of that sum. Over 24 draws of 32 lengths up to 16384, 32/8 heads of 128: 79.9 us in
+//   the mean and 89.7 at most, without the deviations 84.6 and 101.2, with B below 81.3 and 95.8; half as
+//   many items 109.6 where all took 80.5, twice as many 85.0. 16 x 5 tokens: 43.9 and 47.4, 44.3 and 57.2.
 // - A share is four steps at least, one for each wavefront.
+// - A call over more than the last-level cache holds (256 MB of codes at the tables' capacity) finds nothing there from the
+//   last call and loads past it: 32 x 16384 84.2 / 74.4 us. Smaller ones may: 16 x 5 tokens at 8000 repeated over few
+//   caches 40.9 / 44.2 with such loads, over twelve 49.4 / 48.2; 20 x 9000 32.0 / 33.2 and 36.7 / 33.5.
 struct Q4Plan {
     int nc;                  // column tiles of a workgroup
+    bool rep;                // the columns of one tile, once for every group
     int64_t target, least;   // items aimed at, steps of the smallest item
     int64_t items, groups;   // items at most, workgroups an item
     bool few;                // a sequence has few items in the mean
+    bool stream;             // the codes do not stay in the last-level cache from call to call
 };
 Q4Plan q4_plan(int64_t B, int64_t T, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D, int dtype) {
     const int64_t cols = Hq / Hkv * T, steps = cdiv(cap, 32);
-    Q4Plan p{dtype == SPARDA_BF16 && cols > 16 ? 2 : 1, 1, 4, 0, 0, false};
+    Q4Plan p{dtype == SPARDA_BF16 && cols > 16 ? 2 : 1, D >= 64 && cols <= 16 / (D / 32), 1, 4, 0, 0, false, false};
     p.groups = Hkv * cdiv(cols, 16 * p.nc);
     if (steps <= 16 || (steps <= 64 && B * p.groups >= 128)) {
         p.least = steps;
     } else {
-        // (items are target + B at most, target + B / 2 in the mean)
-        const int64_t slots = 256 * ((D == 128 ? 3 : 4) - (p.nc > 1 ? 1 : 0));
-        p.target = slots / p.groups - B / 2;
+        // (items are target + B at most, target + B / 2 in the mean, sqrt(B / 12) to either side)
+        const int64_t slots = 256 * q4_waves(dtype, static_cast<int>(D), p.nc, p.rep);
+        int64_t margin = 0;                          // ceil(0.6 sqrt(B))
+        while (margin * margin * 25 < B * 9) ++margin;
+        p.target = slots / p.groups - B / 2 - margin;
     }
     if (p.target < 1) p.target = 1;
     p.items = p.target + B;
     const int64_t most = B * cdiv(steps, p.least);   // every share the smallest
     if (p.items > most) p.items = most;
     p.few = p.items <= 16 * B;
+    p.stream = B * cap * Hkv * q4_groups(static_cast<int>(D)) * 36 > (256ll << 20);
     return p;
 }
 
@@ -740,16 +846,27 @@ int launch_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = workspace ? a.part_o + p.items * a.Hq * D : nullptr;
     const dim3 grid(static_cast<unsigned>(p.items * p.groups));
-#define SPARDA_DQ_C(DT_, D_, NC_)                                                                 \
-    hipLaunchKernelGGL((decode_paged_q4_kernel<DT_, D_, 4, NC_>), grid, dim3(4 * kWave),          \
+#define SPARDA_DQ_S(DT_, D_, NC_, REP_, S_)                                                       \
+    hipLaunchKernelGGL((decode_paged_q4_kernel<DT_, D_, 4, NC_, REP_, S_>), grid, dim3(4 * kWave), \
                        4 * (a.lds_heads * ((D_) + 4) + 33) * sizeof(float), stream, a)
+#define SPARDA_DQ_C(DT_, D_, NC_, REP_)                                                           \
+    do {                                                                                          \
+        if (p.stream) SPARDA_DQ_S(DT_, D_, NC_, REP_, true);                                      \
+        else SPARDA_DQ_S(DT_, D_, NC_, REP_, false);                                              \
+    } while (0)
 #define SPARDA_DQ(DT_, D_)                                                                        \
     do {                                                                                          \
+        if constexpr (D_ >= 64) {                                                                 \
+            if (p.rep) {                                                                          \
+                SPARDA_DQ_C(DT_, D_, 1, true);                                                    \
+                break;                                                                            \
+            }                                                                                     \
+        }                                                                                         \
         if constexpr (DT_ == SPARDA_BF16) {                                                       \
-            if (p.nc == 2) SPARDA_DQ_C(DT_, D_, 2);                                               \
-            else SPARDA_DQ_C(DT_, D_, 1);                                                         \
+            if (p.nc == 2) SPARDA_DQ_C(DT_, D_, 2, false);                                        \
+            else SPARDA_DQ_C(DT_, D_, 1, false);                                                  \
         } else {                                                                                  \
-            SPARDA_DQ_C(DT_, D_, 1);                                                              \
+            SPARDA_DQ_C(DT_, D_, 1, false);                                                       \
         }                                                                                         \
     } while (0)
 #define SPARDA_DQ_D(DT_)                      \
@@ -764,6 +881,7 @@ int launch_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
 #undef SPARDA_DQ_D
 #undef SPARDA_DQ
 #undef SPARDA_DQ_C
+#undef SPARDA_DQ_S
     if (p.items > B) launch_paged_join(a, D, dtype, p.few, stream);
     return check_hip(hipGetLastError(), "decode_paged_q4_kernel");
 }

@@ -30,20 +30,22 @@ struct RotateAppend {
     uint32_t* status;
 };
 
-// N angles of position pos from dim `at` on; NaN behind the tables
+// N angles of position pos from dim `at` on; NaN behind the tables (whose first row is loaded then: with the
+// loads on one way of a branch the compiler kept a part of them in scratch memory)
 template <int N>
 __device__ __forceinline__ void load_angles(const RotateAppend& a, int64_t pos, int at, bool off_table, float (&c)[N], float (&s)[N]) {
-    if (off_table) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) c[e] = s[e] = __builtin_nanf("");
-        return;
-    }
+    const int64_t from = off_table ? 0 : pos * a.cs_st;
 #pragma unroll
     for (int e = 0; e < N; e += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(a.cos + pos * a.cs_st + at + e);
-        const float4 y = *reinterpret_cast<const float4*>(a.sin + pos * a.cs_st + at + e);
+        const float4 x = *reinterpret_cast<const float4*>(a.cos + from + at + e);
+        const float4 y = *reinterpret_cast<const float4*>(a.sin + from + at + e);
         c[e] = x.x, c[e + 1] = x.y, c[e + 2] = x.z, c[e + 3] = x.w;
         s[e] = y.x, s[e + 1] = y.y, s[e + 2] = y.z, s[e + 3] = y.w;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        c[e] = off_table ? __builtin_nanf("") : c[e];
+        s[e] = off_table ? __builtin_nanf("") : s[e];
     }
 }
 

@@ -232,6 +232,35 @@ def test_decode_over_many_shares(dtype, Hq, Hkv, D, lengths):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("Hq,Hkv,D,T", [(12, 4, 64, 1), (8, 2, 128, 1), (8, 1, 128, 5), (34, 2, 64, 2), (4, 2, 16, 3), (8, 8, 32, 1)])
+def test_decode_with_tables_of_large_capacity(dtype, Hq, Hkv, D, T):
+    """More codes than the last-level cache holds, were the tables full: other loads, the same results."""
+    G = max(1, D // 32)
+    width = (257 << 20) // (2 * 16 * Hkv * G * 36) + 1
+    lengths = [700, 2001]
+    print(f"[case] q4 capacity {dtype} {Hq}/{Hkv}x{D} T={T} width {width}", flush=True)
+    pages, table, rows = cache(lengths, 16, Hkv, D, seed=6, width=width)
+    q = randn(2, T, Hq, D, dtype=dtype, seed=7) * 2
+    got = sparda.decode_paged_q4(dev(q), dev(pages), dev(table), dev(lengths))
+    print("  of the bound:", check(got, q, lengths, rows))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("Hq,Hkv,D", [(4, 1, 128), (5, 1, 128), (8, 1, 64), (9, 1, 64), (2, 2, 128), (16, 1, 32)])
+def test_decode_at_the_number_of_columns_that_changes_the_form(dtype, Hq, Hkv, D):
+    lengths = [333, 31, 32, 0, 2500]
+    print(f"[case] q4 columns {dtype} {Hq}/{Hkv}x{D}", flush=True)
+    pages, table, rows = cache(lengths, 16, Hkv, D, seed=11)
+    q = randn(len(lengths), Hq, D, dtype=dtype, seed=12) * 3
+    got = sparda.decode_paged_q4(dev(q), dev(pages), dev(table), dev(lengths))
+    print("  of the bound:", check(got, q, lengths, rows))
+    # a column does not see what the others hold
+    q[:, :-1] = float("nan")
+    alone = sparda.decode_paged_q4(dev(q), dev(pages), dev(table), dev(lengths)).view(len(lengths), Hq, D)
+    assert torch.equal(alone[:, -1], got.view(len(lengths), Hq, D)[:, -1])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("scale", [0.0, -0.5, 4.0])
 def test_decode_other_scales(dtype, scale):
     print(f"[case] q4 scale {scale} {dtype}", flush=True)
