@@ -63,14 +63,17 @@ __device__ __forceinline__ void q4_codes(const float (&x)[8], _Float16 h, uint32
 }
 
 // Eight elements of a row, as bf16 values in fp32 (round: fp32 rows are rounded)
-template <int DT>
+template <int DT, bool ONCE>
 __device__ __forceinline__ void q4_load8(const char* p, float (&x)[8]) {
+    auto load = [](const char* at) { return ONCE ? load_once(at) : *reinterpret_cast<const uint4*>(at); };
+    const uint4 a = load(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
     if constexpr (DT == SPARDA_F32) {
-        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 16);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        const uint4 b = load(p + 16);
+        const uint32_t r[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(w[e]), x[4 + e] = __uint_as_float(r[e]);
     } else {
-        const uint4 a = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[2 * e] = __uint_as_float(w[e] << 16), x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
     }
@@ -136,9 +139,8 @@ __device__ __forceinline__ uint32_t q4_key_pack(const uint32_t (&c)[8]) {
 // One wavefront per new row. A lane takes eight dims and the eight that they are paired
 // with; the largest magnitude of a group comes from up to four neighbouring lanes. The queries are rotated
 // as for 16-bit pages, four heads at a time. Bound by memory: 16000 rows of 32/8 heads of 128 (196.6 MB read,
-// 149.4 written) take 75-79 us = 4.4-4.6 TB/s where a large copy reaches 5.1; the rest is the values' bytes, of
-// which a row holds every fourth of a word (counted: 171 MB written, 210 read). 64 rows of 12/4 heads of
-// 64 take 5.3 us, a chain of five dependent loads. Neighbouring rows on one XCD: 77.5 against 78.2 us, not taken.
+// 149.4 written) take 65.5 us = 5.3 TB/s (counted: 158 MB written, a row holding single bytes of the values' words). 64 rows of 12/4 heads of 64 take 5.2 us, a chain of five dependent
+// loads. Neighbouring rows on one XCD: 77.5 against 78.2 us (then), not taken.
 template <int DT, int D, bool ROT>
 __global__ void __launch_bounds__(256) append_paged_q4_kernel(RotateAppend a, char* __restrict__ pages) {
     constexpr int G = q4_groups(D), kEs = DT == SPARDA_F32 ? 4 : 2, kPer = D / 16;
@@ -165,8 +167,8 @@ __global__ void __launch_bounds__(256) append_paged_q4_kernel(RotateAppend a, ch
         const char* from = static_cast<const char*>(a.k_new) + (t * a.new_st + h * a.new_sh + c * 8) * kEs;
         char* tile = tiles + h * a.pg.h_st;
         float x[2][8];
-        q4_load8<DT>(from, x[0]);
-        q4_load8<DT>(from + D / 2 * kEs, x[1]);
+        q4_load8<DT, true>(from, x[0]);
+        q4_load8<DT, true>(from + D / 2 * kEs, x[1]);
         if constexpr (ROT) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) turn(x[0][e], x[1][e], cs[e], sn[e]);
@@ -187,7 +189,7 @@ __global__ void __launch_bounds__(256) append_paged_q4_kernel(RotateAppend a, ch
         const int h = i / (2 * kPer), dim = i % (2 * kPer) * 8;
         char* tile = tiles + h * a.pg.h_st;
         float x[8];
-        q4_load8<DT>(static_cast<const char*>(a.v_new) + (t * a.new_st + h * a.new_sh + dim) * kEs, x);
+        q4_load8<DT, true>(static_cast<const char*>(a.v_new) + (t * a.new_st + h * a.new_sh + dim) * kEs, x);
         const _Float16 hh = q4_scale(lanes_max<(D >= 32 ? 4 : 2)>(q4_top(x)));
         uint32_t code[8];
         q4_codes(x, hh, code);
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(256) append_paged_q4_kernel(RotateAppend a, ch
 // ---------------------------------------------------------------------------
 
 // One wavefront per row, eight dims a lane: the values that the codes stand for. Bound by memory: 17486
-// rows of 8 heads of 128 (20.1 MB of codes, 71.6 written) take 21.8-23.1 us = 4.0-4.2 TB/s; the codes of a row
+// rows of 8 heads of 128 (20.1 MB of codes, 71.6 written) take 19.0-23.1 us = 4.0-4.8 TB/s; the codes of a row
 // lie in a third of a tile's lines, and other rows read the same lines again (counted: 37 MB read).
 template <int DT, int D>
 __global__ void __launch_bounds__(256)
@@ -476,7 +478,7 @@ decode_paged_q4_kernel(PagedDecode a) {
         for (int i = 0; i < G; ++i) {
             float x[8];
             if (at < ncol && 32 * i + 8 * grp < D && (!REP || mine == i)) {
-                q4_load8<DT>(q + (32 * i + 8 * grp) * kEs, x);
+                q4_load8<DT, false>(q + (32 * i + 8 * grp) * kEs, x);
                 if (a.negate) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] = -x[e];

@@ -9,8 +9,8 @@ namespace sparda {
 
 // One wavefront per new row: its sequence, position and page, then the heads in pairs of
 // 16-byte pieces (i, i + D/2), the queries' first and the keys' behind them, then the
-// values, copied. Bound by memory: 16000 rows of 32/8 heads of 128, 393 MB read and written, take 76.7 us
-// a call = 5.1 TB/s, what a large copy reaches; 64 rows of 12/4 heads of 64 5.0 us, of which the
+// values, copied. Bound by memory: 16000 rows of 32/8 heads of 128, 393 MB read and written, take 62 us
+// = 6.3 TB/s (part of it stays in the last-level cache), 77 in a row of calls = 5.1 TB/s, as large copies do; 64 rows of 12/4 heads of 64 5.0 us a call, of which the
 // host's part is 4.5.
 template <int DT, int D>
 __global__ void __launch_bounds__(256) rotate_append_paged_kernel(RotateAppend a, char* __restrict__ k, char* __restrict__ v) {
@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(256) rotate_append_paged_kernel(RotateAppend a
     const char* vn = static_cast<const char*>(a.v_new) + t * a.new_st * kEs;
     for (int i = lane; i < a.Hkv * kPieces; i += kWave) {
         const int h = i / kPieces, o = i % kPieces * 16;
-        *reinterpret_cast<uint4*>(v + at + h * a.pg.h_st * kEs + o) = *reinterpret_cast<const uint4*>(vn + h * a.new_sh * kEs + o);
+        *reinterpret_cast<uint4*>(v + at + h * a.pg.h_st * kEs + o) = load_once(vn + h * a.new_sh * kEs + o);
     }
 }
 
