@@ -595,6 +595,7 @@ struct Rotation {
     Rotation(Args& x, PyObject* q_, PyObject* cos_, PyObject* sin_, const NewRows& n, int64_t D)
         : q(x.operand(q_, 3)), cos(x.f32(cos_, 2)), sin(x.f32(sin_, 2)) {
         need(q.scalar_type() == n.k.scalar_type() && q.size(0) == n.N && q.size(1) > 0 && q.size(2) == D && rows16(q));
+        need(!((cos.requires_grad() || sin.requires_grad()) && c10::GradMode::is_enabled()));
         need(cos.sizes() == sin.sizes() && cos.size(0) > 0 && cos.size(1) * 2 == D && aligned(cos, 16) && aligned(sin, 16));
     }
 };

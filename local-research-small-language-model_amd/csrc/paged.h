@@ -81,9 +81,10 @@ struct Share {
     bool bad;        // the length is out of range
 };
 
-__device__ __forceinline__ int paged_steps(int len, int cap, int step) {
-    const int c = len < 0 ? 0 : len > cap ? cap : len;
-    return static_cast<int>((static_cast<int64_t>(c) + step - 1) / step);
+// steps of 2^log_step keys (len at most 2^31 - 64)
+__device__ __forceinline__ int paged_steps(int len, int cap, int log_step) {
+    const uint32_t c = len < 0 ? 0 : len > cap ? cap : len;
+    return static_cast<int>((c + (1u << log_step) - 1) >> log_step);
 }
 
 // Inclusive sums over the lanes: within rows of 16 by shifts, then the rows' totals.
@@ -106,26 +107,26 @@ __device__ __forceinline__ int wave_last(int v) { return __builtin_amdgcn_readla
 // The item's sequence (by_item), or sequence `want`'s items. Wave-uniform. The total
 // of the steps stays below 2^30 (checked by the host against the capacity), so that
 // the sums with the target or a share stay in 32 bits.
-__device__ __forceinline__ Share paged_item(const int32_t* __restrict__ len, int B, int cap, int step, int target,
+__device__ __forceinline__ Share paged_item(const int32_t* __restrict__ len, int B, int cap, int log_step, int target,
                                             int least, bool by_item, int want) {
     const int lane = threadIdx.x % kWave;
     auto at_least = [&](int total) { return max(least, (total + target - 1) / target); };
     auto found = [&](int seq, int l, int parts, int first) {
-        return Share{seq, by_item ? want - first : 0, parts, first, (paged_steps(l, cap, step) + parts - 1) / parts,
+        return Share{seq, by_item ? want - first : 0, parts, first, (paged_steps(l, cap, log_step) + parts - 1) / parts,
                      l < 0 ? 0 : l > cap ? cap : l, l < 0 || l > cap};
     };
     if (B == 1) {
-        const int l = __builtin_amdgcn_readfirstlane(len[0]), steps = paged_steps(l, cap, step), share = at_least(steps);
+        const int l = __builtin_amdgcn_readfirstlane(len[0]), steps = paged_steps(l, cap, log_step), share = at_least(steps);
         const int parts = max(1, (steps + share - 1) / share);
         return by_item && want >= parts ? Share{-1} : found(0, l, parts, 0);
     }
     int total = 0;
-    for (int b0 = 0; b0 < B; b0 += kWave) total += wave_last(wave_scan_i32(b0 + lane < B ? paged_steps(len[b0 + lane], cap, step) : 0));
+    for (int b0 = 0; b0 < B; b0 += kWave) total += wave_last(wave_scan_i32(b0 + lane < B ? paged_steps(len[b0 + lane], cap, log_step) : 0));
     const int share = at_least(total);
     int before = 0;
     for (int b0 = 0; b0 < B; b0 += kWave) {
         const int b = b0 + lane, l = b < B ? len[b] : 0;
-        const int n = b < B ? max(1, (paged_steps(l, cap, step) + share - 1) / share) : 0;
+        const int n = b < B ? max(1, (paged_steps(l, cap, log_step) + share - 1) / share) : 0;
         const int end = before + wave_scan_i32(n);      // items of sequences 0 .. b
         const uint64_t m = __ballot(b < B && (by_item ? end > want : b == want));
         if (m != 0) {
@@ -139,29 +140,33 @@ __device__ __forceinline__ Share paged_item(const int32_t* __restrict__ len, int
 
 constexpr int kPgJoin = 512;        // threads of a join
 
+// (What only several tokens or 4-bit pages need stands at the end, on a cache line of its own: every further line
+// of arguments that a kernel reads at its start costs it 0.3 us.)
 struct PagedDecode {
     const void* q;
-    int64_t q_sb, q_st, q_sh;     // sequence, token, head
+    int64_t q_sb, q_sh;           // sequence, head
     const void *k, *v;
     Pages pg;
     int ps16;                     // 16-key tiles of a page
     const int32_t* len;
     int B, cap;
     int Hq, Hkv, R, head_tiles;   // head tiles of 16 query heads per KV head
-    int T, heads;                 // tokens of a sequence; Hq = T heads, token-major
-    int step;                     // keys of a step
     int target, least;
     int whole;                    // every sequence is one item
     int lds_heads;                // heads of the largest tile
     float scale_log2;             // the scores' scale in log2 units
-    int negate;                   // (4-bit pages: scale_log2 is its magnitude, q takes the sign)
+    int T;                        // tokens of a sequence; Hq = T heads, token-major
     void* out;
     int64_t out_sb;
     float *part_o, *part_ml;      // [items, Hq, D], [items, Hq, 2]
     uint32_t* status;
+    int64_t q_st;                 // between tokens
+    int heads;
+    int negate;                   // (4-bit pages: scale_log2 is its magnitude, q takes the sign)
 };
 
-// joins the items of every sequence that has several (paged.hip); few: they are few in the mean
-void launch_paged_join(const PagedDecode& a, int64_t D, int dtype, bool few, hipStream_t stream);
+// joins the items of every sequence that has several (paged.hip), of steps of 2^log_step keys (5, or 4 with
+// fp32); few: they are few in the mean
+void launch_paged_join(const PagedDecode& a, int64_t D, int dtype, int log_step, bool few, hipStream_t stream);
 
 }  // namespace sparda

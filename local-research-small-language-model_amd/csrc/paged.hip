@@ -121,7 +121,8 @@ __device__ __forceinline__ void paged_store(const PagedDecode& a, const Share& s
 template <int DT, int D, int HG, int KW>
 __global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : DT == SPARDA_F32 ? 3 : 4) decode_paged_kernel(PagedDecode a) {
     typedef PagedStep<DT, D> Step;
-    constexpr int kTiles = Step::kTiles, kV = Step::kV, kQ = Step::kQ, kStep = 16 * kTiles, W = KW;
+    constexpr int kTiles = Step::kTiles, kV = Step::kV, kQ = Step::kQ, kLogStep = kTiles == 1 ? 4 : 5, kStep = 1 << kLogStep, W = KW;
+    static_assert(kStep == 16 * kTiles, "steps of 16 or 32 keys");
     extern __shared__ float lds[];
     const int lane = threadIdx.x % kWave;
     const int wv = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
@@ -134,13 +135,13 @@ __global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : DT == SPARDA_F32
     Share sh;
     if (a.whole) {
         const int l = __builtin_amdgcn_readfirstlane(a.len[item]), n = l < 0 ? 0 : l > a.cap ? a.cap : l;
-        sh = Share{item, 0, 1, item, paged_steps(l, a.cap, kStep), n, l < 0 || l > a.cap};
+        sh = Share{item, 0, 1, item, paged_steps(l, a.cap, kLogStep), n, l < 0 || l > a.cap};
     } else {
-        sh = paged_item(a.len, a.B, a.cap, kStep, a.target, a.least, true, item);
+        sh = paged_item(a.len, a.B, a.cap, kLogStep, a.target, a.least, true, item);
     }
     if (sh.seq < 0) return;                                 // workgroup-uniform
     const int b = sh.seq, len = sh.len;
-    const int steps = paged_steps(len, a.cap, kStep);
+    const int steps = paged_steps(len, a.cap, kLogStep);
     const int s_end = min(steps, (sh.part + 1) * sh.share);
     bool bad = sh.bad;
 
@@ -352,13 +353,13 @@ __device__ __forceinline__ float paged_join_out(const PagedDecode& a, const Shar
 // latencies, the weights' and the partials' (3.7 to 5.4 us): with a whole head a
 // workgroup 1 x 20000 positions take 12.8 against 11.7 us, 1 x 131000 31.6 / 30.8,
 // with 16 dims 8 x 16384 26.1 / 25.5.
-template <int DT, int D>
+template <int DT, int D, int LOG>
 __global__ void __launch_bounds__(kPgJoin) decode_paged_join_kernel(PagedDecode a) {
     constexpr int JD = D < 32 ? D : 32;                       // dims of a workgroup
     constexpr int kG = kPgJoin / JD, kChunk = 1024, kJW = kPgJoin / kWave;
     __shared__ float red[kPgJoin], wts[kChunk], rm[kJW], rl[kJW];
     const int b = blockIdx.y, h = blockIdx.x / (D / JD), d0 = blockIdx.x % (D / JD) * JD, tid = threadIdx.x, wave = tid / kWave;
-    const Share sh = paged_item(a.len, a.B, a.cap, a.step, a.target, a.least, false, b);
+    const Share sh = paged_item(a.len, a.B, a.cap, LOG, a.target, a.least, false, b);
     if (sh.parts <= 1) return;                                // written by its one item
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + static_cast<int64_t>(sh.first) * a.Hq + h;
     const float* po = a.part_o + (static_cast<int64_t>(sh.first) * a.Hq + h) * D + d0 + tid % JD;
@@ -417,10 +418,10 @@ __global__ void __launch_bounds__(kPgJoin) decode_paged_join_kernel(PagedDecode 
 // The same where sequences have few items in the mean: one thread per (query head,
 // dim), items in order, eight in flight. Bound by the launch and two dependent loads: 3.0 us for 1000 positions of 12
 // heads of 64.
-template <int DT, int D>
+template <int DT, int D, int LOG>
 __global__ void __launch_bounds__(256) decode_paged_join_few_kernel(PagedDecode a) {
     const int b = blockIdx.y, h = blockIdx.x * (256 / D) + threadIdx.x / D, d = threadIdx.x % D;
-    const Share sh = paged_item(a.len, a.B, a.cap, a.step, a.target, a.least, false, b);
+    const Share sh = paged_item(a.len, a.B, a.cap, LOG, a.target, a.least, false, b);
     if (sh.parts <= 1 || h >= a.Hq) return;                   // written by its one item
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + static_cast<int64_t>(sh.first) * a.Hq + h;
     const float* po = a.part_o + (static_cast<int64_t>(sh.first) * a.Hq + h) * D + d;
@@ -523,23 +524,25 @@ size_t decode_paged_workspace_bytes(int64_t B, int64_t cap, int64_t Hq, int64_t 
     return p.items <= B ? 0 : static_cast<size_t>(p.items * Hq * (D + 2)) * sizeof(float);
 }
 
-void launch_paged_join(const PagedDecode& a, int64_t D, int dtype, bool few, hipStream_t stream) {
-#define SPARDA_PGJ(DT_, D_)                                                                                       \
+void launch_paged_join(const PagedDecode& a, int64_t D, int dtype, int log_step, bool few, hipStream_t stream) {
+    // (the step is a constant of the kernel: read from its arguments it cost 0.25 us a call)
+#define SPARDA_PGJ(DT_, D_, LOG_)                                                                                 \
     if (few)                                                                                                      \
-        hipLaunchKernelGGL((decode_paged_join_few_kernel<DT_, D_>),                                               \
+        hipLaunchKernelGGL((decode_paged_join_few_kernel<DT_, D_, LOG_>),                                         \
                            dim3(static_cast<unsigned>(cdiv(a.Hq, 256 / D_)), static_cast<unsigned>(a.B)), dim3(256), 0, stream, a); \
     else                                                                                                          \
-        hipLaunchKernelGGL((decode_paged_join_kernel<DT_, D_>),                                                   \
+        hipLaunchKernelGGL((decode_paged_join_kernel<DT_, D_, LOG_>),                                             \
                            dim3(static_cast<unsigned>(a.Hq * (D_ < 32 ? 1 : D_ / 32)), static_cast<unsigned>(a.B)), dim3(kPgJoin), 0, stream, a)
-#define SPARDA_PGJ_D(DT_)                     \
-    switch (D) {                              \
-        case 16: SPARDA_PGJ(DT_, 16); break;  \
-        case 32: SPARDA_PGJ(DT_, 32); break;  \
-        case 64: SPARDA_PGJ(DT_, 64); break;  \
-        default: SPARDA_PGJ(DT_, 128); break; \
+#define SPARDA_PGJ_D(DT_, LOG_)                     \
+    switch (D) {                                    \
+        case 16: SPARDA_PGJ(DT_, 16, LOG_); break;  \
+        case 32: SPARDA_PGJ(DT_, 32, LOG_); break;  \
+        case 64: SPARDA_PGJ(DT_, 64, LOG_); break;  \
+        default: SPARDA_PGJ(DT_, 128, LOG_); break; \
     }
-    if (dtype == SPARDA_F32) SPARDA_PGJ_D(SPARDA_F32)
-    else SPARDA_PGJ_D(SPARDA_BF16)
+    if (dtype != SPARDA_F32) SPARDA_PGJ_D(SPARDA_BF16, 5)
+    else if (log_step == 5) SPARDA_PGJ_D(SPARDA_F32, 5)
+    else SPARDA_PGJ_D(SPARDA_F32, 4)
 #undef SPARDA_PGJ_D
 #undef SPARDA_PGJ
 }
@@ -555,7 +558,7 @@ int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k
     if (const int rc = status_word(&a.status)) return rc;
     a.q = q, a.q_sb = q_sb, a.q_sh = q_sh, a.k = k, a.v = v;
     a.pg = Pages{p_st, s_st, h_st, table, t_st, static_cast<int>(width), static_cast<int>(n_pages)};
-    a.T = 1, a.heads = static_cast<int>(Hq), a.step = dtype == SPARDA_F32 ? 16 : 32;
+    a.T = 1, a.heads = static_cast<int>(Hq);
     a.ps16 = static_cast<int>(ps / 16), a.len = len, a.B = static_cast<int>(B), a.cap = static_cast<int>(cap);
     a.Hq = static_cast<int>(Hq), a.Hkv = static_cast<int>(Hkv), a.R = static_cast<int>(R);
     a.head_tiles = static_cast<int>(cdiv(R, 16));
@@ -574,7 +577,7 @@ int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k
         if (p.hg == 4) SPARDA_PGD_W(DT_, D_, 4, 2);                                                               \
         else if (p.hg == 2) SPARDA_PGD_W(DT_, D_, 2, 4);                                                          \
         else if (p.kw == 4) SPARDA_PGD_W(DT_, D_, 1, 4);                                                          \
-        else SPARDA_PGD_W(DT_, D_, 1, 8);                                                          \
+        else SPARDA_PGD_W(DT_, D_, 1, 8);                                                                         \
     } while (0)
 #define SPARDA_PGD_D(DT_)                     \
     switch (D) {                              \
@@ -588,7 +591,7 @@ int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k
 #undef SPARDA_PGD_D
 #undef SPARDA_PGD_W
 #undef SPARDA_PGD
-    if (p.items > B) launch_paged_join(a, D, dtype, p.few, stream);
+    if (p.items > B) launch_paged_join(a, D, dtype, dtype == SPARDA_F32 ? 4 : 5, p.few, stream);
     return check_hip(hipGetLastError(), "decode_paged_kernel");
 }
 

@@ -437,7 +437,7 @@ constexpr int q4_waves(int DT, int D, int NC, bool REP) {
 template <int DT, int D, int KW, int NC, bool REP, bool STREAM>
 __global__ void __launch_bounds__(KW* kWave, q4_waves(DT, D, NC, REP))
 decode_paged_q4_kernel(PagedDecode a) {
-    constexpr int G = q4_groups(D), kTerms = DT == SPARDA_F32 ? 3 : 1, kStep = 32, kEs = DT == SPARDA_F32 ? 4 : 2;
+    constexpr int G = q4_groups(D), kTerms = DT == SPARDA_F32 ? 3 : 1, kLogStep = 5, kStep = 1 << kLogStep, kEs = DT == SPARDA_F32 ? 4 : 2;
     constexpr int kCols = REP ? 16 / G : 16;                 // columns of a tile
     static_assert(!REP || (NC == 1 && G > 1), "one tile, of several groups");
     extern __shared__ float lds[];
@@ -451,13 +451,13 @@ decode_paged_q4_kernel(PagedDecode a) {
     Share sh;
     if (a.whole) {
         const int l = __builtin_amdgcn_readfirstlane(a.len[item]), n = l < 0 ? 0 : l > a.cap ? a.cap : l;
-        sh = Share{item, 0, 1, item, paged_steps(l, a.cap, kStep), n, l < 0 || l > a.cap};
+        sh = Share{item, 0, 1, item, paged_steps(l, a.cap, kLogStep), n, l < 0 || l > a.cap};
     } else {
-        sh = paged_item(a.len, a.B, a.cap, kStep, a.target, a.least, true, item);
+        sh = paged_item(a.len, a.B, a.cap, kLogStep, a.target, a.least, true, item);
     }
     if (sh.seq < 0) return;                                 // workgroup-uniform
     const int b = sh.seq, len = sh.len;
-    const int steps = paged_steps(len, a.cap, kStep);
+    const int steps = paged_steps(len, a.cap, kLogStep);
     const int s_end = min(steps, (sh.part + 1) * sh.share);
     bool bad = sh.bad;
 
@@ -836,7 +836,7 @@ int launch_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
     if (const int rc = status_word(&a.status)) return rc;
     a.q = q, a.q_sb = q_sb, a.q_st = q_st, a.q_sh = q_sh, a.k = pages;
     a.pg = Pages{p_st, 0, h_st, table, t_st, static_cast<int>(width), static_cast<int>(n_pages)};
-    a.T = static_cast<int>(T), a.heads = static_cast<int>(Hq), a.step = 32;
+    a.T = static_cast<int>(T), a.heads = static_cast<int>(Hq);
     a.ps16 = static_cast<int>(ps / 16), a.len = len, a.B = static_cast<int>(B), a.cap = static_cast<int>(cap);
     a.Hq = static_cast<int>(T * Hq), a.Hkv = static_cast<int>(Hkv), a.R = static_cast<int>(R);
     a.head_tiles = static_cast<int>(cdiv(R * T, 16 * p.nc));
@@ -884,7 +884,7 @@ int launch_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
 #undef SPARDA_DQ
 #undef SPARDA_DQ_C
 #undef SPARDA_DQ_S
-    if (p.items > B) launch_paged_join(a, D, dtype, p.few, stream);
+    if (p.items > B) launch_paged_join(a, D, dtype, 5, p.few, stream);
     return check_hip(hipGetLastError(), "decode_paged_q4_kernel");
 }
 

@@ -1393,7 +1393,7 @@ def rotate_append_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table
         if r is not None:
             return r if type(r) is not int else _lib.fail("sparda_rotate_append_paged", r)
     dev = require_device(k_pages, v_pages, page_table, positions, q, k_new, v_new, cos, sin, cu_seqlens, out)
-    _inference_only(k_pages, v_pages, q, k_new, v_new)
+    _inference_only(k_pages, v_pages, q, k_new, v_new, cos, sin)
     _check_pages(k_pages, v_pages, page_table)
     code = _dtype_code(k_pages)
     if k_new.dtype != k_pages.dtype or v_new.dtype != k_pages.dtype:
@@ -1462,8 +1462,10 @@ def append_paged_q4(pages: torch.Tensor, page_table: torch.Tensor, positions: to
         if r is not None:
             return r if type(r) is not int else None if r == 0 else _lib.fail("sparda_append_paged_q4", r)
     dev = require_device(pages, page_table, positions, k_new, v_new, cu_seqlens, q, cos, sin, out)
-    _inference_only(q, k_new, v_new)
+    _inference_only(q, k_new, v_new, cos, sin)
     code = _dtype_code(k_new)
+    if k_new.dim() != 3:
+        raise ValueError(f"sparda: the new rows must be [N,Hkv,D], got {tuple(k_new.shape)}")
     P, ps, Hkv, D = _check_q4(pages, page_table, k_new.shape[-1])
     B, width = page_table.shape
     k_new, v_new = _new_rows(k_new, v_new, positions, cu_seqlens, B, Hkv, D)
@@ -1538,7 +1540,7 @@ def decode_paged_q4(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tens
     dev = require_device(q, pages, page_table, lengths, out)
     _inference_only(q)
     code = _dtype_code(q)
-    P, ps, Hkv, D = _check_q4(pages, page_table, q.shape[-1])
+    P, ps, Hkv, D = _check_q4(pages, page_table, q.shape[-1] if q.dim() > 0 else None)
     B, width = page_table.shape
     if q.dim() not in (3, 4) or q.shape[0] != B:
         raise ValueError(f"sparda: decode_paged_q4 takes q [{B},Hq,{D}] or [{B},T,Hq,{D}] for this cache, got {tuple(q.shape)}")

@@ -285,6 +285,30 @@ def test_two_streams_at_once():
     assert all(torch.equal(x, y) for i, r in got for x, y in zip(r, want[i]))
 
 
+def test_refusals_of_ranks_and_gradients():
+    print("[case] serving refusals", flush=True)
+    cos, sin = (dev(x) for x in rope_tables(64, 40))
+    pages, table, pos = torch.zeros(sparda.q4_page_shape(4, 16, 2, 64), dtype=torch.uint8, device=DEV), dev([[0, 1], [2, 3]]), dev([0, 0])
+    kp, vp = (torch.zeros(4, 16, 2, 64, dtype=BF, device=DEV) for _ in range(2))
+    q, k, v = (randn(2, h, 64, dtype=BF, seed=h).to(DEV) for h in (4, 2, 2))
+    for bad in (k[0, 0, 0], k[0, 0], k[0], k[None]):
+        with pytest.raises(ValueError):
+            sparda.append_paged_q4(pages, table, pos, bad, bad)
+        with pytest.raises(ValueError):
+            sparda.rotate_append_paged(kp, vp, table, pos, q, bad, bad, cos, sin)
+    for bad in (q[0, 0, 0], q[0, 0], q[0], q[None, None]):
+        with pytest.raises(ValueError):
+            sparda.decode_paged_q4(bad, pages, table, pos)
+    learned = cos.clone().requires_grad_()
+    for call in (lambda c: sparda.rotate_append_paged(kp, vp, table, pos, q, k, v, c, sin),
+                 lambda c: sparda.rotate_append_paged(kp, vp, table, pos, q, k, v, cos, c),
+                 lambda c: sparda.append_paged_q4(pages, table, pos, k, v, None, q, c, sin)):
+        with pytest.raises(RuntimeError):
+            call(learned)
+        with torch.no_grad():
+            assert call(learned).shape == q.shape
+
+
 def _models(vocab=500):
     base = dict(vocab_size=vocab, n_embd=256, n_head=8, n_kv_head=2, head_dim=32, ffn_dim=512, forecast_heads=2,
                 forecast_dim=32, context_length=64, block_size=16, top_k_blocks=8)
