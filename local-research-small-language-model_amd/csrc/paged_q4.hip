@@ -65,7 +65,7 @@ __device__ __forceinline__ void q4_codes(const float (&x)[8], _Float16 h, uint32
 // Eight elements of a row, as bf16 values in fp32 (round: fp32 rows are rounded)
 template <int DT, bool ONCE>
 __device__ __forceinline__ void q4_load8(const char* p, float (&x)[8]) {
-    auto load = [](const char* at) { return ONCE ? load_once(at) : *reinterpret_cast<const uint4*>(at); };
+    auto load = [](const char* at) { return load_row<ONCE>(at); };
     const uint4 a = load(p);
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
     if constexpr (DT == SPARDA_F32) {
@@ -141,7 +141,7 @@ __device__ __forceinline__ uint32_t q4_key_pack(const uint32_t (&c)[8]) {
 // as for 16-bit pages, four heads at a time. Bound by memory: 16000 rows of 32/8 heads of 128 (196.6 MB read,
 // 149.4 written) take 65.5 us = 5.3 TB/s (counted: 158 MB written, a row holding single bytes of the values' words). 64 rows of 12/4 heads of 64 take 5.2 us, a chain of five dependent
 // loads. Neighbouring rows on one XCD: 77.5 against 78.2 us (then), not taken.
-template <int DT, int D, bool ROT>
+template <int DT, int D, bool ROT, bool ONCE>
 __global__ void __launch_bounds__(256) append_paged_q4_kernel(RotateAppend a, char* __restrict__ pages) {
     constexpr int G = q4_groups(D), kEs = DT == SPARDA_F32 ? 4 : 2, kPer = D / 16;
     const int lane = threadIdx.x % kWave;
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(256) append_paged_q4_kernel(RotateAppend a, ch
     if constexpr (ROT) {
         const char* q = static_cast<const char*>(a.q) + t * a.q_st * kEs;
         char* qo = static_cast<char*>(a.q_out) + t * a.qo_st * kEs;
-        turn_heads<DT, D>(a, r.pos, off_table, a.Hq, [&](int h) { return q + h * a.q_sh * kEs; }, [&](int h) { return qo + h * a.qo_sh * kEs; });
+        turn_heads<DT, D, ONCE>(a, r.pos, off_table, a.Hq, [&](int h) { return q + h * a.q_sh * kEs; }, [&](int h) { return qo + h * a.qo_sh * kEs; });
     }
     if (!keep) return;
     const int key = static_cast<int>(r.row % 16);
@@ -167,8 +167,8 @@ __global__ void __launch_bounds__(256) append_paged_q4_kernel(RotateAppend a, ch
         const char* from = static_cast<const char*>(a.k_new) + (t * a.new_st + h * a.new_sh + c * 8) * kEs;
         char* tile = tiles + h * a.pg.h_st;
         float x[2][8];
-        q4_load8<DT, true>(from, x[0]);
-        q4_load8<DT, true>(from + D / 2 * kEs, x[1]);
+        q4_load8<DT, ONCE>(from, x[0]);
+        q4_load8<DT, ONCE>(from + D / 2 * kEs, x[1]);
         if constexpr (ROT) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) turn(x[0][e], x[1][e], cs[e], sn[e]);
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(256) append_paged_q4_kernel(RotateAppend a, ch
         const int h = i / (2 * kPer), dim = i % (2 * kPer) * 8;
         char* tile = tiles + h * a.pg.h_st;
         float x[8];
-        q4_load8<DT, true>(static_cast<const char*>(a.v_new) + (t * a.new_st + h * a.new_sh + dim) * kEs, x);
+        q4_load8<DT, ONCE>(static_cast<const char*>(a.v_new) + (t * a.new_st + h * a.new_sh + dim) * kEs, x);
         const _Float16 hh = q4_scale(lanes_max<(D >= 32 ? 4 : 2)>(q4_top(x)));
         uint32_t code[8];
         q4_codes(x, hh, code);
@@ -249,10 +249,16 @@ int launch_append_paged_q4(const RotateAppend& given, void* pages, int dtype, in
     if (!grid_fits(cdiv(a.N, 4), 256)) return set_error(SPARDA_ERR_SHAPE, "append_paged_q4: grid too large");
     if (const int rc = status_word(&a.status)) return rc;
     const dim3 grid(static_cast<unsigned>(cdiv(a.N, 4)));
-#define SPARDA_AQ(DT_, D_)                                                                                                  \
-    do {                                                                                                                    \
-        if (a.cos) hipLaunchKernelGGL((append_paged_q4_kernel<DT_, D_, true>), grid, dim3(256), 0, stream, a, static_cast<char*>(pages)); \
-        else hipLaunchKernelGGL((append_paged_q4_kernel<DT_, D_, false>), grid, dim3(256), 0, stream, a, static_cast<char*>(pages));      \
+    const bool once = rows_past_cache(a, D, dtype);
+#define SPARDA_AQ_O(DT_, D_, ROT_)                                                                                     \
+    do {                                                                                                               \
+        if (once) hipLaunchKernelGGL((append_paged_q4_kernel<DT_, D_, ROT_, true>), grid, dim3(256), 0, stream, a, static_cast<char*>(pages)); \
+        else hipLaunchKernelGGL((append_paged_q4_kernel<DT_, D_, ROT_, false>), grid, dim3(256), 0, stream, a, static_cast<char*>(pages));     \
+    } while (0)
+#define SPARDA_AQ(DT_, D_)                        \
+    do {                                          \
+        if (a.cos) SPARDA_AQ_O(DT_, D_, true);    \
+        else SPARDA_AQ_O(DT_, D_, false);         \
     } while (0)
 #define SPARDA_AQ_D(DT_)                      \
     switch (D) {                              \
@@ -265,6 +271,7 @@ int launch_append_paged_q4(const RotateAppend& given, void* pages, int dtype, in
     else SPARDA_AQ_D(SPARDA_BF16)
 #undef SPARDA_AQ_D
 #undef SPARDA_AQ
+#undef SPARDA_AQ_O
     return check_hip(hipGetLastError(), "append_paged_q4_kernel");
 }
 

@@ -12,7 +12,7 @@ namespace sparda {
 // values, copied. Bound by memory: 16000 rows of 32/8 heads of 128, 393 MB read and written, take 62 us
 // = 6.3 TB/s (part of it stays in the last-level cache), 77 in a row of calls = 5.1 TB/s, as large copies do; 64 rows of 12/4 heads of 64 5.0 us a call, of which the
 // host's part is 4.5.
-template <int DT, int D>
+template <int DT, int D, bool ONCE>
 __global__ void __launch_bounds__(256) rotate_append_paged_kernel(RotateAppend a, char* __restrict__ k, char* __restrict__ v) {
     constexpr int kEs = DT == SPARDA_F32 ? 4 : 2, kPieces = D * kEs / 16;
     const int lane = threadIdx.x % kWave;
@@ -27,14 +27,14 @@ __global__ void __launch_bounds__(256) rotate_append_paged_kernel(RotateAppend a
     char* qo = static_cast<char*>(a.q_out) + t * a.qo_st * kEs;
     const char* kn = static_cast<const char*>(a.k_new) + t * a.new_st * kEs;
     const int64_t at = (r.page * a.pg.p_st + r.row * a.pg.s_st) * kEs;
-    turn_heads<DT, D>(a, r.pos, off_table, a.Hq + (keep ? a.Hkv : 0),
+    turn_heads<DT, D, ONCE>(a, r.pos, off_table, a.Hq + (keep ? a.Hkv : 0),
                       [&](int h) { return h < a.Hq ? q + h * a.q_sh * kEs : kn + (h - a.Hq) * a.new_sh * kEs; },
                       [&](int h) { return h < a.Hq ? qo + h * a.qo_sh * kEs : k + at + (h - a.Hq) * a.pg.h_st * kEs; });
     if (!keep) return;
     const char* vn = static_cast<const char*>(a.v_new) + t * a.new_st * kEs;
     for (int i = lane; i < a.Hkv * kPieces; i += kWave) {
         const int h = i / kPieces, o = i % kPieces * 16;
-        *reinterpret_cast<uint4*>(v + at + h * a.pg.h_st * kEs + o) = load_once(vn + h * a.new_sh * kEs + o);
+        *reinterpret_cast<uint4*>(v + at + h * a.pg.h_st * kEs + o) = load_row<ONCE>(vn + h * a.new_sh * kEs + o);
     }
 }
 
@@ -43,9 +43,14 @@ int launch_rotate_append_paged(const RotateAppend& given, void* k, void* v, int 
     if (!grid_fits(cdiv(a.N, 4), 256)) return set_error(SPARDA_ERR_SHAPE, "rotate_append_paged: grid too large");
     if (const int rc = status_word(&a.status)) return rc;
     const dim3 grid(static_cast<unsigned>(cdiv(a.N, 4)));
-#define SPARDA_RA(DT_, D_)                                                                              \
-    hipLaunchKernelGGL((rotate_append_paged_kernel<DT_, D_>), grid, dim3(256), 0, stream, a, static_cast<char*>(k), \
-                       static_cast<char*>(v))
+    const bool once = rows_past_cache(a, D, dtype);
+#define SPARDA_RA(DT_, D_)                                                                                          \
+    do {                                                                                                            \
+        if (once) hipLaunchKernelGGL((rotate_append_paged_kernel<DT_, D_, true>), grid, dim3(256), 0, stream, a,    \
+                                     static_cast<char*>(k), static_cast<char*>(v));                                 \
+        else hipLaunchKernelGGL((rotate_append_paged_kernel<DT_, D_, false>), grid, dim3(256), 0, stream, a,        \
+                                static_cast<char*>(k), static_cast<char*>(v));                                      \
+    } while (0)
 #define SPARDA_RA_D(DT_)                      \
     switch (D) {                              \
         case 16: SPARDA_RA(DT_, 16); break;   \

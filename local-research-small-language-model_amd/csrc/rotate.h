@@ -30,13 +30,21 @@ struct RotateAppend {
     uint32_t* status;
 };
 
-// 16 bytes of a new row, which nothing reads again: loaded past the caches, so that they keep what is written.
-// The kernel over 16000 rows of 32/8 heads of 128 76.5 / 63.3 us, rows just written by another kernel 70.4 / 66.3; in
-// a row of such calls, where what earlier ones wrote still goes to memory, and up to 4096 rows no difference. (What is written here is read next and stays in the caches: stores past them make a write of 65
-// MB 3 us shorter and its reader 11 longer.)
-__device__ __forceinline__ uint4 load_once(const char* p) {
+// 16 bytes of a new row. ONCE: loaded past the caches, which nothing reads it from again. Calls that read and
+// write more than the last-level cache holds (256 MB) do so: 16000 rows of 32/8 heads of 128, cold, 76.5 / 63.3 us for
+// the kernel, just written by another one 70.4 / 66.3; in a row of such calls, where what earlier ones wrote still
+// goes to memory, no difference. Smaller ones find their rows in the caches, where the projection has just put
+// them: 4096 rows 32.3 / 33.6, 1501 of 12/4 heads of 64 in fp32 5.5 / 6.1. (What is written here is read next and stays in
+// the caches: stores past them make a write of 65 MB 3 us shorter and its reader 11 longer.)
+template <bool ONCE>
+__device__ __forceinline__ uint4 load_row(const char* p) {
     typedef uint32_t words __attribute__((ext_vector_type(4)));
-    return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const words*>(p)));
+    if constexpr (ONCE) return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const words*>(p)));
+    else return *reinterpret_cast<const uint4*>(p);
+}
+// whether a call does: queries and new rows, each read and (at most) written once
+inline bool rows_past_cache(const RotateAppend& a, int64_t D, int dtype) {
+    return 2 * a.N * (a.Hq + 2 * static_cast<int64_t>(a.Hkv)) * D * (dtype == SPARDA_F32 ? 4 : 2) > (256ll << 20);
 }
 
 // N angles of position pos from dim `at` on; NaN behind the tables (whose first row is loaded then: with the
@@ -98,7 +106,7 @@ __device__ __forceinline__ void turn_pieces(uint4& x, uint4& y, const float (&c)
 // Rotates `heads` heads of row t: head h from from(h) to to(h), both at its first element. A lane takes 16
 // bytes and the 16 that they are paired with, of four heads at a time; D/2 holds 1 to 16
 // such pieces, so that a lane's piece of the angles is the same for every head and is loaded once.
-template <int DT, int D, class From, class To>
+template <int DT, int D, bool ONCE, class From, class To>
 __device__ __forceinline__ void turn_heads(const RotateAppend& a, int64_t pos, bool off_table, int heads, From from, To to) {
     constexpr int kEs = DT == SPARDA_F32 ? 4 : 2, kVe = 16 / kEs, kPer = D / 2 / kVe, kAtOnce = kWave / kPer, kBatch = 4;
     const int lane = threadIdx.x % kWave, c = lane % kPer;
@@ -111,8 +119,8 @@ __device__ __forceinline__ void turn_heads(const RotateAppend& a, int64_t pos, b
             const int h = h0 + e * kAtOnce;
             if (h < heads) {
                 const char* p = from(h) + c * 16;
-                x[e] = load_once(p);
-                y[e] = load_once(p + D / 2 * kEs);
+                x[e] = load_row<ONCE>(p);
+                y[e] = load_row<ONCE>(p + D / 2 * kEs);
             }
         }
 #pragma unroll

@@ -285,6 +285,37 @@ def test_two_streams_at_once():
     assert all(torch.equal(x, y) for i, r in got for x, y in zip(r, want[i]))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+def test_writes_larger_than_the_caches(D, dtype):
+    """A call that reads and writes more than 256 MB loads its rows otherwise: the same bits as four calls of a quarter,
+    whose form the other tests compare with the formula."""
+    Hq, Hkv, ps = 6, 2, 64
+    N = ((128 << 20) // ((Hq + 2 * Hkv) * D * (2 if dtype == BF else 4)) // 4 + 1) * 4
+    print(f"[case] large writes {dtype} D={D} {N} rows", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(D)
+    q, k, v = (torch.randn(N, h, D, device=DEV, generator=g).to(dtype) for h in (Hq, Hkv, Hkv))
+    width = N // ps + 1
+    table = torch.randperm(width, device=DEV, generator=g).int().view(1, width)
+    angles = torch.rand(N, D // 2, device=DEV, generator=g) * 6
+    cos, sin = angles.cos(), angles.sin()
+    def pages():
+        return (torch.zeros(width, ps, Hkv, D, dtype=dtype, device=DEV), torch.zeros(width, ps, Hkv, D, dtype=dtype, device=DEV),
+                *(torch.zeros(sparda.q4_page_shape(width, ps, Hkv, D), dtype=torch.uint8, device=DEV) for _ in range(2)))
+    def write(p, a, b):
+        cu = dev([0, b - a])
+        pos = dev([a])
+        x = sparda.rotate_append_paged(p[0], p[1], table, pos, q[a:b], k[a:b], v[a:b], cos, sin, cu)
+        y = sparda.append_paged_q4(p[2], table, pos, k[a:b], v[a:b], cu, q[a:b], cos, sin)
+        sparda.append_paged_q4(p[3], table, pos, k[a:b], v[a:b], cu)
+        assert torch.equal(x, y)
+        return x
+    whole, parts = pages(), pages()
+    out = write(whole, 0, N)
+    assert torch.equal(out, torch.cat([write(parts, i * N // 4, (i + 1) * N // 4) for i in range(4)]))
+    assert all(torch.equal(a, b) for a, b in zip(whole, parts)) and sparda.status() == 0
+
+
 def test_refusals_of_ranks_and_gradients():
     print("[case] serving refusals", flush=True)
     cos, sin = (dev(x) for x in rope_tables(64, 40))
