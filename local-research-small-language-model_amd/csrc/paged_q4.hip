@@ -410,8 +410,8 @@ struct Q4Place {
 };
 
 // wavefronts of a SIMD
-constexpr int q4_waves(int DT, int D, int NC, bool REP) {
-    return (D == 128 && !REP ? 3 : 4) - (DT == SPARDA_F32 ? 1 : 0) - (NC > 1 ? 1 : 0);
+constexpr int q4_waves(int DT, int D, int NF, int NR) {
+    return (D == 128 && NF > 0 ? 3 : 4) - (DT == SPARDA_F32 ? 1 : 0) - (NF + NR > 1 ? 1 : 0);
 }
 
 }  // namespace
@@ -429,24 +429,26 @@ constexpr int q4_waves(int DT, int D, int NC, bool REP) {
 // the operand that P^T becomes, so P never leaves its lanes, and the order of the codes in memory is that
 // of the operands: no LDS but for the join of the wavefronts.
 //
-// Where the columns fit 16 / G of a tile's 16 (REP), every column stands in it once for each of its G groups: column
+// A tile whose columns fit 16 / G of its 16 (NR = 1; beside NF full ones) holds every column once for each of its G groups: column
 // h + kCols g takes the scores of group g alone (Q's operand is zero elsewhere) and carries the weights of
 // group g alone. The products of all groups then go into one accumulator, which starts at the
 // middle's share of the column (a constant), h is one number a lane and key, and the groups' sums are added
 // across lanes: 16 products a step of 32 keys instead of 32, and 210 vector instructions instead of 307 (D =
 // 128). Unpacking is 128 of them.
 //
-// 32 sequences of up to 16384, 32/8 heads of 128 (401 MB): 74.7 us a call = 5.4 TB/s; without REP and STREAM
-// 87.6, with REP 84.2. Loads alone took 74.5, arithmetic alone 72.9 without REP. 8 x 16384, 12/4 heads of 64 (29
-// MB): 12.3 of 15.5 us a call, a chain of three steps' reads under load; 16 x 5 tokens at up to 8000, 32/8 of
-// 128 (20 columns in two tiles): 35.5 of 41, where arithmetic alone is 35.8; 1 x 1000: 4.9 of 8, a launch and
-// four dependent loads. Steps staged through LDS one or two ahead took 97 and 105 us where this took 95.
-template <int DT, int D, int KW, int NC, bool REP, bool STREAM>
-__global__ void __launch_bounds__(KW* kWave, q4_waves(DT, D, NC, REP))
+// 32 sequences of up to 16384, 32/8 heads of 128 (401 MB): 74.7 us a call = 5.4 TB/s; without a repeated tile and
+// STREAM 87.6, without STREAM 84.2. Loads alone took 74.5, arithmetic alone 72.9 before. 8 x 16384, 12/4 heads of 64 (29
+// MB): 12.3 of 14.8 us a call, a chain of three steps' reads under load; 16 x 5 tokens at up to 8000, 32/8 of
+// 128 (20 columns: a full tile and a repeated one): 32.6 of 36.5, vector issue; in two full tiles 35.5 of 41. 1 x
+// 1000: 4.9 of 8, a launch and four dependent loads. Steps staged through LDS one or two ahead took 97 and 105 us where this took 95.
+template <int DT, int D, int KW, int NF, int NR, bool STREAM>
+__global__ void __launch_bounds__(KW* kWave, q4_waves(DT, D, NF, NR))
 decode_paged_q4_kernel(PagedDecode a) {
     constexpr int G = q4_groups(D), kTerms = DT == SPARDA_F32 ? 3 : 1, kLogStep = 5, kStep = 1 << kLogStep, kEs = DT == SPARDA_F32 ? 4 : 2;
-    constexpr int kCols = REP ? 16 / G : 16;                 // columns of a tile
-    static_assert(!REP || (NC == 1 && G > 1), "one tile, of several groups");
+    constexpr int NC = NF + NR, kCols = 16 / G;              // tiles; columns of a repeated one
+    static_assert(NR == 0 || (NR == 1 && G > 1), "one repeated tile, of several groups");
+    constexpr bool REP = NR > 0;
+    constexpr int kRep = REP ? NF : 0;                       // the repeated tile (tiles before it are full)
     extern __shared__ float lds[];
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
@@ -454,7 +456,7 @@ decode_paged_q4_kernel(PagedDecode a) {
     const int groups = a.Hkv * a.head_tiles;
     const int item = blockIdx.x / groups, gt = blockIdx.x % groups;
     const int g = gt / a.head_tiles, col0 = gt % a.head_tiles * (16 * NC);
-    const int ncol = a.R * a.T - col0 < 16 * NC ? a.R * a.T - col0 : 16 * NC;   // columns of the workgroup
+    const int ncol = a.R * a.T - col0 < 16 * NC ? a.R * a.T - col0 : 16 * NC;   // columns of the workgroup (all, where one is repeated)
     Share sh;
     if (a.whole) {
         const int l = __builtin_amdgcn_readfirstlane(a.len[item]), n = l < 0 ? 0 : l > a.cap ? a.cap : l;
@@ -471,20 +473,21 @@ decode_paged_q4_kernel(PagedDecode a) {
     bf16x8 middle;
 #pragma unroll
     for (int e = 0; e < 8; ++e) middle[e] = static_cast<__bf16>(-24.0f);
-    // this lane's columns of Q (REP: column h of group g in lane h + kCols g, in the product with that group's codes alone)
+    // this lane's columns of Q (a repeated tile's column h of group g in lane h + kCols g, in the product with that group's codes alone)
     const int mine = c16 / kCols;
     int lim[NC];                                             // positions a column sees
     bf16x8 qr[NC][G][kTerms];
-    f32x4 start{0.f, 0.f, 0.f, 0.f};                         // REP: -24 times the sum of the column's q in its group
+    f32x4 start{0.f, 0.f, 0.f, 0.f};                         // repeated tile: -24 times the sum of the column's q in its group
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const int at = 16 * c + c16 % kCols, col = col0 + (at < ncol ? at : ncol - 1), tok = col / a.R, head = g * a.R + col % a.R;
+        const bool repeated = REP && c == kRep;
+        const int at = 16 * c + (repeated ? c16 % kCols : c16), col = col0 + (at < ncol ? at : ncol - 1), tok = col / a.R, head = g * a.R + col % a.R;
         lim[c] = len - a.T + 1 + tok;
         const char* q = static_cast<const char*>(a.q) + (b * a.q_sb + tok * a.q_st + head * a.q_sh) * kEs;
 #pragma unroll
         for (int i = 0; i < G; ++i) {
             float x[8];
-            if (at < ncol && 32 * i + 8 * grp < D && (!REP || mine == i)) {
+            if (at < ncol && 32 * i + 8 * grp < D && (!repeated || mine == i)) {
                 q4_load8<DT, false>(q + (32 * i + 8 * grp) * kEs, x);
                 if (a.negate) {
 #pragma unroll
@@ -495,7 +498,7 @@ decode_paged_q4_kernel(PagedDecode a) {
                 for (int e = 0; e < 8; ++e) x[e] = 0.0f;
             }
             q4_split<kTerms>(x, qr[c][i]);
-            if constexpr (REP) {
+            if (repeated) {
 #pragma unroll
                 for (int n = 0; n < kTerms; ++n) start = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, qr[c][i][n], start, 0, 0, 0);
             }
@@ -508,7 +511,7 @@ decode_paged_q4_kernel(PagedDecode a) {
     const char* kv = static_cast<const char*>(a.k) + g * a.pg.h_st;
     const int last_tile = (len - 1) / 16;
     const int o_keys = (c16 * 4 + grp) * 4 * G, o_values = 256 * G + lane * 4 * G;
-    const int o_scales = 512 * G + grp * 8 * G + (REP ? (c16 % 4 * G + mine) * 2 : 0);
+    const int o_scales = 512 * G + grp * 8 * G, o_own = o_scales + (c16 % 4 * G + mine) * 2;
     int u = sh.part * sh.share + wave;
     int page = 2 * u / a.ps16, rem = 2 * u % a.ps16;
     const int adv_p = 2 * KW / a.ps16, adv_r = 2 * KW % a.ps16;
@@ -523,7 +526,8 @@ decode_paged_q4_kernel(PagedDecode a) {
         return at;
     };
     uint32_t xk[2][G], xv[2][G];                             // the codes of a step, as loaded
-    _Float16 hk[2][REP ? 1 : 4][REP ? 1 : G], hv[2][REP ? 1 : 4][REP ? 1 : G];   // REP: position 4 grp + c16 % 4 and the lane's group
+    _Float16 hk[2][4][G], hv[2][4][G];                       // full tiles: positions 4 grp .. 4 grp + 3
+    _Float16 rk[2], rv[2];                                   // the repeated one: position 4 grp + c16 % 4, the lane's group
     const char* base[2];
     auto locate = [&](const Q4Place& at) __attribute__((always_inline)) {
 #pragma unroll
@@ -538,23 +542,23 @@ decode_paged_q4_kernel(PagedDecode a) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             q4_load_words<G, STREAM>(base[t] + o_keys, xk[t]);
-            if constexpr (REP) hk[t][0][0] = *reinterpret_cast<const _Float16*>(base[t] + o_scales);
-            else q4_load_scales<G>(base[t] + o_scales, hk[t]);
+            if constexpr (REP) rk[t] = *reinterpret_cast<const _Float16*>(base[t] + o_own);
+            if constexpr (NF > 0) q4_load_scales<G>(base[t] + o_scales, hk[t]);
         }
     };
     auto load_values = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             q4_load_words<G, STREAM>(base[t] + o_values, xv[t]);
-            if constexpr (REP) hv[t][0][0] = *reinterpret_cast<const _Float16*>(base[t] + o_scales + 32 * G);
-            else q4_load_scales<G>(base[t] + o_scales + 32 * G, hv[t]);
+            if constexpr (REP) rv[t] = *reinterpret_cast<const _Float16*>(base[t] + o_own + 32 * G);
+            if constexpr (NF > 0) q4_load_scales<G>(base[t] + o_scales + 32 * G, hv[t]);
         }
     };
 
     // m: the columns' references, in the scores' own units, l: this lane's part of their sums
     float m[NC], ref[NC], l[NC];
     const float slack = 16.0f / a.scale_log2;
-    f32x4 o[NC][G][2], less{0.f, 0.f, 0.f, 0.f};             // less: REP: -24 times the sum of the column's weights
+    f32x4 o[NC][G][2], less{0.f, 0.f, 0.f, 0.f};             // less: repeated tile: -24 times the sum of the column's weights
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         m[c] = -__builtin_inff(), ref[c] = l[c] = 0.0f;
@@ -566,37 +570,34 @@ decode_paged_q4_kernel(PagedDecode a) {
     auto scores = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            if constexpr (REP) {
-                f32x4 y = start;
+            f32x4 all = start;                               // the repeated tile's
 #pragma unroll
-                for (int i = 0; i < G; ++i) {
-                    const bf16x8 ka = q4_key_operand(xk[t][i], masks);
-#pragma unroll
-                    for (int n = 0; n < kTerms; ++n) y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qr[0][i][n], y, 0, 0, 0);
-                }
-                const float h = static_cast<float>(hk[t][0][0]);
-                s[0][t][0] = q4_group_sum<G>(q4_by_quad<0>(y[0], h));
-                s[0][t][1] = q4_group_sum<G>(q4_by_quad<1>(y[1], h));
-                s[0][t][2] = q4_group_sum<G>(q4_by_quad<2>(y[2], h));
-                s[0][t][3] = q4_group_sum<G>(q4_by_quad<3>(y[3], h));
-                continue;
-            }
-#pragma unroll
-            for (int c = 0; c < NC; ++c) s[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int c = 0; c < NF; ++c) s[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < G; ++i) {
                 const bf16x8 ka = q4_key_operand(xk[t][i], masks);
+                if constexpr (REP) {
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
+                    for (int n = 0; n < kTerms; ++n) all = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qr[kRep][i][n], all, 0, 0, 0);
+                }
+#pragma unroll
+                for (int c = 0; c < NF; ++c) {
                     f32x4 y{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int n = 0; n < kTerms; ++n) y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, qr[c][i][n], y, 0, 0, 0);
 #pragma unroll
                     for (int n = 0; n < kTerms; ++n) y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qr[c][i][n], y, 0, 0, 0);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[c][t][e] = __builtin_fmaf(y[e], static_cast<float>(hk[t][REP ? 0 : e][REP ? 0 : i]), s[c][t][e]);
+                    for (int e = 0; e < 4; ++e) s[c][t][e] = __builtin_fmaf(y[e], static_cast<float>(hk[t][e][i]), s[c][t][e]);
                 }
-                __builtin_amdgcn_sched_barrier(0);           // (operands of one group at a time: registers)
+                if constexpr (NF > 0) __builtin_amdgcn_sched_barrier(0);   // (operands of one group at a time: registers)
+            }
+            if constexpr (REP) {
+                const float h = static_cast<float>(rk[t]);
+                s[kRep][t][0] = q4_group_sum<G>(q4_by_quad<0>(all[0], h));
+                s[kRep][t][1] = q4_group_sum<G>(q4_by_quad<1>(all[1], h));
+                s[kRep][t][2] = q4_group_sum<G>(q4_by_quad<2>(all[2], h));
+                s[kRep][t][3] = q4_group_sum<G>(q4_by_quad<3>(all[3], h));
             }
         }
     };
@@ -621,7 +622,7 @@ decode_paged_q4_kernel(PagedDecode a) {
                 l[c] *= alpha;
 #pragma unroll
                 for (int i = 0; i < G; ++i) o[c][i][0] *= alpha, o[c][i][1] *= alpha;
-                if constexpr (REP) less *= alpha;
+                if (REP && c == kRep) less *= alpha;
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -630,47 +631,44 @@ decode_paged_q4_kernel(PagedDecode a) {
                 l[c] += p[c][e];
             }
         }
+        bf16x8 own[kTerms];                                  // the repeated tile's weights, of the lane's group
         if constexpr (REP) {
-            const int left = lim[0] - v * kStep - 4 * grp;
+            const int left = lim[kRep] - v * kStep - 4 * grp;
             float ph[8];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const float h = static_cast<float>(hv[t][0][0]);
-                ph[4 * t] = q4_by_quad<0>(p[0][4 * t], h);
-                ph[4 * t + 1] = q4_by_quad<1>(p[0][4 * t + 1], h);
-                ph[4 * t + 2] = q4_by_quad<2>(p[0][4 * t + 2], h);
-                ph[4 * t + 3] = q4_by_quad<3>(p[0][4 * t + 3], h);
+                const float h = static_cast<float>(rv[t]);
+                ph[4 * t] = q4_by_quad<0>(p[kRep][4 * t], h);
+                ph[4 * t + 1] = q4_by_quad<1>(p[kRep][4 * t + 1], h);
+                ph[4 * t + 2] = q4_by_quad<2>(p[kRep][4 * t + 2], h);
+                ph[4 * t + 3] = q4_by_quad<3>(p[kRep][4 * t + 3], h);
             }
             if constexpr (kMask) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) ph[e] = 16 * (e / 4) + e % 4 < left ? ph[e] : 0.0f;   // (as below)
+                for (int e = 0; e < 8; ++e) ph[e] = 16 * (e / 4) + e % 4 < left ? ph[e] : 0.0f;   // (a number behind the column's positions may be anything)
             }
-            bf16x8 pb[kTerms];
-            q4_split<kTerms>(ph, pb);
+            q4_split<kTerms>(ph, own);
 #pragma unroll
-            for (int n = 0; n < kTerms; ++n) less = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, pb[n], less, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < G; ++i) {
-                const bf16x8 v0 = q4_value_operand<0>(xv[0][i], xv[1][i], masks), v1 = q4_value_operand<1>(xv[0][i], xv[1][i], masks);
-#pragma unroll
-                for (int n = 0; n < kTerms; ++n) {
-                    o[0][i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pb[n], o[0][i][0], 0, 0, 0);
-                    o[0][i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pb[n], o[0][i][1], 0, 0, 0);
-                }
-            }
-            return;
+            for (int n = 0; n < kTerms; ++n) less = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, own[n], less, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < G; ++i) {
             const bf16x8 v0 = q4_value_operand<0>(xv[0][i], xv[1][i], masks), v1 = q4_value_operand<1>(xv[0][i], xv[1][i], masks);
+            if constexpr (REP) {
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
+                for (int n = 0; n < kTerms; ++n) {
+                    o[kRep][i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, own[n], o[kRep][i][0], 0, 0, 0);
+                    o[kRep][i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, own[n], o[kRep][i][1], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < NF; ++c) {
                 const int left = lim[c] - v * kStep - 4 * grp;
                 float ph[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    ph[e] = __builtin_fmaf(p[c][e], static_cast<float>(hv[e / 4][REP ? 0 : e % 4][REP ? 0 : i]), 0.0f);
-                    if (kMask) ph[e] = 16 * (e / 4) + e % 4 < left ? ph[e] : 0.0f;   // (a number behind the column's positions may be anything)
+                    ph[e] = __builtin_fmaf(p[c][e], static_cast<float>(hv[e / 4][e % 4][i]), 0.0f);
+                    if (kMask) ph[e] = 16 * (e / 4) + e % 4 < left ? ph[e] : 0.0f;   // (as above)
                 }
                 bf16x8 pb[kTerms];
                 q4_split<kTerms>(ph, pb);
@@ -682,7 +680,7 @@ decode_paged_q4_kernel(PagedDecode a) {
                     o[c][i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pb[n], o[c][i][1], 0, 0, 0);
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (NF > 0) __builtin_amdgcn_sched_barrier(0);
         }
     };
     if (u < s_end) {
@@ -724,19 +722,21 @@ decode_paged_q4_kernel(PagedDecode a) {
         if (nh <= 0) break;                                   // workgroup-uniform
         if (c > 0) __syncthreads();                           // the last ones have been read
         l[c] = pair32_sum(pair16_sum(l[c]));
-        if (c16 % kCols < nh) {
+        const bool repeated = REP && c == kRep;
+        const int cc16 = repeated ? c16 % kCols : c16;        // the lane's column
+        if (cc16 < nh) {
 #pragma unroll
             for (int i = 0; i < G; ++i) {
-                if (REP && mine != i) continue;               // (other groups' weights)
+                if (repeated && mine != i) continue;          // (other groups' weights)
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int d = 32 * i + 2 * (4 * grp + e) + j;
-                        if (d < D) lo[(wave * a.lds_heads + c16 % kCols) * (D + 4) + d] = 2.0f * (o[c][i][j][e] + less[e]);
+                        if (d < D) lo[(wave * a.lds_heads + cc16) * (D + 4) + d] = 2.0f * (repeated ? o[c][i][j][e] + less[e] : o[c][i][j][e]);
                     }
             }
-            if (grp == 0 && mine == 0) {
+            if (grp == 0 && (!repeated || mine == 0)) {
                 lm[(wave * 16 + c16) * 2] = m[c] == -__builtin_inff() ? m[c] : ref[c];   // (log2 units from here)
                 lm[(wave * 16 + c16) * 2 + 1] = l[c];
             }
@@ -783,7 +783,9 @@ namespace {
 // - Two tiles of 16 columns share the unpacked codes where there are more than 16 columns and the products
 //   are single: 16 x 5 tokens of 32/8 heads of 128 at 8000 (20 columns) 41 us, 47 with a tile a workgroup. In
 //   fp32 the terms of two tiles do not fit the registers.
-// - Columns that fit 16 / G of a tile stand in it G times (REP above); a call of 20 columns would take five such tiles.
+// - Columns that fit 16 / G of a tile stand in it G times, and so do those that are left of a full tile (one token of
+//   32/8 heads of 128 88 / 84 us at 32 x 16384; five tokens 41 / 36.5 at 16 x 8000). More would take several such tiles, at 76
+//   vector instructions a step each where a full tile takes 120.
 // - A sequence is one item, with no join, up to 16 steps of 32 keys, or up to 64 where the sequences fill
 //   half of the chip by themselves; otherwise there are as many items as workgroups run at a time (256 CUs
 //   times the wavefronts that a SIMD holds), so that all shares are done in one round: one too many
@@ -796,8 +798,7 @@ namespace {
 //   last call and loads past it: 32 x 16384 84.2 / 74.4 us. Smaller ones may: 16 x 5 tokens at 8000 repeated over few
 //   caches 40.9 / 44.2 with such loads, over twelve 49.4 / 48.2; 20 x 9000 32.0 / 33.2 and 36.7 / 33.5.
 struct Q4Plan {
-    int nc;                  // column tiles of a workgroup
-    bool rep;                // the columns of one tile, once for every group
+    int nf, nr;              // column tiles of a workgroup: full ones, one with its columns once for every group
     int64_t target, least;   // items aimed at, steps of the smallest item
     int64_t items, groups;   // items at most, workgroups an item
     bool few;                // a sequence has few items in the mean
@@ -805,13 +806,16 @@ struct Q4Plan {
 };
 Q4Plan q4_plan(int64_t B, int64_t T, int64_t cap, int64_t Hq, int64_t Hkv, int64_t D, int dtype) {
     const int64_t cols = Hq / Hkv * T, steps = cdiv(cap, 32);
-    Q4Plan p{dtype == SPARDA_BF16 && cols > 16 ? 2 : 1, D >= 64 && cols <= 16 / (D / 32), 1, 4, 0, 0, false, false};
-    p.groups = Hkv * cdiv(cols, 16 * p.nc);
+    Q4Plan p{dtype == SPARDA_BF16 && cols > 16 ? 2 : 1, 0, 1, 4, 0, 0, false, false};
+    const int64_t few = D >= 64 ? 16 / (D / 32) : 0;   // columns of a repeated tile
+    if (cols <= few) p.nf = 0, p.nr = 1;
+    else if (dtype == SPARDA_BF16 && cols > 16 && cols <= 16 + few) p.nf = 1, p.nr = 1;
+    p.groups = Hkv * cdiv(cols, 16 * (p.nf + p.nr));
     if (steps <= 16 || (steps <= 64 && B * p.groups >= 128)) {
         p.least = steps;
     } else {
         // (items are target + B at most, target + B / 2 in the mean, sqrt(B / 12) to either side)
-        const int64_t slots = 256 * q4_waves(dtype, static_cast<int>(D), p.nc, p.rep);
+        const int64_t slots = 256 * q4_waves(dtype, static_cast<int>(D), p.nf, p.nr);
         int64_t margin = 0;                          // ceil(0.6 sqrt(B))
         while (margin * margin * 25 < B * 9) ++margin;
         p.target = slots / p.groups - B / 2 - margin;
@@ -846,7 +850,7 @@ int launch_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
     a.T = static_cast<int>(T), a.heads = static_cast<int>(Hq);
     a.ps16 = static_cast<int>(ps / 16), a.len = len, a.B = static_cast<int>(B), a.cap = static_cast<int>(cap);
     a.Hq = static_cast<int>(T * Hq), a.Hkv = static_cast<int>(Hkv), a.R = static_cast<int>(R);
-    a.head_tiles = static_cast<int>(cdiv(R * T, 16 * p.nc));
+    a.head_tiles = static_cast<int>(cdiv(R * T, 16 * (p.nf + p.nr)));
     a.target = static_cast<int>(p.target), a.least = static_cast<int>(p.least);
     a.whole = p.items <= B;
     a.lds_heads = static_cast<int>(R * T < 16 ? R * T : 16);
@@ -855,27 +859,33 @@ int launch_decode_paged_q4(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = workspace ? a.part_o + p.items * a.Hq * D : nullptr;
     const dim3 grid(static_cast<unsigned>(p.items * p.groups));
-#define SPARDA_DQ_S(DT_, D_, NC_, REP_, S_)                                                       \
-    hipLaunchKernelGGL((decode_paged_q4_kernel<DT_, D_, 4, NC_, REP_, S_>), grid, dim3(4 * kWave), \
+#define SPARDA_DQ_S(DT_, D_, NF_, NR_, S_)                                                        \
+    hipLaunchKernelGGL((decode_paged_q4_kernel<DT_, D_, 4, NF_, NR_, S_>), grid, dim3(4 * kWave), \
                        4 * (a.lds_heads * ((D_) + 4) + 33) * sizeof(float), stream, a)
-#define SPARDA_DQ_C(DT_, D_, NC_, REP_)                                                           \
+#define SPARDA_DQ_C(DT_, D_, NF_, NR_)                                                            \
     do {                                                                                          \
-        if (p.stream) SPARDA_DQ_S(DT_, D_, NC_, REP_, true);                                      \
-        else SPARDA_DQ_S(DT_, D_, NC_, REP_, false);                                              \
+        if (p.stream) SPARDA_DQ_S(DT_, D_, NF_, NR_, true);                                       \
+        else SPARDA_DQ_S(DT_, D_, NF_, NR_, false);                                               \
     } while (0)
 #define SPARDA_DQ(DT_, D_)                                                                        \
     do {                                                                                          \
         if constexpr (D_ >= 64) {                                                                 \
-            if (p.rep) {                                                                          \
-                SPARDA_DQ_C(DT_, D_, 1, true);                                                    \
+            if (p.nr > 0 && p.nf == 0) {                                                          \
+                SPARDA_DQ_C(DT_, D_, 0, 1);                                                       \
+                break;                                                                            \
+            }                                                                                     \
+        }                                                                                         \
+        if constexpr (D_ >= 64 && DT_ == SPARDA_BF16) {                                           \
+            if (p.nr > 0) {                                                                       \
+                SPARDA_DQ_C(DT_, D_, 1, 1);                                                       \
                 break;                                                                            \
             }                                                                                     \
         }                                                                                         \
         if constexpr (DT_ == SPARDA_BF16) {                                                       \
-            if (p.nc == 2) SPARDA_DQ_C(DT_, D_, 2, false);                                        \
-            else SPARDA_DQ_C(DT_, D_, 1, false);                                                  \
+            if (p.nf == 2) SPARDA_DQ_C(DT_, D_, 2, 0);                                            \
+            else SPARDA_DQ_C(DT_, D_, 1, 0);                                                      \
         } else {                                                                                  \
-            SPARDA_DQ_C(DT_, D_, 1, false);                                                       \
+            SPARDA_DQ_C(DT_, D_, 1, 0);                                                           \
         }                                                                                         \
     } while (0)
 #define SPARDA_DQ_D(DT_)                      \

@@ -232,7 +232,7 @@ def test_decode_over_many_shares(dtype, Hq, Hkv, D, lengths):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
-@pytest.mark.parametrize("Hq,Hkv,D,T", [(12, 4, 64, 1), (8, 2, 128, 1), (8, 1, 128, 5), (34, 2, 64, 2), (4, 2, 16, 3), (8, 8, 32, 1)])
+@pytest.mark.parametrize("Hq,Hkv,D,T", [(12, 4, 64, 1), (8, 2, 128, 1), (8, 1, 128, 5), (4, 1, 128, 5), (6, 2, 64, 7), (34, 2, 64, 2), (4, 2, 16, 3), (8, 8, 32, 1)])
 def test_decode_with_tables_of_large_capacity(dtype, Hq, Hkv, D, T):
     """More codes than the last-level cache holds, were the tables full: other loads, the same results."""
     G = max(1, D // 32)
@@ -246,7 +246,8 @@ def test_decode_with_tables_of_large_capacity(dtype, Hq, Hkv, D, T):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
-@pytest.mark.parametrize("Hq,Hkv,D", [(4, 1, 128), (5, 1, 128), (8, 1, 64), (9, 1, 64), (2, 2, 128), (16, 1, 32)])
+@pytest.mark.parametrize("Hq,Hkv,D", [(4, 1, 128), (5, 1, 128), (8, 1, 64), (9, 1, 64), (2, 2, 128), (16, 1, 32), (16, 1, 128), (17, 1, 128),
+                                      (40, 2, 128), (21, 1, 128), (17, 1, 64), (48, 2, 64), (25, 1, 64), (18, 1, 32), (24, 1, 16)])
 def test_decode_at_the_number_of_columns_that_changes_the_form(dtype, Hq, Hkv, D):
     lengths = [333, 31, 32, 0, 2500]
     print(f"[case] q4 columns {dtype} {Hq}/{Hkv}x{D}", flush=True)
