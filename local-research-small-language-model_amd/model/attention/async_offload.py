@@ -243,6 +243,10 @@ class HipAsyncOffloadAttention(BaseAttention):
         return {"steps": n, "transfer_ms": tr / n, "exposed_ms": ex / n,
                 "overlap": 1.0 - ex / tr if tr > 0 else 0.0}
 
+    def rows_ignore_later(self, T: int) -> bool:
+        """Prompts are attended to densely, at any length."""
+        return True
+
     def forward(self, x: torch.Tensor, rotary_emb: RotaryEmbedding, kv_cache=None, mask=None,
                 is_causal: bool = True, forecast_vector: Optional[torch.Tensor] = None, **kwargs) -> torch.Tensor:
         if mask is not None:

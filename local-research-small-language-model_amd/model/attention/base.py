@@ -56,3 +56,8 @@ class BaseAttention(nn.Module, ABC):
     def forward(self, x: torch.Tensor, rotary_emb: RotaryEmbedding, kv_cache: Optional[KVCache] = None,
                 mask: Optional[torch.Tensor] = None, is_causal: bool = True, **kwargs) -> torch.Tensor:
         """x [B,T,n_embd] -> [B,T,n_embd]."""
+
+    def rows_ignore_later(self, T: int) -> bool:
+        """Whether, in uncached causal forwards of up to T tokens, no row's output depends on a
+        later token, through the choice of its blocks for instance. False where that is not known."""
+        return False

@@ -148,6 +148,17 @@ class HipSparseAttention(BaseAttention):
         return self.mode == "dense" or nb <= 2 or (
             self.mode == "forecast" and (forecast_vector is None or self.layer_idx == 0))
 
+    def rows_ignore_later(self, T: int) -> bool:
+        """Dense attention does, and the static window. A forecast's choice does not: a block is scored by the
+        mean of all its keys, those behind the row among them, unless the row's causal blocks are all chosen
+        whatever their scores (or layer 0 attends densely). Past CHUNKED_GATHER_MIN_T rows of a block share a list."""
+        if self.mode == "dense":
+            return True
+        if T > CHUNKED_GATHER_MIN_T:
+            return False
+        blocks = (T + self.block_size - 1) // self.block_size
+        return self.mode == "static" or self.layer_idx == 0 or blocks <= max(2, self.top_k_blocks)
+
     def _selection(self, xq, xk, forecast_vector, is_causal):
         """The allowed-block lists of a prefill (sparse.py:201-253): None for
         the dense fallback, else router lists (forecast) or the static window

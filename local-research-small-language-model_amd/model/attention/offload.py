@@ -181,6 +181,10 @@ class HipOffloadAttention(BaseAttention):
         self.last_profile = {"bytes_transferred": nbytes}
         return self.wo(out.view(B, 1, self.n_head * self.head_dim))
 
+    def rows_ignore_later(self, T: int) -> bool:
+        """Prompts are attended to densely, at any length."""
+        return True
+
     def forward(self, x: torch.Tensor, rotary_emb: RotaryEmbedding, kv_cache=None, mask=None,
                 is_causal: bool = True, forecast_vector: Optional[torch.Tensor] = None, **kwargs) -> torch.Tensor:
         if mask is not None:

@@ -117,7 +117,10 @@ class SparDAResearchModel(nn.Module):
         the reference does. With ``draft_model`` (a smaller model of the same
         vocabulary; one sequence, no caches) it drafts ``num_drafts`` tokens, one forward of this
         model scores them all, and ``sparda.verify_drafts`` keeps those that this model's
-        distribution accepts and draws the next, as if every token had been drawn from it."""
+        distribution accepts and draws the next, as if every token had been drawn from it. That takes rows
+        that do not depend on the drafts behind them: a token is drafted only while it fits the context and
+        ``rows_ignore_later`` holds (dense, static and offloaded attention; forecast attention up to
+        ``top_k_blocks`` blocks). Beyond, every token takes a forward of its own and the draft model is not run."""
         self.eval()
         if draft_model is not None:
             return self._generate_drafted(input_ids, max_new_tokens, temperature, top_k, eos_token_id, kv_caches,
@@ -144,6 +147,10 @@ class SparDAResearchModel(nn.Module):
                 logits = self.forward(nxt, kv_caches=kv_caches)["logits"][:, -1, :]
         return input_ids
 
+    def rows_ignore_later(self, T: int) -> bool:
+        """Whether no row of an uncached forward of up to T tokens depends on a later one, in any layer."""
+        return all(block.attention.rows_ignore_later(T) for block in self.layers)
+
     def _generate_drafted(self, input_ids, max_new_tokens, temperature, top_k, eos_token_id, kv_caches, draft_model,
                           num_drafts) -> torch.Tensor:
         if input_ids.shape[0] != 1 or kv_caches is not None:
@@ -165,7 +172,11 @@ class SparDAResearchModel(nn.Module):
 
         end = input_ids.shape[1] + max_new_tokens
         while input_ids.shape[1] < end:
-            K = min(num_drafts, end - input_ids.shape[1] - 1, self.config.context_length - 1)
+            # (every scored row sees what a forward of the tokens before it alone sees: all of them, and no draft)
+            n = input_ids.shape[1]
+            K = max(0, min(num_drafts, end - n - 1, self.config.context_length - n))
+            while K > 0 and not self.rows_ignore_later(n + K):
+                K -= 1
             ids, probs = input_ids, []
             for _ in range(K):
                 x = kept(logits(draft_model, ids, 1))[:, 0]
@@ -175,11 +186,11 @@ class SparDAResearchModel(nn.Module):
                 else:
                     nxt = torch.argmax(x, dim=-1, keepdim=True)
                 ids = torch.cat((ids, nxt), dim=1)
-            tokens, n = sparda.verify_drafts(kept(logits(self, ids, K + 1)), ids[:, input_ids.shape[1]:].int(),
-                                             torch.rand(1, K + 1, device=ids.device),
-                                             draft_probs=torch.stack(probs, 1) if probs else None,
-                                             temperature=max(float(temperature), 0.0))
-            new = tokens[:, :int(n) + 1].long()
+            tokens, taken = sparda.verify_drafts(kept(logits(self, ids, K + 1)), ids[:, n:].int(),
+                                                 torch.rand(1, K + 1, device=ids.device),
+                                                 draft_probs=torch.stack(probs, 1) if probs else None,
+                                                 temperature=max(float(temperature), 0.0))
+            new = tokens[:, :int(taken) + 1].long()
             if eos_token_id is not None and (new == eos_token_id).any():
                 stop = int((new[0] == eos_token_id).nonzero()[0])
                 return torch.cat((input_ids, new[:, :stop + 1]), dim=1)
