@@ -120,7 +120,8 @@ class SparDAResearchModel(nn.Module):
         distribution accepts and draws the next, as if every token had been drawn from it. That takes rows
         that do not depend on the drafts behind them: a token is drafted only while it fits the context and
         ``rows_ignore_later`` holds (dense, static and offloaded attention; forecast attention up to
-        ``top_k_blocks`` blocks). Beyond, every token takes a forward of its own and the draft model is not run."""
+        ``top_k_blocks`` blocks). Beyond, every token takes a forward of its own and the draft model is not run.
+        Logits that hold no distribution (NaN, +inf, or all -inf) raise RuntimeError where a token is sampled from them."""
         self.eval()
         if draft_model is not None:
             return self._generate_drafted(input_ids, max_new_tokens, temperature, top_k, eos_token_id, kv_caches,
@@ -181,16 +182,23 @@ class SparDAResearchModel(nn.Module):
             for _ in range(K):
                 x = kept(logits(draft_model, ids, 1))[:, 0]
                 if temperature > 0.0:
-                    probs.append(F.softmax(x / temperature, dim=-1))
+                    p = F.softmax(x / temperature, dim=-1)
+                    # (a row without a distribution, NaN all over, drafts token 0)
+                    probs.append(torch.where(p.isnan(), (torch.arange(p.shape[-1], device=p.device) == 0).to(p.dtype), p))
                     nxt = torch.multinomial(probs[-1], num_samples=1)
                 else:
                     nxt = torch.argmax(x, dim=-1, keepdim=True)
                 ids = torch.cat((ids, nxt), dim=1)
-            tokens, taken = sparda.verify_drafts(kept(logits(self, ids, K + 1)), ids[:, n:].int(),
-                                                 torch.rand(1, K + 1, device=ids.device),
+            x = kept(logits(self, ids, K + 1))
+            tokens, taken = sparda.verify_drafts(x, ids[:, n:].int(), torch.rand(1, K + 1, device=ids.device),
                                                  draft_probs=torch.stack(probs, 1) if probs else None,
                                                  temperature=max(float(temperature), 0.0))
-            new = tokens[:, :int(taken) + 1].long()
+            taken = int(taken)
+            new = tokens[:, :taken + 1].long()
+            if int(new[0, taken]) < 0:      # a row without a distribution
+                if temperature > 0.0:
+                    raise RuntimeError(f"generate: the logits behind token {n + taken} hold no distribution (NaN, +inf, or all -inf)")
+                new[0, taken] = torch.argmax(x[0, taken])      # as without a draft model
             if eos_token_id is not None and (new == eos_token_id).any():
                 stop = int((new[0] == eos_token_id).nonzero()[0])
                 return torch.cat((input_ids, new[:, :stop + 1]), dim=1)

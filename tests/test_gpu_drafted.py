@@ -75,3 +75,46 @@ def test_greedy_drafted_generation_equals_plain(backend, prompt_len):
             at = int(other[0, 1])
             x = target(plain[:, :at][:, -CONTEXT:])["logits"][0, -1].topk(2).values
             assert x[0] - x[1] <= 2 * ROW_TOL, at
+
+
+def spoil(model, at, value):
+    """The model's logits are spoiled at the rows that see as many tokens as `at` holds."""
+    forward = model.forward
+
+    def spoiled(ids, **kw):
+        out = forward(ids, **kw)
+        x = out["logits"].clone()
+        for n in at:
+            if n <= ids.shape[1]:
+                x[:, n - 1] = value(x[:, n - 1])
+        return {**out, "logits": x}
+    model.forward = spoiled
+
+
+SPOIL = {"nan": lambda x: x.index_fill(1, torch.tensor([7, 300], device=x.device), float("nan")),
+         "inf": lambda x: x.index_fill(1, torch.tensor([7], device=x.device), float("inf")),
+         "none": lambda x: torch.full_like(x, -float("inf"))}
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("how", list(SPOIL))
+@pytest.mark.parametrize("of", ["target", "draft", "both"])
+def test_rows_without_a_distribution(how, of):
+    """Greedy: the tokens of plain generation. Sampled: an error where the target has no distribution, and the
+    target's tokens where the draft model has none. Never a token of -1."""
+    print(f"[case] drafted spoiled rows {how} {of}", flush=True)
+    target, draft = models("dense")
+    prompt = torch.randint(0, 500, (1, 9), device=DEV)
+    for m, name in ((target, "target"), (draft, "draft")):
+        if of in (name, "both"):
+            spoil(m, {9, 12, 13, 20}, SPOIL[how])
+    plain = target.generate(prompt, max_new_tokens=20, temperature=0.0)
+    out = target.generate(prompt, max_new_tokens=20, temperature=0.0, draft_model=draft, num_drafts=3)
+    assert torch.equal(out, plain)
+    run = lambda: target.generate(prompt, max_new_tokens=20, temperature=1.0, top_k=0, draft_model=draft, num_drafts=3)
+    if of == "draft":
+        out = run()
+        assert out.shape == (1, 29) and 0 <= int(out.min()) and int(out.max()) < 500
+    else:
+        with pytest.raises(RuntimeError, match="no distribution"):
+            run()
