@@ -558,13 +558,20 @@ decode_paged_q4_kernel(PagedDecode a) {
     // m: the columns' references, in the scores' own units, l: this lane's part of their sums
     float m[NC], ref[NC], l[NC];
     const float slack = 16.0f / a.scale_log2;
-    f32x4 o[NC][G][2], less{0.f, 0.f, 0.f, 0.f};             // less: repeated tile: -24 times the sum of the column's weights
+    f32x4 o[NC][G][2], less{0.f, 0.f, 0.f, 0.f};             // less: repeated tile: -24 times the sum of the column's weights, not yet in o
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         m[c] = -__builtin_inff(), ref[c] = l[c] = 0.0f;
 #pragma unroll
         for (int i = 0; i < G; ++i) o[c][i][0] = o[c][i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    // The repeated tile's sums of (16.5 + c) P and of -24 P cancel where values average out, so they must not grow long
+    // apart: 256 steps of a wavefront with flat scores left an fp32 output off by 5.8e-4, now 2.0e-6. fp32 calls join them
+    // in every step (138.5 / 144 us for 32 x 16384, 32/8 heads of 128), the smaller terms first, which the sums hold
+    // better before they are large. bf16 calls, off by 2.4e-3 by their weights' rounding, join them every 64 steps.
+    constexpr bool kEach = DT == SPARDA_F32;
+    constexpr int kFold = 64;
+    int fold = kFold;
     const Q4Masks masks = q4_masks();
     f32x4 s[NC][2];
     auto scores = [&]() __attribute__((always_inline)) {
@@ -648,18 +655,20 @@ decode_paged_q4_kernel(PagedDecode a) {
                 for (int e = 0; e < 8; ++e) ph[e] = 16 * (e / 4) + e % 4 < left ? ph[e] : 0.0f;   // (a number behind the column's positions may be anything)
             }
             q4_split<kTerms>(ph, own);
+            if (kEach) less = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int n = 0; n < kTerms; ++n) less = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, own[n], less, 0, 0, 0);
+            for (int n = kTerms - 1; n >= 0; --n) less = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle, own[n], less, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < G; ++i) {
             const bf16x8 v0 = q4_value_operand<0>(xv[0][i], xv[1][i], masks), v1 = q4_value_operand<1>(xv[0][i], xv[1][i], masks);
             if constexpr (REP) {
 #pragma unroll
-                for (int n = 0; n < kTerms; ++n) {
+                for (int n = kTerms - 1; n >= 0; --n) {
                     o[kRep][i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, own[n], o[kRep][i][0], 0, 0, 0);
                     o[kRep][i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, own[n], o[kRep][i][1], 0, 0, 0);
                 }
+                if constexpr (kEach) o[kRep][i][0] += less, o[kRep][i][1] += less;
             }
 #pragma unroll
             for (int c = 0; c < NF; ++c) {
@@ -681,6 +690,14 @@ decode_paged_q4_kernel(PagedDecode a) {
                 }
             }
             if constexpr (NF > 0) __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (REP && !kEach) {
+            if (--fold == 0) {                               // (wave-uniform)
+                fold = kFold;
+#pragma unroll
+                for (int i = 0; i < G; ++i) o[kRep][i][0] += less, o[kRep][i][1] += less;
+                less = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
         }
     };
     if (u < s_end) {
@@ -733,7 +750,7 @@ decode_paged_q4_kernel(PagedDecode a) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int d = 32 * i + 2 * (4 * grp + e) + j;
-                        if (d < D) lo[(wave * a.lds_heads + cc16) * (D + 4) + d] = 2.0f * (repeated ? o[c][i][j][e] + less[e] : o[c][i][j][e]);
+                        if (d < D) lo[(wave * a.lds_heads + cc16) * (D + 4) + d] = 2.0f * (repeated && !kEach ? o[c][i][j][e] + less[e] : o[c][i][j][e]);
                     }
             }
             if (grp == 0 && (!repeated || mine == 0)) {
