@@ -7,17 +7,19 @@
 //   its total: r = max(p_n - q_n, 0) after a rejection (p_n where that leaves nothing), r = p_n
 //   where no draft is left. Temperature 0: the drafts are compared with the largest logits' lowest indexes.
 //
-// Which token a long sum passes must not hang on how fp32 rounds, so the row that it is drawn from is
-// summed in fp64. Two launches. One reads all logits once and leaves the maximum and the sum of every chunk of
-// every row, for calls of up to 2^21 logits in fp64, in fp32 beyond, where fp64 would take longer than the
-// memory (64 x 8 x 50257: 24.5 us against 12). In the other, workgroups of a (chunk, sequence) find
-// the accepted drafts, which the sums in fp32 decide well enough; each sums its chunk
-// of the row again, and the last one that comes draws. A token from p over sums in fp64 is drawn
-// by the first workgroup alone.
+// What is accepted and which token a long sum passes must not hang on how fp32 rounds, nor on the batch that a
+// sequence is in, so both are decided in fp64. Two launches. One reads all logits once and leaves the maximum and
+// the sum of every chunk of every row, for calls of up to 2^21 logits in fp64, in fp32 beyond, where fp64 would take
+// longer than the memory (64 x 8 x 50257: a call of 47 us against 31). In the other, workgroups of a (chunk, sequence)
+// find the accepted drafts, and each sums its chunk of the row that the token comes from again, in fp64; the last one that
+// comes draws. Where fp32 left an acceptance open (one in 10^5), it does all of this once more in fp64. A token from p
+// over sums in fp64 is drawn by the first workgroup alone.
 //
 // The sums of max(p - q, 0) need p's total Z, which no workgroup has. They are taken apart: over the tokens
 // where w / Z' > q, w = p Z and Z' the total in fp32, sum (w / Z - q) = A / Z - Q with
-// A = sum w, Q = sum q, and the last workgroup has Z. Tokens between the two borders weigh 10^-7 of themselves.
+// A = sum w, Q = sum q, and the last workgroup has Z. Tokens between the two borders are off by at most kVdOff q;
+// where the token that is drawn begins or ends so near to the target that this could matter, the last workgroup
+// does it over too.
 #include "common.h"
 #include "kernels.h"
 
@@ -29,6 +31,10 @@ constexpr int kVdThreads = 256, kVdWaves = kVdThreads / kWave;
 constexpr int kVdRows = 65;           // rows of a sequence (drafts + 1), at most
 constexpr int kVdRounds = 16;         // rounds of a chunk (one 16-byte piece a thread), at most; a row has at most 64 chunks
 constexpr double kVdLog2e = 1.4426950408889634074;
+// How far a row's sum in fp32 may be off, relatively: up to 64 weights a thread (63 2^-24) and six sums of lanes, a
+// weight by its exponential (2^-23) and by three roundings of its exponent t, 3 2^-24 ln 2 |t|, of which the mean over the
+// weights is below 16 (of 2^20 weights at most), 2 10^-6: together 6.4 10^-6.
+constexpr double kVdOff = 0x1p-17;
 
 struct alignas(16) ChunkStat {
     float m;         // largest logit of the chunk
@@ -37,6 +43,7 @@ struct alignas(16) ChunkStat {
 };
 struct ChunkSum {
     double w, above, q;  // of the weights, those above q, q there
+    double near;         // of q where w / Z' is so near to q that w / Z may lie on its other side
 };
 struct SequenceState {
     uint32_t done, pad;  // workgroups of the second launch that are through
@@ -313,7 +320,8 @@ __device__ __forceinline__ void vd_weights(const VdRow& r, int64_t at, int64_t V
 template <int DT>
 __device__ __forceinline__ ChunkSum vd_chunk_sum(const VdRow& r, int64_t first, int rounds, int64_t V, double* red) {
     constexpr int kVe = VdType<DT>::kVe;
-    ChunkSum s{0.0, 0.0, 0.0};
+    ChunkSum s{0.0, 0.0, 0.0, 0.0};
+    float near = 0.0f;                            // (its size matters, not its last bits)
     for (int k = 0; k < rounds; ++k) {
         double w[kVe];
         float q[kVe];
@@ -321,26 +329,31 @@ __device__ __forceinline__ ChunkSum vd_chunk_sum(const VdRow& r, int64_t first, 
 #pragma unroll
         for (int e = 0; e < kVe; ++e) {
             s.w += w[e];
-            if (r.q != nullptr && __builtin_fma(w[e], r.inv_total, -static_cast<double>(q[e])) > 0.0) s.above += w[e], s.q += q[e];
+            if (r.q != nullptr) {
+                const double d = __builtin_fma(w[e], r.inv_total, -static_cast<double>(q[e]));
+                if (d > 0.0) s.above += w[e], s.q += q[e];
+                near += __builtin_fabsf(static_cast<float>(d)) < static_cast<float>(kVdOff) * q[e] ? q[e] : 0.0f;
+            }
         }
     }
     s.w = wave_sum_f64(s.w);
-    if (r.q != nullptr) s.above = wave_sum_f64(s.above), s.q = wave_sum_f64(s.q);
+    if (r.q != nullptr) s.above = wave_sum_f64(s.above), s.q = wave_sum_f64(s.q), s.near = wave_sum(near);
     const int wave = threadIdx.x / kWave;
     __syncthreads();                              // (the array's last use)
-    if (threadIdx.x % kWave == 0) red[3 * wave] = s.w, red[3 * wave + 1] = s.above, red[3 * wave + 2] = s.q;
+    if (threadIdx.x % kWave == 0) red[4 * wave] = s.w, red[4 * wave + 1] = s.above, red[4 * wave + 2] = s.q, red[4 * wave + 3] = s.near;
     __syncthreads();
-    s = ChunkSum{red[0], red[1], red[2]};
+    s = ChunkSum{red[0], red[1], red[2], red[3]};
 #pragma unroll
-    for (int w = 1; w < kVdWaves; ++w) s.w += red[3 * w], s.above += red[3 * w + 1], s.q += red[3 * w + 2];
+    for (int w = 1; w < kVdWaves; ++w) s.w += red[4 * w], s.above += red[4 * w + 1], s.q += red[4 * w + 2], s.near += red[4 * w + 3];
     return s;
 }
 
 // The token of the chunks' sums (lane c of every wavefront holds chunk c's): the chunk where they pass
 // u times their total, the round and the wavefront in it, then the token. All threads of the workgroup; red: one
-// number a round and wavefront.
+// number a round and wavefront; gap: how far the target is from both ends of the token's part of the sum, 0 where
+// no sum passes it.
 template <int DT>
-__device__ __forceinline__ int vd_draw(const VdRow& r, double of_lane, int rounds, int64_t V, float u, double* red, int* found) {
+__device__ __forceinline__ int vd_draw(const VdRow& r, double of_lane, int rounds, int64_t V, float u, double* red, int* found, double* gap) {
     constexpr int kVe = VdType<DT>::kVe;
     const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
     const double upto_chunk = wave_scan_f64(of_lane);
@@ -360,7 +373,7 @@ __device__ __forceinline__ int vd_draw(const VdRow& r, double of_lane, int round
         s = wave_sum_f64(s);
         if (lane == 0) red[k * kVdWaves + wave] = s;
     }
-    if (tid == 0) *found = -1;
+    if (tid == 0) *found = -1, *gap = 0.0;
     __syncthreads();
     // lane: a (round, wavefront), in the order of the row
     const double part = lane < rounds * kVdWaves ? red[lane] : 0.0, upto = wave_scan_f64(part);
@@ -384,7 +397,7 @@ __device__ __forceinline__ int vd_draw(const VdRow& r, double of_lane, int round
                 acc += w[e];
                 if (w[e] > 0.0) {
                     last = e;
-                    if (hit < 0 && acc > target) hit = e;
+                    if (hit < 0 && acc > target) hit = e, *gap = fmin(acc - target, target - (acc - w[e]));
                 }
             }
             *found = last < 0 ? -1 : static_cast<int>(at + (passes && hit >= 0 ? hit : last));
@@ -400,12 +413,18 @@ __device__ __forceinline__ int vd_draw(const VdRow& r, double of_lane, int round
 // workgroup: 35 us a launch of 1024.)
 __device__ __forceinline__ double vd_read(const double* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ void vd_write(double* p, double v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ ChunkSum vd_read_sum(const ChunkSum* p) {   // (all on their way at once)
+    ChunkSum s;
+    s.w = vd_read(&p->w), s.above = vd_read(&p->above), s.q = vd_read(&p->q), s.near = vd_read(&p->near);
+    return s;
+}
 // writes the workgroup's sums and counts it; true in the last of `all`
 __device__ __forceinline__ bool vd_last(ChunkSum* to, const ChunkSum& s, uint32_t* done, uint32_t all, int* flag) {
     if (threadIdx.x == 0) {
         vd_write(&to->w, s.w);
         vd_write(&to->above, s.above);
         vd_write(&to->q, s.q);
+        vd_write(&to->near, s.near);
         __builtin_amdgcn_s_waitcnt(0x0f70);       // vmcnt(0): the stores have arrived
         asm volatile("" ::: "memory");
         *flag = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == all;
@@ -422,10 +441,14 @@ __device__ __forceinline__ bool vd_last(ChunkSum* to, const ChunkSum& s, uint32_
 // q (19 MB) 15.2 us, of which the last workgroups' draw is 2.2 and the exponentials in fp64 1.7 (measured
 // without each); 32 of 32000 11.7; one sequence 6.0. Drafts' logits and q fetched by the first launch instead of
 // here: no difference in a call (28.5 / 28.3, 20.1 / 20.1 us).
+// Where fp32 leaves a decision open (a call of 64 x 7 in a hundred), the last workgroup goes through the sequence again:
+// some 30 us a row. It is inlined, with the registers of six wavefronts a SIMD, which run the 1600 workgroups of 64 x 50257
+// at once: a call of 31.6 us; without the bound 33.3, out of line 34.2, without that way 31.0.
 template <int DT>
-__global__ void __launch_bounds__(kVdThreads, 4) verify_draw_kernel(Verify a) {
+__global__ void __launch_bounds__(kVdThreads, 6) verify_draw_kernel(Verify a) {
     constexpr int kEs = VdType<DT>::kEs;
-    __shared__ double red[kVdRounds * kVdWaves], rz[kVdRows];   // (red: a number a round and wavefront, three a wavefront)
+    __shared__ double red[kVdRounds * kVdWaves], rz[kVdRows];   // (red: a number a round and wavefront, four a wavefront)
+    __shared__ double gap;
     __shared__ float rmax[kVdRows];
     __shared__ int rarg[kVdRows], ok[kVdRows], found, flag;
     const int tid = threadIdx.x, lane = tid % kWave, chunk = blockIdx.x, b = blockIdx.y;
@@ -473,28 +496,40 @@ __global__ void __launch_bounds__(kVdThreads, 4) verify_draw_kernel(Verify a) {
             const bool inside = d >= 0 && d < a.V;
             const double p = valid && inside ? vd_weight((static_cast<double>(x) - m) * c) : 0.0;
             rmax[i] = m, rz[i] = z, rarg[i] = valid ? (greedy ? arg : 0) : -1;
-            ok[i] = valid && inside && (greedy ? d == arg : static_cast<double>(u) * q < p / z) ? 1 : 0;
+            const double uq = static_cast<double>(u) * q;
+            const bool yes = greedy ? d == arg : uq < p / z;
+            // bit 1: open, z in fp32 may be wrong by as much (or c is one that fp32 does not hold)
+            const bool unsure = !a.exact && !greedy && p > 0.0 && (__builtin_fabs(uq * z - p) <= kVdOff * p || c > 3e38);
+            ok[i] = valid && inside ? (yes ? 1 : 0) | (unsure ? 2 : 0) : 0;
         }
     }
     __syncthreads();
-    int n = 0;
-    while (n < count && ok[n] != 0) ++n;
+    int n = 0, open = 0;
+    for (; n < count; ++n) {
+        const int yes = ok[n];
+        open |= yes;
+        if ((yes & 1) == 0) break;
+    }
     auto write = [&](int token) {
         for (int i = tid; i <= a.K; i += kVdThreads)
             a.tokens[static_cast<int64_t>(b) * (a.K + 1) + i] = i < n ? a.drafts[b * a.d_sb + i] : i == n ? token : -1;
         if (tid == 0) a.accepted[b] = n;
     };
-    if (rarg[n] < 0 || greedy) {
+    if ((rarg[n] < 0 && (open & 2) == 0) || greedy) {
         if (chunk == 0) write(rarg[n]);
         return;
     }
     const float u01 = a.uniform[b * a.u_sb + a.K], u = u01 < 0.0f ? 0.0f : u01;
-    VdRow r{};
-    r.row = static_cast<const char*>(a.logits) + (b * a.l_sb + n * a.l_st) * kEs;
-    r.c = c, r.m = rmax[n], r.inv_total = 1.0 / rz[n], r.without = -1;
-    const bool rejected = n < count, against = rejected && a.probs != nullptr;
-    const int64_t d = rejected && !against ? a.drafts[b * a.d_sb + n] : -1;   // the rejected draft weighs nothing
-    if (d >= 0 && d < a.V) r.without = d;
+    auto of_row = [&](double total) {                         // row n, as the token is drawn from it where q is not taken off
+        VdRow r{};
+        r.row = static_cast<const char*>(a.logits) + (b * a.l_sb + n * a.l_st) * kEs;
+        r.c = c, r.m = rmax[n], r.inv_total = 1.0 / total, r.without = -1;
+        const int64_t d = n < count && a.probs == nullptr ? a.drafts[b * a.d_sb + n] : -1;   // the rejected draft weighs nothing
+        if (d >= 0 && d < a.V) r.without = d;
+        return r;
+    };
+    VdRow r = of_row(rz[n]);
+    const bool against = n < count && a.probs != nullptr;
     const int64_t shift = vd_shift<DT>(r.row);
     double of_lane;                                           // a chunk's weight
     int rounds = a.rounds2, token = -1;
@@ -504,12 +539,61 @@ __global__ void __launch_bounds__(kVdThreads, 4) verify_draw_kernel(Verify a) {
         ChunkSum* sums = a.sums + static_cast<int64_t>(b) * a.chunks2;
         const ChunkSum s = vd_chunk_sum<DT>(less, static_cast<int64_t>(chunk) * rounds * VdType<DT>::kRound - shift, rounds, a.V, red);
         if (!vd_last(&sums[chunk], s, &a.state[b].done, static_cast<uint32_t>(a.chunks2), &flag)) return;
-        of_lane = lane < a.chunks2 ? vd_read(&sums[lane].w) : 0.0;
+        const ChunkSum of = lane < a.chunks2 ? vd_read_sum(&sums[lane]) : ChunkSum{0.0, 0.0, 0.0, 0.0};
+        of_lane = of.w;
+        bool again = (open & 2) != 0;
         if (against) {
             less.inv_total = 1.0 / wave_sum_f64(of_lane);
-            const double left = lane < a.chunks2 ? __builtin_fma(vd_read(&sums[lane].above), less.inv_total, -vd_read(&sums[lane].q)) : 0.0;
+            const double left = __builtin_fma(of.above, less.inv_total, -of.q);
             const double of_less = left > 0.0 ? left : 0.0;
-            if (__ballot(of_less > 0.0) != 0) token = vd_draw<DT>(less, of_less, rounds, a.V, u, red, &found);
+            // (the sums up to the token and the target each move by `off` at most)
+            const double off = a.exact ? 0.0 : kVdOff * wave_sum_f64(of.near);
+            if (__ballot(of_less > 0.0) != 0) token = vd_draw<DT>(less, of_less, rounds, a.V, u, red, &found, &gap);
+            again = again || (off > 0.0 && (token < 0 || gap <= 3.0 * off));
+        }
+        if (__builtin_expect(again, 0)) {                     // (workgroup-uniform) the sequence again, all sums in fp64
+            double of_p = 0.0;
+            bool last = false;                                // row n's total is known: now what the token is drawn from
+            for (n = 0;;) {
+                const int yes = n < count ? ok[n] : 0;
+                if (!last) {
+                    if (yes == 1) {
+                        ++n;
+                        continue;
+                    }
+                    if (rarg[n] < 0) {
+                        write(-1);
+                        return;
+                    }
+                    r = of_row(1.0);
+                }
+                const int64_t without = r.without;
+                r.without = last ? without : -1;
+                double z = 0.0;
+                of_lane = 0.0;
+                for (int i = 0; i < a.chunks2; ++i) {
+                    const ChunkSum s = vd_chunk_sum<DT>(r, static_cast<int64_t>(i) * rounds * VdType<DT>::kRound - vd_shift<DT>(r.row), rounds, a.V, red);
+                    z += s.w;
+                    const double left = r.q != nullptr ? __builtin_fma(s.above, r.inv_total, -s.q) : s.w;
+                    if (lane == i) of_lane = left > 0.0 ? left : 0.0;
+                }
+                r.without = without;
+                if (last) break;
+                if (yes != 0) {                               // open: its draft is in the vocabulary
+                    const int32_t d = a.drafts[b * a.d_sb + n];
+                    const double w = vd_weight((static_cast<double>(load_elem<DT>(a.logits, b * a.l_sb + n * a.l_st + d)) - r.m) * c);
+                    const float q = a.probs ? a.probs[b * a.p_sb + n * a.p_st + d] : 1.0f;
+                    if (static_cast<double>(a.uniform[b * a.u_sb + n]) * q < w / z) {
+                        ++n;
+                        continue;
+                    }
+                }
+                if (n < count && a.probs != nullptr) r.q = a.probs + b * a.p_sb + n * a.p_st;
+                else if (without < 0) break;
+                of_p = of_lane, r.inv_total = 1.0 / z, last = true;
+            }
+            if (r.q != nullptr && __ballot(of_lane > 0.0) == 0) r.q = nullptr, of_lane = of_p;   // nothing is left
+            token = -1;
         }
     } else {
         if (chunk != 0) return;
@@ -522,7 +606,7 @@ __global__ void __launch_bounds__(kVdThreads, 4) verify_draw_kernel(Verify a) {
         }
     }
     // from p (without the draft, which holds all of it where nothing is left)
-    if (token < 0) token = __ballot(of_lane > 0.0) != 0 ? vd_draw<DT>(r, of_lane, rounds, a.V, u, red, &found) : static_cast<int>(r.without);
+    if (token < 0) token = __ballot(of_lane > 0.0) != 0 ? vd_draw<DT>(r, of_lane, rounds, a.V, u, red, &found, &gap) : static_cast<int>(r.without);
     write(token);
 }
 
@@ -530,7 +614,7 @@ namespace {
 
 // Sizes, with what was measured on either side (us a call):
 // - fp64 statistics up to 2^21 logits, where the launch and the loads hide them (5 x 32000: 10.1 either way) and
-//   a token from p needs no second pass; beyond, 64 x 8 x 50257 31.5 with them, 28.3 without.
+//   a token from p needs no second pass; beyond, 64 x 8 x 50257 47 with them, 31 without.
 // - The first launch's chunks grow from one round (256 pieces of 16 bytes) to eight while there are more than
 //   4096 of them: two / four / eight rounds at 64 x 8 x 50257 32.3 / 31.4 / 34.5 (then; four is the rule's).
 // - The second launch's grow while there are more than 2048: limits of 256 / 512 / 1024 / 2048 / 4096 at 64 x
