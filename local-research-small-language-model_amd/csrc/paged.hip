@@ -339,13 +339,6 @@ __global__ void __launch_bounds__(HG* KW* kWave, D == 128 ? 2 : DT == SPARDA_F32
     }
 }
 
-// A joined output; zeros for a token that comes before the sequence's first position (of a
-// bad sequence, whose sums are NaN: NaN)
-__device__ __forceinline__ float paged_join_out(const PagedDecode& a, const Share& sh, int h, float O, float L) {
-    const bool none = a.T > 1 && sh.len - a.T + 1 + h / a.heads <= 0;
-    return none && O == O ? 0.0f : O / L;
-}
-
 // Joins the items of a sequence, one workgroup per (32 dims of a query head, sequence):
 //     M = max m_i, out = sum exp2(m_i - M) O_i / sum exp2(m_i - M) l_i.
 // The items' weights once into LDS, then dims over the lanes and the items over the
@@ -412,7 +405,7 @@ __global__ void __launch_bounds__(kPgJoin) decode_paged_join_kernel(PagedDecode 
     for (int w = 0; w < kJW; ++w) den += rl[w];
 #pragma unroll
     for (int i = 1; i < kG; ++i) O += red[i * JD + tid];
-    store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d0 + tid, paged_join_out(a, sh, h, O, den));
+    store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d0 + tid, O / den);
 }
 
 // The same where sequences have few items in the mean: one thread per (query head,
@@ -451,7 +444,7 @@ __global__ void __launch_bounds__(256) decode_paged_join_few_kernel(PagedDecode 
                 O = __builtin_fmaf(wt, y[e], O);
             }
     }
-    store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d, paged_join_out(a, sh, h, O, L));
+    store_elem<DT>(a.out, b * a.out_sb + static_cast<int64_t>(h) * D + d, O / L);
 }
 
 namespace {
@@ -558,7 +551,6 @@ int launch_decode_paged(const void* q, int64_t q_sb, int64_t q_sh, const void* k
     if (const int rc = status_word(&a.status)) return rc;
     a.q = q, a.q_sb = q_sb, a.q_sh = q_sh, a.k = k, a.v = v;
     a.pg = Pages{p_st, s_st, h_st, table, t_st, static_cast<int>(width), static_cast<int>(n_pages)};
-    a.T = 1, a.heads = static_cast<int>(Hq);
     a.ps16 = static_cast<int>(ps / 16), a.len = len, a.B = static_cast<int>(B), a.cap = static_cast<int>(cap);
     a.Hq = static_cast<int>(Hq), a.Hkv = static_cast<int>(Hkv), a.R = static_cast<int>(R);
     a.head_tiles = static_cast<int>(cdiv(R, 16));

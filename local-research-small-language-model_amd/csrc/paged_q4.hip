@@ -810,7 +810,8 @@ namespace {
 //   by two standard deviations of that sum. Over 24 draws of 32 lengths up to 16384, 32/8 heads of 128: 79.9 us in
 //   the mean and 89.7 at most, without the deviations 84.6 and 101.2, with B below 81.3 and 95.8; half as
 //   many items 109.6 where all took 80.5, twice as many 85.0. 16 x 5 tokens: 43.9 and 47.4, 44.3 and 57.2.
-// - A share is four steps at least, one for each wavefront.
+// - A share is four steps at least, one for each wavefront. (A sequence of several items, the only kind that is joined,
+//   therefore holds more than 128 positions: all of its tokens, 64 at most, see some.)
 // - A call over more than the last-level cache holds (256 MB of codes at the tables' capacity) finds nothing there from the
 //   last call and loads past it: 32 x 16384 84.2 / 74.4 us. Smaller ones may: 16 x 5 tokens at 8000 repeated over few
 //   caches 40.9 / 44.2 with such loads, over twelve 49.4 / 48.2; 20 x 9000 32.0 / 33.2 and 36.7 / 33.5.
