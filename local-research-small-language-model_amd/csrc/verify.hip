@@ -67,7 +67,6 @@ struct Verify {
     int chunks1, chunks2;
     ChunkStat* stats;            // [B, K + 1, chunks1]
     ChunkSum* sums;              // [B, chunks2]
-    int exact;                   // the statistics' sums are fp64's
     SequenceState* state;        // [B]
     int32_t *tokens, *accepted;  // [B, K + 1], [B]
 };
@@ -316,8 +315,8 @@ __device__ __forceinline__ void vd_weights(const VdRow& r, int64_t at, int64_t V
     }
 }
 
-// the sums of a chunk's weights, by all threads; the result in every one
-template <int DT>
+// the sums of a chunk's weights, by all threads; the result in every one (NEAR: `near` among them)
+template <int DT, bool NEAR>
 __device__ __forceinline__ ChunkSum vd_chunk_sum(const VdRow& r, int64_t first, int rounds, int64_t V, double* red) {
     constexpr int kVe = VdType<DT>::kVe;
     ChunkSum s{0.0, 0.0, 0.0, 0.0};
@@ -332,12 +331,15 @@ __device__ __forceinline__ ChunkSum vd_chunk_sum(const VdRow& r, int64_t first, 
             if (r.q != nullptr) {
                 const double d = __builtin_fma(w[e], r.inv_total, -static_cast<double>(q[e]));
                 if (d > 0.0) s.above += w[e], s.q += q[e];
-                near += __builtin_fabsf(static_cast<float>(d)) < static_cast<float>(kVdOff) * q[e] ? q[e] : 0.0f;
+                if constexpr (NEAR) near += __builtin_fabsf(static_cast<float>(d)) < static_cast<float>(kVdOff) * q[e] ? q[e] : 0.0f;
             }
         }
     }
     s.w = wave_sum_f64(s.w);
-    if (r.q != nullptr) s.above = wave_sum_f64(s.above), s.q = wave_sum_f64(s.q), s.near = wave_sum(near);
+    if (r.q != nullptr) {
+        s.above = wave_sum_f64(s.above), s.q = wave_sum_f64(s.q);
+        if constexpr (NEAR) s.near = wave_sum(near);
+    }
     const int wave = threadIdx.x / kWave;
     __syncthreads();                              // (the array's last use)
     if (threadIdx.x % kWave == 0) red[4 * wave] = s.w, red[4 * wave + 1] = s.above, red[4 * wave + 2] = s.q, red[4 * wave + 3] = s.near;
@@ -444,7 +446,7 @@ __device__ __forceinline__ bool vd_last(ChunkSum* to, const ChunkSum& s, uint32_
 // Where fp32 leaves a decision open (a call of 64 x 7 in a hundred), the last workgroup goes through the sequence again:
 // some 30 us a row. It is inlined, with the registers of six wavefronts a SIMD, which run the 1600 workgroups of 64 x 50257
 // at once: a call of 31.6 us; without the bound 33.3, out of line 34.2, without that way 31.0.
-template <int DT>
+template <int DT, bool EXACT>
 __global__ void __launch_bounds__(kVdThreads, 6) verify_draw_kernel(Verify a) {
     constexpr int kEs = VdType<DT>::kEs;
     __shared__ double red[kVdRounds * kVdWaves], rz[kVdRows];   // (red: a number a round and wavefront, four a wavefront)
@@ -499,7 +501,7 @@ __global__ void __launch_bounds__(kVdThreads, 6) verify_draw_kernel(Verify a) {
             const double uq = static_cast<double>(u) * q;
             const bool yes = greedy ? d == arg : uq < p / z;
             // bit 1: open, z in fp32 may be wrong by as much (or c is one that fp32 does not hold)
-            const bool unsure = !a.exact && !greedy && p > 0.0 && (__builtin_fabs(uq * z - p) <= kVdOff * p || c > 3e38);
+            const bool unsure = !EXACT && !greedy && p > 0.0 && (__builtin_fabs(uq * z - p) <= kVdOff * p || c > 3e38);
             ok[i] = valid && inside ? (yes ? 1 : 0) | (unsure ? 2 : 0) : 0;
         }
     }
@@ -535,9 +537,9 @@ __global__ void __launch_bounds__(kVdThreads, 6) verify_draw_kernel(Verify a) {
     int rounds = a.rounds2, token = -1;
     VdRow less = r;
     if (against) less.q = a.probs + b * a.p_sb + n * a.p_st;
-    if (!a.exact || against) {
+    if (!EXACT || against) {
         ChunkSum* sums = a.sums + static_cast<int64_t>(b) * a.chunks2;
-        const ChunkSum s = vd_chunk_sum<DT>(less, static_cast<int64_t>(chunk) * rounds * VdType<DT>::kRound - shift, rounds, a.V, red);
+        const ChunkSum s = vd_chunk_sum<DT, !EXACT>(less, static_cast<int64_t>(chunk) * rounds * VdType<DT>::kRound - shift, rounds, a.V, red);
         if (!vd_last(&sums[chunk], s, &a.state[b].done, static_cast<uint32_t>(a.chunks2), &flag)) return;
         const ChunkSum of = lane < a.chunks2 ? vd_read_sum(&sums[lane]) : ChunkSum{0.0, 0.0, 0.0, 0.0};
         of_lane = of.w;
@@ -547,11 +549,11 @@ __global__ void __launch_bounds__(kVdThreads, 6) verify_draw_kernel(Verify a) {
             const double left = __builtin_fma(of.above, less.inv_total, -of.q);
             const double of_less = left > 0.0 ? left : 0.0;
             // (the sums up to the token and the target each move by `off` at most)
-            const double off = a.exact ? 0.0 : kVdOff * wave_sum_f64(of.near);
+            const double off = EXACT ? 0.0 : kVdOff * wave_sum_f64(of.near);
             if (__ballot(of_less > 0.0) != 0) token = vd_draw<DT>(less, of_less, rounds, a.V, u, red, &found, &gap);
             again = again || (off > 0.0 && (token < 0 || gap <= 3.0 * off));
         }
-        if (__builtin_expect(again, 0)) {                     // (workgroup-uniform) the sequence again, all sums in fp64
+        if (!EXACT && __builtin_expect(again, 0)) {           // (workgroup-uniform) the sequence again, all sums in fp64
             double of_p = 0.0;
             bool last = false;                                // row n's total is known: now what the token is drawn from
             for (n = 0;;) {
@@ -572,7 +574,7 @@ __global__ void __launch_bounds__(kVdThreads, 6) verify_draw_kernel(Verify a) {
                 double z = 0.0;
                 of_lane = 0.0;
                 for (int i = 0; i < a.chunks2; ++i) {
-                    const ChunkSum s = vd_chunk_sum<DT>(r, static_cast<int64_t>(i) * rounds * VdType<DT>::kRound - vd_shift<DT>(r.row), rounds, a.V, red);
+                    const ChunkSum s = vd_chunk_sum<DT, false>(r, static_cast<int64_t>(i) * rounds * VdType<DT>::kRound - vd_shift<DT>(r.row), rounds, a.V, red);
                     z += s.w;
                     const double left = r.q != nullptr ? __builtin_fma(s.above, r.inv_total, -s.q) : s.w;
                     if (lane == i) of_lane = left > 0.0 ? left : 0.0;
@@ -601,7 +603,7 @@ __global__ void __launch_bounds__(kVdThreads, 6) verify_draw_kernel(Verify a) {
         of_lane = lane < a.chunks1 ? in_row(stats[n * a.chunks1 + lane], rmax[n]) : 0.0;
         if (r.without >= 0) {
             const int at = static_cast<int>((r.without + shift) / (static_cast<int64_t>(rounds) * VdType<DT>::kRound));
-            const ChunkSum s = vd_chunk_sum<DT>(r, static_cast<int64_t>(at) * rounds * VdType<DT>::kRound - shift, rounds, a.V, red);
+            const ChunkSum s = vd_chunk_sum<DT, false>(r, static_cast<int64_t>(at) * rounds * VdType<DT>::kRound - shift, rounds, a.V, red);
             of_lane = lane == at ? s.w : of_lane;
         }
     }
@@ -654,7 +656,7 @@ int launch_verify_drafts(const void* logits, int dtype, int64_t l_sb, int64_t l_
     char* ws = static_cast<char*>(workspace);
     const Verify a{logits, l_sb, l_st, drafts, d_sb, uniform, u_sb, probs, p_sb, p_st, counts, temperature, all_temperature,
                    static_cast<int>(K), V, p.rounds1, p.rounds2, p.chunks1, p.chunks2,
-                   reinterpret_cast<ChunkStat*>(ws + p.stats), reinterpret_cast<ChunkSum*>(ws + p.sums), p.exact ? 1 : 0,
+                   reinterpret_cast<ChunkStat*>(ws + p.stats), reinterpret_cast<ChunkSum*>(ws + p.sums),
                    reinterpret_cast<SequenceState*>(ws + p.state), tokens, accepted};
     if (!grid_fits(static_cast<int64_t>(p.chunks1) * B * (K + 1), kVdThreads) || !grid_fits(static_cast<int64_t>(p.chunks2) * B, kVdThreads))
         return set_error(SPARDA_ERR_SHAPE, "verify_drafts: grid too large");
@@ -674,7 +676,8 @@ int launch_verify_drafts(const void* logits, int dtype, int64_t l_sb, int64_t l_
             case 8: SPARDA_VD_R(DT_, 8); break;                                              \
             default: SPARDA_VD_R(DT_, 16); break;                                            \
         }                                                                                    \
-        hipLaunchKernelGGL((verify_draw_kernel<DT_>), grid2, threads, 0, stream, a);         \
+        if (p.exact) hipLaunchKernelGGL((verify_draw_kernel<DT_, true>), grid2, threads, 0, stream, a); \
+        else hipLaunchKernelGGL((verify_draw_kernel<DT_, false>), grid2, threads, 0, stream, a);        \
     } while (0)
     if (dtype == SPARDA_F32) SPARDA_VD(SPARDA_F32);
     else SPARDA_VD(SPARDA_BF16);
