@@ -1028,7 +1028,7 @@ SPARDA_API size_t sparda_verify_drafts_workspace_bytes(int64_t B, int64_t K, int
  *   uniform[b,i] q_i(draft_i) < p_i(draft_i);
  * behind n accepted drafts the token is the lowest one at which the cumulated sum of r
  * passes uniform[b,K] times its total, r = max(p_n - q_n, 0) after a rejection (p_n where that is
- * zero everywhere), r = p_n behind the last draft; sums that decide the token in fp64. A
+ * zero everywhere), r = p_n behind the last draft; acceptances and tokens are those of sums in fp64, whatever the batch. A
  * temperature that is not above 0: draft i is accepted if it is the lowest index of
  * row i's largest logit, and the token is that of row n; +inf counts as 3.4e38. A row without a distribution (no logit above
  * -inf, or NaN or +inf among them) accepts nothing and gives token -1; so does a

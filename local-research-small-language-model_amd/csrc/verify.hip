@@ -440,8 +440,8 @@ __device__ __forceinline__ bool vd_last(ChunkSum* to, const ChunkSum& s, uint32_
 // One workgroup per (chunk, sequence), or per sequence where all sums are there and no distributions are given.
 // Bound by its chain: the statistics, the row (a load that waits for what was accepted), a reduction,
 // the sums' way through memory, the last workgroup's loads of them and of its chunk again. 64 rows of 50257 with
-// q (19 MB) 15.2 us, of which the last workgroups' draw is 2.2 and the exponentials in fp64 1.7 (measured
-// without each); 32 of 32000 11.7; one sequence 6.0. Drafts' logits and q fetched by the first launch instead of
+// q (19 MB) 17.0 us, of which the last workgroups' draw is 2.2 and the exponentials in fp64 1.7 (measured
+// without each); 32 of 32000 in fp32 12.7; one sequence 6.0. Drafts' logits and q fetched by the first launch instead of
 // here: no difference in a call (28.5 / 28.3, 20.1 / 20.1 us).
 // Where fp32 leaves a decision open (a call of 64 x 7 in a hundred), the last workgroup goes through the sequence again:
 // some 30 us a row. It is inlined, with the registers of six wavefronts a SIMD, which run the 1600 workgroups of 64 x 50257
