@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(kVdThreads, 6) verify_draw_kernel(Verify a) {
         }
     }
     __syncthreads();
-    int n = 0, open = 0;
+    int n = 0, open = !EXACT && c > 3e38 ? 2 : 0;
     for (; n < count; ++n) {
         const int yes = ok[n];
         open |= yes;

@@ -15,8 +15,8 @@ B, V = 24, 50257                       # 2.4 M logits with a draft each
 
 def case(dtype, temperature, seed):
     g = torch.Generator().manual_seed(seed)
-    x = (torch.randn(B, 2, V, generator=g) * 3).to(dtype)
-    p = torch.softmax(x.double() / temperature, -1)
+    x = (torch.randn(B, 2, V, generator=g) * 3 * (temperature if temperature < 1e-30 else 1)).to(dtype)
+    p = torch.softmax(x.double() / float(np.float32(temperature)), -1)
     return g, x, p
 
 
@@ -27,8 +27,7 @@ def alone(x, drafts, u, probs, temperature):
     return torch.cat([t for t, _ in r]), torch.cat([n for _, n in r])
 
 
-@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
-@pytest.mark.parametrize("temperature", [1.0, 0.5])
+@pytest.mark.parametrize("dtype,temperature", [(BF, 1.0), (BF, 0.5), (F32, 1.0), (F32, 0.5), (F32, 1e-39)])   # (the last: 1 / T is no fp32 number)
 @pytest.mark.parametrize("given", [True, False], ids=["probs", "tokens"])
 def test_acceptance_next_to_its_border(dtype, temperature, given):
     """u q and p closer than fp32 tells apart: u is the fp32 number below or above p / q. (p in float64 is right to 1e-14;
